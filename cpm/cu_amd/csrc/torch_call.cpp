@@ -148,7 +148,7 @@ struct Caller<R (*)(A...)> {
     X(kv_append) X(rope_table) X(rope_apply) X(gather_rows) X(head_weight_tile) X(head_workspace_bytes)                   \
     X(frspec_head_topk) X(lm_head_argmax) X(log_softmax_sliced) X(log_softmax_workspace_bytes) X(topk)                    \
     X(topk_workspace_bytes) X(remap) X(tree_accept) X(kv_compact) X(accept_commit) X(verify_tail) X(verify_tail_inplace)  \
-    X(draft_tree_begin) X(draft_tree_extend) X(draft_tree_finish) X(draft_tree_finish_root)
+    X(draft_tree_begin) X(draft_tree_extend) X(draft_tree_finish) X(draft_tree_finish_root) X(int8_weight_tile)
 
 #define X(name)                                                                                                    \
     decltype(&cpmcu_##name) fn_##name = nullptr;                                                                   \
@@ -258,6 +258,193 @@ PyObject* call_tree_attention_rows(PyObject*, PyObject* const* args, Py_ssize_t 
     }));
 }
 
+// ---- batches: operators whose tensors may be views of wider rows; types, shapes and the device are checked here ----
+
+// A tensor of this type on the current device (whose stream the call goes to); null with an AssertionError set.
+const at::Tensor* device_tensor(PyObject* o, at::ScalarType type, const char* what) {
+    const at::Tensor* t = tensor_or_null(o);
+    if (t && t->is_cuda() && t->scalar_type() == type && t->device().index() == c10::hip::current_device()) return t;
+    PyErr_Format(PyExc_AssertionError, "%s on the current device required", what);
+    return nullptr;
+}
+const at::Tensor* dense_tensor(PyObject* o, at::ScalarType type, const char* what) {
+    const at::Tensor* t = device_tensor(o, type, what);
+    return t && expect(t->is_contiguous(), "device-resident contiguous tensor required") ? t : nullptr;
+}
+int32_t* ints(const at::Tensor* t) { return static_cast<int32_t*>(t->data_ptr()); }
+at::Tensor new_tensor(const at::Tensor& like, at::ScalarType type, at::IntArrayRef sizes) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
+bool integer(PyObject* o, int* out) { return convert(o, out); }
+
+decltype(&cpmcu_batch_tables) fn_batch_tables = nullptr;
+decltype(&cpmcu_rope_rows) fn_rope_rows = nullptr;
+decltype(&cpmcu_kv_append_slots) fn_kv_append_slots = nullptr;
+decltype(&cpmcu_quantize_rows) fn_quantize_rows = nullptr;
+decltype(&cpmcu_int8_linear) fn_int8_linear = nullptr;
+
+bool arguments(Py_ssize_t nargs, Py_ssize_t expected) {
+    if (nargs != expected) PyErr_Format(PyExc_TypeError, "%zd arguments given, %zd expected", nargs, expected);
+    return nargs == expected;
+}
+
+// batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, max_rows): (kv_lens, held, counts, row_offsets, positions, slots)
+PyObject* call_batch_tables(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 7)) return nullptr;
+    const char* const what = "batch_tables: int32 tensors";
+    const at::Tensor* t[6];
+    for (int i = 0; i < 6; ++i)
+        if (!(t[i] = dense_tensor(args[i], at::kInt, what))) return nullptr;
+    int max_rows;
+    if (!integer(args[6], &max_rows)) return nullptr;
+    const at::Tensor &kv = *t[0], &tables = *t[2], &stack = *t[4];
+    const int64_t B = kv.numel();
+    if (!expect(tables.dim() == 2 && tables.size(0) == B && t[1]->numel() == B && t[3]->numel() == B && t[5]->numel() == 2,
+                "batch_tables: lengths and held pages are [B], the tables [B, max_blocks], the counts [2]") ||
+        !expect(B <= INT32_MAX && tables.size(1) <= INT32_MAX && stack.numel() <= INT32_MAX, "batch_tables: sizes beyond 32 bits"))
+        return nullptr;
+    const int64_t rows = max_rows > 0 ? max_rows : 0;
+    const int64_t sizes[6] = {B, B, 2, B + 1, rows, rows};
+    at::Tensor out[6];
+    for (int i = 0; i < 6; ++i) out[i] = new_tensor(kv, at::kInt, at::IntArrayRef(&sizes[i], 1));
+    void* const st = current_stream();
+    const int rc = without_gil([&] {
+        return fn_batch_tables(ints(t[0]), ints(t[1]), static_cast<int>(B), ints(t[2]), static_cast<int>(tables.size(1)), ints(t[3]), ints(t[4]), static_cast<int>(stack.numel()),
+                               ints(t[5]), ints(&out[0]), ints(&out[1]), ints(&out[2]), ints(&out[3]), ints(&out[4]), ints(&out[5]), max_rows, st);
+    });
+    if (rc != CPMCU_OK) return status(rc);
+    THPObjectPtr result(PyTuple_New(6));
+    if (!result) return nullptr;
+    for (int i = 0; i < 6; ++i) {
+        PyObject* o = THPVariable_Wrap(std::move(out[i]));
+        if (!o) return nullptr;
+        PyTuple_SET_ITEM(result.get(), i, o);
+    }
+    return result.release();
+}
+
+// Rows of heads, [n, heads, D] of 16-bit floats whose heads follow each other; rows may be further apart.
+struct HeadRows {
+    void* at = nullptr;
+    int64_t stride = 0, n = 0, heads = 0, dim = 0;
+};
+bool head_rows(PyObject* o, const char* what, HeadRows* r) {
+    const at::Tensor* t = device_tensor(o, at::kHalf, what);
+    if (!t) return false;
+    if (t->dim() != 3 || t->size(0) > INT32_MAX || t->size(1) > INT32_MAX || t->size(2) > INT32_MAX ||
+        (t->numel() > 0 && (t->stride(2) != 1 || (t->size(1) > 1 && t->stride(1) != t->size(2))))) {
+        PyErr_Format(PyExc_AssertionError, "%s: [n, heads, D] with the heads of a row one after the other required", what);
+        return false;
+    }
+    *r = HeadRows{t->data_ptr(), t->size(0) > 1 ? t->stride(0) : t->size(1) * t->size(2), t->size(0), t->size(1), t->size(2)};
+    return true;
+}
+bool alike(const HeadRows& a, const HeadRows& b) { return a.n == b.n && a.heads == b.heads && a.dim == b.dim; }
+
+// rope_rows(q, k, positions, inv_freq, interleaved, magnitude, transposed, q_out, k_out): k and k_out may be None.
+PyObject* call_rope_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 9)) return nullptr;
+    HeadRows q, k, q_out, k_out;
+    int interleaved, transposed;
+    float magnitude;
+    if (!head_rows(args[0], "rope_rows: q of 16-bit floats", &q) || !head_rows(args[7], "rope_rows: q_out of 16-bit floats", &q_out) ||
+        (args[1] != Py_None && (!head_rows(args[1], "rope_rows: k of 16-bit floats", &k) || !head_rows(args[8], "rope_rows: k_out of 16-bit floats", &k_out))))
+        return nullptr;
+    const at::Tensor *pos = dense_tensor(args[2], at::kInt, "rope_rows: int32 positions"), *freq = pos ? dense_tensor(args[3], at::kFloat, "rope_rows: float32 inv_freq") : nullptr;
+    if (!freq || !integer(args[4], &interleaved) || !convert(args[5], &magnitude) || !integer(args[6], &transposed)) return nullptr;
+    if (!expect(alike(q, q_out) && alike(k, k_out) && (args[1] == Py_None || (k.n == q.n && k.dim == q.dim)), "rope_rows: q, k and their results differ in shape") ||
+        !expect(pos->numel() == q.n && freq->numel() <= INT32_MAX / 2, "rope_rows: a position for each row required"))
+        return nullptr;
+    void* const st = current_stream();
+    return status(without_gil([&] {
+        return fn_rope_rows(ints(pos), static_cast<const float*>(freq->data_ptr()), static_cast<int>(2 * freq->numel()), interleaved, magnitude, transposed, q.at, q.stride, q_out.at,
+                            q_out.stride, static_cast<int>(q.heads), k.at, k.stride, k_out.at, k_out.stride, static_cast<int>(k.heads), static_cast<int>(q.dim), static_cast<int>(q.n), st);
+    }));
+}
+
+// kv_append_slots(k_pool, v_pool, k, v, slots, q, q_out, positions, inv_freq, interleaved, magnitude): q and q_out, positions and inv_freq may be None.
+PyObject* call_kv_append_slots(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 11)) return nullptr;
+    const char* const pools = "kv_append_slots: pools of 16-bit floats";
+    const at::Tensor *k_pool = dense_tensor(args[0], at::kHalf, pools), *v_pool = k_pool ? dense_tensor(args[1], at::kHalf, pools) : nullptr;
+    HeadRows k, v, q, q_out;
+    if (!v_pool || !head_rows(args[2], "kv_append_slots: k of 16-bit floats", &k) || !head_rows(args[3], "kv_append_slots: v of 16-bit floats", &v) ||
+        (args[5] != Py_None && (!head_rows(args[5], "kv_append_slots: q of 16-bit floats", &q) || !head_rows(args[6], "kv_append_slots: q_out of 16-bit floats", &q_out))))
+        return nullptr;
+    const at::Tensor *slots = dense_tensor(args[4], at::kInt, "kv_append_slots: int32 slots"), *pos = nullptr, *freq = nullptr;
+    if (!slots || (args[7] != Py_None && !(pos = dense_tensor(args[7], at::kInt, "kv_append_slots: int32 positions"))) ||
+        (args[8] != Py_None && !(freq = dense_tensor(args[8], at::kFloat, "kv_append_slots: float32 inv_freq"))))
+        return nullptr;
+    int interleaved;
+    float magnitude;
+    if (!integer(args[9], &interleaved) || !convert(args[10], &magnitude)) return nullptr;
+    if (!expect(k_pool->dim() == 4 && k_pool->size(2) == CPMCU_PAGE_SIZE && k_pool->size(3) == CPMCU_HEAD_DIM && v_pool->dim() == 4 && v_pool->size(0) == k_pool->size(0) &&
+                    v_pool->size(1) == k_pool->size(1) && v_pool->size(2) == CPMCU_HEAD_DIM && v_pool->size(3) == CPMCU_PAGE_SIZE && k_pool->size(0) <= INT32_MAX,
+                "kv_append_slots: pools are [pages, Hkv, 256, 128] and [pages, Hkv, 128, 256]") ||
+        !expect(alike(k, v) && k.heads == k_pool->size(1) && k.dim == CPMCU_HEAD_DIM && slots->numel() == k.n, "kv_append_slots: k and v are [n, Hkv, 128], slots [n]") ||
+        !expect(alike(q, q_out) && (args[5] == Py_None || (q.n == k.n && q.dim == CPMCU_HEAD_DIM)), "kv_append_slots: q and q_out are [n, Hq, 128]") ||
+        !expect((pos != nullptr) == (freq != nullptr) && (!pos || pos->numel() == k.n) && (!freq || freq->numel() <= CPMCU_HEAD_DIM), "kv_append_slots: positions [n] and inv_freq go together"))
+        return nullptr;
+    void* const st = current_stream();
+    return status(without_gil([&] {
+        return fn_kv_append_slots(k_pool->data_ptr(), v_pool->data_ptr(), static_cast<int>(k_pool->size(0)), ints(slots), k.at, k.stride, v.at, v.stride, static_cast<int>(k.n),
+                                  static_cast<int>(k.heads), pos ? ints(pos) : nullptr, freq ? static_cast<const float*>(freq->data_ptr()) : nullptr,
+                                  freq ? static_cast<int>(2 * freq->numel()) : 0, interleaved, magnitude, q.at, q.stride, q_out.at, q_out.stride, static_cast<int>(q.heads), st);
+    }));
+}
+
+// quantize_rows(x): (xq [n, K rounded up to 64] of int8, scales [n])
+PyObject* call_quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 1)) return nullptr;
+    const at::Tensor* x = device_tensor(args[0], at::kHalf, "quantize_rows: rows of 16-bit floats");
+    if (!x || !expect(x->dim() == 2 && (x->numel() == 0 || x->size(1) == 1 || x->stride(1) == 1) && x->size(0) <= INT32_MAX && x->size(1) <= INT32_MAX - 64, "quantize_rows: [n, K] with whole rows required"))
+        return nullptr;
+    const int64_t n = x->size(0), K = x->size(1), sizes[2] = {n, (K + 63) / 64 * 64};
+    at::Tensor xq = new_tensor(*x, at::kChar, at::IntArrayRef(sizes, 2)), scales = new_tensor(*x, at::kFloat, at::IntArrayRef(sizes, 1));
+    if (n == 0 || K == 0) return expect(K > 0, "quantize_rows: rows without values") ? Py_BuildValue("NN", THPVariable_Wrap(xq), THPVariable_Wrap(scales)) : nullptr;
+    void* const st = current_stream();
+    const int rc = without_gil([&] {
+        return fn_quantize_rows(x->data_ptr(), n > 1 ? x->stride(0) : K, static_cast<int>(n), static_cast<int>(K), static_cast<int8_t*>(xq.data_ptr()), static_cast<float*>(scales.data_ptr()), st);
+    });
+    if (rc != CPMCU_OK) return status(rc);
+    return Py_BuildValue("NN", THPVariable_Wrap(std::move(xq)), THPVariable_Wrap(std::move(scales)));
+}
+
+// int8_linear(xq, x_scales, w_tiled, w_scales, V, K, out or None): out [n, V]
+PyObject* call_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 7)) return nullptr;
+    const at::Tensor* t[4];
+    for (int i = 0; i < 4; ++i)
+        if (!(t[i] = dense_tensor(args[i], i % 2 ? at::kFloat : at::kChar, i % 2 ? "int8_linear: float32 scales" : "int8_linear: int8 rows and weights"))) return nullptr;
+    int V, K;
+    if (!integer(args[4], &V) || !integer(args[5], &K)) return nullptr;
+    const at::Tensor& xq = *t[0];
+    if (!expect(V >= 1 && K >= 1 && xq.dim() == 2 && xq.size(1) == (K + 63) / 64 * 64 && xq.size(0) <= INT32_MAX && t[1]->numel() == xq.size(0),
+                "int8_linear: rows are [n, K rounded up to 64], with a scale each") ||
+        !expect(t[3]->numel() == V && t[2]->numel() == (V + 15) / 16 * 16 * ((K + 63) / 64 * 64), "int8_linear: the weight is tiled from [V, K], with a scale for each channel"))
+        return nullptr;
+    const int64_t n = xq.size(0), sizes[2] = {n, V};
+    at::Tensor made;
+    const at::Tensor* out;
+    if (args[6] == Py_None) {
+        made = new_tensor(xq, at::kHalf, at::IntArrayRef(sizes, 2));
+        out = &made;
+    } else if (!(out = dense_tensor(args[6], at::kHalf, "int8_linear: out of 16-bit floats")) || !expect(out->dim() == 2 && out->size(0) == n && out->size(1) == V, "int8_linear: out is [n, V]")) {
+        return nullptr;
+    }
+    if (n > 0) {
+        void* const st = current_stream();
+        const int rc = without_gil([&] {
+            return fn_int8_linear(static_cast<const int8_t*>(xq.data_ptr()), static_cast<const float*>(t[1]->data_ptr()), static_cast<const int8_t*>(t[2]->data_ptr()),
+                                  static_cast<const float*>(t[3]->data_ptr()), static_cast<int>(n), V, K, out->data_ptr(), st);
+        });
+        if (rc != CPMCU_OK) return status(rc);
+    }
+    if (args[6] != Py_None) {
+        Py_INCREF(args[6]);
+        return args[6];
+    }
+    return THPVariable_Wrap(std::move(made));
+}
+
 // empty(like, dtype, rows, cols, dtype, rows, cols, ...): uninitialised [rows, cols] tensors ([rows] where cols is 0) on like's
 // device, as a tuple.  dtype: 'h' 16-bit float, 'f' fp32, 'i' int32, 'l' int64.
 PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -315,7 +502,9 @@ PyObject* bind(PyObject*, PyObject* handle) {
     };
     bool ok = find("cpmcu_last_error", &g_last_error) && find("cpmcu_lm_head_partials", &fn_lm_head_partials) &&
               find("cpmcu_tree_attention_window", &fn_tree_attention_window) &&
-              find("cpmcu_tree_attention_workspace_bytes", &fn_tree_attention_workspace_bytes);
+              find("cpmcu_tree_attention_workspace_bytes", &fn_tree_attention_workspace_bytes) && find("cpmcu_batch_tables", &fn_batch_tables) &&
+              find("cpmcu_rope_rows", &fn_rope_rows) && find("cpmcu_kv_append_slots", &fn_kv_append_slots) &&
+              find("cpmcu_quantize_rows", &fn_quantize_rows) && find("cpmcu_int8_linear", &fn_int8_linear);
 #define X(name) ok = ok && find("cpmcu_" #name, &fn_##name);
     CPMCU_TORCH_CALLS(X)
 #undef X
@@ -330,6 +519,11 @@ PyMethodDef g_methods[] = {
     X(lm_head_partials)
     X(kv_append_rows)
     X(tree_attention_rows)
+    X(batch_tables)
+    X(rope_rows)
+    X(kv_append_slots)
+    X(quantize_rows)
+    X(int8_linear)
     ENTRY("empty", empty)
     {"pinned", entry<pinned>, METH_O, nullptr},
     {"synchronize", entry<synchronize>, METH_NOARGS, nullptr},

@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libcpmcu_amd.so")
 OK, ERR_INVALID_ARGUMENT, ERR_RUNTIME, ERR_UNSUPPORTED, ERR_HIP = range(5)
 
 c_int, c_float, c_size_t = ctypes.c_int, ctypes.c_float, ctypes.c_size_t
-c_void_p, c_char_p, c_u64 = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_uint64
+c_void_p, c_char_p, c_u64, c_i64 = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_uint64, ctypes.c_int64
 _P = c_void_p
 
 # name -> (restype, argtypes); status-returning functions are wrapped to raise
@@ -90,6 +90,13 @@ SIGNATURES = {
     "cpmcu_draft_tree_begin": (c_int, [_P, c_int, c_int, _P, _P, _P, _P, _P, _P]),
     "cpmcu_draft_tree_extend": (c_int, [_P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P]),
     "cpmcu_draft_tree_finish": (c_int, [_P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P]),
+    "cpmcu_batch_tables": (c_int, [_P, _P, c_int, _P, c_int, _P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P]),
+    "cpmcu_rope_rows": (c_int, [_P, _P, c_int, c_int, c_float, c_int, _P, c_i64, _P, c_i64, c_int, _P, c_i64, _P, c_i64, c_int, c_int, c_int, _P]),
+    "cpmcu_kv_append_slots": (c_int, [_P, _P, c_int, _P, _P, c_i64, _P, c_i64, c_int, c_int, _P, _P, c_int, c_int, c_float, _P, c_i64, _P, c_i64, c_int, _P]),
+    "cpmcu_quantize_rows": (c_int, [_P, c_i64, c_int, c_int, _P, _P, _P]),
+    "cpmcu_int8_weight_bytes": (c_size_t, [c_int, c_int]),
+    "cpmcu_int8_weight_tile": (c_int, [_P, c_int, c_int, _P, _P]),
+    "cpmcu_int8_linear": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, _P, _P]),
     "cpmcu_draft_tree_finish_root": (c_int, [_P, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P]),
 }
 

@@ -4,6 +4,7 @@ torch only supplies device memory and the current stream; every function here is
 ``libcpmcu_amd.so`` through the C-ABI (``include/cpmcu_amd.h``), made by the native binding
 ``_torch_call``.  Nothing falls back to torch math.
 """
+import copy
 import ctypes
 import math
 
@@ -134,6 +135,161 @@ def tree_attention(q, cache, layer, kv_len, max_kv_len, mask=None, scale=None, n
     if need is not None:
         native.tree_attention_rows(*args, _workspace("attn", need, q.device), int(num_splits))
     return out
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=None, length=None):
+    """(inv_freq fp32 [rotary_dim / 2] on the host, magnitude) for rope_rows: base ** (-2i / rotary_dim), stretched for contexts longer
+    than the model was trained on.  scaling is None or a dict whose "type" is
+
+    * "linear": positions as if factor times closer, inv_freq / factor;
+    * "ntk": the base grows so that the slowest pair is stretched by factor and the fastest not at all,
+      base * factor ** (rotary_dim / (rotary_dim - 2));
+    * "yarn": pairs that turn more than beta_fast (32) times within original (the trained length) stay, those of fewer than beta_slow (1)
+      turns are divided by factor, with a linear ramp over the pairs in between; magnitude 0.1 ln(factor) + 1 (or "magnitude");
+    * "longrope": inv_freq / short_factor[i], from lengths above original on / long_factor[i] (length: the context this step works
+      with); magnitude sqrt(1 + ln(factor) / ln(original)) where factor > 1 (or "magnitude").
+
+    Computed in 64 bits."""
+    half = int(rotary_dim) // 2
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim=%r is not an even number" % (rotary_dim,))
+    i = torch.arange(half, dtype=torch.float64)
+    freq = float(base) ** (-i / half)
+    magnitude = 1.0
+    if scaling is not None:
+        kind = scaling.get("type")
+        factor = float(scaling.get("factor", 1.0))
+        if not factor >= 1.0:
+            raise ValueError("scaling factor %r below 1" % (factor,))
+        if kind == "linear":
+            freq = freq / factor
+        elif kind == "ntk":
+            if half < 2:
+                raise ValueError("ntk scaling of a single pair")
+            freq = (float(base) * factor ** (half / (half - 1.0))) ** (-i / half)
+        elif kind == "yarn":
+            original = float(scaling["original"])
+            # the pair (a fraction of one) that turns `turns` times within the trained length
+            pair_of = lambda turns: half * math.log(original / (turns * 2.0 * math.pi)) / math.log(float(base))  # noqa: E731
+            low = max(math.floor(pair_of(float(scaling.get("beta_fast", 32.0)))), 0)
+            high = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1.0)))), 2 * half - 1)
+            ramp = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+            freq = freq * (1.0 - ramp) + freq / factor * ramp
+            magnitude = float(scaling.get("magnitude", 0.1 * math.log(factor) + 1.0))
+        elif kind == "longrope":
+            original = float(scaling["original"])
+            if length is None:
+                raise ValueError("longrope frequencies depend on the length")
+            by = torch.as_tensor(scaling["long_factor" if length > original else "short_factor"], dtype=torch.float64)
+            if by.numel() != half:
+                raise ValueError("%d factors for %d pairs" % (by.numel(), half))
+            freq = freq / by
+            magnitude = float(scaling.get("magnitude", math.sqrt(1.0 + math.log(factor) / math.log(original))))
+        else:
+            raise ValueError("rotary scaling of type %r" % (kind,))
+    return freq.float(), magnitude
+
+
+def rope_rows(q, k, positions, inv_freq, interleaved=False, magnitude=1.0, transposed=False, q_out=None, k_out=None):
+    """Rotary positions of q [n, Hq, D] and k [n, Hkv, D] (or None): (q_out, k_out), new tensors unless given (q and k themselves: in place).
+
+    positions int32 [n] (rows of a negative one are left out), inv_freq fp32 [rotary_dim / 2] (see rope_frequencies): the first rotary_dim
+    values of each head turn, in pairs (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1).  Rows may be views of wider ones (a fused
+    projection's output).  transposed: gradients of the results back to q and k.
+    """
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k is not None and k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    (_native or _calls()).rope_rows(q, k, positions, inv_freq, 1 if interleaved else 0, magnitude, 1 if transposed else 0, q_out, k_out)
+    return q_out, k_out
+
+
+def batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, max_rows):
+    """Pages and slots of a batch's new rows, from the requests' lengths, in one launch (int32 device tensors).
+
+    kv_lens [B] cached and new_lens [B] new tokens of each request (negative: it has ended and gives its pages back); block_tables
+    [B, max_blocks], of which the first held[r] entries of row r are request r's pages; free_pages, a stack of which counts[0] are free.
+    Returns dict(kv_lens [B], held [B], counts [2] = (free pages, refused requests), row_offsets [B + 1], positions [max_rows], slots
+    [max_rows]), which the next step takes in place of the inputs; block_tables and free_pages change in place.  Rows without a slot
+    (refused requests', and behind the last one) have slot and position -1.  See PageBatch for an object that keeps all this.
+    """
+    lens, held, counts, offsets, positions, slots = (_native or _calls()).batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, int(max_rows))
+    return dict(kv_lens=lens, held=held, counts=counts, row_offsets=offsets, positions=positions, slots=slots)
+
+
+def kv_append_slots(cache, layer, k, v, slots, q=None, q_out=None, positions=None, inv_freq=None, interleaved=False, magnitude=1.0):
+    """Rows k, v [n, Hkv, 128] of several requests to slots[t] = page * 256 + place of the cache (rows without a slot: left out).
+
+    With positions and inv_freq, as rope_rows takes them, k is rotated on its way, and q [n, Hq, 128] (if given) into q_out, which is
+    returned; rows left out keep what q_out held."""
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    (_native or _calls()).kv_append_slots(cache.k[layer], cache.v[layer], k, v, slots, q, q_out, positions, inv_freq, 1 if interleaved else 0, magnitude)
+    return q_out
+
+
+class PageBatch:
+    """The pages of up to max_requests requests on one paged cache, kept on the device: tables, lengths and the stack of free pages.
+
+    ``plan(new_lens, max_rows)`` gives every request room for its new rows and returns where they go (batch_tables); ``kv_lens[r:r + 1]`` and
+    ``block_tables[r]`` are then what tree_attention takes for request r (through ``cache_of``)."""
+
+    def __init__(self, cache, max_requests, max_blocks, num_pages=None):
+        ints = dict(dtype=torch.int32, device=cache.device)
+        self.cache = cache
+        pages = cache.num_pages if num_pages is None else int(num_pages)
+        assert 1 <= pages <= cache.num_pages
+        self.block_tables = torch.zeros((max_requests, max_blocks), **ints)
+        self.kv_lens = torch.zeros(max_requests, **ints)
+        self.held = torch.zeros(max_requests, **ints)
+        self.free_pages = torch.arange(pages - 1, -1, -1, **ints)
+        self.counts = torch.tensor([pages, 0], **ints)
+
+    def plan(self, new_lens, max_rows):
+        """new_lens int32 [max_requests]: rows of this step, -1 for a request that has ended.  The step is taken: lengths and pages
+        are those with the new rows from here on (counts[1] says how many requests were refused)."""
+        step = batch_tables(self.kv_lens, new_lens, self.block_tables, self.held, self.free_pages, self.counts, max_rows)
+        # (copied, not replaced: views of them, and launches captured with them, see the new values)
+        for name in ("kv_lens", "held", "counts"):
+            getattr(self, name).copy_(step[name])
+        return step
+
+    def cache_of(self, r):
+        """Request r's view of the cache, for tree_attention."""
+        view = copy.copy(self.cache)
+        view.block_table = self.block_tables[r]
+        return view
+
+
+def quantize_rows(x):
+    """16-bit rows [n, K] to 8 bits: (xq int8 [n, K rounded up to 64], zeros behind K; scales fp32 [n] = max |x| / 127)."""
+    return (_native or _calls()).quantize_rows(x)
+
+
+class Int8Weight:
+    """8-bit weights [V, K] with a scale for each channel, in matrix-operand order: built once."""
+
+    def __init__(self, w, scales):
+        """w int8 [V, K], scales fp32 [V]: the weight of channel c is w[c] * scales[c]."""
+        assert w.dtype == torch.int8 and w.dim() == 2 and scales.dtype == torch.float32 and scales.numel() == w.shape[0]
+        self.V, self.K = w.shape
+        self.shape = (self.V, self.K)
+        self.scales = scales.contiguous()
+        w = w.contiguous()
+        self.data = torch.empty(_lib().raw.cpmcu_int8_weight_bytes(self.V, self.K), dtype=torch.int8, device=w.device)
+        _calls().int8_weight_tile(w, self.V, self.K, self.data)
+
+    @classmethod
+    def quantized(cls, w):
+        """From 16-bit weights [V, K]: each channel to 8 bits as quantize_rows does a row."""
+        wq, scales = quantize_rows(w)
+        return cls(wq[:, :w.shape[1]], scales)
+
+
+def int8_linear(xq, x_scales, weight, out=None):
+    """[n, V] = (xq . weight^T in 32-bit integers) * x_scales * weight.scales, in 16 bits; xq and x_scales from quantize_rows."""
+    return (_native or _calls()).int8_linear(xq, x_scales, weight.data, weight.scales, weight.V, weight.K, out)
 
 
 def gather_rows(src, remap):

@@ -640,6 +640,68 @@ int cpmcu_draft_tree_finish_root(void* state, int k, int num_iter, int tree_size
                                  const int32_t* token_id_remap, int32_t root_id, int32_t* tree_draft_ids, int32_t* tree_position_ids,
                                  uint64_t* tree_attn_mask, int32_t* tree_parent, void* stream);
 
+/* ---- Batches: pages, slots, rotary positions and 8-bit products of several requests' rows ----
+ * No counterpart in the reference, which serves one sequence (its cache rows are [P, P + T), src/model/attn.cuh:14-21, its block
+ * table is null, src/flash_attn/flash_api.hpp:379, its rotary layout is one, src/model/rotary.cuh:7-34, and its 8-bit types are weights
+ * alone).  What a host that serves several requests needs between their hidden rows and cpmcu_tree_attention* on one of them: request
+ * r attends with block_table = block_tables + r * max_blocks and kv_len = kv_lens_out + r.
+ *
+ * Block tables, slot map and positions of a batch's rows from the requests' lengths (one launch, no host round trip).
+ *   kv_lens, new_lens int32[num_requests], 1 to 4096 requests: tokens in the cache, and rows of this step.  A negative new_lens[r] says
+ *       that request r has ended: its pages are free again, its length is 0.
+ *   block_tables int32[num_requests][max_blocks], held int32[num_requests]: each request's pages in order, the first held[r] are its own.
+ *       The others are left as they are; keep them valid page numbers (zeros, at the start), since attention may look one up.
+ *   free_pages int32[num_pages] / counts int32[2]: a stack of counts[0] free pages, each of them below num_pages, the next one to give
+ *       at counts[0] - 1.  Ended requests' pages are put on it first, in request order; then every request takes what it lacks for
+ *       kv_lens + new_lens tokens, in request order.  Both arrays and block_tables change in place.
+ *   A request is refused -- its length, pages and table stay, its rows have no slot -- if it needs more than max_blocks pages or than are
+ *       left (then so is every later one that needs any), if its rows end behind max_rows, or if kv_lens[r] is negative.
+ *   outputs, apart from the inputs (a caller who does not want the step drops them: the stack below counts[0] and the pages in
+ *       the tables below held[r] are as they were): kv_lens_out, held_out int32[num_requests]; counts_out int32[2] = (free pages, refused
+ *       requests); row_offsets int32[num_requests + 1]: request r's rows are [row_offsets[r], row_offsets[r + 1]); positions, slots
+ *       int32[max_rows]: a row's position in its request and its place page * 256 + position % 256 in the cache; both -1 for
+ *       refused requests' rows and behind the last row. */
+int cpmcu_batch_tables(const int32_t* kv_lens, const int32_t* new_lens, int num_requests, int32_t* block_tables, int max_blocks,
+                       const int32_t* held, int32_t* free_pages, int num_pages, const int32_t* counts, int32_t* kv_lens_out,
+                       int32_t* held_out, int32_t* counts_out, int32_t* row_offsets, int32_t* positions, int32_t* slots, int max_rows,
+                       void* stream);
+
+/* Rotary positions of n rows of q and k heads: with p = positions[t], m = magnitude and half = rotary_dim / 2, the pair of values
+ * (x, y) = (i, i + half) of a head, or (2i, 2i + 1) when interleaved, becomes
+ *   (m (x cos a - y sin a), m (x sin a + y cos a)),  a = p * inv_freq[i],
+ * the values from rotary_dim on are copied, and rows of a negative position are left out (their results stay as they were).  The
+ * angle is formed in 64 bits: exact far into a context, unlike cpmcu_rope_table's float product (which is the reference's).
+ *   inv_freq float[half]: with whatever scaling the model's long contexts have (see ops.rope_frequencies);
+ *   transposed: the transposed matrix, that takes gradients of the results back to the inputs (with m = 1 the inverse);
+ *   q [n][q_stride], heads of head_dim values one after the other from the row's start; q_out likewise, the same memory and stride (in
+ *       place) or memory apart; k alike; Hq or Hkv may be 0.  head_dim even, up to 256; rotary_dim even.  Rows on 16 bytes with
+ *       rotary_dim and head_dim multiples of 16 are read and written in 16-byte pieces, others value by value. */
+int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, int rotary_dim, int interleaved, float magnitude, int transposed,
+                    const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, const void* k, int64_t k_stride, void* k_out,
+                    int64_t k_out_stride, int Hkv, int head_dim, int n, void* stream);
+
+/* The K and V rows of several requests into the paged cache of a layer, row t of [n] to slots[t] = page * 256 + place in the page (as
+ * cpmcu_batch_tables writes them; no slot twice).  Rows whose slot is negative or lies behind num_pages are left out whole.
+ *   k, v [n][stride], Hkv heads of 128 values from the row's start; rows and pools on 16 bytes.
+ *   positions, inv_freq (or both NULL): K is rotated on its way as by cpmcu_rope_rows, and so are the Hq heads of q into q_out (Hq
+ *       may be 0); rotary_dim a multiple of 16; rows of a negative position are left out as well. */
+int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, const int32_t* slots, const void* k, int64_t k_stride, const void* v,
+                          int64_t v_stride, int n, int Hkv, const int32_t* positions, const float* inv_freq, int rotary_dim, int interleaved,
+                          float magnitude, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, void* stream);
+
+/* Rows of 16-bit floats to 8 bits with a scale for each row: scales[t] = max |x| / 127, xq[t][k] = rint(127 x / max |x|) (ties to even,
+ * the quotient as if exact).  An empty (all zero) row has scale 0 and zeros, a row with an infinity or NaN scale NaN and zeros.
+ *   x [n][x_stride], K <= 131071 values from the row's start; xq [n][K rounded up to 64], zeros behind column K, on 16 bytes. */
+int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K, int8_t* xq, float* scales, void* stream);
+/* 8-bit weights [V][K], row-major, in matrix-operand order [ceil(V/16)][ceil(K/64)][64 lanes][16 bytes]: once, at load time. */
+size_t cpmcu_int8_weight_bytes(int V, int K);
+int cpmcu_int8_weight_tile(const int8_t* w, int V, int K, int8_t* w_tiled, void* stream);
+/* out[t][c] = (sum over k of xq[t][k] w[c][k]) * (x_scales[t] * w_scales[c]), [n][V] in the element type: the sum exact in 32-bit
+ * integers, one rounding to float, one product, one rounding to the element type.  xq as cpmcu_quantize_rows leaves it (what lies
+ * behind column K does not matter), w_tiled as cpmcu_int8_weight_tile does.  K <= 131071. */
+int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_tiled, const float* w_scales, int n, int V, int K, void* out,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

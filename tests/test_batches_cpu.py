@@ -1,0 +1,154 @@
+"""Batches on the CPU: what the operators refuse before any device call, and the rotary frequencies of long contexts."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+P = ctypes.c_void_p
+A, B, C, D, E, F = (P(1 << 20 << i) for i in range(6))  # never looked at: far apart, on 16 bytes
+
+
+def _lib():
+    from cpm.cu_amd import lib
+    return lib.get()
+
+
+def _tables(**kw):
+    a = dict(kv=P(1 << 32), new=P(2 << 32), n=4, tables=P(3 << 32), blocks=8, held=P(4 << 32), free=P(5 << 32), pages=64, counts=P(6 << 32), kv_out=P(7 << 32), held_out=P(8 << 32),
+             counts_out=P(9 << 32), offsets=P(10 << 32), positions=P(11 << 32), slots=P(12 << 32), rows=100)
+    a.update(kw)
+    _lib().batch_tables(a["kv"], a["new"], a["n"], a["tables"], a["blocks"], a["held"], a["free"], a["pages"], a["counts"], a["kv_out"], a["held_out"], a["counts_out"], a["offsets"],
+                        a["positions"], a["slots"], a["rows"], None)
+
+
+@pytest.mark.parametrize("kw, match", [
+    (dict(kv=None), "null"), (dict(counts_out=None), "null"), (dict(positions=None), "null"), (dict(slots=None), "null"),
+    (dict(n=0), "0 requests"), (dict(n=4097), "4097 requests"), (dict(blocks=0), "max_blocks=0"), (dict(blocks=(1 << 18) + 1), "max_blocks"),
+    (dict(pages=0), "num_pages=0"), (dict(pages=1 << 23), "num_pages"), (dict(rows=-1), "max_rows=-1"), (dict(rows=(1 << 30) + 1), "max_rows"),
+    (dict(kv_out=P(1 << 32)), "memory of an input"), (dict(held_out=P((4 << 32) + 12)), "memory of an input"), (dict(counts_out=P(6 << 32)), "memory of an input"),
+    (dict(slots=P((3 << 32) + 4 * 4 * 8 - 4)), "memory of an input"), (dict(positions=P((5 << 32) - 396)), "memory of an input")])
+def test_batch_tables_refuses(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _tables(**kw)
+
+
+def _rope(**kw):
+    a = dict(pos=A, freq=B, rotary=128, il=0, m=1.0, tr=0, q=P(1 << 32), qs=4096, qo=P(2 << 32), qos=4096, hq=32, k=P(3 << 32), ks=256, ko=P(4 << 32), kos=256, hkv=2, dim=128, n=60)
+    a.update(kw)
+    _lib().rope_rows(a["pos"], a["freq"], a["rotary"], a["il"], ctypes.c_float(a["m"]), a["tr"], a["q"], a["qs"], a["qo"], a["qos"], a["hq"], a["k"], a["ks"], a["ko"], a["kos"], a["hkv"], a["dim"], a["n"], None)
+
+
+@pytest.mark.parametrize("kw, match", [
+    (dict(pos=None), "null"), (dict(freq=None), "null"), (dict(q=None), "null"), (dict(ko=None), "null"), (dict(rotary=0), "rotary_dim=0"), (dict(rotary=127), "rotary_dim=127"),
+    (dict(rotary=130), "rotary_dim=130"), (dict(dim=127), "head_dim=127"), (dict(dim=258), "head_dim=258"), (dict(n=-1), "n=-1"), (dict(hq=1025, qs=1 << 20, qos=1 << 20), "1025 heads of q"),
+    (dict(hkv=-1), "-1 heads of k"), (dict(qs=4095), "rows of q closer"), (dict(kos=255), "rows of k closer"), (dict(qo=P((1 << 32) + 256)), "results of q"),
+    (dict(qo=P(1 << 32), qos=8192), "results of q"), (dict(ko=P((3 << 32) + 2 * 60 * 256 - 16)), "results of k"), (dict(m=math.inf), "magnitude"), (dict(m=math.nan), "magnitude")])
+def test_rope_rows_refuses(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _rope(**kw)
+
+
+def test_empty_calls_are_no_calls():
+    """No rows or heads: nothing to do, and no device is asked for."""
+    _rope(n=0)
+    _rope(hq=0, hkv=0)
+    _append(n=0)
+    _lib().quantize_rows(A, 64, 0, 64, B, C, None)
+    _lib().int8_linear(A, B, C, D, 0, 16, 64, E, None)
+
+
+def _append(**kw):
+    a = dict(kp=P(1 << 32), vp=P(2 << 32), pages=4, slots=A, k=P(3 << 32), ks=256, v=P(4 << 32), vs=256, n=60, hkv=2, pos=B, freq=C, rotary=128, il=0, m=1.0, q=P(5 << 32), qs=4096, qo=P(6 << 32), qos=4096, hq=32)
+    a.update(kw)
+    _lib().kv_append_slots(a["kp"], a["vp"], a["pages"], a["slots"], a["k"], a["ks"], a["v"], a["vs"], a["n"], a["hkv"], a["pos"], a["freq"], a["rotary"], a["il"], ctypes.c_float(a["m"]), a["q"], a["qs"],
+                           a["qo"], a["qos"], a["hq"], None)
+
+
+@pytest.mark.parametrize("kw, match", [
+    (dict(kp=None), "null"), (dict(slots=None), "null"), (dict(v=None), "null"), (dict(q=None), "null"), (dict(pos=None), "null"), (dict(freq=None), "null"), (dict(pages=0), "num_pages=0"),
+    (dict(pages=1 << 23), "num_pages"), (dict(n=-1), "n=-1"), (dict(hkv=0), "Hkv=0"), (dict(rotary=24), "multiple of 16"), (dict(rotary=144), "rotary_dim=144"), (dict(pos=None, freq=None), "q is rotated here"),
+    (dict(ks=255), "closer"), (dict(vs=248), "closer"), (dict(k=P((3 << 32) + 8)), "16 bytes"), (dict(vs=260), "16 bytes"), (dict(qs=4100), "16 bytes"), (dict(vp=P((2 << 32) + 2)), "16 bytes"), (dict(m=math.inf), "magnitude")])
+def test_kv_append_slots_refuses(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _append(**kw)
+
+
+def test_int8_operators_refuse():
+    L = _lib()
+    for args in ((None, 64, 1, 64, B, C), (A, 64, 1, 64, None, C), (A, 64, 1, 64, B, None), (A, 64, -1, 64, B, C), (A, 64, 1, 0, B, C), (A, 1 << 20, 1, 131072, B, C), (A, 63, 1, 64, B, C),
+                 (A, 64, 1, 64, P(24), C)):
+        with pytest.raises(ValueError, match="quantize_rows"):
+            L.quantize_rows(*args, None)
+    for args in ((None, 16, 64, B), (A, 16, 64, None), (A, 16, 64, A), (A, 0, 64, B), (A, 16, 0, B), (A, 16, 131072, B), (A, 16, 64, P(8))):
+        with pytest.raises(ValueError, match="int8_weight_tile"):
+            L.int8_weight_tile(*args, None)
+    for args in ((None, B, C, D, 1, 16, 64, E), (A, None, C, D, 1, 16, 64, E), (A, B, None, D, 1, 16, 64, E), (A, B, C, None, 1, 16, 64, E), (A, B, C, D, 1, 16, 64, None), (A, B, C, D, -1, 16, 64, E),
+                 (A, B, C, D, 1, 0, 64, E), (A, B, C, D, 1, 16, 0, E), (A, B, C, D, 1, 16, 131072, E), (P(8), B, C, D, 1, 16, 64, E), (A, B, P(8), D, 1, 16, 64, E)):
+        with pytest.raises(ValueError, match="int8_linear"):
+            L.int8_linear(*args, None)
+    assert L.raw.cpmcu_int8_weight_bytes(17, 65) == 2 * 2 * 1024 and L.raw.cpmcu_int8_weight_bytes(0, 65) == 0
+
+
+def test_binding_refuses_host_tensors_and_counts_arguments():
+    import torch
+    from cpm.cu_amd import ops
+    native = ops._calls()
+    h, i, f, b = torch.zeros((4, 2, 128), dtype=torch.float16), torch.zeros(4, dtype=torch.int32), torch.zeros(64), torch.zeros((4, 64), dtype=torch.int8)
+    for call in (lambda: ops.rope_rows(h, None, i, f), lambda: ops.batch_tables(i, i, i.view(4, 1), i, i, i[:2], 4), lambda: ops.quantize_rows(h.view(4, 256)),
+                 lambda: native.int8_linear(b, f[:4], b, f[:16], 16, 64, None), lambda: native.kv_append_slots(h, h, h, h, i, None, None, None, None, 0, 1.0)):
+        with pytest.raises(AssertionError, match="current device required"):
+            call()
+    for name in ("rope_rows", "batch_tables", "quantize_rows", "int8_linear", "kv_append_slots"):
+        with pytest.raises(TypeError, match="arguments given"):
+            getattr(native, name)(*[None] * 17)
+        with pytest.raises((AssertionError, TypeError)):
+            getattr(native, name)(*[None] * dict(rope_rows=9, batch_tables=7, quantize_rows=1, int8_linear=7, kv_append_slots=11)[name])
+
+
+# ---- rotary frequencies: against the formulas, pair by pair ----
+
+def test_plain_linear_and_ntk_frequencies():
+    from cpm.cu_amd import ops
+    for dim, base in ((128, 10000.0), (64, 500000.0), (42, 1e6)):
+        plain = np.array([base ** (-2.0 * i / dim) for i in range(dim // 2)])
+        for scaling, want in ((None, plain), (dict(type="linear", factor=4.0), plain / 4), (dict(type="ntk", factor=8.0), [(base * 8.0 ** (dim / (dim - 2.0))) ** (-2.0 * i / dim) for i in range(dim // 2)])):
+            freq, magnitude = ops.rope_frequencies(dim, base, scaling)
+            # one rounding to 32 bits, and the powers' own in 64
+            assert magnitude == 1.0 and np.allclose(freq.numpy().astype(np.float64), want, rtol=2.0 ** -24 + 1e-13, atol=0)
+    # what the base is grown for: the slowest pair is stretched by the factor
+    freq, _ = ops.rope_frequencies(128, 10000.0, dict(type="ntk", factor=8.0))
+    assert np.isclose(float(freq[-1]) * 8.0, 10000.0 ** (-126 / 128), rtol=1e-6)
+
+
+def test_yarn_frequencies():
+    from cpm.cu_amd import ops
+    dim, base, factor, original = 128, 10000.0, 16.0, 4096.0
+    freq, magnitude = ops.rope_frequencies(dim, base, dict(type="yarn", factor=factor, original=original))
+    assert magnitude == pytest.approx(0.1 * math.log(16.0) + 1.0, rel=1e-12)
+    low, high = (dim * math.log(original / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (32.0, 1.0))
+    low, high = math.floor(low), math.ceil(high)
+    for i in range(dim // 2):
+        f = base ** (-2.0 * i / dim)
+        ramp = min(max((i - low) / (high - low), 0.0), 1.0)
+        assert float(freq[i]) == pytest.approx(f * (1 - ramp) + f / factor * ramp, rel=1e-7)
+    assert ops.rope_frequencies(dim, base, dict(type="yarn", factor=factor, original=original, magnitude=1.5))[1] == 1.5
+
+
+def test_longrope_frequencies_follow_the_length():
+    from cpm.cu_amd import ops
+    short, long = np.linspace(1.0, 2.0, 32), np.linspace(1.0, 40.0, 32)
+    scaling = dict(type="longrope", factor=32.0, original=4096, short_factor=list(short), long_factor=list(long))
+    plain = 10000.0 ** (-np.arange(32) / 32)
+    for length, by in ((4096, short), (4097, long)):
+        freq, magnitude = ops.rope_frequencies(64, 10000.0, scaling, length=length)
+        assert np.allclose(freq.numpy().astype(np.float64), plain / by, rtol=1e-7) and magnitude == pytest.approx(math.sqrt(1 + math.log(32) / math.log(4096)))
+
+
+@pytest.mark.parametrize("dim, scaling, length", [(7, None, None), (0, None, None), (64, dict(type="other"), None), (64, dict(type="linear", factor=0.5), None), (64, dict(type="linear", factor=math.nan), None),
+                                                  (2, dict(type="ntk", factor=2.0), None), (64, dict(type="longrope", factor=2.0, original=4096, short_factor=[1.0] * 32, long_factor=[1.0] * 32), None),
+                                                  (64, dict(type="longrope", factor=2.0, original=4096, short_factor=[1.0] * 31, long_factor=[1.0] * 32), 10)])
+def test_rope_frequencies_refuse(dim, scaling, length):
+    from cpm.cu_amd import ops
+    with pytest.raises(ValueError):
+        ops.rope_frequencies(dim, 10000.0, scaling, length=length)
