@@ -121,9 +121,22 @@ struct LinearParams {
     const int8_t *xq, *w;
     const float *x_scales, *w_scales;
     void* out;
-    int n, V, steps;
+    int n, V, steps, blocks;  // (blocks of channels)
+    int row_tiles, channel_tiles;
     bool quads;  // four channels' results are stored at once
 };
+
+// The tile of a workgroup.  Workgroups of equal number modulo 8 share an XCD and its L2: each XCD takes a run of tiles, in columns of up to
+// eight row tiles, so that those that run at the same time use few rows and weights.
+constexpr int kXcds = 8;
+constexpr int kColumn = 8;
+__device__ inline void tile_of(const LinearParams& p, int block, int* tx, int* tv) {
+    const int total = p.row_tiles * p.channel_tiles, each = total / kXcds, more = total % kXcds, xcd = block % kXcds;
+    const int i = xcd * each + min(xcd, more) + block / kXcds;
+    const int band = i / (kColumn * p.channel_tiles), rows = min(kColumn, p.row_tiles - band * kColumn), in_band = i - band * kColumn * p.channel_tiles;
+    *tx = band * kColumn + in_band % rows;
+    *tv = in_band / rows;
+}
 
 // Channels c .. c + 3 of row t.
 template <typename E>
@@ -171,6 +184,77 @@ __global__ __launch_bounds__(512) void int8_linear_kernel(LinearParams p) {
     }
 }
 
+// Tiles of (WX NX) x (WV NV) blocks for more rows: WX x WV waves, each with NX x NV of the blocks in its accumulators.
+// Rows go to LDS by direct loads, in operand order (a block's step is 1 KB, read back without bank conflicts), kAhead steps in advance
+// in a ring of kStages; weights lie in operand order already and go straight into registers, two steps in advance, so that LDS
+// is read for the rows alone.  The loads are numbered as they return: waiting for the weights of step s (which the compiler does, in front of their
+// first use) waits for every request in front of them, among them the rows of step s + 1; the wait in front of the barrier says so.
+constexpr int kStages = 4;
+constexpr int kAhead = kStages - 1;
+
+template <typename E, int NX, int NV, int WX, int WV>
+__global__ __launch_bounds__(64 * WX * WV, 2) void int8_linear_tile_kernel(LinearParams p) {
+    constexpr int kWaves = WX * WV, kBlocks = WX * NX, kLoads = kBlocks / kWaves;
+    static_assert(kBlocks % kWaves == 0, "every wave requests as many blocks of rows");
+    __shared__ __attribute__((aligned(16))) int8_t ring[kStages][kBlocks][kTile];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wx = wave / WV, wv = wave % WV;
+    int tx, tv;
+    tile_of(p, blockIdx.x, &tx, &tv);
+    const int t0 = tx * kBlocks * 16, b0 = (tv * WV + wv) * NV, last = p.steps - 1;
+    const int8_t* row[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) row[j] = p.xq + (size_t)min(t0 + (wave * kLoads + j) * 16 + (lane & 15), p.n - 1) * p.steps * kStep + (lane >> 4) * 16;
+    const int8_t* w[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) w[v] = p.w + (size_t)min(b0 + v, p.blocks - 1) * p.steps * kTile + lane * 16;
+    const auto request = [&](int s) {
+        const size_t at = (size_t)min(s, last) * kStep;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&ring[s % kStages][wave * kLoads + j][0]);
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(row[j] + at), "s"(dst) : "memory", "m0");
+        }
+    };
+    const auto weights = [&](int s, i32x4* a) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) a[v] = *reinterpret_cast<const i32x4*>(w[v] + (size_t)min(s, last) * kTile);
+    };
+    i32x4 acc[NX][NV] = {};
+    const auto step = [&](int s, const i32x4* now, i32x4* next) {
+        request(s + kAhead);
+        weights(s + 2, next);
+        const int8_t* x = &ring[s % kStages][wx * NX][0] + lane * 16;
+#pragma unroll
+        for (int b = 0; b < NX; ++b) {
+            const i32x4 rows = *reinterpret_cast<const i32x4*>(x + b * kTile);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) acc[b][v] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[v], rows, acc[b][v], 0, 0, 0);
+        }
+        // this step's rows are read, the next one's are there: behind them two steps' requests at most
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(2 * (kLoads + NV)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" : : : "memory");
+    };
+    i32x4 a0[NV], a1[NV], a2[NV];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) request(s);
+    weights(0, a0);
+    weights(1, a1);
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    for (int s = 0; s < p.steps; s += 3) {
+        step(s, a0, a2);
+        if (s + 1 < p.steps) step(s + 1, a1, a0);
+        if (s + 2 < p.steps) step(s + 2, a2, a1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (requests beyond the last step write to LDS, too)
+#pragma unroll
+    for (int b = 0; b < NX; ++b)
+#pragma unroll
+        for (int v = 0; v < NV; ++v) store_quad<E>(p, t0 + (wx * NX + b) * 16 + (lane & 15), (b0 + v) * kBlock + (lane >> 4) * 4, acc[b][v]);
+}
+
 }  // namespace
 }  // namespace cpmcu
 
@@ -216,14 +300,31 @@ extern "C" int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const 
     CPMCU_CHECK_ARG(n >= 0 && V >= 1 && K >= 1 && K <= kMaxColumns, "int8_linear: n=%d, V=%d, K=%d outside [1, %d]", n, V, K, kMaxColumns);
     CPMCU_CHECK_ARG(((uintptr_t)xq | (uintptr_t)w_tiled) % 16 == 0, "int8_linear: xq and w_tiled have to lie on 16 bytes");
     if (n == 0) return CPMCU_OK;
-    LinearParams p{xq, w_tiled, x_scales, w_scales, out, n, V, ceil_div(K, kStep), V % 4 == 0 && (uintptr_t)out % 8 == 0};
+    LinearParams p{xq, w_tiled, x_scales, w_scales, out, n, V, ceil_div(K, kStep), ceil_div(V, kBlock), 0, 0, V % 4 == 0 && (uintptr_t)out % 8 == 0};
     hipStream_t st = resolve_stream(stream);
-    const int nx = n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 : 8;
-    const dim3 grid(ceil_div(V, kBlock), ceil_div(n, 16 * nx));
-    CPMCU_CHECK_ARG(grid.y <= 65535, "int8_linear: n=%d rows", n);
-#define CPMCU_LINEAR(E)                                                                                                  \
-    (nx == 1 ? int8_linear_kernel<E, 1> : nx == 2 ? int8_linear_kernel<E, 2> : nx == 4 ? int8_linear_kernel<E, 4> : int8_linear_kernel<E, 8>)
-    hipLaunchKernelGGL(options().dtype == 1 ? CPMCU_LINEAR(bf16) : CPMCU_LINEAR(f16), grid, dim3(512), 0, st, p);
+    const bool is_bf16 = options().dtype == 1;
+    if (n > 64) {
+#define CPMCU_TILE(E, NX, NV, WX, WV)                                                                                                   \
+    do {                                                                                                                                \
+        p.row_tiles = ceil_div(n, 16 * NX * WX);                                                                                        \
+        p.channel_tiles = ceil_div(p.blocks, NV * WV);                                                                                  \
+        hipLaunchKernelGGL((int8_linear_tile_kernel<E, NX, NV, WX, WV>), dim3(p.row_tiles * p.channel_tiles), dim3(64 * WX * WV), 0, st, p); \
+    } while (0)
+        if (n > 512) {
+            if (is_bf16) CPMCU_TILE(bf16, 8, 4, 2, 4);
+            else CPMCU_TILE(f16, 8, 4, 2, 4);
+        } else {
+            if (is_bf16) CPMCU_TILE(bf16, 8, 2, 1, 4);
+            else CPMCU_TILE(f16, 8, 2, 1, 4);
+        }
+#undef CPMCU_TILE
+        CPMCU_LAUNCH_CHECK();
+        return CPMCU_OK;
+    }
+    const int nx = n <= 16 ? 1 : n <= 32 ? 2 : 4;
+    const dim3 grid(p.blocks, 1);
+#define CPMCU_LINEAR(E) (nx == 1 ? int8_linear_kernel<E, 1> : nx == 2 ? int8_linear_kernel<E, 2> : int8_linear_kernel<E, 4>)
+    hipLaunchKernelGGL(is_bf16 ? CPMCU_LINEAR(bf16) : CPMCU_LINEAR(f16), grid, dim3(512), 0, st, p);
 #undef CPMCU_LINEAR
     CPMCU_LAUNCH_CHECK();
     return CPMCU_OK;
