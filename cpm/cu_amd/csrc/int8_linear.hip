@@ -7,6 +7,7 @@
 #include "internal.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace cpmcu {
 namespace {
@@ -16,6 +17,7 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxColumns = 131071;
+constexpr int kCus = 256;             // of an MI355X
 constexpr int kStep = 64;             // columns of a matrix instruction; rows and weights are padded to whole steps
 constexpr int kBlock = 16;            // channels of a weight block
 constexpr int kTile = kBlock * kStep; // bytes of a weight tile: lane l holds channel l & 15, columns (l >> 4) * 16 ..
@@ -156,103 +158,371 @@ __device__ inline void store_quad(const LinearParams& p, int t, int c, i32x4 sum
     }
 }
 
-// A block of channels and NX blocks of rows per workgroup; the waves take K's steps in turn.
-template <typename E, int NX>
-__global__ __launch_bounds__(512) void int8_linear_kernel(LinearParams p) {
-    __shared__ i32x4 part[8][NX][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t0 = blockIdx.y * NX * 16;
-    const int8_t* w = p.w + (size_t)blockIdx.x * p.steps * kTile + lane * 16;
-    const int8_t* x[NX];
+// NX blocks of rows and NV blocks of channels per workgroup, for few rows: the weights are the bytes, each is read by one workgroup, and the
+// waves take K's steps in turn, so that a workgroup's requests are whole kilobytes one behind the other.  A wave requests U steps at once
+// while it works on the U before them; the waves' sums meet in LDS.
+constexpr int kSplit = 8;
+
+template <typename E, int NX, int NV, int U>
+__global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearParams p) {
+    constexpr int kQuads = NX * NV;
+    __shared__ i32x4 part[kSplit / 2][kQuads][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int tx, tv;
+    tile_of(p, blockIdx.x, &tx, &tv);
+    const int t0 = tx * NX * 16, b0 = tv * NV, last = p.steps - 1;
+    const int8_t *x[NX], *w[NV];
 #pragma unroll
     for (int b = 0; b < NX; ++b) x[b] = p.xq + (size_t)min(t0 + b * 16 + (lane & 15), p.n - 1) * p.steps * kStep + (lane >> 4) * 16;
-    i32x4 acc[NX] = {};
-    for (int s = wave; s < p.steps; s += 8) {
-        const i32x4 a = *reinterpret_cast<const i32x4*>(w + (size_t)s * kTile);
 #pragma unroll
-        for (int b = 0; b < NX; ++b)
-            acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *reinterpret_cast<const i32x4*>(x[b] + (size_t)s * kStep), acc[b], 0, 0, 0);
+    for (int v = 0; v < NV; ++v) w[v] = p.w + (size_t)min(b0 + v, p.blocks - 1) * p.steps * kTile + lane * 16;
+    struct Group {
+        i32x4 a[U][NV], x[U][NX];
+    };
+    const auto load = [&](int s, Group& g) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t at = min(s + u * kSplit, last);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) g.a[u][v] = *reinterpret_cast<const i32x4*>(w[v] + at * kTile);
+#pragma unroll
+            for (int b = 0; b < NX; ++b) g.x[u][b] = *reinterpret_cast<const i32x4*>(x[b] + at * kStep);
+        }
+    };
+    i32x4 acc[NX][NV] = {};
+    const auto multiply = [&](int s, const Group& g) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s + u * kSplit > last) break;  // (the same for the whole wave)
+#pragma unroll
+            for (int b = 0; b < NX; ++b)
+#pragma unroll
+                for (int v = 0; v < NV; ++v) acc[b][v] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.a[u][v], g.x[u][b], acc[b][v], 0, 0, 0);
+        }
+    };
+    constexpr int kTurn = U * kSplit;
+    Group g0, g1;
+    load(wave, g0);
+    for (int s = wave; s <= last; s += 2 * kTurn) {
+        if (s + kTurn <= last) load(s + kTurn, g1);
+        multiply(s, g0);
+        if (s + kTurn > last) break;
+        if (s + 2 * kTurn <= last) load(s + 2 * kTurn, g0);
+        multiply(s + kTurn, g1);
     }
+    // eight sums to four to two to one
 #pragma unroll
-    for (int b = 0; b < NX; ++b) part[wave][b][lane] = acc[b];
-    __syncthreads();
-    for (int b = wave; b < NX; b += 8) {
-        i32x4 sum = part[0][b][lane];
+    for (int half = kSplit / 2; half; half >>= 1) {
+        if (wave >= half && wave < 2 * half) {
 #pragma unroll
-        for (int k = 1; k < 8; ++k) sum += part[k][b][lane];
-        store_quad<E>(p, t0 + b * 16 + (lane & 15), blockIdx.x * kBlock + (lane >> 4) * 4, sum);
+            for (int b = 0; b < NX; ++b)
+#pragma unroll
+                for (int v = 0; v < NV; ++v) part[wave - half][b * NV + v][lane] = acc[b][v];
+        }
+        __syncthreads();
+        if (half > 1 && wave < half) {
+#pragma unroll
+            for (int b = 0; b < NX; ++b)
+#pragma unroll
+                for (int v = 0; v < NV; ++v) acc[b][v] += part[wave][b * NV + v][lane];
+        }
+        if (half > 1) __syncthreads();
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int b = 0; b < NX; ++b)
+#pragma unroll
+        for (int v = 0; v < NV; ++v) store_quad<E>(p, t0 + b * 16 + (lane & 15), (b0 + v) * kBlock + (lane >> 4) * 4, acc[b][v] + part[0][b * NV + v][lane]);
+}
+
+// A wave's tile: NX blocks of rows from t0 on, NV blocks of channels from c0 on.  The results go through LDS, as many blocks of rows at a time
+// as ROOM bytes of the wave's own hold, so that a row's are stored as one run of NV * 32 bytes (as they lie in the accumulators a row has 8);
+// rows of an uneven V start anywhere, which 16-byte stores may.
+struct __attribute__((packed, aligned(2))) Piece {
+    uint32_t v[4];
+};
+template <typename E, int NX, int NV, int ROOM>
+__device__ inline void store_tile(const LinearParams& p, int t0, int c0, i32x4 (&acc)[NX][NV], int8_t* part) {
+    constexpr int kRoom = ROOM / (512 * NV), kPieces = 2 * NV, kPass = NX <= kRoom ? NX : kRoom < 4 ? 2 : kRoom < 8 ? 4 : 8;
+    static_assert(kRoom >= 2 && NX % kPass == 0, "passes of whole blocks");
+    const int lane = threadIdx.x & 63;
+    float sw[NV][4];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sw[v][j] = p.w_scales[min(c0 + v * kBlock + (lane >> 4) * 4 + j, p.V - 1)];
+#pragma unroll
+    for (int b1 = 0; b1 < NX; b1 += kPass) {
+        const int t1 = t0 + b1 * 16;
+#pragma unroll
+        for (int b = 0; b < kPass; ++b) {
+            const int r = b * 16 + (lane & 15);
+            const float sx = p.x_scales[min(t1 + r, p.n - 1)];
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const i32x4 sum = acc[b1 + b][v];
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = Elem<E>::to_bits((float)sum[j] * (sx * sw[v][j]));
+                const int piece = (v * 2 + (lane >> 5)) ^ (r & (kPieces - 1));
+                *reinterpret_cast<uint2*>(part + r * (kPieces * 16) + piece * 16 + ((lane >> 4) & 1) * 8) = make_uint2(y[0] | y[1] << 16, y[2] | y[3] << 16);
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // (one wave's own: no barrier)
+#pragma unroll
+        for (int i = 0; i < kPass * 16 * kPieces / 64; ++i) {
+            const int r = i * (64 / kPieces) + lane / kPieces, piece = lane % kPieces, t = t1 + r, c = c0 + piece * 8;
+            const uint4 y = *reinterpret_cast<const uint4*>(part + r * (kPieces * 16) + (piece ^ (r & (kPieces - 1))) * 16);
+            if (t >= p.n || c >= p.V) continue;
+            uint16_t* to = (uint16_t*)p.out + (size_t)t * p.V + c;
+            if (c + 8 <= p.V) {
+                *reinterpret_cast<Piece*>(to) = Piece{{y.x, y.y, y.z, y.w}};
+            } else {
+                const uint32_t v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int j = 0; j < 7; ++j)
+                    if (c + j < p.V) to[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     }
 }
 
 // Tiles of (WX NX) x (WV NV) blocks for more rows: WX x WV waves, each with NX x NV of the blocks in its accumulators.
-// Rows go to LDS by direct loads, in operand order (a block's step is 1 KB, read back without bank conflicts), kAhead steps in advance
-// in a ring of kStages; weights lie in operand order already and go straight into registers, two steps in advance, so that LDS
-// is read for the rows alone.  The loads are numbered as they return: waiting for the weights of step s (which the compiler does, in front of their
-// first use) waits for every request in front of them, among them the rows of step s + 1; the wait in front of the barrier says so.
-constexpr int kStages = 4;
-constexpr int kAhead = kStages - 1;
-
-template <typename E, int NX, int NV, int WX, int WV>
-__global__ __launch_bounds__(64 * WX * WV, 2) void int8_linear_tile_kernel(LinearParams p) {
-    constexpr int kWaves = WX * WV, kBlocks = WX * NX, kLoads = kBlocks / kWaves;
-    static_assert(kBlocks % kWaves == 0, "every wave requests as many blocks of rows");
-    __shared__ __attribute__((aligned(16))) int8_t ring[kStages][kBlocks][kTile];
+// Rows go to LDS by direct loads, two steps at a time, so that a request takes whole 128-byte lines, eight rows of them; the eight rows of a
+// 16-byte column lie side by side, which is how the operands are read back, without bank conflicts.  Weights lie
+// in operand order already and go straight into registers, AHEAD pairs of steps in advance, so that LDS is read for the rows alone.
+// Half of a step's rows are read from LDS while the other half is multiplied, so the next pair's have to be there a pair early: its
+// rows are requested in front of the weights of two pairs before.  Requests return in order, and the wait for the weights of pair j, which the
+// compiler puts in front of their first use, is one for the rows of pair j + 2 as well; the one in front of the barrier says so.
+template <typename E, int NX, int NV, int WX, int WV, int AHEAD>
+__global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_tile_kernel(LinearParams p) {
+    constexpr int kWaves = WX * WV, kBlocks = WX * NX, kLoads = 2 * kBlocks / kWaves, kStages = AHEAD + 3, kHalf = NX / 2, kSets = 2 * (AHEAD + 1);
+    static_assert(2 * kBlocks % kWaves == 0 && NX % 2 == 0, "every wave requests as many kilobytes of rows");
+    constexpr int kStageBytes = kBlocks * 2 * kTile;
+    __shared__ __attribute__((aligned(16))) int8_t ring[kStages * kStageBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wx = wave / WV, wv = wave % WV;
     int tx, tv;
     tile_of(p, blockIdx.x, &tx, &tv);
-    const int t0 = tx * kBlocks * 16, b0 = (tv * WV + wv) * NV, last = p.steps - 1;
-    const int8_t* row[kLoads];
+    const int t0 = tx * kBlocks * 16, b0 = (tv * WV + wv) * NV, last = p.steps - 1, last_pair = last / 2, pairs = p.steps / 2;  // (whole pairs)
+    // (an uneven last step: its pair takes the columns of the one step twice, and only the first is multiplied)
+    const uint32_t no_second = (p.steps & 1) && lane >= 32 ? kStep : 0;
+    const int8_t* x_tile = p.xq + (size_t)t0 * p.steps * kStep;
+    uint32_t row[kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) row[j] = p.xq + (size_t)min(t0 + (wave * kLoads + j) * 16 + (lane & 15), p.n - 1) * p.steps * kStep + (lane >> 4) * 16;
+    for (int j = 0; j < kLoads; ++j) row[j] = (uint32_t)(min((wave * kLoads + j) * 8 + (lane & 7), p.n - 1 - t0) * p.steps * kStep + (lane >> 3) * 16);
     const int8_t* w[NV];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) w[v] = p.w + (size_t)min(b0 + v, p.blocks - 1) * p.steps * kTile + lane * 16;
-    const auto request = [&](int s) {
-        const size_t at = (size_t)min(s, last) * kStep;
+    for (int v = 0; v < NV; ++v) w[v] = p.w + (size_t)min(b0 + v, p.blocks - 1) * p.steps * kTile;
+    const uint32_t lane16 = lane * 16, ring_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)ring + wave * (kLoads * kTile);
+    const auto request = [&](int pair, int stage) {
+        const int8_t* from = x_tile + (size_t)min(pair, last_pair) * (2 * kStep);
+        const uint32_t back = pair >= last_pair ? no_second : 0;
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&ring[s % kStages][wave * kLoads + j][0]);
-            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(row[j] + at), "s"(dst) : "memory", "m0");
-        }
+        for (int j = 0; j < kLoads; ++j)
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(row[j] - back), "s"(from), "s"(ring_at + stage * kStageBytes + j * kTile) : "memory", "m0");
     };
     const auto weights = [&](int s, i32x4* a) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) a[v] = *reinterpret_cast<const i32x4*>(w[v] + (size_t)min(s, last) * kTile);
+        for (int v = 0; v < NV; ++v) a[v] = *reinterpret_cast<const i32x4*>(w[v] + (size_t)min(s, last) * kTile + lane16);
     };
-    i32x4 acc[NX][NV] = {};
-    const auto step = [&](int s, const i32x4* now, i32x4* next) {
-        request(s + kAhead);
-        weights(s + 2, next);
-        const int8_t* x = &ring[s % kStages][wx * NX][0] + lane * 16;
+    i32x4 acc[NX][NV] = {}, x0[kHalf], x1[kHalf];
+    const int8_t* mine = ring + wx * (NX * 2 * kTile) + ((lane & 15) >> 3) * kTile + (lane & 7) * 16 + (lane >> 4) * 128;
+    // The order below is kept: what is read comes ahead of the products that hide its way.
+    const auto read = [&](int stage, int second, int half, i32x4* x) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < NX; ++b) {
-            const i32x4 rows = *reinterpret_cast<const i32x4*>(x + b * kTile);
+        for (int b = 0; b < kHalf; ++b) x[b] = *reinterpret_cast<const i32x4*>(mine + stage * kStageBytes + (half * kHalf + b) * (2 * kTile) + second * 512);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto multiply = [&](const i32x4* a, const i32x4* x, int half) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) acc[b][v] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[v], rows, acc[b][v], 0, 0, 0);
+        for (int b = 0; b < kHalf; ++b)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) acc[half * kHalf + b][v] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[v], x[b], acc[half * kHalf + b][v], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto after = [](int stage, int n) { return stage + n >= kStages ? stage + n - kStages : stage + n; };
+    i32x4 a[kSets][NV];
+    request(0, 0);
+    request(1, 1);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+        request(j + 2, j + 2);
+        weights(2 * j, a[2 * j]);
+        weights(2 * j + 1, a[2 * j + 1]);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(AHEAD * (kLoads + 2 * NV)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    int stage = 0;
+    read(0, 0, 0, x0);
+    for (int j0 = 0; j0 < pairs; j0 += AHEAD + 1) {
+#pragma unroll
+        for (int u = 0; u <= AHEAD; ++u) {
+            const int j = j0 + u;
+            if (j < pairs) {
+                read(stage, 0, 1, x1);
+                request(j + AHEAD + 2, after(stage, AHEAD + 2));
+                weights(2 * (j + AHEAD), a[2 * (u + AHEAD) % kSets]);
+                multiply(a[2 * u], x0, 0);
+                read(stage, 1, 0, x0);
+                multiply(a[2 * u], x1, 1);
+                read(stage, 1, 1, x1);
+                weights(2 * (j + AHEAD) + 1, a[(2 * (u + AHEAD) + 1) % kSets]);
+                multiply(a[2 * u + 1], x0, 0);
+                stage = after(stage, 1);
+                read(stage, 0, 0, x0);
+                multiply(a[2 * u + 1], x1, 1);
+                // the rows read so far are in registers, those of pair j + 2 in LDS: behind them AHEAD pairs' requests at most
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(AHEAD * (kLoads + 2 * NV)) : "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" : : : "memory");
+            }
         }
-        // this step's rows are read, the next one's are there: behind them two steps' requests at most
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(2 * (kLoads + NV)) : "memory");
+    }
+    if (p.steps & 1) {
+        read(stage, 0, 1, x1);
+#pragma unroll
+        for (int u = 0; u <= AHEAD; ++u)
+            if (pairs % (AHEAD + 1) == u) {
+                multiply(a[2 * u], x0, 0);
+                multiply(a[2 * u], x1, 1);
+            }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (requests beyond the last pair write to LDS, too)
+    __syncthreads();
+    store_tile<E, NX, NV, kStages * kLoads * kTile>(p, t0 + wx * NX * 16, b0 * kBlock, acc, ring + wave * (kStages * kLoads * kTile));
+}
+
+// Larger tiles for many rows.  What crosses from L2 bounds the tiles above (50 to 60 GB/s a CU, 17 TB/s in all), and with waves that share channels
+// each weight crosses once for every one of them; here rows and weights are both in LDS and a CU takes each once.  A step is requested three in
+// advance and has to be there one early, as above.  A CU with 256 x 256 to do takes 0.61 us a step where few CUs run and 0.85 to 0.95 where all
+// do: 2535 TOP/s at 8192 x 16384 x 4096 (rows, columns, channels), 10 % more on zeros, which draw less power; deeper rings and other orders
+// of the tiles change nothing.
+template <typename E, int NX, int NV, int WX, int WV>
+__global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_kernel(LinearParams p) {
+    constexpr int kWaves = WX * WV, kRows = WX * NX, kChannels = WV * NV, kStages = 4, kStageBytes = (kRows + kChannels) * kTile, kHalf = NX / 2;
+    constexpr int kX = kRows / kWaves, kW = kChannels / kWaves, kRoom = kStages * kStageBytes / kWaves;
+    __shared__ __attribute__((aligned(16))) int8_t ring[kStages * kStageBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wx = wave / WV, wv = wave % WV;
+    int tx, tv;
+    tile_of(p, blockIdx.x, &tx, &tv);
+    const int t0 = tx * kRows * 16, last = p.steps - 1;
+    const int8_t* x_tile = p.xq + (size_t)t0 * p.steps * kStep;
+    uint32_t row[kX];
+    const int8_t* w[kW];
+#pragma unroll
+    for (int j = 0; j < kX; ++j) row[j] = (uint32_t)(min((wave * kX + j) * 16 + (lane & 15), p.n - 1 - t0) * p.steps * kStep + (lane >> 4) * 16);
+#pragma unroll
+    for (int j = 0; j < kW; ++j) w[j] = p.w + (size_t)min(tv * kChannels + wave * kW + j, p.blocks - 1) * p.steps * kTile;
+    const uint32_t lane16 = lane * 16, ring_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)ring;
+    const auto request = [&](int s, int stage) {
+        const size_t at = min(s, last);
+        const uint32_t to = ring_at + stage * kStageBytes;
+#pragma unroll
+        for (int j = 0; j < kX; ++j)
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(row[j]), "s"(x_tile + at * kStep), "s"(to + (wave * kX + j) * kTile) : "memory", "m0");
+#pragma unroll
+        for (int j = 0; j < kW; ++j)
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane16), "s"(w[j] + at * kTile), "s"(to + (kRows + wave * kW + j) * kTile) : "memory", "m0");
+    };
+    i32x4 acc[NX][NV] = {}, x0[kHalf], x1[kHalf], a0[NV], a1[NV];
+    const int8_t* x_at = ring + wx * (NX * kTile) + lane16;
+    const int8_t* w_at = ring + (kRows + wv * NV) * kTile + lane16;
+    const auto read_x = [&](int stage, int half, i32x4* x) {
+#pragma unroll
+        for (int b = 0; b < kHalf; ++b) x[b] = *reinterpret_cast<const i32x4*>(x_at + stage * kStageBytes + (half * kHalf + b) * kTile);
+    };
+    const auto read_w = [&](int stage, i32x4* a) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) a[v] = *reinterpret_cast<const i32x4*>(w_at + stage * kStageBytes + v * kTile);
+    };
+    // The order is kept: what is read comes ahead of the products that hide its way.
+    const auto multiply = [&](const i32x4* a, const i32x4* x, int half) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < kHalf; ++b)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) acc[half * kHalf + b][v] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[v], x[b], acc[half * kHalf + b][v], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto step = [&](int s, const i32x4* a, i32x4* next) {
+        const int now = s % kStages, then = (s + 1) % kStages;
+        read_x(now, 1, x1);
+        request(s + 3, (s + 3) % kStages);
+        multiply(a, x0, 0);
+        read_w(then, next);
+        read_x(then, 0, x0);
+        multiply(a, x1, 1);
+        // what was read is in registers, step s + 2 in LDS: behind it the requests of step s + 3
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(kX + kW) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" : : : "memory");
     };
-    i32x4 a0[NV], a1[NV], a2[NV];
-#pragma unroll
-    for (int s = 0; s < kAhead; ++s) request(s);
-    weights(0, a0);
-    weights(1, a1);
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    request(0, 0);
+    request(1, 1);
+    request(2, 2);
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kX + kW) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" : : : "memory");
-    for (int s = 0; s < p.steps; s += 3) {
-        step(s, a0, a2);
+    read_w(0, a0);
+    read_x(0, 0, x0);
+    for (int s = 0; s < p.steps; s += 2) {
+        step(s, a0, a1);
         if (s + 1 < p.steps) step(s + 1, a1, a0);
-        if (s + 2 < p.steps) step(s + 2, a2, a1);
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (requests beyond the last step write to LDS, too)
-#pragma unroll
-    for (int b = 0; b < NX; ++b)
-#pragma unroll
-        for (int v = 0; v < NV; ++v) store_quad<E>(p, t0 + (wx * NX + b) * 16 + (lane & 15), (b0 + v) * kBlock + (lane >> 4) * 4, acc[b][v]);
+    __syncthreads();
+    store_tile<E, NX, NV, kRoom>(p, t0 + wx * NX * 16, (tv * kChannels + wv * NV) * kBlock, acc, ring + wave * kRoom);
+}
+
+// The shapes, and what one of their tiles costs, as measured over 1 to 8192 rows, 512 to 73448 channels and 512 to 16384 columns: `start` us
+// of a launch and `step` us for every 64 columns of a round (a tile on every CU), `busy` more of them where all CUs work.  The choice is the
+// shape with the least cost; it is within 10 % of the best one over that range (60 x 4096 x 16384: 32 x 128 14.5 us, 32 x 64 split 33.9, 64 x 128
+// 18.1; 333 x 4099 x 12289: 128 x 256 28.5, 64 x 128 34.8, 64 x 256 36.6, 256 x 256 48.9; 2048 x 4096 x 16384: 256 x 256 125, 128 x 256 151, 64 x 256 167).
+struct Variant {
+    const char* name;
+    void (*f16_kernel)(LinearParams);
+    void (*bf16_kernel)(LinearParams);
+    int rows, channels, threads;
+    float start, step, busy;
+    bool shared;  // workgroups share a CU: rounds need not be whole
+};
+#define CPMCU_SPLIT(nx, nv, u) "int8_linear_split_kernel<" #nx "," #nv ">", int8_linear_split_kernel<f16, nx, nv, u>, int8_linear_split_kernel<bf16, nx, nv, u>, 16 * nx, kBlock* nv, 64 * kSplit
+#define CPMCU_TILE(nx, nv, wx, wv, ahead)                                                                                                                   \
+    "int8_linear_tile_kernel<" #nx "," #nv "," #wx "," #wv ">", int8_linear_tile_kernel<f16, nx, nv, wx, wv, ahead>, int8_linear_tile_kernel<bf16, nx, nv, wx, wv, ahead>, \
+        16 * nx * wx, kBlock* nv* wv, 64 * wx * wv
+#define CPMCU_WIDE(nx, nv, wx, wv)                                                                                                                     \
+    "int8_linear_wide_kernel<" #nx "," #nv "," #wx "," #wv ">", int8_linear_wide_kernel<f16, nx, nv, wx, wv>, int8_linear_wide_kernel<bf16, nx, nv, wx, wv>, \
+        16 * nx * wx, kBlock* nv* wv, 64 * wx * wv
+const Variant kVariants[kInt8LinearShapes] = {
+    {CPMCU_SPLIT(1, 2, 4), 4.f, 0.052f, 0.f, true},   {CPMCU_SPLIT(2, 2, 4), 5.f, 0.065f, 0.f, false},  {CPMCU_SPLIT(2, 4, 2), 5.6f, 0.09f, 0.f, false},
+    {CPMCU_TILE(2, 2, 1, 4, 4), 4.5f, 0.133f, 0.f, false}, {CPMCU_TILE(4, 2, 1, 4, 3), 4.5f, 0.205f, 0.f, false}, {CPMCU_TILE(4, 4, 1, 4, 2), 4.5f, 0.28f, 0.03f, false},
+    {CPMCU_WIDE(4, 4, 2, 4), 5.f, 0.345f, 0.17f, false}, {CPMCU_WIDE(8, 4, 2, 4), 5.f, 0.61f, 0.3f, false}};
+#undef CPMCU_SPLIT
+#undef CPMCU_TILE
+#undef CPMCU_WIDE
+
+int choose_variant(int n, int V, int K) {
+    if (options().int8_linear_shape >= 0) return options().int8_linear_shape;
+    const int steps = ceil_div(K, kStep);
+    int best = 0;
+    float least = 0.f;
+    for (int i = 0; i < kInt8LinearShapes; ++i) {
+        const Variant& v = kVariants[i];
+        const float tiles = (float)ceil_div(n, v.rows) * (float)ceil_div(V, v.channels) / kCus;
+        const float rounds = v.shared ? std::max(tiles, 0.5f) : std::ceil(tiles);
+        float step = v.step + v.busy * std::min(tiles, 1.f);
+        if (v.shared && n < 16) step -= 0.016f * (float)(16 - n) / 16.f;  // (rows that are not there take no way from L2)
+        const float cost = v.start + (float)steps * rounds * step, floor = (float)V * (float)K / 6e6f;  // (weights at 6 TB/s)
+        const float total = std::max(cost, floor) + 0.1f * cost;
+        if (i == 0 || total < least) {
+            best = i;
+            least = total;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -294,6 +564,14 @@ extern "C" int cpmcu_int8_weight_tile(const int8_t* w, int V, int K, int8_t* w_t
     return CPMCU_OK;
 }
 
+extern "C" int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, size_t kernel_name_bytes, int* num_workgroups) {
+    CPMCU_CHECK_ARG(n >= 1 && V >= 1 && K >= 1 && K <= kMaxColumns, "int8_linear_plan: n=%d, V=%d, K=%d outside [1, %d]", n, V, K, kMaxColumns);
+    const Variant& v = kVariants[choose_variant(n, V, K)];
+    if (kernel_name && kernel_name_bytes) snprintf(kernel_name, kernel_name_bytes, "%s", v.name);
+    if (num_workgroups) *num_workgroups = (int)std::min<int64_t>((int64_t)ceil_div(n, v.rows) * ceil_div(V, v.channels), INT32_MAX);
+    return CPMCU_OK;
+}
+
 extern "C" int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_tiled, const float* w_scales, int n, int V, int K, void* out,
                                  void* stream) {
     CPMCU_CHECK_ARG(xq && x_scales && w_tiled && w_scales && out, "int8_linear: null pointer argument");
@@ -301,31 +579,12 @@ extern "C" int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const 
     CPMCU_CHECK_ARG(((uintptr_t)xq | (uintptr_t)w_tiled) % 16 == 0, "int8_linear: xq and w_tiled have to lie on 16 bytes");
     if (n == 0) return CPMCU_OK;
     LinearParams p{xq, w_tiled, x_scales, w_scales, out, n, V, ceil_div(K, kStep), ceil_div(V, kBlock), 0, 0, V % 4 == 0 && (uintptr_t)out % 8 == 0};
-    hipStream_t st = resolve_stream(stream);
-    const bool is_bf16 = options().dtype == 1;
-    if (n > 64) {
-#define CPMCU_TILE(E, NX, NV, WX, WV)                                                                                                   \
-    do {                                                                                                                                \
-        p.row_tiles = ceil_div(n, 16 * NX * WX);                                                                                        \
-        p.channel_tiles = ceil_div(p.blocks, NV * WV);                                                                                  \
-        hipLaunchKernelGGL((int8_linear_tile_kernel<E, NX, NV, WX, WV>), dim3(p.row_tiles * p.channel_tiles), dim3(64 * WX * WV), 0, st, p); \
-    } while (0)
-        if (n > 512) {
-            if (is_bf16) CPMCU_TILE(bf16, 8, 4, 2, 4);
-            else CPMCU_TILE(f16, 8, 4, 2, 4);
-        } else {
-            if (is_bf16) CPMCU_TILE(bf16, 8, 2, 1, 4);
-            else CPMCU_TILE(f16, 8, 2, 1, 4);
-        }
-#undef CPMCU_TILE
-        CPMCU_LAUNCH_CHECK();
-        return CPMCU_OK;
-    }
-    const int nx = n <= 16 ? 1 : n <= 32 ? 2 : 4;
-    const dim3 grid(p.blocks, 1);
-#define CPMCU_LINEAR(E) (nx == 1 ? int8_linear_kernel<E, 1> : nx == 2 ? int8_linear_kernel<E, 2> : int8_linear_kernel<E, 4>)
-    hipLaunchKernelGGL(is_bf16 ? CPMCU_LINEAR(bf16) : CPMCU_LINEAR(f16), grid, dim3(512), 0, st, p);
-#undef CPMCU_LINEAR
+    const Variant v = kVariants[choose_variant(n, V, K)];
+    p.row_tiles = ceil_div(n, v.rows);
+    p.channel_tiles = ceil_div(V, v.channels);
+    CPMCU_CHECK_ARG((int64_t)p.row_tiles * p.channel_tiles <= INT32_MAX, "int8_linear: n=%d rows of V=%d channels", n, V);
+    const dim3 grid(p.row_tiles * p.channel_tiles);
+    hipLaunchKernelGGL(options().dtype == 1 ? v.bf16_kernel : v.f16_kernel, grid, dim3(v.threads), 0, resolve_stream(stream), p);
     CPMCU_LAUNCH_CHECK();
     return CPMCU_OK;
 }

@@ -19,8 +19,10 @@ struct Options {
     int frspec_fused = 0;          // 1: the FR-Spec head with its top-k as one launch where the shape allows (measured no faster: off)
     int frspec_wait_us = 50000;    // longest wait of a finisher of the fused FR-Spec launch for the other workgroups' words
     int topk_row_kernel = 1;       // 0: top-k by k rounds per chunk of 2048 elements and a merge launch (tests compare the two)
+    int int8_linear_shape = -1;    // -1 = chosen per call; 0 .. kInt8LinearShapes - 1: that shape of the 8-bit product
 };
 Options& options();
+constexpr int kInt8LinearShapes = 8;  // int8_linear.hip
 
 // tree_attention.hip -- what an attention launch can leave behind for the host: a device-side length outside
 // [max(T, mask_k_range), max_kv_len] (the launch worked on the clamped length), merge waits that ran out, partials of the

@@ -258,6 +258,9 @@ extern "C" int cpmcu_set_option(const char* name, int value) {
     } else if (nm == "topk_row_kernel") {
         CPMCU_CHECK_ARG(value == 0 || value == 1, "set_option: topk_row_kernel=%d must be 0 or 1", value);
         options().topk_row_kernel = value;
+    } else if (nm == "int8_linear_shape") {
+        CPMCU_CHECK_ARG(value >= -1 && value < kInt8LinearShapes, "set_option: int8_linear_shape=%d outside [-1, %d]", value, kInt8LinearShapes - 1);
+        options().int8_linear_shape = value;
     } else if (nm == "frspec_wait_us") {
         CPMCU_CHECK_ARG(value >= 0 && value <= 1000000, "set_option: frspec_wait_us=%d outside [0, 1000000]", value);
         options().frspec_wait_us = value;

@@ -97,6 +97,7 @@ SIGNATURES = {
     "cpmcu_int8_weight_bytes": (c_size_t, [c_int, c_int]),
     "cpmcu_int8_weight_tile": (c_int, [_P, c_int, c_int, _P, _P]),
     "cpmcu_int8_linear": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, _P, _P]),
+    "cpmcu_int8_linear_plan": (c_int, [c_int, c_int, c_int, c_char_p, c_size_t, ctypes.POINTER(c_int)]),
     "cpmcu_draft_tree_finish_root": (c_int, [_P, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P]),
 }
 

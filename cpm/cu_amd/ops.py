@@ -527,3 +527,10 @@ def head_plan(n, w):
     wg = ctypes.c_int(0)
     _lib().head_plan(n, V, H, layout, buf, 96, ctypes.byref(wg))
     return buf.value.decode(), wg.value
+
+
+def int8_linear_plan(n, V, K):
+    """(kernel name, workgroups) of an int8_linear call of n rows on a weight [V, K]."""
+    buf, wg = ctypes.create_string_buffer(96), ctypes.c_int(0)
+    _lib().int8_linear_plan(int(n), int(V), int(K), buf, 96, ctypes.byref(wg))
+    return buf.value.decode(), wg.value

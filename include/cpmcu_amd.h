@@ -113,7 +113,9 @@ const char* cpmcu_version(void);
  *   "topk_row_kernel"       1 = top-k by the one-launch row kernel (rows of more than 32768 elements in slices and a
  *                           merge of the slices' k best) (default), 0 = k rounds of a maximum search per chunk of 2048
  *                           elements and a merge launch, for chunks x k up to 2048: the same results, bit for bit,
- *                           from independent code. */
+ *                           from independent code;
+ *   "int8_linear_shape"     -1 = chosen per call (default), 0 to 7 = that shape of the 8-bit product's kernel (cpmcu_int8_linear_plan names
+ *                           it): the same results, bit for bit. */
 int cpmcu_set_option(const char* name, int value);
 
 /* ------------------------------------------------------------------------- */
@@ -701,6 +703,8 @@ int cpmcu_int8_weight_tile(const int8_t* w, int V, int K, int8_t* w_tiled, void*
  * behind column K does not matter), w_tiled as cpmcu_int8_weight_tile does.  K <= 131071. */
 int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_tiled, const float* w_scales, int n, int V, int K, void* out,
                       void* stream);
+/* The kernel a cpmcu_int8_linear call of this shape launches and its workgroup count, without launching (the outputs may be NULL). */
+int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, size_t kernel_name_bytes, int* num_workgroups);
 
 #ifdef __cplusplus
 }

@@ -90,6 +90,25 @@ def test_int8_operators_refuse():
     assert L.raw.cpmcu_int8_weight_bytes(17, 65) == 2 * 2 * 1024 and L.raw.cpmcu_int8_weight_bytes(0, 65) == 0
 
 
+def test_int8_linear_plans():
+    """Every shape of the kernel is somebody's, from one row to many."""
+    from cpm.cu_amd import lib, ops
+    seen = {}
+    for n in (1, 16, 32, 60, 128, 333, 512, 1024, 2048, 8192):
+        for V, K in ((512, 1000), (4608, 4096), (16384, 4096), (73448, 4096), (4096, 16384), (12289, 4099)):
+            name, workgroups = ops.int8_linear_plan(n, V, K)
+            seen.setdefault(name, []).append((n, V, K))
+            assert workgroups >= 1
+    assert len(seen) == 8
+    assert "split" in ops.int8_linear_plan(1, 4608, 4096)[0] and "wide" in ops.int8_linear_plan(8192, 16384, 4096)[0]
+    for args in ((0, 16, 64), (1, 0, 64), (1, 16, 131072)):
+        with pytest.raises(ValueError, match="int8_linear_plan"):
+            ops.int8_linear_plan(*args)
+    for value in (-2, 8):
+        with pytest.raises(ValueError, match="int8_linear_shape"):
+            lib.get().set_option(b"int8_linear_shape", value)
+
+
 def test_binding_refuses_host_tensors_and_counts_arguments():
     import torch
     from cpm.cu_amd import ops

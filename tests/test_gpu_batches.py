@@ -487,6 +487,35 @@ def test_int8_linear(gpu, set_option, dtype, n, V, K):
     assert same.data_ptr() == out[1:n + 1].data_ptr() and torch.equal(same.view(torch.int16), got.view(torch.int16)) and (out[0] == 7.0).all() and (out[n + 1] == 7.0).all()
 
 
+@pytest.fixture
+def int8_shape():
+    from cpm.cu_amd import lib
+    yield lambda i: lib.get().set_option(b"int8_linear_shape", i)
+    lib.get().set_option(b"int8_linear_shape", -1)
+
+
+@pytest.mark.parametrize("shape", range(8))
+def test_int8_linear_shapes_agree(gpu, set_option, int8_shape, shape):
+    """Each shape of the kernel at sizes about its tiles': odd rows, channels and steps, one step, many, and stores off 16 bytes."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    int8_shape(shape)
+    names = set()
+    for n, V, K, dtype in ((1, 1, 1, 0), (7, 300, 64, 1), (31, 130, 65, 0), (33, 127, 129, 0), (64, 128, 192, 1), (65, 257, 256, 0), (130, 513, 1000, 1), (255, 255, 1027, 0), (257, 259, 2048, 0), (300, 770, 4099, 1),
+                           (600, 264, 640, 0), (3, 5003, 333, 0)):
+        set_option("dtype", dtype)
+        names.add(ops.int8_linear_plan(n, V, K)[0])
+        xq, w = _int8(torch, n + K, n, (K + 63) // 64 * 64), _int8(torch, V + K, V, K)
+        x_scales, w_scales = torch.rand(n, device="cuda") * 0.01, torch.rand(V, device="cuda") * 0.001
+        out = torch.full((n + 1, V), 7.0, dtype=torch.float16, device="cuda")
+        got = _check_product(torch, dtype, xq, x_scales, w, w_scales, K, out=out[:n])
+        assert (out[n] == 7.0).all(), "written behind the last row"
+        int8_shape(0)
+        assert torch.equal(ops.int8_linear(xq, x_scales, ops.Int8Weight(w, w_scales)).view(torch.int16), got.view(torch.int16))
+        int8_shape(shape)
+    assert len(names) == 1
+
+
 @pytest.mark.parametrize("n", [1, 20, 70, 200, 600])
 def test_int8_linear_sums_to_the_ends_of_32_bits(gpu, n):
     """The longest rows of the largest values, and a row of scale NaN."""
