@@ -478,7 +478,7 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_ke
 }
 
 // The shapes, and what one of their tiles costs, as measured over 1 to 8192 rows, 512 to 73448 channels and 512 to 16384 columns: `start` us
-// of a launch and `step` us for every 64 columns of a round (a tile on every CU), `busy` more of them where all CUs work.  The choice is the
+// of a launch, for a round (a tile on every CU) `round` us and `step` more for every 64 columns, `busy` more of them where all CUs work.  The choice is the
 // shape with the least cost; it is within 10 % of the best one over that range (60 x 4096 x 16384: 32 x 128 14.5 us, 32 x 64 split 33.9, 64 x 128
 // 18.1; 333 x 4099 x 12289: 128 x 256 28.5, 64 x 128 34.8, 64 x 256 36.6, 256 x 256 48.9; 2048 x 4096 x 16384: 256 x 256 125, 128 x 256 151, 64 x 256 167).
 struct Variant {
@@ -486,7 +486,7 @@ struct Variant {
     void (*f16_kernel)(LinearParams);
     void (*bf16_kernel)(LinearParams);
     int rows, channels, threads;
-    float start, step, busy;
+    float start, round, step, busy;
     bool shared;  // workgroups share a CU: rounds need not be whole
 };
 #define CPMCU_SPLIT(nx, nv, u) "int8_linear_split_kernel<" #nx "," #nv ">", int8_linear_split_kernel<f16, nx, nv, u>, int8_linear_split_kernel<bf16, nx, nv, u>, 16 * nx, kBlock* nv, 64 * kSplit
@@ -497,9 +497,9 @@ struct Variant {
     "int8_linear_wide_kernel<" #nx "," #nv "," #wx "," #wv ">", int8_linear_wide_kernel<f16, nx, nv, wx, wv>, int8_linear_wide_kernel<bf16, nx, nv, wx, wv>, \
         16 * nx * wx, kBlock* nv* wv, 64 * wx * wv
 const Variant kVariants[kInt8LinearShapes] = {
-    {CPMCU_SPLIT(1, 2, 4), 4.f, 0.052f, 0.f, true},   {CPMCU_SPLIT(2, 2, 4), 5.f, 0.065f, 0.f, false},  {CPMCU_SPLIT(2, 4, 2), 5.6f, 0.09f, 0.f, false},
-    {CPMCU_TILE(2, 2, 1, 4, 4), 4.5f, 0.133f, 0.f, false}, {CPMCU_TILE(4, 2, 1, 4, 3), 4.5f, 0.205f, 0.f, false}, {CPMCU_TILE(4, 4, 1, 4, 2), 4.5f, 0.28f, 0.03f, false},
-    {CPMCU_WIDE(4, 4, 2, 4), 5.f, 0.345f, 0.17f, false}, {CPMCU_WIDE(8, 4, 2, 4), 5.f, 0.61f, 0.3f, false}};
+    {CPMCU_SPLIT(1, 2, 4), 4.f, 0.8f, 0.042f, 0.f, true},   {CPMCU_SPLIT(2, 2, 4), 5.f, 0.f, 0.065f, 0.f, false},  {CPMCU_SPLIT(2, 4, 2), 5.6f, 0.f, 0.09f, 0.f, false},
+    {CPMCU_TILE(2, 2, 1, 4, 4), 3.2f, 0.f, 0.148f, 0.f, false}, {CPMCU_TILE(4, 2, 1, 4, 3), 4.5f, 0.f, 0.205f, 0.f, false}, {CPMCU_TILE(4, 4, 1, 4, 2), 4.5f, 0.f, 0.28f, 0.03f, false},
+    {CPMCU_WIDE(4, 4, 2, 4), 5.f, 0.f, 0.345f, 0.17f, false}, {CPMCU_WIDE(8, 4, 2, 4), 5.f, 0.f, 0.61f, 0.3f, false}};
 #undef CPMCU_SPLIT
 #undef CPMCU_TILE
 #undef CPMCU_WIDE
@@ -515,7 +515,7 @@ int choose_variant(int n, int V, int K) {
         const float rounds = v.shared ? std::max(tiles, 0.5f) : std::ceil(tiles);
         float step = v.step + v.busy * std::min(tiles, 1.f);
         if (v.shared && n < 16) step -= 0.016f * (float)(16 - n) / 16.f;  // (rows that are not there take no way from L2)
-        const float cost = v.start + (float)steps * rounds * step, floor = (float)V * (float)K / 6e6f;  // (weights at 6 TB/s)
+        const float cost = v.start + rounds * (v.round + (float)steps * step), floor = (float)V * (float)K / 6e6f;  // (weights at 6 TB/s)
         const float total = std::max(cost, floor) + 0.1f * cost;
         if (i == 0 || total < least) {
             best = i;

@@ -17,7 +17,6 @@ constexpr int kThreads = 256;
 constexpr int kMaxHalf = 128;    // heads of up to 256 values
 constexpr int kMaxHeads = 1024;
 constexpr int kRows = 4;         // rows of a workgroup: their angles are formed once for all heads
-constexpr int kBatch = 4;        // items of a thread in flight
 
 struct Turns {
     const int32_t* positions;
@@ -41,34 +40,55 @@ __device__ inline float2 turn_of(const Turns& t, int position, int i) {
     return make_float2(c * t.magnitude, s * t.sine);
 }
 
-// An item of a head is eight pairs in two 16-byte pieces, behind the rotated values sixteen values (WIDE); or one pair, two values.
+// An item of a head is two 16-byte pieces (WideItem) or two values (NarrowItem) that lie so far apart that neighbouring lanes' pieces are
+// neighbours in memory: the two halves of pairs (i, i + half), behind those and with interleaved pairs the two halves of what there is.
+struct ItemPlace {
+    int first, second;   // values from the head's start
+    int turn_a, turn_b;  // the pieces' angles: with pairs (i, i + half) both pieces have turn_a's; -1: none, the piece is copied
+};
+template <int W, bool IL>
+__device__ inline ItemPlace item_place(int i, int half, int head_dim) {
+    if constexpr (IL) {
+        const int a = W * i, b = head_dim / 2 + W * i;
+        return {a, b, a < 2 * half ? a / 2 : -1, b < 2 * half ? b / 2 : -1};
+    } else {
+        if (W * i < half) return {W * i, half + W * i, W * i, -1};
+        const int rest = head_dim - 2 * half, j = W * i - half;
+        return {2 * half + j, 2 * half + rest / 2 + j, -1, -1};
+    }
+}
 template <typename E, bool IL>
 struct WideItem {
     typedef typename Elem<E>::x8 X8;
-    static constexpr int kPairs = 8;
+    static constexpr int kWidth = 8;
     X8 a, b;
-    __device__ inline void load(const E* head, int i, int half) {
-        a = *reinterpret_cast<const X8*>(head + first(i, half));
-        b = *reinterpret_cast<const X8*>(head + second(i, half));
+    __device__ static inline ItemPlace place(int i, int half, int head_dim) { return item_place<8, IL>(i, half, head_dim); }
+    __device__ inline void load(const E* head, const ItemPlace& at) {
+        a = *reinterpret_cast<const X8*>(head + at.first);
+        b = *reinterpret_cast<const X8*>(head + at.second);
     }
-    __device__ inline void store(E* head, int i, int half) const {
-        *reinterpret_cast<X8*>(head + first(i, half)) = a;
-        *reinterpret_cast<X8*>(head + second(i, half)) = b;
+    __device__ inline void store(E* head, const ItemPlace& at) const {
+        __builtin_nontemporal_store(a, reinterpret_cast<X8*>(head + at.first));
+        __builtin_nontemporal_store(b, reinterpret_cast<X8*>(head + at.second));
     }
-    __device__ static inline int first(int i, int half) { return !IL && 8 * i < half ? 8 * i : 16 * i; }
-    __device__ static inline int second(int i, int half) { return !IL && 8 * i < half ? half + 8 * i : 16 * i + 8; }
-    __device__ inline void turn(const float2* cs) {
+    __device__ static inline void turn_pairs(X8& x, const float2* cs) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (IL) {
-                X8& x = j < 4 ? a : b;
-                E u = x[2 * (j & 3)], v = x[2 * (j & 3) + 1];
-                rotate_pair(u, v, cs[j]);
-                x[2 * (j & 3)] = u;
-                x[2 * (j & 3) + 1] = v;
-            } else {
+        for (int j = 0; j < 4; ++j) {
+            E u = x[2 * j], v = x[2 * j + 1];
+            rotate_pair(u, v, cs[j]);
+            x[2 * j] = u;
+            x[2 * j + 1] = v;
+        }
+    }
+    __device__ inline void turn(const float2* cs, const ItemPlace& at) {
+        if constexpr (IL) {
+            if (at.turn_a >= 0) turn_pairs(a, cs + at.turn_a);
+            if (at.turn_b >= 0) turn_pairs(b, cs + at.turn_b);
+        } else if (at.turn_a >= 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
                 E u = a[j], v = b[j];
-                rotate_pair(u, v, cs[j]);
+                rotate_pair(u, v, cs[at.turn_a + j]);
                 a[j] = u;
                 b[j] = v;
             }
@@ -77,52 +97,47 @@ struct WideItem {
 };
 template <typename E, bool IL>
 struct NarrowItem {
-    static constexpr int kPairs = 1;
+    static constexpr int kWidth = 1;
     E a, b;
-    __device__ inline void load(const E* head, int i, int half) { a = head[first(i, half)], b = head[second(i, half)]; }
-    __device__ inline void store(E* head, int i, int half) const { head[first(i, half)] = a, head[second(i, half)] = b; }
-    __device__ static inline int first(int i, int half) { return !IL && i < half ? i : 2 * i; }
-    __device__ static inline int second(int i, int half) { return !IL && i < half ? half + i : 2 * i + 1; }
-    __device__ inline void turn(const float2* cs) { rotate_pair(a, b, cs[0]); }
+    // (interleaved pairs are neighbours: the item is the pair)
+    __device__ static inline ItemPlace place(int i, int half, int head_dim) { return IL ? ItemPlace{2 * i, 2 * i + 1, i < half ? i : -1, -1} : item_place<1, false>(i, half, head_dim); }
+    __device__ inline void load(const E* head, const ItemPlace& at) { a = head[at.first], b = head[at.second]; }
+    __device__ inline void store(E* head, const ItemPlace& at) const { head[at.first] = a, head[at.second] = b; }
+    __device__ inline void turn(const float2* cs, const ItemPlace& at) {
+        if (at.turn_a >= 0) rotate_pair(a, b, cs[at.turn_a]);
+    }
 };
 
-// Rows [r0, r0 + kRows) of q and k, this workgroup's part of their items.  present(r): whether row r has a position and a place.
-template <typename E, typename Item, typename Present>
+// Rows [r0, r0 + kRows) of q and k, this workgroup's part of their items.  place_of(r): a number >= 0, if row r has a position and a place;
+// k_head(r, place, head): where the result of a key head goes.  Results are stored past the L2, whose dirty lines a launch would have to
+// write back at its end (8191 rows of 40 heads 36.3 us, so 29.2); one item a thread at a time leaves most waves in flight (39 with four).
+template <typename E, typename Item, typename PlaceOf, typename KHead>
 __device__ inline void rope_run(const Turns& t, const HeadRows& q, const HeadRows& k, int n, int head_dim, int r0, int part, int parts, float2* cs, int* there,
-                                Present&& present) {
+                                PlaceOf&& place_of, KHead&& k_head) {
     const int tid = threadIdx.x, half = t.half;
-    const int items = head_dim / (2 * Item::kPairs), per_row = (q.heads + k.heads) * items;
+    const int items = head_dim / (2 * Item::kWidth), per_row = (q.heads + k.heads) * items;
     const int rows = min(kRows, n - r0), total = rows * per_row;
-    const int start = part * kThreads * kBatch;
-    for (int base = start; base < total; base += parts * kThreads * kBatch) {
-        Item x[kBatch];
-        int row[kBatch], item[kBatch];
-        E* to[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = base + u * kThreads + tid;
-            row[u] = -1;
-            if (i >= total) continue;
-            row[u] = i / per_row;
-            const int in_row = i - row[u] * per_row;
-            int head = in_row / items;
-            item[u] = in_row - head * items;
-            const bool is_q = head < q.heads;
-            if (!is_q) head -= q.heads;
-            const E* from = (const E*)(is_q ? q.in : k.in) + (r0 + row[u]) * (is_q ? q.in_stride : k.in_stride) + (long)head * head_dim;
-            to[u] = (E*)(is_q ? q.out : k.out) + (r0 + row[u]) * (is_q ? q.out_stride : k.out_stride) + (long)head * head_dim;
-            x[u].load(from, item[u], half);
+    const int start = part * kThreads;
+    for (int base = start; base < total; base += parts * kThreads) {
+        const int i = base + tid;
+        Item x;
+        ItemPlace at;
+        int row = 0, head = 0;
+        if (i < total) {
+            row = i / per_row;
+            const int in_row = i - row * per_row;
+            head = in_row / items;
+            at = Item::place(in_row - head * items, half, head_dim);
+            x.load(head < q.heads ? (const E*)q.in + (r0 + row) * q.in_stride + (long)head * head_dim : (const E*)k.in + (r0 + row) * k.in_stride + (long)(head - q.heads) * head_dim, at);
         }
         if (base == start) {
-            for (int i = tid; i < rows * half; i += kThreads) cs[i] = turn_of(t, t.positions[r0 + i / half], i % half);
-            if (tid < rows) there[tid] = present(r0 + tid);
+            for (int j = tid; j < rows * half; j += kThreads) cs[j] = turn_of(t, t.positions[r0 + j / half], j % half);
+            if (tid < rows) there[tid] = place_of(r0 + tid);
             __syncthreads();
         }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            if (row[u] < 0 || !there[row[u]]) continue;
-            if (item[u] * Item::kPairs < half) x[u].turn(cs + row[u] * half + item[u] * Item::kPairs);
-            x[u].store(to[u], item[u], half);
+        if (i < total && there[row] >= 0) {
+            x.turn(cs + row * half, at);
+            x.store(head < q.heads ? (E*)q.out + (r0 + row) * q.out_stride + (long)head * head_dim : (E*)k_head(r0 + row, there[row], head - q.heads), at);
         }
     }
 }
@@ -137,12 +152,13 @@ template <typename E, template <typename, bool> class Item, bool IL>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeParams p) {
     __shared__ float2 cs[kRows * kMaxHalf];
     __shared__ int there[kRows];
-    rope_run<E, Item<E, IL>>(p.t, p.q, p.k, p.n, p.head_dim, blockIdx.x * kRows, blockIdx.y, p.parts, cs, there, [&](int r) { return p.t.positions[r] >= 0; });
+    rope_run<E, Item<E, IL>>(p.t, p.q, p.k, p.n, p.head_dim, blockIdx.x * kRows, blockIdx.y, p.parts, cs, there, [&](int r) { return p.t.positions[r]; },
+                              [&](int r, int, int head) { return (E*)p.k.out + r * p.k.out_stride + (long)head * p.head_dim; });
 }
 
-// How many workgroups share kRows rows: enough to give every thread one batch while the launch is small.
+// How many workgroups share kRows rows: enough to give every thread one item while the launch is small.
 int row_parts(int n, int heads, int items) {
-    const int most = ceil_div(std::min(n, kRows) * heads * items, kThreads * kBatch);
+    const int most = ceil_div(std::min(n, kRows) * heads * items, kThreads);
     return std::min(most, std::max(1, 1024 / ceil_div(n, kRows)));
 }
 
@@ -172,104 +188,123 @@ int check_turns(const char* op, const int32_t* positions, const float* inv_freq,
 
 // ---- append ----
 
-constexpr int kSpan = 2 * kAppendRows;  // the row before a workgroup's sixteen, they, and the fifteen that may complete a group of slots
-
 struct SlotParams {
-    RopeParams rope;       // q alone; rope.t.positions null: rows that come rotated
+    RopeParams rope;  // q, and k without a place of its own; rope.t.positions null: rows that come rotated
     f16 *k_pool, *v_pool;
     const int32_t* slots;
-    const void *k, *v;
-    long k_stride, v_stride;
-    int Hkv, heads_per_wg, kv_blocks, num_slots;
+    const uint16_t* v;
+    long v_stride;
+    int v_blocks, num_slots;
 };
 
-// Sixteen rows of heads_per_wg KV heads.  K rows go on as 16-byte pieces.  V is transposed through LDS: what a page holds of a dim is
-// in aligned groups of 16 slots (two 16-byte pieces), so whoever has the first row of a run of consecutive slots inside such a group
-// writes all of the group -- up to fifteen rows beyond its own sixteen -- and pieces are whole wherever the rows of a request follow
-// each other, however the sixteen lie to the groups.
-template <typename E, bool IL>
-__device__ inline void append_run(const SlotParams& p, int block, float2* cs, int* slot, uint16_t* stage) {
-    typedef WideItem<E, IL> Item;
-    const int tid = threadIdx.x, n = p.rope.n, half = p.rope.t.half;
-    const int groups_of_heads = p.Hkv / p.heads_per_wg;
-    const int r0 = block / groups_of_heads * kAppendRows, g0 = block % groups_of_heads * p.heads_per_wg;
-    const bool rope = p.rope.t.positions != nullptr;
-    if (tid < kSpan) {
-        const int r = r0 - 1 + tid;
-        int s = -1;
-        if (r >= 0 && r < n) {
-            s = p.slots[r];
-            if (s < 0 || s >= p.num_slots || (rope && p.rope.t.positions[r] < 0)) s = -1;
-        }
-        slot[tid] = s;
-    }
-    if (rope)
-        for (int i = tid; i < min(kAppendRows, n - r0) * half; i += kThreads) cs[i] = turn_of(p.rope.t, p.rope.t.positions[r0 + i / half], i % half);
-    __syncthreads();
-    const int lane = tid & 63, at = lane & (kSpan - 1);
-    // bit i: row r0 - 1 + i has a place; it continues the group of the row before it
-    const int mine = slot[at];
-    const uint32_t present = (uint32_t)__ballot(mine >= 0);
-    const uint32_t joined = (uint32_t)__ballot(mine >= 0 && at > 0 && (mine & 15) != 0 && slot[max(at, 1) - 1] == mine - 1);
-    const uint32_t leaders = present & ~joined & 0x1FFFEu;
-    if ((present & 0x1FFFEu) == 0) return;
-    const auto run_of = [&](int i) { return 1 + __builtin_ctz(~((uint64_t)joined >> (i + 1))); };  // rows of the group that row i leads
-    const int last_leader = leaders ? 31 - __builtin_clz(leaders) : 0;
-    const int staged = leaders ? max(last_leader + run_of(last_leader) - 1, kAppendRows) : kAppendRows;  // rows r0 .. r0 + staged - 1
-    for (int g = g0; g < g0 + p.heads_per_wg; ++g) {
-        const int row = tid >> 4, ch = tid & 15;
-        for (int r = row; r < staged; r += kAppendRows) {
-            if (slot[1 + r] < 0) continue;
-            const uint4 vx = *reinterpret_cast<const uint4*>((const uint16_t*)p.v + (r0 + r) * p.v_stride + (long)g * kHeadDim + ch * 8);
-            uint2* to = reinterpret_cast<uint2*>(stage + r * kAppendStride + ch * 8);
-            to[0] = make_uint2(vx.x, vx.y);
-            to[1] = make_uint2(vx.z, vx.w);
-        }
-        if (tid < kAppendRows * 8) {
-            const int r = tid >> 3, i = tid & 7, s = slot[1 + r];
-            if (s >= 0) {
-                Item x;
-                x.load((const E*)p.k + (r0 + r) * p.k_stride + (long)g * kHeadDim, i, half);
-                if (rope && 8 * i < half) x.turn(cs + r * half + 8 * i);
-                x.store((E*)p.k_pool + (((size_t)(s / kPage) * p.Hkv + g) * kPage + s % kPage) * kHeadDim, i, half);
-            }
-        }
-        __syncthreads();
-        const int d = tid >> 1, piece = tid & 1;
-        for (uint32_t rest = leaders; rest; rest &= rest - 1) {
-            const int i = __builtin_ctz(rest), s = slot[i], len = run_of(i);
-            uint16_t* dst = reinterpret_cast<uint16_t*>(p.v_pool) + (((size_t)(s / kPage) * p.Hkv + g) * kHeadDim + d) * kPage + (s % kPage & ~15) + piece * 8;
-            uint32_t v[8], in = 0;
+__device__ inline int slot_of(const SlotParams& p, int r) {
+    const int s = p.slots[r];
+    return s >= 0 && s < p.num_slots && (p.rope.t.positions == nullptr || p.rope.t.positions[r] >= 0) ? s : -1;
+}
+
+// V of ROWS rows and one head.  A page holds a dim in aligned groups of 16 slots (two 16-byte pieces), so V is transposed through LDS, and whoever has
+// the first row of a run of consecutive slots inside such a group writes all of the run, up to fifteen rows beyond its own: pieces are
+// whole wherever the rows of a request follow each other, however a workgroup's rows lie to the groups.  64 rows fill whole lines of four groups; where
+// that leaves CUs idle, 16 rows do.  Everything is requested before anything is known of the slots: a decode step's rows are one round trip.
+template <int ROWS>
+struct VStage {
+    int slot[ROWS + 16];  // [i + 1]: row i of the workgroup's, -1: none
+    uint16_t v[(ROWS + 15) * kAppendStride];
+};
+template <int ROWS>
+__device__ inline void append_v(const SlotParams& p, int block, VStage<ROWS>& lds) {
+    constexpr int kAll = ROWS + 15, kSide = ROWS / 16;  // rows that may be needed; groups that are written side by side
+    const int tid = threadIdx.x, lane = tid & 63, n = p.rope.n, Hkv = p.rope.k.heads;
+    const int g = block % Hkv, r0 = block / Hkv * ROWS;
+    uint4 v[(kAll * 16 + kThreads - 1) / kThreads];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int r = piece * 4 + (j & 3) + (j >> 2) * 8 - (s & 15);  // the token of slot j, counted from the group's leader
-                v[j] = stage[(i - 1 + min(max(r, 0), len - 1)) * kAppendStride + d];
-                in |= r >= 0 && r < len ? 1u << j : 0u;
-            }
+    for (int u = 0; u * kThreads < kAll * 16; ++u) {
+        const int r = (u * kThreads + tid) >> 4;
+        if (r < kAll && r0 + r < n) v[u] = *reinterpret_cast<const uint4*>(p.v + (r0 + r) * p.v_stride + (long)g * kHeadDim + (tid & 15) * 8);
+    }
+    if (tid <= kAll) lds.slot[tid] = r0 + tid >= 1 && r0 + tid - 1 < n ? slot_of(p, r0 + tid - 1) : -1;
+#pragma unroll
+    for (int u = 0; u * kThreads < kAll * 16; ++u) {
+        const int r = (u * kThreads + tid) >> 4;
+        if (r < kAll && r0 + r < n) {
+            uint2* to = reinterpret_cast<uint2*>(lds.v + r * kAppendStride + (tid & 15) * 8);
+            to[0] = make_uint2(v[u].x, v[u].y);
+            to[1] = make_uint2(v[u].z, v[u].w);
+        }
+    }
+    __syncthreads();
+    // bit i: row i has a place; it goes on with the run of the row before it
+    const auto joins = [&](int i) { return i < kAll && lds.slot[i + 1] >= 0 && (lds.slot[i + 1] & 15) != 0 && lds.slot[i] == lds.slot[i + 1] - 1; };
+    const uint64_t joined = __ballot(joins(lane)), joined_hi = ROWS + 15 > 64 ? __ballot(joins(64 + lane)) : 0;
+    const uint64_t leaders = __ballot(lane < ROWS && lds.slot[min(lane, ROWS) + 1] >= 0) & ~joined;
+    if (leaders == 0) return;
+    const auto run_of = [&](int i) {  // rows of the run that row i leads
+        const uint32_t next = (uint32_t)(joined >> i >> 1) | (i >= 32 ? (uint32_t)(joined_hi << (63 - i)) : 0u);
+        return 1 + __builtin_ctz(~(next & 0x7FFFu));
+    };
+    const size_t head = (size_t)g * kHeadDim;
+    const auto dim_row = [&](int s, int d) { return reinterpret_cast<uint16_t*>(p.v_pool) + ((size_t)(s / kPage) * Hkv * kHeadDim + head + d) * kPage + (s % kPage & ~15); };
+    if (__popcll(leaders) > ROWS / 4) {
+        // short runs: value by value, all rows from the first leader's to the last run's end
+        const int d = tid & (kHeadDim - 1), last = 63 - __builtin_clzll(leaders), end = last + run_of(last);
+        for (int i = __builtin_ctzll(leaders) + (tid >> 7); i < end; i += 2) {
+            const int s = lds.slot[i + 1];
+            if (s >= 0) dim_row(s, d)[v_slot16(s & 15)] = lds.v[i * kAppendStride + d];
+        }
+        return;
+    }
+    const int piece = tid & 1, side = (tid >> 1) % kSide, d0 = tid / (2 * kSide);
+    uint64_t rest = leaders;
+    while (rest) {
+        int i = -1;
+#pragma unroll
+        for (int k = 0; k < kSide; ++k) {
+            if (k == side && rest) i = __builtin_ctzll(rest);
+            rest &= rest - 1;  // (of none: none)
+        }
+        if (i < 0) continue;
+        const int s = lds.slot[i + 1], len = run_of(i), first = piece * 4 - (s & 15);  // row i + first + (j & 3) + (j >> 2) * 8 is slot j's
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = first + (j & 3) + (j >> 2) * 8;
+            in |= r >= 0 && r < len ? 1u << j : 0u;
+        }
+        if (in == 0) continue;
+        for (int d = d0; d < kHeadDim; d += kThreads / (2 * kSide)) {
+            uint32_t y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = lds.v[(i + min(max(first + (j & 3) + (j >> 2) * 8, 0), len - 1)) * kAppendStride + d];
+            uint16_t* dst = dim_row(s, d) + piece * 8;
             if (in == 0xFFu) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(v[0] | (v[1] << 16), v[2] | (v[3] << 16), v[4] | (v[5] << 16), v[6] | (v[7] << 16));
+                typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+                __builtin_nontemporal_store(U4{y[0] | y[1] << 16, y[2] | y[3] << 16, y[4] | y[5] << 16, y[6] | y[7] << 16}, reinterpret_cast<U4*>(dst));
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if ((in >> j) & 1u) dst[j] = (uint16_t)v[j];
+                    if ((in >> j) & 1u) dst[j] = (uint16_t)y[j];
             }
         }
-        __syncthreads();
     }
 }
 
-template <typename E, bool IL>
+template <typename E, bool IL, int ROWS>
 __global__ __launch_bounds__(kThreads) void kv_append_slots_kernel(SlotParams p) {
-    __shared__ float2 cs[kAppendRows * kHeadDim / 2];
-    __shared__ int slot[kSpan];
-    __shared__ __attribute__((aligned(8))) uint16_t stage[kSpan * kAppendStride];
-    if ((int)blockIdx.x < p.kv_blocks) {
-        append_run<E, IL>(p, blockIdx.x, cs, slot, stage);
+    __shared__ union {
+        VStage<ROWS> v;
+        struct {
+            float2 cs[kRows * kMaxHalf];
+            int there[kRows];
+        } rope;
+    } lds;
+    if ((int)blockIdx.x < p.v_blocks) {
+        append_v<ROWS>(p, blockIdx.x, lds.v);
         return;
     }
-    const int b = blockIdx.x - p.kv_blocks;
-    rope_run<E, WideItem<E, IL>>(p.rope.t, p.rope.q, p.rope.k, p.rope.n, kHeadDim, b / p.rope.parts * kRows, b % p.rope.parts, p.rope.parts, cs, slot,
-                                 [&](int r) { return p.rope.t.positions[r] >= 0 && p.slots[r] >= 0 && p.slots[r] < p.num_slots; });
+    const int b = blockIdx.x - p.v_blocks, Hkv = p.rope.k.heads;
+    rope_run<E, WideItem<E, IL>>(p.rope.t, p.rope.q, p.rope.k, p.rope.n, kHeadDim, b / p.rope.parts * kRows, b % p.rope.parts, p.rope.parts, lds.rope.cs, lds.rope.there,
+                                 [&](int r) { return slot_of(p, r); },
+                                 [&](int, int s, int head) { return p.k_pool + (((size_t)(s / kPage) * Hkv + head) * kPage + s % kPage) * kHeadDim; });
 }
 
 }  // namespace
@@ -313,7 +348,7 @@ extern "C" int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, 
     }
     CPMCU_CHECK_ARG(rope || Hq == 0, "kv_append_slots: q is rotated here or not given");
     SlotParams p{};
-    p.rope = RopeParams{{positions, inv_freq, rope ? rotary_dim / 2 : 0, magnitude, magnitude}, {q, q_out, q_stride, q_out_stride, Hq}, {}, n, kHeadDim, 1};
+    p.rope = RopeParams{{positions, inv_freq, rope ? rotary_dim / 2 : 0, magnitude, magnitude}, {q, q_out, q_stride, q_out_stride, Hq}, {k, nullptr, k_stride, 0, Hkv}, n, kHeadDim, 1};
     if (int rc = check_rows("kv_append_slots", "q", p.rope.q, std::max(n, 1), kHeadDim)) return rc;
     const long width = (long)Hkv * kHeadDim;
     CPMCU_CHECK_ARG(k_stride >= width && v_stride >= width, "kv_append_slots: rows closer than their %ld values", width);
@@ -323,19 +358,17 @@ extern "C" int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, 
     p.k_pool = (f16*)k_pool;
     p.v_pool = (f16*)v_pool;
     p.slots = slots;
-    p.k = k;
-    p.v = v;
-    p.k_stride = k_stride;
+    p.v = (const uint16_t*)v;
     p.v_stride = v_stride;
-    p.Hkv = Hkv;
     p.num_slots = num_pages * kPage;
-    p.heads_per_wg = 1;
-    p.kv_blocks = ceil_div(n, kAppendRows) * (Hkv / p.heads_per_wg);
-    p.rope.parts = Hq ? row_parts(n, Hq, kHeadDim / 16) : 1;
-    const int q_blocks = Hq ? ceil_div(n, kRows) * p.rope.parts : 0;
+    const bool long_runs = (int64_t)ceil_div(n, 64) * Hkv >= 128;  // (4001 rows of 4 heads 8.3 us in 16s, 6.1 in 64s; 64 rows of 8 heads, a page each, 6.3 and 7.5)
+    p.v_blocks = ceil_div(n, long_runs ? 64 : 16) * Hkv;
+    p.rope.parts = row_parts(n, Hq + Hkv, kHeadDim / 16);
     hipStream_t st = resolve_stream(stream);
-    const dim3 grid(p.kv_blocks + q_blocks);
-#define CPMCU_SLOTS(E) (interleaved ? kv_append_slots_kernel<E, true> : kv_append_slots_kernel<E, false>)
+    const dim3 grid(p.v_blocks + ceil_div(n, kRows) * p.rope.parts);
+#define CPMCU_SLOTS(E)                                                                                                              \
+    (long_runs ? interleaved ? kv_append_slots_kernel<E, true, 64> : kv_append_slots_kernel<E, false, 64>                           \
+               : interleaved ? kv_append_slots_kernel<E, true, 16> : kv_append_slots_kernel<E, false, 16>)
     hipLaunchKernelGGL(options().dtype == 1 ? CPMCU_SLOTS(bf16) : CPMCU_SLOTS(f16), grid, dim3(kThreads), 0, st, p);
 #undef CPMCU_SLOTS
     CPMCU_LAUNCH_CHECK();
