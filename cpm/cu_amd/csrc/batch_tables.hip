@@ -19,9 +19,7 @@ namespace {
 
 constexpr int kMaxRequests = 4096;
 constexpr int kMaxBlocks = 1 << 18;   // 2^26 tokens of a request; the pages of kMaxRequests such requests add up in 32 bits
-constexpr int kMaxRows = 1 << 30;     // (the totals of rows stop at the capacity)
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kMaxRows = 1 << 29;     // (the totals of rows stop behind the capacity; two of them have to add up)
 constexpr int kRowsPerThread = 4;     // one 16-byte piece of positions and one of slots
 
 struct TableParams {
@@ -42,79 +40,116 @@ __device__ inline int first_above(const int* totals, int n, int x) {
     return lo;
 }
 
-// The total of the threads before this one, and of all of them, each `cap` at most (totals that stop at a cap can be added up in any grouping).
-__device__ inline int block_total(int v, int cap, int* wave_total, int* all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d);
-        if (lane >= d) v = min(v + o, cap);
-    }
-    if (lane == 63) wave_total[wave] = v;
-    __syncthreads();
-    int before = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w == wave) before = sum;
-        sum = min(sum + wave_total[w], cap);
-    }
-    __syncthreads();
-    *all = sum;
-    v = __shfl_up(v, 1);
-    return lane == 0 ? before : min(before + v, cap);
+// Inclusive running totals over a wave's lanes, each `cap` at most (totals that stop at a cap can be added up in any grouping).
+__device__ inline int wave_totals(int v, int cap) {
+    const auto add = [&](int from) { v = min(v + from, cap); };
+    add(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // rows of 16 lanes: from 1, 2, 4 and 8 lanes before,
+    add(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // lane 15 of rows 0 and 2 to the rows behind,
+    add(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // lane 31 to the upper half
+    return v;
 }
 
-__global__ __launch_bounds__(kThreads) void batch_tables_kernel(TableParams p) {
+// One workgroup of 256 threads with a request each where there are few, 1024 with four each beyond: a launch of 16 requests' single rows is
+// the round trip for their lengths, one exchange of totals, and the round trip for their pages.
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void batch_tables_kernel(TableParams p) {
+    constexpr int kMost = THREADS * EACH, kWaves = THREADS / 64;
     // running totals of rows, needed pages and pages given back; and each request's cached length, -1 where no row of it has a slot
-    __shared__ int row_end[kMaxRequests], need_end[kMaxRequests], back_end[kMaxRequests], length[kMaxRequests];
-    __shared__ int wave_total[kWaves], granted, refused;
-    const int tid = threadIdx.x, B = p.B, M = p.M;
-    const int each = (B + kThreads - 1) / kThreads, r0 = min(tid * each, B), r1 = min(r0 + each, B);  // this thread's requests
+    __shared__ int row_end[kMost], need_end[kMost], back_end[kMost], length[kMost];
+    __shared__ int wave_total[3][kWaves], served, lacking;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = p.B, M = p.M;
     const int row_cap = p.max_rows + 1;  // more rows than there is room for
     const auto held_by = [&](int r) { return min(max(p.held[r], 0), M); };
 
-    int rows = 0, back = 0, need = 0, lacking = 0, all_rows, all_back, all_need;
-    for (int r = r0; r < r1; ++r) {
-        const int n = p.new_lens[r];
-        rows = min(rows + min(max(n, 0), row_cap), row_cap);
-        if (n < 0) back += held_by(r);
+    int n[EACH], h[EACH], len[EACH], need[EACH];
+    int rows = 0, back = 0, needs = 0, bad = 0;
+    const int given = p.counts[0];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int r = tid * EACH + e;
+        n[e] = r < B ? p.new_lens[r] : 0;
+        h[e] = r < B ? held_by(r) : 0;
+        len[e] = r < B ? p.kv_lens[r] : 0;
     }
-    if (tid == 0) granted = refused = 0;
-    rows = block_total(rows, row_cap, wave_total, &all_rows);
-    back = block_total(back, INT32_MAX, wave_total, &all_back);
-    const int count = min(max(p.counts[0], 0), p.num_pages);
-    const int top = min(count + all_back, p.num_pages);
-    for (int r = r0; r < r1; ++r) {
-        const int n = p.new_lens[r], h = held_by(r), len = p.kv_lens[r];
-        const int64_t blocks = ((int64_t)len + max(n, 0) + kPage - 1) / kPage;
-        rows = min(rows + min(max(n, 0), row_cap), row_cap);
-        if (n < 0) back += h;
-        const bool bad = n >= 0 && (len < 0 || blocks > M || (n > 0 && rows > p.max_rows));
-        if (n >= 0 && !bad) need += max(0, (int)blocks - h);
-        lacking += bad;
-        row_end[r] = rows;
-        back_end[r] = back;
-        need_end[r] = need;
-        length[r] = n < 0 || bad ? -1 : len;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int64_t blocks = ((int64_t)len[e] + max(n[e], 0) + kPage - 1) / kPage;
+        const bool never = n[e] >= 0 && (len[e] < 0 || blocks > M);
+        bad |= never ? 1 << e : 0;
+        need[e] = n[e] < 0 || never ? 0 : max(0, (int)blocks - h[e]);
+        rows = min(rows + min(max(n[e], 0), row_cap), row_cap);
+        back += n[e] < 0 ? h[e] : 0;
+        needs += need[e];
     }
-    const int need_before = block_total(need, INT32_MAX, wave_total, &all_need);
-    int last = 0, served = 0;
-    for (int r = r0; r < r1; ++r) {
-        const int end = need_end[r];
-        need_end[r] = need_before + end;
-        if (end > last) {
-            if (need_before + end > top) {
-                length[r] = -1;
-                ++lacking;
-            } else {
-                served = need_before + end;
-            }
+    if (tid == 0) served = lacking = 0;
+    // totals in front of this thread's requests, and of all of them
+    int all[3], mine[3] = {rows, back, needs};
+    const auto totals = [&](int from, int to) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            if (k < from || k >= to) continue;
+            const int cap = k == 0 ? row_cap : INT32_MAX, upto = wave_totals(mine[k], cap);
+            if (lane == 63) wave_total[k][wave] = upto;
+            mine[k] = __builtin_amdgcn_update_dpp(0, upto, 0x138, 0xf, 0xf, false);  // the lane before
         }
-        last = end;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            if (k < from || k >= to) continue;
+            const int cap = k == 0 ? row_cap : INT32_MAX;
+            int before = 0, sum = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                if (w == wave) before = sum;
+                sum = min(sum + wave_total[k][w], cap);
+            }
+            mine[k] = min(before + mine[k], cap);
+            all[k] = sum;
+        }
+    };
+    totals(0, 3);
+    if (all[0] > p.max_rows) {  // some requests' rows have no place: they need no pages
+        needs = 0;
+        rows = mine[0];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            rows = min(rows + min(max(n[e], 0), row_cap), row_cap);
+            if (n[e] > 0 && rows > p.max_rows) {
+                bad |= 1 << e;
+                need[e] = 0;
+            }
+            needs += need[e];
+        }
+        mine[2] = needs;
+        __syncthreads();
+        totals(2, 3);
     }
-    if (served > 0) atomicMax(&granted, served);
-    if (lacking > 0) atomicAdd(&refused, lacking);
+    const int all_rows = all[0], all_back = all[1];
+    const int count = min(max(given, 0), p.num_pages);
+    const int top = min(count + all_back, p.num_pages);
+    int last = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int r = tid * EACH + e;
+        mine[0] = min(mine[0] + min(max(n[e], 0), row_cap), row_cap);
+        mine[1] += n[e] < 0 ? h[e] : 0;
+        mine[2] += need[e];
+        if (need[e] > 0 && mine[2] > top) bad |= 1 << e;
+        else if (need[e] > 0) last = mine[2];
+        if (r < B) {
+            row_end[r] = mine[0];
+            back_end[r] = mine[1];
+            need_end[r] = mine[2];
+            length[r] = n[e] < 0 || (bad >> e & 1) ? -1 : len[e];
+        }
+    }
+    if (all[2] > top && last > 0) atomicMax(&served, last);
+    if (bad) atomicAdd(&lacking, __popc(bad));
     __syncthreads();
+    const int granted = all[2] > top ? served : all[2];
 
     const auto begin = [&](const int* totals, int r) { return r > 0 ? totals[r - 1] : 0; };
     const auto on_stack = [&](int at) {  // entry `at` of the stack with the ended requests' pages on it
@@ -122,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void batch_tables_kernel(TableParams p) {
         const int i = at - count, r = first_above(back_end, B, i);
         return p.tables[(size_t)r * M + i - begin(back_end, r)];
     };
-    const int first = blockIdx.x * kThreads + tid, threads = gridDim.x * kThreads;
+    const int first = blockIdx.x * THREADS + tid, threads = gridDim.x * THREADS;
     for (int g = first; g * kRowsPerThread < p.max_rows; g += threads) {
         int at[kRowsPerThread], slot[kRowsPerThread];
         const int i0 = g * kRowsPerThread;
@@ -169,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void batch_tables_kernel(TableParams p) {
         p.tables[(size_t)r * M + held_by(r) + j - begin(need_end, r)] = on_stack(top - 1 - j);
     }
     if (blockIdx.x != 0) return;
-    for (int r = tid; r < B; r += kThreads) {
+    for (int r = tid; r < B; r += THREADS) {
         const int n = p.new_lens[r];
         const bool has = length[r] >= 0;
         p.kv_lens_out[r] = has ? length[r] + n : n < 0 ? 0 : p.kv_lens[r];
@@ -179,7 +214,7 @@ __global__ __launch_bounds__(kThreads) void batch_tables_kernel(TableParams p) {
     if (tid == 0) {
         p.row_offsets[0] = 0;
         p.counts_out[0] = top - granted;
-        p.counts_out[1] = refused;
+        p.counts_out[1] = lacking;
     }
 }
 
@@ -212,8 +247,9 @@ extern "C" int cpmcu_batch_tables(const int32_t* kv_lens, const int32_t* new_len
         for (const auto& i : in) CPMCU_CHECK_ARG(!overlap(o.at, o.bytes, i.at, i.bytes), "batch_tables: an output is the memory of an input");
     TableParams p{kv_lens, new_lens, held, counts, block_tables, free_pages, kv_lens_out, held_out, counts_out, row_offsets, positions, slots,
                   num_requests, max_blocks, num_pages, max_rows, ((uintptr_t)positions | (uintptr_t)slots) % 16 == 0};
-    const int grid = std::min(std::max(ceil_div(max_rows, kThreads * kRowsPerThread), 1), 1024);
-    hipLaunchKernelGGL(batch_tables_kernel, dim3(grid), dim3(kThreads), 0, resolve_stream(stream), p);
+    const bool few = num_requests <= 256;
+    const int grid = std::min(std::max(ceil_div(max_rows, (few ? 256 : 1024) * kRowsPerThread), 1), 1024);
+    hipLaunchKernelGGL((few ? batch_tables_kernel<256, 1> : batch_tables_kernel<1024, 4>), dim3(grid), dim3(few ? 256 : 1024), 0, resolve_stream(stream), p);
     CPMCU_LAUNCH_CHECK();
     return CPMCU_OK;
 }

@@ -531,11 +531,11 @@ int choose_variant(int n, int V, int K) {
 using namespace cpmcu;
 
 extern "C" int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K, int8_t* xq, float* scales, void* stream) {
-    CPMCU_CHECK_ARG(x && xq && scales, "quantize_rows: null pointer argument");
     CPMCU_CHECK_ARG(n >= 0 && K >= 1 && K <= kMaxColumns, "quantize_rows: n=%d, K=%d outside [1, %d]", n, K, kMaxColumns);
+    if (n == 0) return CPMCU_OK;  // (rows that are not there may have no memory)
+    CPMCU_CHECK_ARG(x && xq && scales, "quantize_rows: null pointer argument");
     CPMCU_CHECK_ARG(x_stride >= K, "quantize_rows: rows closer than their %d values", K);
     CPMCU_CHECK_ARG((uintptr_t)xq % 16 == 0, "quantize_rows: xq has to lie on 16 bytes");
-    if (n == 0) return CPMCU_OK;
     const bool wide = (uintptr_t)x % 16 == 0 && x_stride % 8 == 0 && K % 8 == 0;
     const int padded = ceil_div(K, kStep) * kStep;
     hipStream_t st = resolve_stream(stream);
@@ -574,10 +574,10 @@ extern "C" int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, si
 
 extern "C" int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_tiled, const float* w_scales, int n, int V, int K, void* out,
                                  void* stream) {
-    CPMCU_CHECK_ARG(xq && x_scales && w_tiled && w_scales && out, "int8_linear: null pointer argument");
     CPMCU_CHECK_ARG(n >= 0 && V >= 1 && K >= 1 && K <= kMaxColumns, "int8_linear: n=%d, V=%d, K=%d outside [1, %d]", n, V, K, kMaxColumns);
-    CPMCU_CHECK_ARG(((uintptr_t)xq | (uintptr_t)w_tiled) % 16 == 0, "int8_linear: xq and w_tiled have to lie on 16 bytes");
     if (n == 0) return CPMCU_OK;
+    CPMCU_CHECK_ARG(xq && x_scales && w_tiled && w_scales && out, "int8_linear: null pointer argument");
+    CPMCU_CHECK_ARG(((uintptr_t)xq | (uintptr_t)w_tiled) % 16 == 0, "int8_linear: xq and w_tiled have to lie on 16 bytes");
     LinearParams p{xq, w_tiled, x_scales, w_scales, out, n, V, ceil_div(K, kStep), ceil_div(V, kBlock), 0, 0, V % 4 == 0 && (uintptr_t)out % 8 == 0};
     const Variant v = kVariants[choose_variant(n, V, K)];
     p.row_tiles = ceil_div(n, v.rows);

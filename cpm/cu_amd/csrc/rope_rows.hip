@@ -317,11 +317,12 @@ extern "C" int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, 
                                int64_t k_out_stride, int Hkv, int head_dim, int n, void* stream) {
     CPMCU_CHECK_ARG(head_dim >= 2 && head_dim % 2 == 0 && head_dim <= 2 * kMaxHalf, "rope_rows: head_dim=%d is not an even number up to %d", head_dim, 2 * kMaxHalf);
     CPMCU_CHECK_ARG(n >= 0, "rope_rows: n=%d", n);
+    if (n == 0) return CPMCU_OK;  // (rows that are not there may have no memory)
     if (int rc = check_turns("rope_rows", positions, inv_freq, rotary_dim, head_dim, magnitude)) return rc;
     RopeParams p{{positions, inv_freq, rotary_dim / 2, magnitude, transposed ? -magnitude : magnitude}, {q, q_out, q_stride, q_out_stride, Hq}, {k, k_out, k_stride, k_out_stride, Hkv}, n, head_dim, 1};
-    if (int rc = check_rows("rope_rows", "q", p.q, std::max(n, 1), head_dim)) return rc;
-    if (int rc = check_rows("rope_rows", "k", p.k, std::max(n, 1), head_dim)) return rc;
-    if (n == 0 || Hq + Hkv == 0) return CPMCU_OK;
+    if (int rc = check_rows("rope_rows", "q", p.q, n, head_dim)) return rc;
+    if (int rc = check_rows("rope_rows", "k", p.k, n, head_dim)) return rc;
+    if (Hq + Hkv == 0) return CPMCU_OK;
     const bool wide = rotary_dim % 16 == 0 && head_dim % 16 == 0 && on_16_bytes(p.q) && on_16_bytes(p.k);
     p.parts = row_parts(n, Hq + Hkv, head_dim / (wide ? 16 : 2));
     const dim3 grid(ceil_div(n, kRows), p.parts);
@@ -338,9 +339,10 @@ extern "C" int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, 
 extern "C" int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, const int32_t* slots, const void* k, int64_t k_stride, const void* v,
                                      int64_t v_stride, int n, int Hkv, const int32_t* positions, const float* inv_freq, int rotary_dim, int interleaved,
                                      float magnitude, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, void* stream) {
-    CPMCU_CHECK_ARG(k_pool && v_pool && slots && k && v, "kv_append_slots: null pointer argument");
     CPMCU_CHECK_ARG(num_pages >= 1 && num_pages <= INT32_MAX / kPage, "kv_append_slots: num_pages=%d outside [1, %d]", num_pages, INT32_MAX / kPage);
     CPMCU_CHECK_ARG(n >= 0 && Hkv >= 1 && Hkv <= kMaxHeads, "kv_append_slots: n=%d Hkv=%d", n, Hkv);
+    if (n == 0) return CPMCU_OK;  // (rows that are not there may have no memory)
+    CPMCU_CHECK_ARG(k_pool && v_pool && slots && k && v, "kv_append_slots: null pointer argument");
     const bool rope = positions != nullptr || inv_freq != nullptr;
     if (rope) {
         if (int rc = check_turns("kv_append_slots", positions, inv_freq, rotary_dim, kHeadDim, magnitude)) return rc;
@@ -349,12 +351,11 @@ extern "C" int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, 
     CPMCU_CHECK_ARG(rope || Hq == 0, "kv_append_slots: q is rotated here or not given");
     SlotParams p{};
     p.rope = RopeParams{{positions, inv_freq, rope ? rotary_dim / 2 : 0, magnitude, magnitude}, {q, q_out, q_stride, q_out_stride, Hq}, {k, nullptr, k_stride, 0, Hkv}, n, kHeadDim, 1};
-    if (int rc = check_rows("kv_append_slots", "q", p.rope.q, std::max(n, 1), kHeadDim)) return rc;
+    if (int rc = check_rows("kv_append_slots", "q", p.rope.q, n, kHeadDim)) return rc;
     const long width = (long)Hkv * kHeadDim;
     CPMCU_CHECK_ARG(k_stride >= width && v_stride >= width, "kv_append_slots: rows closer than their %ld values", width);
     CPMCU_CHECK_ARG(on_16_bytes(p.rope.q) && ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0,
                     "kv_append_slots: rows and pools have to lie on 16 bytes");
-    if (n == 0) return CPMCU_OK;
     p.k_pool = (f16*)k_pool;
     p.v_pool = (f16*)v_pool;
     p.slots = slots;

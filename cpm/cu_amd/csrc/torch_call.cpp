@@ -105,8 +105,8 @@ bool convert(PyObject* o, T* out) {
 // torch's current stream.  torch's default stream is HIP's null stream, which the library has to be told apart from "its own
 // blocking stream": every launch on a blocking stream is ordered behind the null stream by a marker packet, 7-8 us between two
 // launches (append of 9 rows in a row: 10.5 us each, 3 on the null stream itself).
-void* current_stream() {
-    void* const st = reinterpret_cast<void*>(c10::hip::getCurrentHIPStream().stream());
+void* current_stream(c10::DeviceIndex device = -1) {
+    void* const st = reinterpret_cast<void*>(c10::hip::getCurrentHIPStream(device).stream());
     return st ? st : CPMCU_STREAM_LEGACY;
 }
 
@@ -260,19 +260,33 @@ PyObject* call_tree_attention_rows(PyObject*, PyObject* const* args, Py_ssize_t 
 
 // ---- batches: operators whose tensors may be views of wider rows; types, shapes and the device are checked here ----
 
-// A tensor of this type on the current device (whose stream the call goes to); null with an AssertionError set.
-const at::Tensor* device_tensor(PyObject* o, at::ScalarType type, const char* what) {
-    const at::Tensor* t = tensor_or_null(o);
-    if (t && t->is_cuda() && t->scalar_type() == type && t->device().index() == c10::hip::current_device()) return t;
-    PyErr_Format(PyExc_AssertionError, "%s on the current device required", what);
-    return nullptr;
-}
-const at::Tensor* dense_tensor(PyObject* o, at::ScalarType type, const char* what) {
-    const at::Tensor* t = device_tensor(o, type, what);
-    return t && expect(t->is_contiguous(), "device-resident contiguous tensor required") ? t : nullptr;
-}
+// The tensors of a call: on the current device, whose current stream the call goes to.  Null or false with an AssertionError set.
+struct Call {
+    c10::DeviceIndex device = -1;  // (asked for with the first device tensor: there may be none)
+    const at::Tensor* strided(PyObject* o, at::ScalarType type, const char* what) {
+        const at::Tensor* t = tensor_or_null(o);
+        if (t && t->is_cuda() && t->scalar_type() == type) {
+            if (device < 0) device = c10::hip::current_device();
+            if (t->device().index() == device) return t;
+        }
+        PyErr_Format(PyExc_AssertionError, "%s on the current device required", what);
+        return nullptr;
+    }
+    const at::Tensor* dense(PyObject* o, at::ScalarType type, const char* what) {
+        const at::Tensor* t = strided(o, type, what);
+        return t && expect(t->is_contiguous(), "device-resident contiguous tensor required") ? t : nullptr;
+    }
+    void* stream() const { return current_stream(device); }
+};
 int32_t* ints(const at::Tensor* t) { return static_cast<int32_t*>(t->data_ptr()); }
 at::Tensor new_tensor(const at::Tensor& like, at::ScalarType type, at::IntArrayRef sizes) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
+// n values of a one-dimensional tensor, from `at` on, as a tensor of their own on the same memory.
+at::Tensor part_of(const at::Tensor& whole, int64_t at, int64_t n) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    impl->set_storage_offset(at);
+    impl->set_sizes_contiguous(n);
+    return at::Tensor(std::move(impl));
+}
 bool integer(PyObject* o, int* out) { return convert(o, out); }
 
 decltype(&cpmcu_batch_tables) fn_batch_tables = nullptr;
@@ -286,35 +300,38 @@ bool arguments(Py_ssize_t nargs, Py_ssize_t expected) {
     return nargs == expected;
 }
 
-// batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, max_rows): (kv_lens, held, counts, row_offsets, positions, slots)
+// batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, max_rows): (kv_lens, held, counts, row_offsets, positions, slots, state).
+// One allocation (six cost 2.5 us of host time more), each part on 16 bytes; state is the first three as they lie in it, counts, held, kv_lens.
 PyObject* call_batch_tables(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!arguments(nargs, 7)) return nullptr;
-    const char* const what = "batch_tables: int32 tensors";
+    Call call;
     const at::Tensor* t[6];
     for (int i = 0; i < 6; ++i)
-        if (!(t[i] = dense_tensor(args[i], at::kInt, what))) return nullptr;
+        if (!(t[i] = call.dense(args[i], at::kInt, "batch_tables: int32 tensors"))) return nullptr;
     int max_rows;
     if (!integer(args[6], &max_rows)) return nullptr;
-    const at::Tensor &kv = *t[0], &tables = *t[2], &stack = *t[4];
-    const int64_t B = kv.numel();
+    const at::Tensor &tables = *t[2], &stack = *t[4];
+    const int64_t B = t[0]->numel();
     if (!expect(tables.dim() == 2 && tables.size(0) == B && t[1]->numel() == B && t[3]->numel() == B && t[5]->numel() == 2,
                 "batch_tables: lengths and held pages are [B], the tables [B, max_blocks], the counts [2]") ||
         !expect(B <= INT32_MAX && tables.size(1) <= INT32_MAX && stack.numel() <= INT32_MAX, "batch_tables: sizes beyond 32 bits"))
         return nullptr;
-    const int64_t rows = max_rows > 0 ? max_rows : 0;
-    const int64_t sizes[6] = {B, B, 2, B + 1, rows, rows};
-    at::Tensor out[6];
-    for (int i = 0; i < 6; ++i) out[i] = new_tensor(kv, at::kInt, at::IntArrayRef(&sizes[i], 1));
-    void* const st = current_stream();
+    const int64_t rows = max_rows > 0 ? max_rows : 0, sizes[6] = {2, B, B, B + 1, rows, rows};
+    int64_t at[7] = {0};
+    for (int i = 0; i < 6; ++i) at[i + 1] = at[i] + (sizes[i] + 3) / 4 * 4;
+    const at::Tensor whole = new_tensor(*t[0], at::kInt, at::IntArrayRef(&at[6], 1));
+    int32_t* const out = ints(&whole);
+    void* const st = call.stream();
     const int rc = without_gil([&] {
         return fn_batch_tables(ints(t[0]), ints(t[1]), static_cast<int>(B), ints(t[2]), static_cast<int>(tables.size(1)), ints(t[3]), ints(t[4]), static_cast<int>(stack.numel()),
-                               ints(t[5]), ints(&out[0]), ints(&out[1]), ints(&out[2]), ints(&out[3]), ints(&out[4]), ints(&out[5]), max_rows, st);
+                               ints(t[5]), out + at[2], out + at[1], out, out + at[3], out + at[4], out + at[5], max_rows, st);
     });
     if (rc != CPMCU_OK) return status(rc);
-    THPObjectPtr result(PyTuple_New(6));
+    THPObjectPtr result(PyTuple_New(7));
     if (!result) return nullptr;
-    for (int i = 0; i < 6; ++i) {
-        PyObject* o = THPVariable_Wrap(std::move(out[i]));
+    const int order[6] = {2, 1, 0, 3, 4, 5};
+    for (int i = 0; i < 7; ++i) {
+        PyObject* o = THPVariable_Wrap(i < 6 ? part_of(whole, at[order[i]], sizes[order[i]]) : part_of(whole, 0, at[3]));
         if (!o) return nullptr;
         PyTuple_SET_ITEM(result.get(), i, o);
     }
@@ -326,8 +343,8 @@ struct HeadRows {
     void* at = nullptr;
     int64_t stride = 0, n = 0, heads = 0, dim = 0;
 };
-bool head_rows(PyObject* o, const char* what, HeadRows* r) {
-    const at::Tensor* t = device_tensor(o, at::kHalf, what);
+bool head_rows(Call& call, PyObject* o, const char* what, HeadRows* r) {
+    const at::Tensor* t = call.strided(o, at::kHalf, what);
     if (!t) return false;
     if (t->dim() != 3 || t->size(0) > INT32_MAX || t->size(1) > INT32_MAX || t->size(2) > INT32_MAX ||
         (t->numel() > 0 && (t->stride(2) != 1 || (t->size(1) > 1 && t->stride(1) != t->size(2))))) {
@@ -342,18 +359,19 @@ bool alike(const HeadRows& a, const HeadRows& b) { return a.n == b.n && a.heads 
 // rope_rows(q, k, positions, inv_freq, interleaved, magnitude, transposed, q_out, k_out): k and k_out may be None.
 PyObject* call_rope_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!arguments(nargs, 9)) return nullptr;
+    Call call;
     HeadRows q, k, q_out, k_out;
     int interleaved, transposed;
     float magnitude;
-    if (!head_rows(args[0], "rope_rows: q of 16-bit floats", &q) || !head_rows(args[7], "rope_rows: q_out of 16-bit floats", &q_out) ||
-        (args[1] != Py_None && (!head_rows(args[1], "rope_rows: k of 16-bit floats", &k) || !head_rows(args[8], "rope_rows: k_out of 16-bit floats", &k_out))))
+    if (!head_rows(call, args[0], "rope_rows: q of 16-bit floats", &q) || !head_rows(call, args[7], "rope_rows: q_out of 16-bit floats", &q_out) ||
+        (args[1] != Py_None && (!head_rows(call, args[1], "rope_rows: k of 16-bit floats", &k) || !head_rows(call, args[8], "rope_rows: k_out of 16-bit floats", &k_out))))
         return nullptr;
-    const at::Tensor *pos = dense_tensor(args[2], at::kInt, "rope_rows: int32 positions"), *freq = pos ? dense_tensor(args[3], at::kFloat, "rope_rows: float32 inv_freq") : nullptr;
+    const at::Tensor *pos = call.dense(args[2], at::kInt, "rope_rows: int32 positions"), *freq = pos ? call.dense(args[3], at::kFloat, "rope_rows: float32 inv_freq") : nullptr;
     if (!freq || !integer(args[4], &interleaved) || !convert(args[5], &magnitude) || !integer(args[6], &transposed)) return nullptr;
     if (!expect(alike(q, q_out) && alike(k, k_out) && (args[1] == Py_None || (k.n == q.n && k.dim == q.dim)), "rope_rows: q, k and their results differ in shape") ||
         !expect(pos->numel() == q.n && freq->numel() <= INT32_MAX / 2, "rope_rows: a position for each row required"))
         return nullptr;
-    void* const st = current_stream();
+    void* const st = call.stream();
     return status(without_gil([&] {
         return fn_rope_rows(ints(pos), static_cast<const float*>(freq->data_ptr()), static_cast<int>(2 * freq->numel()), interleaved, magnitude, transposed, q.at, q.stride, q_out.at,
                             q_out.stride, static_cast<int>(q.heads), k.at, k.stride, k_out.at, k_out.stride, static_cast<int>(k.heads), static_cast<int>(q.dim), static_cast<int>(q.n), st);
@@ -363,15 +381,16 @@ PyObject* call_rope_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // kv_append_slots(k_pool, v_pool, k, v, slots, q, q_out, positions, inv_freq, interleaved, magnitude): q and q_out, positions and inv_freq may be None.
 PyObject* call_kv_append_slots(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!arguments(nargs, 11)) return nullptr;
+    Call call;
     const char* const pools = "kv_append_slots: pools of 16-bit floats";
-    const at::Tensor *k_pool = dense_tensor(args[0], at::kHalf, pools), *v_pool = k_pool ? dense_tensor(args[1], at::kHalf, pools) : nullptr;
+    const at::Tensor *k_pool = call.dense(args[0], at::kHalf, pools), *v_pool = k_pool ? call.dense(args[1], at::kHalf, pools) : nullptr;
     HeadRows k, v, q, q_out;
-    if (!v_pool || !head_rows(args[2], "kv_append_slots: k of 16-bit floats", &k) || !head_rows(args[3], "kv_append_slots: v of 16-bit floats", &v) ||
-        (args[5] != Py_None && (!head_rows(args[5], "kv_append_slots: q of 16-bit floats", &q) || !head_rows(args[6], "kv_append_slots: q_out of 16-bit floats", &q_out))))
+    if (!v_pool || !head_rows(call, args[2], "kv_append_slots: k of 16-bit floats", &k) || !head_rows(call, args[3], "kv_append_slots: v of 16-bit floats", &v) ||
+        (args[5] != Py_None && (!head_rows(call, args[5], "kv_append_slots: q of 16-bit floats", &q) || !head_rows(call, args[6], "kv_append_slots: q_out of 16-bit floats", &q_out))))
         return nullptr;
-    const at::Tensor *slots = dense_tensor(args[4], at::kInt, "kv_append_slots: int32 slots"), *pos = nullptr, *freq = nullptr;
-    if (!slots || (args[7] != Py_None && !(pos = dense_tensor(args[7], at::kInt, "kv_append_slots: int32 positions"))) ||
-        (args[8] != Py_None && !(freq = dense_tensor(args[8], at::kFloat, "kv_append_slots: float32 inv_freq"))))
+    const at::Tensor *slots = call.dense(args[4], at::kInt, "kv_append_slots: int32 slots"), *pos = nullptr, *freq = nullptr;
+    if (!slots || (args[7] != Py_None && !(pos = call.dense(args[7], at::kInt, "kv_append_slots: int32 positions"))) ||
+        (args[8] != Py_None && !(freq = call.dense(args[8], at::kFloat, "kv_append_slots: float32 inv_freq"))))
         return nullptr;
     int interleaved;
     float magnitude;
@@ -383,7 +402,7 @@ PyObject* call_kv_append_slots(PyObject*, PyObject* const* args, Py_ssize_t narg
         !expect(alike(q, q_out) && (args[5] == Py_None || (q.n == k.n && q.dim == CPMCU_HEAD_DIM)), "kv_append_slots: q and q_out are [n, Hq, 128]") ||
         !expect((pos != nullptr) == (freq != nullptr) && (!pos || pos->numel() == k.n) && (!freq || freq->numel() <= CPMCU_HEAD_DIM), "kv_append_slots: positions [n] and inv_freq go together"))
         return nullptr;
-    void* const st = current_stream();
+    void* const st = call.stream();
     return status(without_gil([&] {
         return fn_kv_append_slots(k_pool->data_ptr(), v_pool->data_ptr(), static_cast<int>(k_pool->size(0)), ints(slots), k.at, k.stride, v.at, v.stride, static_cast<int>(k.n),
                                   static_cast<int>(k.heads), pos ? ints(pos) : nullptr, freq ? static_cast<const float*>(freq->data_ptr()) : nullptr,
@@ -394,13 +413,14 @@ PyObject* call_kv_append_slots(PyObject*, PyObject* const* args, Py_ssize_t narg
 // quantize_rows(x): (xq [n, K rounded up to 64] of int8, scales [n])
 PyObject* call_quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!arguments(nargs, 1)) return nullptr;
-    const at::Tensor* x = device_tensor(args[0], at::kHalf, "quantize_rows: rows of 16-bit floats");
+    Call call;
+    const at::Tensor* x = call.strided(args[0], at::kHalf, "quantize_rows: rows of 16-bit floats");
     if (!x || !expect(x->dim() == 2 && (x->numel() == 0 || x->size(1) == 1 || x->stride(1) == 1) && x->size(0) <= INT32_MAX && x->size(1) <= INT32_MAX - 64, "quantize_rows: [n, K] with whole rows required"))
         return nullptr;
     const int64_t n = x->size(0), K = x->size(1), sizes[2] = {n, (K + 63) / 64 * 64};
     at::Tensor xq = new_tensor(*x, at::kChar, at::IntArrayRef(sizes, 2)), scales = new_tensor(*x, at::kFloat, at::IntArrayRef(sizes, 1));
     if (n == 0 || K == 0) return expect(K > 0, "quantize_rows: rows without values") ? Py_BuildValue("NN", THPVariable_Wrap(xq), THPVariable_Wrap(scales)) : nullptr;
-    void* const st = current_stream();
+    void* const st = call.stream();
     const int rc = without_gil([&] {
         return fn_quantize_rows(x->data_ptr(), n > 1 ? x->stride(0) : K, static_cast<int>(n), static_cast<int>(K), static_cast<int8_t*>(xq.data_ptr()), static_cast<float*>(scales.data_ptr()), st);
     });
@@ -411,9 +431,10 @@ PyObject* call_quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 // int8_linear(xq, x_scales, w_tiled, w_scales, V, K, out or None): out [n, V]
 PyObject* call_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!arguments(nargs, 7)) return nullptr;
+    Call call;
     const at::Tensor* t[4];
     for (int i = 0; i < 4; ++i)
-        if (!(t[i] = dense_tensor(args[i], i % 2 ? at::kFloat : at::kChar, i % 2 ? "int8_linear: float32 scales" : "int8_linear: int8 rows and weights"))) return nullptr;
+        if (!(t[i] = call.dense(args[i], i % 2 ? at::kFloat : at::kChar, i % 2 ? "int8_linear: float32 scales" : "int8_linear: int8 rows and weights"))) return nullptr;
     int V, K;
     if (!integer(args[4], &V) || !integer(args[5], &K)) return nullptr;
     const at::Tensor& xq = *t[0];
@@ -427,11 +448,11 @@ PyObject* call_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (args[6] == Py_None) {
         made = new_tensor(xq, at::kHalf, at::IntArrayRef(sizes, 2));
         out = &made;
-    } else if (!(out = dense_tensor(args[6], at::kHalf, "int8_linear: out of 16-bit floats")) || !expect(out->dim() == 2 && out->size(0) == n && out->size(1) == V, "int8_linear: out is [n, V]")) {
+    } else if (!(out = call.dense(args[6], at::kHalf, "int8_linear: out of 16-bit floats")) || !expect(out->dim() == 2 && out->size(0) == n && out->size(1) == V, "int8_linear: out is [n, V]")) {
         return nullptr;
     }
     if (n > 0) {
-        void* const st = current_stream();
+        void* const st = call.stream();
         const int rc = without_gil([&] {
             return fn_int8_linear(static_cast<const int8_t*>(xq.data_ptr()), static_cast<const float*>(t[1]->data_ptr()), static_cast<const int8_t*>(t[2]->data_ptr()),
                                   static_cast<const float*>(t[3]->data_ptr()), static_cast<int>(n), V, K, out->data_ptr(), st);

@@ -214,7 +214,7 @@ def batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, max_
     [max_rows]), which the next step takes in place of the inputs; block_tables and free_pages change in place.  Rows without a slot
     (refused requests', and behind the last one) have slot and position -1.  See PageBatch for an object that keeps all this.
     """
-    lens, held, counts, offsets, positions, slots = (_native or _calls()).batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, int(max_rows))
+    lens, held, counts, offsets, positions, slots, _ = (_native or _calls()).batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, int(max_rows))
     return dict(kv_lens=lens, held=held, counts=counts, row_offsets=offsets, positions=positions, slots=slots)
 
 
@@ -236,24 +236,24 @@ class PageBatch:
     ``block_tables[r]`` are then what tree_attention takes for request r (through ``cache_of``)."""
 
     def __init__(self, cache, max_requests, max_blocks, num_pages=None):
-        ints = dict(dtype=torch.int32, device=cache.device)
         self.cache = cache
         pages = cache.num_pages if num_pages is None else int(num_pages)
         assert 1 <= pages <= cache.num_pages
-        self.block_tables = torch.zeros((max_requests, max_blocks), **ints)
-        self.kv_lens = torch.zeros(max_requests, **ints)
-        self.held = torch.zeros(max_requests, **ints)
-        self.free_pages = torch.arange(pages - 1, -1, -1, **ints)
-        self.counts = torch.tensor([pages, 0], **ints)
+        self.max_requests, padded = int(max_requests), (int(max_requests) + 3) // 4 * 4
+        self.block_tables = torch.zeros((self.max_requests, max_blocks), dtype=torch.int32, device=cache.device)
+        self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=cache.device)
+        # one tensor, laid out as batch_tables' results are, so that a step is taken by one copy: views of it, and launches captured with them, see the new values
+        self._state = torch.zeros(4 + 2 * padded, dtype=torch.int32, device=cache.device)
+        self.counts, self.held, self.kv_lens = self._state[:2], self._state[4:4 + self.max_requests], self._state[4 + padded:4 + padded + self.max_requests]
+        self._state[0] = pages
 
     def plan(self, new_lens, max_rows):
         """new_lens int32 [max_requests]: rows of this step, -1 for a request that has ended.  The step is taken: lengths and pages
         are those with the new rows from here on (counts[1] says how many requests were refused)."""
-        step = batch_tables(self.kv_lens, new_lens, self.block_tables, self.held, self.free_pages, self.counts, max_rows)
-        # (copied, not replaced: views of them, and launches captured with them, see the new values)
-        for name in ("kv_lens", "held", "counts"):
-            getattr(self, name).copy_(step[name])
-        return step
+        lens, held, counts, offsets, positions, slots, state = (_native or _calls()).batch_tables(self.kv_lens, new_lens, self.block_tables, self.held, self.free_pages,
+                                                                                                  self.counts, int(max_rows))
+        self._state.copy_(state)
+        return dict(kv_lens=lens, held=held, counts=counts, row_offsets=offsets, positions=positions, slots=slots)
 
     def cache_of(self, r):
         """Request r's view of the cache, for tree_attention."""

@@ -25,7 +25,7 @@ def _tables(**kw):
 @pytest.mark.parametrize("kw, match", [
     (dict(kv=None), "null"), (dict(counts_out=None), "null"), (dict(positions=None), "null"), (dict(slots=None), "null"),
     (dict(n=0), "0 requests"), (dict(n=4097), "4097 requests"), (dict(blocks=0), "max_blocks=0"), (dict(blocks=(1 << 18) + 1), "max_blocks"),
-    (dict(pages=0), "num_pages=0"), (dict(pages=1 << 23), "num_pages"), (dict(rows=-1), "max_rows=-1"), (dict(rows=(1 << 30) + 1), "max_rows"),
+    (dict(pages=0), "num_pages=0"), (dict(pages=1 << 23), "num_pages"), (dict(rows=-1), "max_rows=-1"), (dict(rows=(1 << 29) + 1), "max_rows"),
     (dict(kv_out=P(1 << 32)), "memory of an input"), (dict(held_out=P((4 << 32) + 12)), "memory of an input"), (dict(counts_out=P(6 << 32)), "memory of an input"),
     (dict(slots=P((3 << 32) + 4 * 4 * 8 - 4)), "memory of an input"), (dict(positions=P((5 << 32) - 396)), "memory of an input")])
 def test_batch_tables_refuses(kw, match):
@@ -54,6 +54,7 @@ def test_empty_calls_are_no_calls():
     _rope(n=0)
     _rope(hq=0, hkv=0)
     _append(n=0)
+    _append(n=0, k=None, v=None, slots=None, q=None, qo=None, pos=None)
     _lib().quantize_rows(A, 64, 0, 64, B, C, None)
     _lib().int8_linear(A, B, C, D, 0, 16, 64, E, None)
 
@@ -76,7 +77,7 @@ def test_kv_append_slots_refuses(kw, match):
 
 def test_int8_operators_refuse():
     L = _lib()
-    for args in ((None, 64, 1, 64, B, C), (A, 64, 1, 64, None, C), (A, 64, 1, 64, B, None), (A, 64, -1, 64, B, C), (A, 64, 1, 0, B, C), (A, 1 << 20, 1, 131072, B, C), (A, 63, 1, 64, B, C),
+    for args in ((None, 64, 1, 64, B, C), (A, 64, 1, 64, None, C), (A, 64, 1, 64, B, None), (A, 64, -1, 64, B, C), (A, 64, 0, 0, B, C), (A, 64, 1, 0, B, C), (A, 1 << 20, 1, 131072, B, C), (A, 63, 1, 64, B, C),
                  (A, 64, 1, 64, P(24), C)):
         with pytest.raises(ValueError, match="quantize_rows"):
             L.quantize_rows(*args, None)

@@ -120,7 +120,7 @@ def _check_tables(torch, kv, new, tables, held, stack, count, max_rows):
     (1, 1, 1, 1, {}, 1), (1, 4, 300, 700, {}, 1000), (16, 512, 8000, 1, {}, 16), (16, 512, 8000, 1, dict(ended=0.3, idle=0.3), 64), (60, 8, 500, 300, dict(ended=0.1), 20001),
     (64, 3, 256, 256, dict(over=0.3), 40000), (333, 16, 1000, 100, dict(ended=0.2, idle=0.2, spare=0.5), 33333), (1023, 8, 200, 5, {}, 6001), (1024, 4, 300, 20, dict(ended=0.5), 30000),
     (1025, 4, 300, 20, dict(ended=0.1, spare=0.0), 30000), (4096, 5, 400, 30, dict(ended=0.1, idle=0.5, spare=0.9), 70003), (4096, 64, 1000, 1, {}, 4096), (100, 40, 2000, 500, dict(spare=0.8), 25000),
-    (3, 2000, 200000, 100000, {}, 400000), (5, 8, 100, 100, dict(ended=1.0), 64), (5, 8, 100, 100, dict(idle=1.0), 64), (7, 8, 100, 100, {}, 0)])
+    (3, 2000, 200000, 100000, {}, 400000), (255, 16, 900, 300, dict(ended=0.1, spare=0.7), 60001), (256, 9, 700, 3, dict(idle=0.2), 999), (257, 9, 700, 3, dict(idle=0.2), 999), (200, 9, 300, 400, dict(over=0.2), 30000), (2000, 9, 300, 100, dict(over=0.2, ended=0.1), 100000), (5, 8, 100, 100, dict(ended=1.0), 64), (5, 8, 100, 100, dict(idle=1.0), 64), (7, 8, 100, 100, {}, 0)])
 def test_batch_tables_is_the_walk_through_the_requests(gpu, B, M, mean_cached, mean_new, kw, rows):
     for seed in range(3):
         _check_tables(gpu, *_batch(B * 31 + seed, B, M, mean_cached, mean_new, **kw), rows)
@@ -668,6 +668,24 @@ def test_batch_operators_on_another_stream(gpu):
         got = calls()
     side.synchronize()
     assert torch.equal(got[0], -want[0]) and torch.equal(got[1], -want[1]) and torch.equal(got[2], -want[2])
+
+
+def test_no_rows_at_all(gpu):
+    torch = gpu
+    from cpm.cu_amd import ops
+    from cpm.cu_amd.kvcache import PagedKVCache
+    h = lambda *s: torch.empty(s, dtype=torch.float16, device="cuda")  # noqa: E731
+    none, f = torch.empty(0, dtype=torch.int32, device="cuda"), torch.ones(64, device="cuda")
+    cache = PagedKVCache(1, 2, 2, fill=3.0)
+    assert ops.rope_rows(h(0, 4, D), h(0, 2, D), none, f)[1].shape == (0, 2, D)
+    assert ops.rope_rows(h(3, 0, D), None, torch.zeros(3, dtype=torch.int32, device="cuda"), f)[0].shape == (3, 0, D)
+    assert ops.kv_append_slots(cache, 0, h(0, 2, D), h(0, 2, D), none) is None
+    assert ops.kv_append_slots(cache, 0, h(0, 2, D), h(0, 2, D), none, q=h(0, 4, D), positions=none, inv_freq=f).shape == (0, 4, D)
+    xq, scales = ops.quantize_rows(h(0, 100))
+    assert xq.shape == (0, 128) and scales.shape == (0,)
+    assert ops.int8_linear(xq, scales, ops.Int8Weight(torch.ones((5, 100), dtype=torch.int8, device="cuda"), f[:5])).shape == (0, 5)
+    torch.cuda.synchronize()
+    assert (cache.k[0] == 3.0).all() and (cache.v[0] == 3.0).all()
 
 
 def test_wrong_tensors_are_refused(gpu):
