@@ -126,6 +126,14 @@ def test_batch_tables_is_the_walk_through_the_requests(gpu, B, M, mean_cached, m
         _check_tables(gpu, *_batch(B * 31 + seed, B, M, mean_cached, mean_new, **kw), rows)
 
 
+@pytest.mark.parametrize("B, M, mean_cached, mean_new, kw, rows", [
+    (256, 16, 900, 300, dict(ended=0.1), 65537), (30, 200, 900, 5000, dict(over=0.1), 131333), (257, 40, 900, 1100, dict(ended=0.1, spare=0.9), 262145),
+    (1024, 9, 100, 300, dict(idle=0.5), 300001), (1025, 9, 100, 300, dict(idle=0.2, ended=0.2), 270000), (4096, 4, 100, 80, dict(idle=0.1), 262209)])
+def test_batch_tables_of_many_rows(gpu, B, M, mean_cached, mean_new, kw, rows):
+    """More rows than there are threads: several runs of rows a wave."""
+    _check_tables(gpu, *_batch(B * 37, B, M, mean_cached, mean_new, **kw), rows)
+
+
 def test_batch_tables_by_hand(gpu):
     """Boundaries of pages, requests that do not fit (the table, the stack, the rows), and lengths that are none."""
     I = 2 ** 31 - 1
