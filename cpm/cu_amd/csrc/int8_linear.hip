@@ -16,6 +16,10 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
+struct __attribute__((packed, aligned(2))) Piece {  // (moved as 16 bytes at any even address)
+    uint32_t v[4];
+};
+
 constexpr int kMaxColumns = 131071;
 constexpr int kCus = 256;             // of an MI355X
 constexpr int kStep = 64;             // columns of a matrix instruction; rows and weights are padded to whole steps
@@ -25,26 +29,32 @@ constexpr int kTile = kBlock * kStep; // bytes of a weight tile: lane l holds ch
 // ---- rows ----
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantPieces = 8;  // pieces of eight values that a thread keeps between the two passes: rows of up to 16384 values are read once
+constexpr int kQuantPieces = 8;   // pieces of eight values that a thread keeps between the two passes
+constexpr int kQuantRows = 1024;  // as many rows get a wave each
 
 __device__ inline u16x8 max_bits(u16x8 a, u16x8 b) { return __builtin_elementwise_max(a, b); }
 
-// One workgroup a row.  |x| is ordered as its bits are, so the maximum is taken on packed 16-bit integers, and an infinity or NaN is a
+// A workgroup a row, which reads rows of up to 16384 values once; a wave a row where there are many rows of up to 4096 values, which spares
+// the meeting of the waves and fills the card with loads: 8192 rows of 4096 values 19.3 us (5.2 TB/s, a copy's rate) and 24 by workgroups,
+// 8192 of 1024 9.0 and 17.7, 1024 of 4096 4.4 and 5.1, but 512 4.0 and 3.5 and a single one 3.4 and 2.7.  Rows start at any even address:
+// 16-byte loads may, and only a row's last values are loaded one by one (8192 rows of 4099: 28 us, 48 with every value by itself).
+// |x| is ordered as its bits are, so the maximum is taken on packed 16-bit integers, and an infinity or NaN is a
 // maximum from the infinity's pattern on: such a row gets scale NaN and zeros, and its products are NaN.  127 x is exact in 32 bits, and
 // the quotient's error is mended by one Newton step, which is exact where the quotient is: rint sees a tie where there is one, and a
 // quotient that is none is at least 2^-19 of itself away from the next one.
-template <typename E, bool WIDE>
-__global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const E* x, long stride, int K, int padded, int8_t* xq, float* scales) {
+template <typename E, int THREADS, bool WHOLE>
+__global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const E* x, long stride, int n, int K, int padded, int8_t* xq, float* scales) {
     __shared__ uint32_t wave_max[kQuantThreads / 64];
-    const int tid = threadIdx.x;
-    const E* row = x + blockIdx.x * stride;
+    const int tid = threadIdx.x % THREADS, at = blockIdx.x * (kQuantThreads / THREADS) + threadIdx.x / THREADS;
+    if (at >= n) return;  // (only whole waves, and only where no barrier follows)
+    const E* row = x + at * stride;
     const auto load = [&](int i) {
         u16x8 v = {};
-        if constexpr (WIDE) {
-            if (8 * i < K) v = *reinterpret_cast<const u16x8*>(row + 8 * i);
-        } else {
+        if (WHOLE ? 8 * i < K : 8 * i + 8 <= K) {
+            v = __builtin_bit_cast(u16x8, *reinterpret_cast<const Piece*>(row + 8 * i));
+        } else if (8 * i < K) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 7; ++j)
                 if (8 * i + j < K) v[j] = __builtin_bit_cast(uint16_t, row[8 * i + j]);
         }
         return v;
@@ -53,26 +63,28 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const E* x
     u16x8 kept[kQuantPieces], m = {};
 #pragma unroll
     for (int u = 0; u < kQuantPieces; ++u) {
-        kept[u] = load(tid + u * kQuantThreads);
+        kept[u] = load(tid + u * THREADS);
         m = max_bits(m, kept[u] & (uint16_t)0x7FFF);
     }
-    for (int i = tid + kQuantPieces * kQuantThreads; i < pieces; i += kQuantThreads) m = max_bits(m, load(i) & (uint16_t)0x7FFF);
+    for (int i = tid + kQuantPieces * THREADS; i < pieces; i += THREADS) m = max_bits(m, load(i) & (uint16_t)0x7FFF);
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, (uint32_t)m[j]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    if ((tid & 63) == 0) wave_max[tid >> 6] = top;
-    __syncthreads();
+    if constexpr (THREADS > 64) {
+        if ((tid & 63) == 0) wave_max[tid >> 6] = top;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kQuantThreads / 64; ++w) top = max(top, wave_max[w]);
+        for (int w = 0; w < THREADS / 64; ++w) top = max(top, wave_max[w]);
+    }
     const float amax = Elem<E>::from_bits((uint16_t)top);
     const bool finite = amax <= Elem<E>::kMaxFinite;
     // (bfloat16 reaches as far as 32 bits do: 127 x and 1 / amax stay in range by a power of two on both)
     const float pre = amax > 0x1p100f ? 0x1p-30f : amax < 0x1p-100f ? 0x1p30f : 1.f;
     const float a = amax * pre, inverse = finite && amax > 0.f ? 1.f / a : 0.f, to127 = 127.f * pre;
-    if (tid == 0) scales[blockIdx.x] = finite ? amax / 127.f : __builtin_nanf("");
-    uint2* out = reinterpret_cast<uint2*>(xq + (size_t)blockIdx.x * padded);
+    if (tid == 0) scales[at] = finite ? amax / 127.f : __builtin_nanf("");
+    uint2* out = reinterpret_cast<uint2*>(xq + (size_t)at * padded);
     const auto put = [&](int i, u16x8 v) {
         uint32_t w[2] = {};
 #pragma unroll
@@ -87,8 +99,8 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const E* x
     };
 #pragma unroll
     for (int u = 0; u < kQuantPieces; ++u)
-        if (tid + u * kQuantThreads < pieces) put(tid + u * kQuantThreads, kept[u]);
-    for (int i = tid + kQuantPieces * kQuantThreads; i < pieces; i += kQuantThreads) put(i, load(i));
+        if (tid + u * THREADS < pieces) put(tid + u * THREADS, kept[u]);
+    for (int i = tid + kQuantPieces * THREADS; i < pieces; i += THREADS) put(i, load(i));
 }
 
 // ---- weights ----
@@ -238,9 +250,6 @@ __global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearPa
 // A wave's tile: NX blocks of rows from t0 on, NV blocks of channels from c0 on.  The results go through LDS, as many blocks of rows at a time
 // as ROOM bytes of the wave's own hold, so that a row's are stored as one run of NV * 32 bytes (as they lie in the accumulators a row has 8);
 // rows of an uneven V start anywhere, which 16-byte stores may.
-struct __attribute__((packed, aligned(2))) Piece {
-    uint32_t v[4];
-};
 template <typename E, int NX, int NV, int ROOM>
 __device__ inline void store_tile(const LinearParams& p, int t0, int c0, i32x4 (&acc)[NX][NV], int8_t* part) {
     constexpr int kRoom = ROOM / (512 * NV), kPieces = 2 * NV, kPass = NX <= kRoom ? NX : kRoom < 4 ? 2 : kRoom < 8 ? 4 : 8;
@@ -534,12 +543,16 @@ extern "C" int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K
     CPMCU_CHECK_ARG(n >= 0 && K >= 1 && K <= kMaxColumns, "quantize_rows: n=%d, K=%d outside [1, %d]", n, K, kMaxColumns);
     if (n == 0) return CPMCU_OK;  // (rows that are not there may have no memory)
     CPMCU_CHECK_ARG(x && xq && scales, "quantize_rows: null pointer argument");
+    CPMCU_CHECK_ARG(n < 1 << 24, "quantize_rows: n=%d, more rows than a launch has workgroups", n);
     CPMCU_CHECK_ARG(x_stride >= K, "quantize_rows: rows closer than their %d values", K);
     CPMCU_CHECK_ARG((uintptr_t)xq % 16 == 0, "quantize_rows: xq has to lie on 16 bytes");
-    const bool wide = (uintptr_t)x % 16 == 0 && x_stride % 8 == 0 && K % 8 == 0;
     const int padded = ceil_div(K, kStep) * kStep;
     hipStream_t st = resolve_stream(stream);
-#define CPMCU_QUANT(E) hipLaunchKernelGGL((wide ? quantize_rows_kernel<E, true> : quantize_rows_kernel<E, false>), dim3(n), dim3(kQuantThreads), 0, st, (const E*)x, (long)x_stride, K, padded, xq, scales)
+    const bool whole = K % 8 == 0, waves = n >= kQuantRows && padded <= 64 * 8 * kQuantPieces;
+#define CPMCU_QUANT(E)                                                                                                                              \
+    hipLaunchKernelGGL((waves ? whole ? quantize_rows_kernel<E, 64, true> : quantize_rows_kernel<E, 64, false>                                      \
+                              : whole ? quantize_rows_kernel<E, kQuantThreads, true> : quantize_rows_kernel<E, kQuantThreads, false>),              \
+                       dim3(waves ? ceil_div(n, kQuantThreads / 64) : n), dim3(kQuantThreads), 0, st, (const E*)x, (long)x_stride, n, K, padded, xq, scales)
     if (options().dtype == 1) CPMCU_QUANT(bf16);
     else CPMCU_QUANT(f16);
 #undef CPMCU_QUANT

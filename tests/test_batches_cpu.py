@@ -78,7 +78,7 @@ def test_kv_append_slots_refuses(kw, match):
 def test_int8_operators_refuse():
     L = _lib()
     for args in ((None, 64, 1, 64, B, C), (A, 64, 1, 64, None, C), (A, 64, 1, 64, B, None), (A, 64, -1, 64, B, C), (A, 64, 0, 0, B, C), (A, 64, 1, 0, B, C), (A, 1 << 20, 1, 131072, B, C), (A, 63, 1, 64, B, C),
-                 (A, 64, 1, 64, P(24), C)):
+                 (A, 64, 1, 64, P(24), C), (A, 64, 1 << 24, 64, B, C)):
         with pytest.raises(ValueError, match="quantize_rows"):
             L.quantize_rows(*args, None)
     for args in ((None, 16, 64, B), (A, 16, 64, None), (A, 16, 64, A), (A, 0, 64, B), (A, 16, 0, B), (A, 16, 131072, B), (A, 16, 64, P(8))):

@@ -435,6 +435,21 @@ def test_quantize_rows(gpu, set_option, dtype, n, K):
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n, K", [(1023, 129), (1024, 1), (1025, 64), (1026, 71), (1027, 512), (1030, 4090), (1031, 4096), (1024, 4097), (1024, 4161)])
+def test_quantize_many_rows(gpu, set_option, dtype, n, K):
+    """A wave a row, and rows that are just too long for one."""
+    torch = gpu
+    set_option("dtype", dtype)
+    x = _rows(torch, n + K, dtype, n, K)
+    x[0] *= 0.001
+    x[1] = 0
+    x[2, K // 2] = float("inf")
+    x[-1, K - 1] = float("nan")
+    _check_quantized(torch, x)
+    _check_quantized(torch, torch.cat([x, x], 1)[:, 3 % K:3 % K + K].contiguous().view(n, K))
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
 def test_quantize_rows_at_the_types_limits(gpu, set_option, dtype):
     """Ties, the largest and the smallest values, signed zeros, -inf and NaN of either sign."""
     torch = gpu
@@ -457,6 +472,14 @@ def test_quantize_rows_of_wider_rows(gpu):
     x = _rows(torch, 8, 0, 20, 700)
     for lo, hi in ((0, 512), (8, 648), (3, 700), (64, 65)):
         _check_quantized(torch, x[:, lo:hi])
+
+
+def test_quantize_rows_at_any_address(gpu):
+    torch = gpu
+    for n in (20, 1100):
+        x = _rows(torch, 9, 0, n, 701)
+        for lo, hi in ((1, 513), (2, 642), (5, 701), (7, 71)):
+            _check_quantized(torch, x[:, lo:hi])
 
 
 def _int8(torch, seed, *shape):
