@@ -21,6 +21,7 @@ struct __attribute__((packed, aligned(2))) Piece {  // (moved as 16 bytes at any
 };
 
 constexpr int kMaxColumns = 131071;
+constexpr int kMaxChannels = 1 << 30, kMaxRows = 1 << 30;
 constexpr int kCus = 256;             // of an MI355X
 constexpr int kStep = 64;             // columns of a matrix instruction; rows and weights are padded to whole steps
 constexpr int kBlock = 16;            // channels of a weight block
@@ -561,13 +562,13 @@ extern "C" int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K
 }
 
 extern "C" size_t cpmcu_int8_weight_bytes(int V, int K) {
-    if (V < 1 || K < 1) return 0;
+    if (V < 1 || V > kMaxChannels || K < 1 || K > kMaxColumns) return 0;
     return (size_t)ceil_div(V, kBlock) * ceil_div(K, kStep) * kTile;
 }
 
 extern "C" int cpmcu_int8_weight_tile(const int8_t* w, int V, int K, int8_t* w_tiled, void* stream) {
     CPMCU_CHECK_ARG(w && w_tiled && (const void*)w != (const void*)w_tiled, "int8_weight_tile: null or aliased pointer argument");
-    CPMCU_CHECK_ARG(V >= 1 && K >= 1 && K <= kMaxColumns, "int8_weight_tile: V=%d, K=%d outside [1, %d]", V, K, kMaxColumns);
+    CPMCU_CHECK_ARG(V >= 1 && V <= kMaxChannels && K >= 1 && K <= kMaxColumns, "int8_weight_tile: V=%d outside [1, %d] or K=%d outside [1, %d]", V, kMaxChannels, K, kMaxColumns);
     CPMCU_CHECK_ARG((uintptr_t)w_tiled % 16 == 0, "int8_weight_tile: w_tiled has to lie on 16 bytes");
     const bool wide = (uintptr_t)w % 16 == 0 && K % 16 == 0;
     const int steps = ceil_div(K, kStep);
@@ -578,7 +579,7 @@ extern "C" int cpmcu_int8_weight_tile(const int8_t* w, int V, int K, int8_t* w_t
 }
 
 extern "C" int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, size_t kernel_name_bytes, int* num_workgroups) {
-    CPMCU_CHECK_ARG(n >= 1 && V >= 1 && K >= 1 && K <= kMaxColumns, "int8_linear_plan: n=%d, V=%d, K=%d outside [1, %d]", n, V, K, kMaxColumns);
+    CPMCU_CHECK_ARG(n >= 1 && n <= kMaxRows && V >= 1 && V <= kMaxChannels && K >= 1 && K <= kMaxColumns, "int8_linear_plan: n=%d, V=%d, K=%d outside [1, %d]", n, V, K, kMaxColumns);
     const Variant& v = kVariants[choose_variant(n, V, K)];
     if (kernel_name && kernel_name_bytes) snprintf(kernel_name, kernel_name_bytes, "%s", v.name);
     if (num_workgroups) *num_workgroups = (int)std::min<int64_t>((int64_t)ceil_div(n, v.rows) * ceil_div(V, v.channels), INT32_MAX);
@@ -587,7 +588,7 @@ extern "C" int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, si
 
 extern "C" int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_tiled, const float* w_scales, int n, int V, int K, void* out,
                                  void* stream) {
-    CPMCU_CHECK_ARG(n >= 0 && V >= 1 && K >= 1 && K <= kMaxColumns, "int8_linear: n=%d, V=%d, K=%d outside [1, %d]", n, V, K, kMaxColumns);
+    CPMCU_CHECK_ARG(n >= 0 && n <= kMaxRows && V >= 1 && V <= kMaxChannels && K >= 1 && K <= kMaxColumns, "int8_linear: n=%d, V=%d, K=%d outside [1, %d]", n, V, K, kMaxColumns);
     if (n == 0) return CPMCU_OK;
     CPMCU_CHECK_ARG(xq && x_scales && w_tiled && w_scales && out, "int8_linear: null pointer argument");
     CPMCU_CHECK_ARG(((uintptr_t)xq | (uintptr_t)w_tiled) % 16 == 0, "int8_linear: xq and w_tiled have to lie on 16 bytes");
@@ -595,7 +596,7 @@ extern "C" int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const 
     const Variant v = kVariants[choose_variant(n, V, K)];
     p.row_tiles = ceil_div(n, v.rows);
     p.channel_tiles = ceil_div(V, v.channels);
-    CPMCU_CHECK_ARG((int64_t)p.row_tiles * p.channel_tiles <= INT32_MAX, "int8_linear: n=%d rows of V=%d channels", n, V);
+    CPMCU_CHECK_ARG((int64_t)p.row_tiles * p.channel_tiles * v.threads <= UINT32_MAX, "int8_linear: n=%d rows of V=%d channels are more than a launch has threads", n, V);
     const dim3 grid(p.row_tiles * p.channel_tiles);
     hipLaunchKernelGGL(options().dtype == 1 ? v.bf16_kernel : v.f16_kernel, grid, dim3(v.threads), 0, resolve_stream(stream), p);
     CPMCU_LAUNCH_CHECK();

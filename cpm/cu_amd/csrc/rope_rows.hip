@@ -16,6 +16,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 128;    // heads of up to 256 values
 constexpr int kMaxHeads = 1024;
+constexpr int kMaxRows = 1 << 24; // of an append kMaxRows * 8 of all V heads (a launch has fewer than 2^32 threads)
 constexpr int kRows = 4;         // rows of a workgroup: their angles are formed once for all heads
 
 struct Turns {
@@ -316,7 +317,7 @@ extern "C" int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, 
                                const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, const void* k, int64_t k_stride, void* k_out,
                                int64_t k_out_stride, int Hkv, int head_dim, int n, void* stream) {
     CPMCU_CHECK_ARG(head_dim >= 2 && head_dim % 2 == 0 && head_dim <= 2 * kMaxHalf, "rope_rows: head_dim=%d is not an even number up to %d", head_dim, 2 * kMaxHalf);
-    CPMCU_CHECK_ARG(n >= 0, "rope_rows: n=%d", n);
+    CPMCU_CHECK_ARG(n >= 0 && n < kMaxRows, "rope_rows: n=%d outside [0, %d)", n, kMaxRows);
     if (n == 0) return CPMCU_OK;  // (rows that are not there may have no memory)
     if (int rc = check_turns("rope_rows", positions, inv_freq, rotary_dim, head_dim, magnitude)) return rc;
     RopeParams p{{positions, inv_freq, rotary_dim / 2, magnitude, transposed ? -magnitude : magnitude}, {q, q_out, q_stride, q_out_stride, Hq}, {k, k_out, k_stride, k_out_stride, Hkv}, n, head_dim, 1};
@@ -340,7 +341,7 @@ extern "C" int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, 
                                      int64_t v_stride, int n, int Hkv, const int32_t* positions, const float* inv_freq, int rotary_dim, int interleaved,
                                      float magnitude, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, void* stream) {
     CPMCU_CHECK_ARG(num_pages >= 1 && num_pages <= INT32_MAX / kPage, "kv_append_slots: num_pages=%d outside [1, %d]", num_pages, INT32_MAX / kPage);
-    CPMCU_CHECK_ARG(n >= 0 && Hkv >= 1 && Hkv <= kMaxHeads, "kv_append_slots: n=%d Hkv=%d", n, Hkv);
+    CPMCU_CHECK_ARG(n >= 0 && Hkv >= 1 && Hkv <= kMaxHeads && n < kMaxRows && (int64_t)n * Hkv < kMaxRows * 8, "kv_append_slots: n=%d Hkv=%d", n, Hkv);
     if (n == 0) return CPMCU_OK;  // (rows that are not there may have no memory)
     CPMCU_CHECK_ARG(k_pool && v_pool && slots && k && v, "kv_append_slots: null pointer argument");
     const bool rope = positions != nullptr || inv_freq != nullptr;

@@ -193,7 +193,7 @@ def rope_frequencies(rotary_dim, base=10000.0, scaling=None, length=None):
 def rope_rows(q, k, positions, inv_freq, interleaved=False, magnitude=1.0, transposed=False, q_out=None, k_out=None):
     """Rotary positions of q [n, Hq, D] and k [n, Hkv, D] (or None): (q_out, k_out), new tensors unless given (q and k themselves: in place).
 
-    positions int32 [n] (rows of a negative one are left out), inv_freq fp32 [rotary_dim / 2] (see rope_frequencies): the first rotary_dim
+    positions int32 [n] (rows of a negative one are left out: a new tensor has no values there), inv_freq fp32 [rotary_dim / 2] (see rope_frequencies): the first rotary_dim
     values of each head turn, in pairs (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1).  Rows may be views of wider ones (a fused
     projection's output).  transposed: gradients of the results back to q and k.
     """
@@ -222,7 +222,7 @@ def kv_append_slots(cache, layer, k, v, slots, q=None, q_out=None, positions=Non
     """Rows k, v [n, Hkv, 128] of several requests to slots[t] = page * 256 + place of the cache (rows without a slot: left out).
 
     With positions and inv_freq, as rope_rows takes them, k is rotated on its way, and q [n, Hq, 128] (if given) into q_out, which is
-    returned; rows left out keep what q_out held."""
+    returned; rows left out keep what q_out held (a new tensor has no values there)."""
     if q is not None and q_out is None:
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     (_native or _calls()).kv_append_slots(cache.k[layer], cache.v[layer], k, v, slots, q, q_out, positions, inv_freq, 1 if interleaved else 0, magnitude)
@@ -273,6 +273,7 @@ class Int8Weight:
     def __init__(self, w, scales):
         """w int8 [V, K], scales fp32 [V]: the weight of channel c is w[c] * scales[c]."""
         assert w.dtype == torch.int8 and w.dim() == 2 and scales.dtype == torch.float32 and scales.numel() == w.shape[0]
+        assert w.is_cuda and w.device == scales.device and w.device.index == torch.cuda.current_device(), "weights and scales on the current device required"
         self.V, self.K = w.shape
         self.shape = (self.V, self.K)
         self.scales = scales.contiguous()

@@ -676,7 +676,7 @@ int cpmcu_batch_tables(const int32_t* kv_lens, const int32_t* new_lens, int num_
  *   inv_freq float[half]: with whatever scaling the model's long contexts have (see ops.rope_frequencies);
  *   transposed: the transposed matrix, that takes gradients of the results back to the inputs (with m = 1 the inverse);
  *   q [n][q_stride], heads of head_dim values one after the other from the row's start; q_out likewise, the same memory and stride (in
- *       place) or memory apart; k alike; Hq or Hkv may be 0.  head_dim even, up to 256; rotary_dim even.  Rows on 16 bytes with
+ *       place) or memory apart, from k too; k alike; Hq or Hkv may be 0.  n < 2^24.  head_dim even, up to 256; rotary_dim even.  Rows on 16 bytes with
  *       rotary_dim and head_dim multiples of 16 are read and written in 16-byte pieces, others value by value. */
 int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, int rotary_dim, int interleaved, float magnitude, int transposed,
                     const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, const void* k, int64_t k_stride, void* k_out,
@@ -684,6 +684,7 @@ int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, int rotary_
 
 /* The K and V rows of several requests into the paged cache of a layer, row t of [n] to slots[t] = page * 256 + place in the page (as
  * cpmcu_batch_tables writes them; no slot twice).  Rows whose slot is negative or lies behind num_pages are left out whole.
+ * n < 2^24, n * Hkv < 2^27.
  *   k, v [n][stride], Hkv heads of 128 values from the row's start; rows and pools on 16 bytes.
  *   positions, inv_freq (or both NULL): K is rotated on its way as by cpmcu_rope_rows, and so are the Hq heads of q into q_out (Hq
  *       may be 0); rotary_dim a multiple of 16; rows of a negative position are left out as well. */
@@ -693,14 +694,14 @@ int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, const int32
 
 /* Rows of 16-bit floats to 8 bits with a scale for each row: scales[t] = max |x| / 127, xq[t][k] = rint(127 x / max |x|) (ties to even,
  * the quotient as if exact).  An empty (all zero) row has scale 0 and zeros, a row with an infinity or NaN scale NaN and zeros.
- *   x [n][x_stride], K <= 131071 values from the row's start; xq [n][K rounded up to 64], zeros behind column K, on 16 bytes. */
+ *   x [n][x_stride], n < 2^24, K <= 131071 values from the row's start; xq [n][K rounded up to 64], zeros behind column K, on 16 bytes. */
 int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K, int8_t* xq, float* scales, void* stream);
 /* 8-bit weights [V][K], row-major, in matrix-operand order [ceil(V/16)][ceil(K/64)][64 lanes][16 bytes]: once, at load time. */
 size_t cpmcu_int8_weight_bytes(int V, int K);
 int cpmcu_int8_weight_tile(const int8_t* w, int V, int K, int8_t* w_tiled, void* stream);
 /* out[t][c] = (sum over k of xq[t][k] w[c][k]) * (x_scales[t] * w_scales[c]), [n][V] in the element type: the sum exact in 32-bit
  * integers, one rounding to float, one product, one rounding to the element type.  xq as cpmcu_quantize_rows leaves it (what lies
- * behind column K does not matter), w_tiled as cpmcu_int8_weight_tile does.  K <= 131071. */
+ * behind column K does not matter), w_tiled as cpmcu_int8_weight_tile does; out apart from the inputs.  K <= 131071. */
 int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_tiled, const float* w_scales, int n, int V, int K, void* out,
                       void* stream);
 /* The kernel a cpmcu_int8_linear call of this shape launches and its workgroup count, without launching (the outputs may be NULL). */

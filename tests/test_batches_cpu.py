@@ -91,6 +91,35 @@ def test_int8_operators_refuse():
     assert L.raw.cpmcu_int8_weight_bytes(17, 65) == 2 * 2 * 1024 and L.raw.cpmcu_int8_weight_bytes(0, 65) == 0
 
 
+def test_sizes_beyond_a_launch_are_refused():
+    """Before any grid is made of them: rows, channels and their products up to the largest 32-bit numbers."""
+    L, I = _lib(), 2 ** 31 - 1
+    for n in (1 << 24, I - 3, I):
+        with pytest.raises(ValueError, match="rope_rows: n="):
+            _rope(n=n)
+        with pytest.raises(ValueError, match="kv_append_slots: n="):
+            _append(n=n)
+        with pytest.raises(ValueError, match="quantize_rows: n="):
+            L.quantize_rows(A, 64, n, 64, B, C, None)
+    with pytest.raises(ValueError, match="kv_append_slots: n="):
+        _append(n=(1 << 24) - 1, hkv=16, ks=2048, vs=2048)
+    for n, V in ((I, 16), (16, I), ((1 << 30) + 1, 16), (16, (1 << 30) + 1), (1 << 30, 1 << 30), (1 << 24, 1 << 24)):
+        with pytest.raises(ValueError, match="int8_linear: n="):
+            L.int8_linear(A, B, C, D, n, V, 64, E, None)
+    for V in (I, (1 << 30) + 1):
+        with pytest.raises(ValueError, match="int8_weight_tile"):
+            L.int8_weight_tile(A, V, 64, B, None)
+        assert L.raw.cpmcu_int8_weight_bytes(V, 64) == 0
+    assert L.raw.cpmcu_int8_weight_bytes(16, 131072) == 0
+
+
+def test_weights_are_on_the_current_device():
+    import torch
+    from cpm.cu_amd import ops
+    with pytest.raises(AssertionError, match="current device required"):
+        ops.Int8Weight(torch.zeros((16, 64), dtype=torch.int8), torch.zeros(16))
+
+
 def test_int8_linear_plans():
     """Every shape of the kernel is somebody's, from one row to many."""
     from cpm.cu_amd import lib, ops
