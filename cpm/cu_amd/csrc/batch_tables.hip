@@ -54,8 +54,8 @@ __device__ inline int wave_totals(int v, int cap) {
 // requests' single rows is the round trip for their lengths, one exchange of totals, and the round trip for their pages.
 // A wave looks up RUNS runs of 64 rows at once: the requests of their first rows with the whole wave in two reads of LDS, and each row's by
 // halving what lies between, which is nothing where requests have many rows.  One run where a workgroup per CU covers all rows, four beyond
-// (the runs' round trips overlap).  4096 requests' single rows 9.4 us with one run and 11.7 with four, a million rows of 4096 requests
-// 21.6 and 17.1.  1.1 million rows of 1000 requests: 11.8 us, of which 8.8 MB written are 1.8; the totals take 6, the round trips behind
+// (the runs' round trips overlap).  4096 requests' single rows 9.0 us with one run and 11.3 with four, a million rows of 4096 requests
+// 21.2 and 16.8.  1.1 million rows of 1000 requests: 11.8 us, of which 8.8 MB written are 1.8; the totals take 5, the round trips behind
 // them (row to request, to page, to slot) the rest.
 template <int THREADS, int EACH, int RUNS>
 __global__ __launch_bounds__(THREADS) void batch_tables_kernel(TableParams p) {
@@ -105,10 +105,16 @@ __global__ __launch_bounds__(THREADS) void batch_tables_kernel(TableParams p) {
             if (k < from || k >= to) continue;
             const int cap = k == 0 ? row_cap : INT32_MAX;
             int before = 0, sum = 0;
+            if constexpr (kWaves > 4) {  // (16 totals one after the other take 0.5 us, the running totals over lanes again 0.2)
+                const int upto = wave_totals(lane < kWaves ? wave_total[k][lane] : 0, cap);
+                sum = __builtin_amdgcn_readlane(upto, kWaves - 1);
+                if (wave > 0) before = __builtin_amdgcn_readlane(upto, __builtin_amdgcn_readfirstlane(wave - 1));
+            } else {
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                if (w == wave) before = sum;
-                sum = min(sum + wave_total[k][w], cap);
+                for (int w = 0; w < kWaves; ++w) {
+                    if (w == wave) before = sum;
+                    sum = min(sum + wave_total[k][w], cap);
+                }
             }
             mine[k] = min(before + mine[k], cap);
             all[k] = sum;
