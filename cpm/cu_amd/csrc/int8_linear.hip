@@ -488,7 +488,7 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_ke
 
 // The shapes, and what one of their tiles costs, as measured over 1 to 8192 rows, 512 to 73448 channels and 512 to 16384 columns: `start` us
 // of a launch, for a round (a tile on every CU) `round` us and `step` more for every 64 columns, `busy` more of them where all CUs work.  The choice is the
-// shape with the least cost; it is within 10 % of the best one over that range (60 x 4096 x 16384: 32 x 128 14.5 us, 32 x 64 split 33.9, 64 x 128
+// shape with the least cost; it is within 11 % of the best one over that range (60 x 4096 x 16384: 32 x 128 14.5 us, 32 x 64 split 33.9, 64 x 128
 // 18.1; 333 x 4099 x 12289: 128 x 256 28.5, 64 x 128 34.8, 64 x 256 36.6, 256 x 256 48.9; 2048 x 4096 x 16384: 256 x 256 125, 128 x 256 151, 64 x 256 167).
 struct Variant {
     const char* name;
@@ -496,7 +496,7 @@ struct Variant {
     void (*bf16_kernel)(LinearParams);
     int rows, channels, threads;
     float start, round, step, busy;
-    bool shared;  // workgroups share a CU: rounds need not be whole
+    bool shared;  // a round with CUs to spare costs less
 };
 #define CPMCU_SPLIT(nx, nv, u) "int8_linear_split_kernel<" #nx "," #nv ">", int8_linear_split_kernel<f16, nx, nv, u>, int8_linear_split_kernel<bf16, nx, nv, u>, 16 * nx, kBlock* nv, 64 * kSplit
 #define CPMCU_TILE(nx, nv, wx, wv, ahead)                                                                                                                   \
@@ -521,7 +521,7 @@ int choose_variant(int n, int V, int K) {
     for (int i = 0; i < kInt8LinearShapes; ++i) {
         const Variant& v = kVariants[i];
         const float tiles = (float)ceil_div(n, v.rows) * (float)ceil_div(V, v.channels) / kCus;
-        const float rounds = v.shared ? std::max(tiles, 0.5f) : std::ceil(tiles);
+        const float rounds = v.shared && tiles < 1.f ? std::max(tiles, 0.5f) : std::ceil(tiles);
         float step = v.step + v.busy * std::min(tiles, 1.f);
         if (v.shared && n < 16) step -= 0.016f * (float)(16 - n) / 16.f;  // (rows that are not there take no way from L2)
         const float cost = v.start + rounds * (v.round + (float)steps * step), floor = (float)V * (float)K / 6e6f;  // (weights at 6 TB/s)
