@@ -151,6 +151,12 @@ __device__ inline void tile_of(const LinearParams& p, int block, int* tx, int* t
     *tv = in_band / rows;
 }
 
+// Rows are requested so that four lanes take 64 neighbouring bytes: requests whose neighbouring lanes are in different rows, as the operands are, reach
+// 38 to 51 GB/s a CU from L2, and 110 to 150 this way.  LDS puts the operands together: row r of a block has piece c of a step's four in place c ^ turned(r), so that
+// the rows that are read at once lie in different banks.
+__device__ inline int turned(int r) { return ((r >> 1 & 1) << 1) ^ (r >> 2 & 3); }
+__device__ inline int operand_place(int lane) { return (lane & 15) * 4 + ((lane >> 4) ^ turned(lane & 15)); }  // in 16-byte places
+
 // Channels c .. c + 3 of row t.
 template <typename E>
 __device__ inline void store_quad(const LinearParams& p, int t, int c, i32x4 sum) {
@@ -171,20 +177,25 @@ __device__ inline void store_quad(const LinearParams& p, int t, int c, i32x4 sum
 
 // NX blocks of rows and NV blocks of channels per workgroup, for few rows: the weights are the bytes, each is read by one workgroup, and the
 // waves take K's steps in turn, so that a workgroup's requests are whole kilobytes one behind the other.  A wave requests U steps at once
-// while it works on the U before them; the waves' sums meet in LDS.
+// while it works on the U before them; rows go through LDS for the operands' order (17 rows of 4096 columns to 4608 channels 7.6 us, 9.5 requested in
+// that order); the waves' sums meet in LDS.  One row: 5.9 us, 18.9 MB.
 constexpr int kSplit = 8;
 
 template <typename E, int NX, int NV, int U>
 __global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearParams p) {
     constexpr int kQuads = NX * NV;
-    __shared__ i32x4 part[kSplit / 2][kQuads][64];
+    __shared__ union {
+        i32x4 part[kSplit / 2][kQuads][64];
+        i32x4 rows[kSplit][U][NX][64];
+    } lds;
+    auto& part = lds.part;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tx, tv;
     tile_of(p, blockIdx.x, &tx, &tv);
     const int t0 = tx * NX * 16, b0 = tv * NV, last = p.steps - 1;
     const int8_t *x[NX], *w[NV];
 #pragma unroll
-    for (int b = 0; b < NX; ++b) x[b] = p.xq + (size_t)min(t0 + b * 16 + (lane & 15), p.n - 1) * p.steps * kStep + (lane >> 4) * 16;
+    for (int b = 0; b < NX; ++b) x[b] = p.xq + (size_t)min(t0 + b * 16 + (lane >> 2), p.n - 1) * p.steps * kStep + ((lane & 3) ^ turned(lane >> 2)) * 16;
 #pragma unroll
     for (int v = 0; v < NV; ++v) w[v] = p.w + (size_t)min(b0 + v, p.blocks - 1) * p.steps * kTile + lane * 16;
     struct Group {
@@ -202,13 +213,20 @@ __global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearPa
     };
     i32x4 acc[NX][NV] = {};
     const auto multiply = [&](int s, const Group& g) {
+        i32x4(&rows)[U][NX][64] = lds.rows[wave];  // (one wave's own: no barrier)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int b = 0; b < NX; ++b) rows[u][b][lane] = g.x[u][b];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (s + u * kSplit > last) break;  // (the same for the whole wave)
 #pragma unroll
-            for (int b = 0; b < NX; ++b)
+            for (int b = 0; b < NX; ++b) {
+                const i32x4 r = rows[u][b][operand_place(lane)];
 #pragma unroll
-                for (int v = 0; v < NV; ++v) acc[b][v] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.a[u][v], g.x[u][b], acc[b][v], 0, 0, 0);
+                for (int v = 0; v < NV; ++v) acc[b][v] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.a[u][v], r, acc[b][v], 0, 0, 0);
+            }
         }
     };
     constexpr int kTurn = U * kSplit;
@@ -221,6 +239,7 @@ __global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearPa
         if (s + 2 * kTurn <= last) load(s + 2 * kTurn, g0);
         multiply(s + kTurn, g1);
     }
+    __syncthreads();  // (the sums lie where rows were)
     // eight sums to four to two to one
 #pragma unroll
     for (int half = kSplit / 2; half; half >>= 1) {
@@ -279,10 +298,10 @@ __device__ inline void store_tile(const LinearParams& p, int t0, int c0, i32x4 (
         }
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // (one wave's own: no barrier)
 #pragma unroll
-        for (int i = 0; i < kPass * 16 * kPieces / 64; ++i) {
+        for (int i = 0; i < (kPass * 16 * kPieces + 63) / 64; ++i) {
             const int r = i * (64 / kPieces) + lane / kPieces, piece = lane % kPieces, t = t1 + r, c = c0 + piece * 8;
             const uint4 y = *reinterpret_cast<const uint4*>(part + r * (kPieces * 16) + (piece ^ (r & (kPieces - 1))) * 16);
-            if (t >= p.n || c >= p.V) continue;
+            if (r >= kPass * 16 || t >= p.n || c >= p.V) continue;
             uint16_t* to = (uint16_t*)p.out + (size_t)t * p.V + c;
             if (c + 8 <= p.V) {
                 __builtin_nontemporal_store(Piece{y.x, y.y, y.z, y.w}, reinterpret_cast<Piece*>(to));
@@ -297,51 +316,59 @@ __device__ inline void store_tile(const LinearParams& p, int t0, int c0, i32x4 (
     }
 }
 
-// Tiles of (WX NX) x (WV NV) blocks for more rows: WX x WV waves, each with NX x NV of the blocks in its accumulators.
-// Rows go to LDS by direct loads, two steps at a time, so that a request takes whole 128-byte lines, eight rows of them; the eight rows of a
-// 16-byte column lie side by side, which is how the operands are read back, without bank conflicts.  Weights lie
+// Tiles of (WX NX) x (WV NV) blocks for more rows: WX x WV waves, each with NX x NV of the blocks in its accumulators, and KS such groups, each with
+// a share of K: a second group hides the first one's waits where a CU has one tile (256 rows of 4096 columns to 4608 channels 12.6 us, 14.9 with one
+// group, 17.7 with one and requests in the operands' order).
+// Rows go to LDS by direct loads, two steps at a time, eight rows of whole 128-byte lines a request; row r has piece c of a line's eight in place
+// c ^ (r % 8), so that the operands are read back without bank conflicts.  Weights lie
 // in operand order already and go straight into registers, AHEAD pairs of steps in advance, so that LDS is read for the rows alone.
 // Half of a step's rows are read from LDS while the other half is multiplied, so the next pair's have to be there a pair early: its
 // rows are requested in front of the weights of two pairs before.  Requests return in order, and the wait for the weights of pair j, which the
 // compiler puts in front of their first use, is one for the rows of pair j + 2 as well; the one in front of the barrier says so.
-template <typename E, int NX, int NV, int WX, int WV, int AHEAD>
-__global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_tile_kernel(LinearParams p) {
+template <typename E, int NX, int NV, int WX, int WV, int AHEAD, int KS>
+__global__ __launch_bounds__(64 * WX * WV * KS, WX * WV * KS / 4) void int8_linear_tile_kernel(LinearParams p) {
     constexpr int kWaves = WX * WV, kBlocks = WX * NX, kLoads = 2 * kBlocks / kWaves, kStages = AHEAD + 3, kHalf = NX / 2, kSets = 2 * (AHEAD + 1);
+    static_assert(KS == 1 || (KS == 2 && kHalf * NV * 1024 <= kStages * kLoads * kTile), "the groups' sums have room in the ring");
     static_assert(2 * kBlocks % kWaves == 0 && NX % 2 == 0, "every wave requests as many kilobytes of rows");
     constexpr int kStageBytes = kBlocks * 2 * kTile;
-    __shared__ __attribute__((aligned(16))) int8_t ring[kStages * kStageBytes];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wx = wave / WV, wv = wave % WV;
+    __shared__ __attribute__((aligned(16))) int8_t ring[KS * kStages * kStageBytes];
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = all / kWaves, wave = all % kWaves, wx = wave / WV, wv = wave % WV;
     int tx, tv;
     tile_of(p, blockIdx.x, &tx, &tv);
-    const int t0 = tx * kBlocks * 16, b0 = (tv * WV + wv) * NV, last = p.steps - 1, last_pair = last / 2, pairs = p.steps / 2;  // (whole pairs)
+    const int t0 = tx * kBlocks * 16, b0 = (tv * WV + wv) * NV, last_pair = (p.steps - 1) / 2;
+    // this group's pairs of steps: [first, end), of which `pairs` are whole
+    const int per = last_pair / KS + 1, first = min(group * per, last_pair), end = min(group * per + per, last_pair + 1), pairs = max(min(end, p.steps / 2) - group * per, 0);
+    const bool odd = (p.steps & 1) && group * per <= last_pair && end == last_pair + 1;
     // (an uneven last step: its pair takes the columns of the one step twice, and only the first is multiplied)
-    const uint32_t no_second = (p.steps & 1) && lane >= 32 ? kStep : 0;
+    const uint32_t piece = (lane & 7) ^ (lane >> 3), no_second = (p.steps & 1) && piece >= 4 ? kStep : 0;
     const int8_t* x_tile = p.xq + (size_t)t0 * p.steps * kStep;
     uint32_t row[kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) row[j] = (uint32_t)(min((wave * kLoads + j) * 8 + (lane & 7), p.n - 1 - t0) * p.steps * kStep + (lane >> 3) * 16);
+    for (int j = 0; j < kLoads; ++j) row[j] = (uint32_t)(min((wave * kLoads + j) * 8 + (lane >> 3), p.n - 1 - t0) * p.steps * kStep) + piece * 16;
     const int8_t* w[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) w[v] = p.w + (size_t)min(b0 + v, p.blocks - 1) * p.steps * kTile;
-    const uint32_t lane16 = lane * 16, ring_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)ring + wave * (kLoads * kTile);
+    const uint32_t lane16 = lane * 16, ring_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)ring + group * (kStages * kStageBytes) + wave * (kLoads * kTile);
     const auto request = [&](int pair, int stage) {
-        const int8_t* from = x_tile + (size_t)min(pair, last_pair) * (2 * kStep);
-        const uint32_t back = pair >= last_pair ? no_second : 0;
+        const int at = min(first + pair, max(end - 1, first));
+        const int8_t* from = x_tile + (size_t)at * (2 * kStep);
+        const uint32_t back = at == last_pair ? no_second : 0;
 #pragma unroll
         for (int j = 0; j < kLoads; ++j)
             asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(row[j] - back), "s"(from), "s"(ring_at + stage * kStageBytes + j * kTile) : "memory", "m0");
     };
     const auto weights = [&](int s, i32x4* a) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) a[v] = *reinterpret_cast<const i32x4*>(w[v] + (size_t)min(s, last) * kTile + lane16);
+        for (int v = 0; v < NV; ++v) a[v] = *reinterpret_cast<const i32x4*>(w[v] + (size_t)min(2 * first + s, min(max(2 * end, 2 * first + 1), p.steps) - 1) * kTile + lane16);
     };
     i32x4 acc[NX][NV] = {}, x0[kHalf], x1[kHalf];
-    const int8_t* mine = ring + wx * (NX * 2 * kTile) + ((lane & 15) >> 3) * kTile + (lane & 7) * 16 + (lane >> 4) * 128;
+    const int8_t* mine = ring + group * (kStages * kStageBytes) + wx * (NX * 2 * kTile) + ((lane & 15) >> 3) * kTile + (lane & 7) * 128;
+    const int at[2] = {((lane >> 4) ^ (lane & 7)) * 16, ((4 + (lane >> 4)) ^ (lane & 7)) * 16};
     // The order below is kept: what is read comes ahead of the products that hide its way.
     const auto read = [&](int stage, int second, int half, i32x4* x) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < kHalf; ++b) x[b] = *reinterpret_cast<const i32x4*>(mine + stage * kStageBytes + (half * kHalf + b) * (2 * kTile) + second * 512);
+        for (int b = 0; b < kHalf; ++b) x[b] = *reinterpret_cast<const i32x4*>(mine + stage * kStageBytes + (half * kHalf + b) * (2 * kTile) + at[second]);
         __builtin_amdgcn_sched_barrier(0);
     };
     const auto multiply = [&](const i32x4* a, const i32x4* x, int half) {
@@ -390,7 +417,10 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_tile_ke
             }
         }
     }
-    if (p.steps & 1) {
+    if constexpr (KS > 1) {  // (a barrier for every pair of the group that has most)
+        for (int j = pairs; j < min(per, p.steps / 2); ++j) __builtin_amdgcn_s_barrier();
+    }
+    if (odd) {
         read(stage, 0, 1, x1);
 #pragma unroll
         for (int u = 0; u <= AHEAD; ++u)
@@ -401,14 +431,33 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_tile_ke
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (requests beyond the last pair write to LDS, too)
     __syncthreads();
-    store_tile<E, NX, NV, kStages * kLoads * kTile>(p, t0 + wx * NX * 16, b0 * kBlock, acc, ring + wave * (kStages * kLoads * kTile));
+    if constexpr (KS == 1) {
+        store_tile<E, NX, NV, kStages * kLoads * kTile>(p, t0 + wx * NX * 16, b0 * kBlock, acc, ring + wave * (kStages * kLoads * kTile));
+    } else {  // each group takes half of the rows, and gives the sums of the others
+        i32x4 half[kHalf][NV];
+        i32x4* given = reinterpret_cast<i32x4*>(ring) + all * (kHalf * NV * 64) + lane;
+        const i32x4* taken = reinterpret_cast<const i32x4*>(ring) + ((1 - group) * kWaves + wave) * (kHalf * NV * 64) + lane;
+#pragma unroll
+        for (int b = 0; b < kHalf; ++b)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                given[(b * NV + v) * 64] = group == 0 ? acc[kHalf + b][v] : acc[b][v];
+                half[b][v] = group == 0 ? acc[b][v] : acc[kHalf + b][v];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < kHalf; ++b)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) half[b][v] += taken[(b * NV + v) * 64];
+        __syncthreads();
+        store_tile<E, kHalf, NV, kStages * kLoads * kTile>(p, t0 + (wx * NX + group * kHalf) * 16, b0 * kBlock, half, ring + all * (kStages * kLoads * kTile));
+    }
 }
 
-// Larger tiles for many rows.  What crosses from L2 bounds the tiles above (50 to 60 GB/s a CU, 17 TB/s in all), and with waves that share channels
-// each weight crosses once for every one of them; here rows and weights are both in LDS and a CU takes each once.  A step is requested three in
-// advance and has to be there one early, as above.  A CU with 256 x 256 to do takes 0.61 us a step where few CUs run and 0.85 to 0.95 where all
-// do: 2535 TOP/s at 8192 x 16384 x 4096 (rows, columns, channels), 10 % more on zeros, which draw less power; deeper rings and other orders
-// of the tiles change nothing.
+// Larger tiles for many rows.  With waves that share channels each weight crosses from L2 once for every one of them; here rows and weights are both in
+// LDS and a CU takes each once.  A step is requested three in advance and has to be there one early, as above.  A CU with 256 x 256 to do takes
+// 0.6 us a step where few CUs run and 0.8 to 0.9 where all do, of which the matrix cores need 0.43 at their peak: 2260 TOP/s at 8192 x 4096 x 16384 (rows,
+// columns, channels), 2510 at 8192 x 16384 x 4096, 10 % more on zeros, which draw less power; deeper rings and other orders of the tiles change nothing.
 template <typename E, int NX, int NV, int WX, int WV>
 __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_kernel(LinearParams p) {
     constexpr int kWaves = WX * WV, kRows = WX * NX, kChannels = WV * NV, kStages = 4, kStageBytes = (kRows + kChannels) * kTile, kHalf = NX / 2;
@@ -422,7 +471,7 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_ke
     uint32_t row[kX];
     const int8_t* w[kW];
 #pragma unroll
-    for (int j = 0; j < kX; ++j) row[j] = (uint32_t)(min((wave * kX + j) * 16 + (lane & 15), p.n - 1 - t0) * p.steps * kStep + (lane >> 4) * 16);
+    for (int j = 0; j < kX; ++j) row[j] = (uint32_t)(min((wave * kX + j) * 16 + (lane >> 2), p.n - 1 - t0) * p.steps * kStep) + ((lane & 3) ^ turned(lane >> 2)) * 16;
 #pragma unroll
     for (int j = 0; j < kW; ++j) w[j] = p.w + (size_t)min(tv * kChannels + wave * kW + j, p.blocks - 1) * p.steps * kTile;
     const uint32_t lane16 = lane * 16, ring_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)ring;
@@ -437,7 +486,7 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_ke
             asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane16), "s"(w[j] + at * kTile), "s"(to + (kRows + wave * kW + j) * kTile) : "memory", "m0");
     };
     i32x4 acc[NX][NV] = {}, x0[kHalf], x1[kHalf], a0[NV], a1[NV];
-    const int8_t* x_at = ring + wx * (NX * kTile) + lane16;
+    const int8_t* x_at = ring + wx * (NX * kTile) + operand_place(lane) * 16;
     const int8_t* w_at = ring + (kRows + wv * NV) * kTile + lane16;
     const auto read_x = [&](int stage, int half, i32x4* x) {
 #pragma unroll
@@ -486,29 +535,31 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_ke
     store_tile<E, NX, NV, kRoom>(p, t0 + wx * NX * 16, (tv * kChannels + wv * NV) * kBlock, acc, ring + wave * kRoom);
 }
 
-// The shapes, and what one of their tiles costs, as measured over 1 to 8192 rows, 512 to 73448 channels and 512 to 16384 columns: `start` us
-// of a launch, for a round (a tile on every CU) `round` us and `step` more for every 64 columns, `busy` more of them where all CUs work.  The choice is the
-// shape with the least cost; it is within 11 % of the best one over that range (60 x 4096 x 16384: 32 x 128 14.5 us, 32 x 64 split 33.9, 64 x 128
-// 18.1; 333 x 4099 x 12289: 128 x 256 28.5, 64 x 128 34.8, 64 x 256 36.6, 256 x 256 48.9; 2048 x 4096 x 16384: 256 x 256 125, 128 x 256 151, 64 x 256 167).
+// The shapes, and what they cost, fitted to 448 sizes of 1 to 8192 rows, 512 to 73448 channels and 512 to 16384 columns: `start` us of a launch; for a
+// round (a tile on every CU) `round` us and `step` more for every 64 columns, `busy` more of them where all CUs work; and `whole` says how much of a
+// last round that is not full counts as a full one.  The choice is the shape with the least cost, 0.3 % above the best of them in the mean and 11 % at
+// most (in us, rows x columns x channels: 1 x 4096 x 4608 16 x 16 split 5.9, 16 x 32 split 6.0, 32 x 64 7.7; 64 x 4096 x 16384 32 x 64 13.7, 64 x 64 14.2, 16 x 32
+// split 26.2; 256 x 4096 x 4608 64 x 128 12.6, 32 x 64 16.2, 64 x 256 19.3; 333 x 4099 x 12289 128 x 256 27.5, 64 x 128 34.3, 64 x 256 34.9, 256 x 256 45.6;
+// 2048 x 4096 x 16384: 256 x 256 120, 128 x 256 133, 64 x 256 142).
 struct Variant {
     const char* name;
     void (*f16_kernel)(LinearParams);
     void (*bf16_kernel)(LinearParams);
     int rows, channels, threads;
-    float start, round, step, busy;
-    bool shared;  // a round with CUs to spare costs less
+    float start, round, step, busy, whole;
 };
 #define CPMCU_SPLIT(nx, nv, u) "int8_linear_split_kernel<" #nx "," #nv ">", int8_linear_split_kernel<f16, nx, nv, u>, int8_linear_split_kernel<bf16, nx, nv, u>, 16 * nx, kBlock* nv, 64 * kSplit
-#define CPMCU_TILE(nx, nv, wx, wv, ahead)                                                                                                                   \
-    "int8_linear_tile_kernel<" #nx "," #nv "," #wx "," #wv ">", int8_linear_tile_kernel<f16, nx, nv, wx, wv, ahead>, int8_linear_tile_kernel<bf16, nx, nv, wx, wv, ahead>, \
-        16 * nx * wx, kBlock* nv* wv, 64 * wx * wv
+#define CPMCU_TILE(nx, nv, wx, wv, ahead, ks)                                                                                                                   \
+    "int8_linear_tile_kernel<" #nx "," #nv "," #wx "," #wv "," #ks ">", int8_linear_tile_kernel<f16, nx, nv, wx, wv, ahead, ks>, \
+        int8_linear_tile_kernel<bf16, nx, nv, wx, wv, ahead, ks>, 16 * nx * wx, kBlock* nv* wv, 64 * wx * wv * ks
 #define CPMCU_WIDE(nx, nv, wx, wv)                                                                                                                     \
     "int8_linear_wide_kernel<" #nx "," #nv "," #wx "," #wv ">", int8_linear_wide_kernel<f16, nx, nv, wx, wv>, int8_linear_wide_kernel<bf16, nx, nv, wx, wv>, \
         16 * nx * wx, kBlock* nv* wv, 64 * wx * wv
 const Variant kVariants[kInt8LinearShapes] = {
-    {CPMCU_SPLIT(1, 2, 4), 4.f, 0.8f, 0.042f, 0.f, true},   {CPMCU_SPLIT(2, 2, 4), 5.f, 0.f, 0.065f, 0.f, false},  {CPMCU_SPLIT(2, 4, 2), 5.6f, 0.f, 0.09f, 0.f, false},
-    {CPMCU_TILE(2, 2, 1, 4, 4), 3.2f, 0.f, 0.148f, 0.f, false}, {CPMCU_TILE(4, 2, 1, 4, 3), 4.5f, 0.f, 0.205f, 0.f, false}, {CPMCU_TILE(4, 4, 1, 4, 2), 4.5f, 0.f, 0.28f, 0.03f, false},
-    {CPMCU_WIDE(4, 4, 2, 4), 5.f, 0.f, 0.345f, 0.17f, false}, {CPMCU_WIDE(8, 4, 2, 4), 5.f, 0.f, 0.61f, 0.3f, false}};
+    {CPMCU_SPLIT(1, 1, 4), 2.8f, 0.36f, 0.0057f, 0.017f, 0.3f},        {CPMCU_SPLIT(1, 2, 4), 2.9f, 0.83f, 0.0319f, 0.0032f, 0.1f},
+    {CPMCU_TILE(2, 1, 1, 4, 3, 2), 2.6f, 0.84f, 0.0785f, 0.f, 0.4f},   {CPMCU_TILE(4, 1, 1, 4, 5, 2), 1.f, 2.84f, 0.0769f, 0.046f, 0.7f},
+    {CPMCU_TILE(4, 2, 1, 4, 2, 2), 2.2f, 1.6f, 0.116f, 0.044f, 0.6f},  {CPMCU_TILE(4, 4, 1, 4, 2, 1), 3.5f, 0.92f, 0.222f, 0.081f, 0.5f},
+    {CPMCU_WIDE(4, 4, 2, 4), 1.f, 3.72f, 0.272f, 0.2f, 1.f},           {CPMCU_WIDE(8, 4, 2, 4), 3.7f, 3.7f, 0.431f, 0.38f, 0.8f}};
 #undef CPMCU_SPLIT
 #undef CPMCU_TILE
 #undef CPMCU_WIDE
@@ -521,10 +572,9 @@ int choose_variant(int n, int V, int K) {
     for (int i = 0; i < kInt8LinearShapes; ++i) {
         const Variant& v = kVariants[i];
         const float tiles = (float)ceil_div(n, v.rows) * (float)ceil_div(V, v.channels) / kCus;
-        const float rounds = v.shared && tiles < 1.f ? std::max(tiles, 0.5f) : std::ceil(tiles);
-        float step = v.step + v.busy * std::min(tiles, 1.f);
-        if (v.shared && n < 16) step -= 0.016f * (float)(16 - n) / 16.f;  // (rows that are not there take no way from L2)
-        const float cost = v.start + rounds * (v.round + (float)steps * step), floor = (float)V * (float)K / 6e6f;  // (weights at 6 TB/s)
+        const float rounds = tiles <= 1.f ? 1.f : v.whole * std::ceil(tiles) + (1.f - v.whole) * tiles;
+        const float cost = v.start + rounds * (v.round + (float)steps * (v.step + v.busy * std::min(tiles, 1.f)));
+        const float floor = (float)V * (float)K / 6e6f;  // (weights at 6 TB/s)
         const float total = std::max(cost, floor) + 0.1f * cost;
         if (i == 0 || total < least) {
             best = i;
