@@ -177,18 +177,17 @@ __device__ inline void store_quad(const LinearParams& p, int t, int c, i32x4 sum
 
 // NX blocks of rows and NV blocks of channels per workgroup, for few rows: the weights are the bytes, each is read by one workgroup, and the
 // waves take K's steps in turn, so that a workgroup's requests are whole kilobytes one behind the other.  A wave requests U steps at once
-// while it works on the U before them; rows go through LDS for the operands' order (17 rows of 4096 columns to 4608 channels 7.6 us, 9.5 requested in
-// that order); the waves' sums meet in LDS.  One row: 5.9 us, 18.9 MB.
+// while it works on the U before them; rows go through LDS for the operands' order (which spares 1.8 of 9.5 us at 17 rows of
+// 4096 columns to 4608 channels); the waves' sums meet in LDS, where a wave adds up each block's (0.4 us less than halving the waves).  One row: 5.6 us.
 constexpr int kSplit = 8;
 
 template <typename E, int NX, int NV, int U>
 __global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearParams p) {
     constexpr int kQuads = NX * NV;
     __shared__ union {
-        i32x4 part[kSplit / 2][kQuads][64];
+        i32x4 part[kSplit][kQuads][64];
         i32x4 rows[kSplit][U][NX][64];
     } lds;
-    auto& part = lds.part;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tx, tv;
     tile_of(p, blockIdx.x, &tx, &tv);
@@ -240,29 +239,17 @@ __global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearPa
         multiply(s + kTurn, g1);
     }
     __syncthreads();  // (the sums lie where rows were)
-    // eight sums to four to two to one
-#pragma unroll
-    for (int half = kSplit / 2; half; half >>= 1) {
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int b = 0; b < NX; ++b)
-#pragma unroll
-                for (int v = 0; v < NV; ++v) part[wave - half][b * NV + v][lane] = acc[b][v];
-        }
-        __syncthreads();
-        if (half > 1 && wave < half) {
-#pragma unroll
-            for (int b = 0; b < NX; ++b)
-#pragma unroll
-                for (int v = 0; v < NV; ++v) acc[b][v] += part[wave][b * NV + v][lane];
-        }
-        if (half > 1) __syncthreads();
-    }
-    if (wave != 0) return;
 #pragma unroll
     for (int b = 0; b < NX; ++b)
 #pragma unroll
-        for (int v = 0; v < NV; ++v) store_quad<E>(p, t0 + b * 16 + (lane & 15), (b0 + v) * kBlock + (lane >> 4) * 4, acc[b][v] + part[0][b * NV + v][lane]);
+        for (int v = 0; v < NV; ++v) lds.part[wave][b * NV + v][lane] = acc[b][v];
+    __syncthreads();
+    static_assert(kQuads <= kSplit, "a wave for each block of sums");
+    if (wave >= kQuads) return;
+    i32x4 sum = {};
+#pragma unroll
+    for (int u = 0; u < kSplit; ++u) sum += lds.part[u][wave][lane];
+    store_quad<E>(p, t0 + wave / NV * 16 + (lane & 15), (b0 + wave % NV) * kBlock + (lane >> 4) * 4, sum);
 }
 
 // A wave's tile: NX blocks of rows from t0 on, NV blocks of channels from c0 on.  The results go through LDS, as many blocks of rows at a time
@@ -537,10 +524,10 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_ke
 
 // The shapes, and what they cost, fitted to 448 sizes of 1 to 8192 rows, 512 to 73448 channels and 512 to 16384 columns: `start` us of a launch; for a
 // round (a tile on every CU) `round` us and `step` more for every 64 columns, `busy` more of them where all CUs work; and `whole` says how much of a
-// last round that is not full counts as a full one.  The choice is the shape with the least cost, 0.3 % above the best of them in the mean and 11 % at
-// most (in us, rows x columns x channels: 1 x 4096 x 4608 16 x 16 split 5.9, 16 x 32 split 6.0, 32 x 64 7.7; 64 x 4096 x 16384 32 x 64 13.7, 64 x 64 14.2, 16 x 32
-// split 26.2; 256 x 4096 x 4608 64 x 128 12.6, 32 x 64 16.2, 64 x 256 19.3; 333 x 4099 x 12289 128 x 256 27.5, 64 x 128 34.3, 64 x 256 34.9, 256 x 256 45.6;
-// 2048 x 4096 x 16384: 256 x 256 120, 128 x 256 133, 64 x 256 142).
+// last round that is not full counts as a full one.  The choice is the shape with the least cost, 0.4 % above the best of them in the mean and 11 % at
+// most (in us, rows x columns x channels: 1 x 4096 x 4608 16 x 32 split 5.6, 16 x 16 5.8, 32 x 64 7.8; 64 x 4096 x 4608 32 x 64 8.5, 16 x 64 split 9.6, 64 x 128
+// 12.0; 64 x 4096 x 4096 16 x 64 split 6.7, 32 x 64 8.4; 256 x 4096 x 4608 64 x 128 12.6, 32 x 64 15.7, 64 x 256 19.4; 333 x 4099 x 12289 128 x 256 27.2,
+// 64 x 128 33.1, 64 x 256 33.8, 256 x 256 46.7; 2048 x 4096 x 16384: 256 x 256 117, 128 x 256 125, 64 x 256 136).
 struct Variant {
     const char* name;
     void (*f16_kernel)(LinearParams);
@@ -556,10 +543,10 @@ struct Variant {
     "int8_linear_wide_kernel<" #nx "," #nv "," #wx "," #wv ">", int8_linear_wide_kernel<f16, nx, nv, wx, wv>, int8_linear_wide_kernel<bf16, nx, nv, wx, wv>, \
         16 * nx * wx, kBlock* nv* wv, 64 * wx * wv
 const Variant kVariants[kInt8LinearShapes] = {
-    {CPMCU_SPLIT(1, 1, 4), 2.8f, 0.36f, 0.0057f, 0.017f, 0.3f},        {CPMCU_SPLIT(1, 2, 4), 2.9f, 0.83f, 0.0319f, 0.0032f, 0.1f},
-    {CPMCU_TILE(2, 1, 1, 4, 3, 2), 2.6f, 0.84f, 0.0785f, 0.f, 0.4f},   {CPMCU_TILE(4, 1, 1, 4, 5, 2), 1.f, 2.84f, 0.0769f, 0.046f, 0.7f},
-    {CPMCU_TILE(4, 2, 1, 4, 2, 2), 2.2f, 1.6f, 0.116f, 0.044f, 0.6f},  {CPMCU_TILE(4, 4, 1, 4, 2, 1), 3.5f, 0.92f, 0.222f, 0.081f, 0.5f},
-    {CPMCU_WIDE(4, 4, 2, 4), 1.f, 3.72f, 0.272f, 0.2f, 1.f},           {CPMCU_WIDE(8, 4, 2, 4), 3.7f, 3.7f, 0.431f, 0.38f, 0.8f}};
+    {CPMCU_SPLIT(1, 1, 4), 2.7f, 0.51f, 0.0027f, 0.02f, 0.6f},        {CPMCU_SPLIT(1, 2, 4), 2.5f, 0.33f, 0.0245f, 0.011f, 0.4f},
+    {CPMCU_SPLIT(1, 4, 2), 2.4f, 0.33f, 0.0437f, 0.0095f, 0.4f},      {CPMCU_TILE(2, 1, 1, 4, 3, 2), 2.4f, 0.44f, 0.0754f, 0.f, 0.4f},
+    {CPMCU_TILE(4, 2, 1, 4, 2, 2), 2.7f, 1.48f, 0.116f, 0.043f, 0.5f}, {CPMCU_TILE(4, 4, 1, 4, 2, 1), 3.5f, 1.16f, 0.229f, 0.037f, 0.6f},
+    {CPMCU_WIDE(4, 4, 2, 4), 1.5f, 3.46f, 0.279f, 0.16f, 1.f},        {CPMCU_WIDE(8, 4, 2, 4), 4.3f, 4.f, 0.457f, 0.37f, 0.6f}};
 #undef CPMCU_SPLIT
 #undef CPMCU_TILE
 #undef CPMCU_WIDE
