@@ -701,6 +701,66 @@ def test_batch_operators_on_another_stream(gpu):
     assert torch.equal(got[0], -want[0]) and torch.equal(got[1], -want[1]) and torch.equal(got[2], -want[2])
 
 
+def test_batch_operators_in_two_graphs_at_once(gpu):
+    """Two captured steps on data of their own, replayed side by side on two streams and between eager calls: they share no memory."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    from cpm.cu_amd.kvcache import PagedKVCache
+    Hq, Hkv, R, n = 4, 2, 3, 700
+    weight = ops.Int8Weight.quantized(_rows(torch, 3, 0, (Hq + 2 * Hkv) * D, 900) * 0.05)
+    inv_freq = _freq(torch, 64)
+
+    class Step:
+        def __init__(self, seed):
+            self.cache = PagedKVCache(1, Hkv, 12, fill=0.0)
+            self.batch = ops.PageBatch(self.cache, R, 4)
+            self.hidden = _rows(torch, seed, 0, n, 900)
+            self.new = torch.tensor([100 + seed, 200, 300 - seed], dtype=torch.int32, device="cuda")
+            self.q = torch.zeros((n, Hq, D), dtype=torch.float16, device="cuda")
+            self.free = self.batch.free_pages.clone()
+
+        def again(self):
+            self.batch._state.zero_()
+            self.batch._state[0] = 12
+            self.batch.free_pages.copy_(self.free)
+
+        def run(self):
+            where = self.batch.plan(self.new, n)
+            qkv = ops.int8_linear(*ops.quantize_rows(self.hidden), weight)
+            q, k, v = (x.view(n, -1, D) for x in qkv.split([Hq * D, Hkv * D, Hkv * D], 1))
+            ops.kv_append_slots(self.cache, 0, k, v, where["slots"], q=q, q_out=self.q, positions=where["positions"], inv_freq=inv_freq)
+
+        def results(self):
+            return [t.clone() for t in (self.q, self.cache.k[0], self.cache.v[0], self.batch.block_tables, self.batch.kv_lens, self.batch.counts)]
+
+    steps, streams, graphs, want = [Step(1), Step(2)], [torch.cuda.Stream(), torch.cuda.Stream()], [], []
+    for s in steps:
+        s.run()
+        want.append(s.results())
+        s.again()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            s.run()
+        graphs.append(graph)
+    for turn in range(4):
+        for s in steps:
+            s.again()
+            s.q.zero_()
+            s.cache.k[0].zero_()
+            s.cache.v[0].zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        other = ops.int8_linear(*ops.quantize_rows(steps[turn % 2].hidden), weight)
+        torch.cuda.synchronize()
+        assert torch.isfinite(other).all()
+        for s, w in zip(steps, want):
+            for got, ref in zip(s.results(), w):
+                assert torch.equal(got, ref)
+
+
 def test_no_rows_at_all(gpu):
     torch = gpu
     from cpm.cu_amd import ops
