@@ -294,6 +294,7 @@ decltype(&cpmcu_rope_rows) fn_rope_rows = nullptr;
 decltype(&cpmcu_kv_append_slots) fn_kv_append_slots = nullptr;
 decltype(&cpmcu_quantize_rows) fn_quantize_rows = nullptr;
 decltype(&cpmcu_int8_linear) fn_int8_linear = nullptr;
+decltype(&cpmcu_int8_weight_bytes) fn_int8_weight_bytes = nullptr;
 
 bool arguments(Py_ssize_t nargs, Py_ssize_t expected) {
     if (nargs != expected) PyErr_Format(PyExc_TypeError, "%zd arguments given, %zd expected", nargs, expected);
@@ -428,6 +429,21 @@ PyObject* call_quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     return Py_BuildValue("NN", THPVariable_Wrap(std::move(xq)), THPVariable_Wrap(std::move(scales)));
 }
 
+// Whether a tensor is as large as a weight [V, K] is when it is tiled (the bytes pass 32 bits); never where there is no such weight.
+bool tiled_from(const at::Tensor& w, int V, int K) {
+    const size_t bytes = fn_int8_weight_bytes(V, K);
+    return bytes > 0 && static_cast<size_t>(w.numel()) == bytes;
+}
+
+// int8_weight_fits(w_tiled, V, K): the check that int8_linear makes, for any tensor.
+PyObject* call_int8_weight_fits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 3)) return nullptr;
+    const at::Tensor* w = tensor_or_null(args[0]);
+    int V, K;
+    if (!expect(w, "int8_weight_fits: tensor required") || !integer(args[1], &V) || !integer(args[2], &K)) return nullptr;
+    return PyBool_FromLong(w->scalar_type() == at::kChar && tiled_from(*w, V, K));
+}
+
 // int8_linear(xq, x_scales, w_tiled, w_scales, V, K, out or None): out [n, V]
 PyObject* call_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!arguments(nargs, 7)) return nullptr;
@@ -438,9 +454,9 @@ PyObject* call_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int V, K;
     if (!integer(args[4], &V) || !integer(args[5], &K)) return nullptr;
     const at::Tensor& xq = *t[0];
-    if (!expect(V >= 1 && K >= 1 && xq.dim() == 2 && xq.size(1) == (K + 63) / 64 * 64 && xq.size(0) <= INT32_MAX && t[1]->numel() == xq.size(0),
+    if (!expect(V >= 1 && K >= 1 && xq.dim() == 2 && xq.size(1) == (int64_t{K} + 63) / 64 * 64 && xq.size(0) <= INT32_MAX && t[1]->numel() == xq.size(0),
                 "int8_linear: rows are [n, K rounded up to 64], with a scale each") ||
-        !expect(t[3]->numel() == V && t[2]->numel() == (V + 15) / 16 * 16 * ((K + 63) / 64 * 64), "int8_linear: the weight is tiled from [V, K], with a scale for each channel"))
+        !expect(t[3]->numel() == V && tiled_from(*t[2], V, K), "int8_linear: the weight is tiled from [V, K], with a scale for each channel"))
         return nullptr;
     const int64_t n = xq.size(0), sizes[2] = {n, V};
     at::Tensor made;
@@ -525,7 +541,8 @@ PyObject* bind(PyObject*, PyObject* handle) {
               find("cpmcu_tree_attention_window", &fn_tree_attention_window) &&
               find("cpmcu_tree_attention_workspace_bytes", &fn_tree_attention_workspace_bytes) && find("cpmcu_batch_tables", &fn_batch_tables) &&
               find("cpmcu_rope_rows", &fn_rope_rows) && find("cpmcu_kv_append_slots", &fn_kv_append_slots) &&
-              find("cpmcu_quantize_rows", &fn_quantize_rows) && find("cpmcu_int8_linear", &fn_int8_linear);
+              find("cpmcu_quantize_rows", &fn_quantize_rows) && find("cpmcu_int8_linear", &fn_int8_linear) &&
+              find("cpmcu_int8_weight_bytes", &fn_int8_weight_bytes);
 #define X(name) ok = ok && find("cpmcu_" #name, &fn_##name);
     CPMCU_TORCH_CALLS(X)
 #undef X
@@ -545,6 +562,7 @@ PyMethodDef g_methods[] = {
     X(kv_append_slots)
     X(quantize_rows)
     X(int8_linear)
+    X(int8_weight_fits)
     ENTRY("empty", empty)
     {"pinned", entry<pinned>, METH_O, nullptr},
     {"synchronize", entry<synchronize>, METH_NOARGS, nullptr},

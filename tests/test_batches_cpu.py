@@ -120,6 +120,23 @@ def test_weights_are_on_the_current_device():
         ops.Int8Weight(torch.zeros((16, 64), dtype=torch.int8), torch.zeros(16))
 
 
+def test_weights_of_2_gib_and_more_fit_their_sizes():
+    """Sizes in 64 bits: neither is a large weight refused, nor does a tensor fit that is shorter by a multiple of 2^32 (or 2^31)."""
+    import torch
+    from cpm.cu_amd import ops
+    fits = ops._calls().int8_weight_fits
+    weight = lambda n, t=torch.int8: torch.empty(n, dtype=t, device="meta")  # noqa: E731
+    for V, K in ((256000, 12288), (131072, 16384), (131088, 16384), (262144, 16448), (1 << 20, 131071), (17, 65), (1, 1)):
+        size = -(-V // 16) * 16 * (-(-K // 64) * 64)
+        assert ops._lib().raw.cpmcu_int8_weight_bytes(V, K) == size
+        assert fits(weight(size), V, K) and not fits(weight(size, torch.uint8), V, K)
+        for other in (size - 1, size + 1, size % 2 ** 32, size % 2 ** 31):
+            assert other == size or not fits(weight(other), V, K)
+    I = 2 ** 31 - 1
+    for V, K in ((0, 64), (-16, 64), (16, 0), (16, 131072), (16, I), (I, 64), (I, I)):
+        assert not fits(weight(0), V, K) and not fits(weight(1 << 30), V, K)
+
+
 def test_int8_linear_plans():
     """Every shape of the kernel is somebody's, from one row to many."""
     from cpm.cu_amd import lib, ops

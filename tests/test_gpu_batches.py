@@ -563,6 +563,43 @@ def test_int8_linear_sums_to_the_ends_of_32_bits(gpu, n):
     assert got[0].isnan().all() and not got[1:].isnan().any()
 
 
+@pytest.mark.parametrize("n, shapes", [(5, (0, 1, 2)), (70, (3, 4, 5)), (300, (6, 7))])
+def test_int8_linear_with_a_weight_beyond_2_gib(gpu, int8_shape, n, shapes):
+    """Channels on both sides of byte 2^31 of the weight and at its ends, in every shape of the kernel."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    V, K = 131072 + 40, 16384
+    w, xq = _int8(torch, 1, V, K), _int8(torch, 2, n, K)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x_scales, w_scales = (torch.empty(m, device="cuda").uniform_(0.5, 1.0, generator=g) * 0.001 for m in (n, V))
+    weight = ops.Int8Weight(w, w_scales)
+    assert weight.data.numel() > 2 ** 31
+    some = torch.cat([torch.arange(0, 40), torch.arange(131072 - 300, V)]).cuda()
+    ref = torch.matmul(xq.double(), w[some].double().t().contiguous()) * x_scales.double()[:, None] * w_scales.double()[some][None, :]
+    for shape in (-1,) + shapes:
+        int8_shape(shape)
+        got = ops.int8_linear(xq, x_scales, weight)
+        torch.cuda.synchronize()
+        _close(got[:, some], ref, 0, ref.abs() * 2.0 ** -22)  # (as in _check_product)
+
+
+@pytest.mark.parametrize("shape", [1, 4, 7])
+def test_int8_linear_with_results_beyond_2_gib(gpu, int8_shape, shape):
+    """Results on both sides of value 2^31 and of byte 2^31 (value 2^30), and the last ones."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    n, V, K = 32768 + 70, 65536, 64
+    w, xq = _int8(torch, 1, V, K), _int8(torch, 2, n, K)
+    x_scales, w_scales = torch.full((n,), 2.0 ** -8, device="cuda"), torch.full((V,), 2.0 ** -8, device="cuda")
+    int8_shape(shape)
+    got = ops.int8_linear(xq, x_scales, ops.Int8Weight(w, w_scales))
+    torch.cuda.synchronize()
+    assert got.numel() > 2 ** 31
+    some = torch.cat([torch.arange(0, 20), torch.arange(16384 - 20, 16384 + 20), torch.arange(n - 100, n)]).cuda()
+    ref = torch.matmul(xq[some].double(), w.double().t().contiguous()) * 2.0 ** -16
+    _close(got[some], ref, 0, ref.abs() * 2.0 ** -22)
+
+
 def test_int8_weight_from_16_bits(gpu):
     """Weights and rows quantised here: the product is near the 16-bit one, by at most half a step of either side's 8 bits a column."""
     torch = gpu
