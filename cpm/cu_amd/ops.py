@@ -271,12 +271,13 @@ class Int8Weight:
     """8-bit weights [V, K] with a scale for each channel, in matrix-operand order: built once."""
 
     def __init__(self, w, scales):
-        """w int8 [V, K], scales fp32 [V]: the weight of channel c is w[c] * scales[c]."""
+        """w int8 [V, K], scales fp32 [V]: the weight of channel c is w[c] * scales[c].  Both are copied: what is written to them later
+        does not change the weight."""
         assert w.dtype == torch.int8 and w.dim() == 2 and scales.dtype == torch.float32 and scales.numel() == w.shape[0]
         assert w.is_cuda and w.device == scales.device and w.device.index == torch.cuda.current_device(), "weights and scales on the current device required"
         self.V, self.K = w.shape
         self.shape = (self.V, self.K)
-        self.scales = scales.contiguous()
+        self.scales = scales.detach().reshape(self.V).clone(memory_format=torch.contiguous_format)
         w = w.contiguous()
         self.data = torch.empty(_lib().raw.cpmcu_int8_weight_bytes(self.V, self.K), dtype=torch.int8, device=w.device)
         _calls().int8_weight_tile(w, self.V, self.K, self.data)

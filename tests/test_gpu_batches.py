@@ -563,6 +563,23 @@ def test_int8_linear_sums_to_the_ends_of_32_bits(gpu, n):
     assert got[0].isnan().all() and not got[1:].isnan().any()
 
 
+@pytest.mark.parametrize("step", [1, 2])
+def test_int8_weight_is_a_copy(gpu, step):
+    """Neither the values nor the scales are the caller's memory, contiguous or not."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    V, K = 50, 128
+    w, scales = _int8(torch, 1, V, K), torch.rand(V * step, device="cuda")[::step]
+    weight = ops.Int8Weight(w, scales)
+    xq, x_scales = _int8(torch, 2, 3, K), torch.rand(3, device="cuda")
+    want = ops.int8_linear(xq, x_scales, weight)
+    w.zero_()
+    scales.fill_(5.0)
+    assert torch.equal(ops.int8_linear(xq, x_scales, weight), want) and want.any()
+    rows = torch.rand((V, 1), device="cuda")
+    assert ops.Int8Weight(w, rows).scales.shape == (V,)
+
+
 @pytest.mark.parametrize("n, shapes", [(5, (0, 1, 2)), (70, (3, 4, 5)), (300, (6, 7))])
 def test_int8_linear_with_a_weight_beyond_2_gib(gpu, int8_shape, n, shapes):
     """Channels on both sides of byte 2^31 of the weight and at its ends, in every shape of the kernel."""
