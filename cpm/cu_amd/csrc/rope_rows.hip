@@ -167,6 +167,19 @@ bool on_16_bytes(const HeadRows& x) {
     return x.heads == 0 || (((uintptr_t)x.in | (uintptr_t)x.out) % 16 == 0 && x.in_stride % 8 == 0 && x.out_stride % 8 == 0);
 }
 
+// n rows in memory, and whether two such sets share any: never where one ends before the other begins, nor where they are columns apart of rows
+// of one stride (the parts of a fused projection); rows of different strides that run through each other are taken to.
+struct RowSet {
+    const void* at;
+    long stride, width;
+};
+bool share(const RowSet& a, const RowSet& b, int n) {
+    const intptr_t d = (intptr_t)b.at - (intptr_t)a.at, s = 2 * a.stride;
+    if (n == 0 || a.width == 0 || b.width == 0 || d >= (n - 1) * s + 2 * a.width || -d >= 2 * ((n - 1) * b.stride + b.width)) return false;
+    const intptr_t column = (d % s + s) % s;
+    return a.stride != b.stride || column < 2 * a.width || column + 2 * b.width > s;
+}
+
 int check_rows(const char* op, const char* name, const HeadRows& x, int n, int head_dim) {
     CPMCU_CHECK_ARG(x.heads >= 0 && x.heads <= kMaxHeads, "%s: %d heads of %s outside [0, %d]", op, x.heads, name, kMaxHeads);
     if (x.heads == 0) return CPMCU_OK;
@@ -174,9 +187,7 @@ int check_rows(const char* op, const char* name, const HeadRows& x, int n, int h
     const long width = (long)x.heads * head_dim;
     CPMCU_CHECK_ARG(x.in_stride >= width && x.out_stride >= width, "%s: rows of %s closer than their %ld values", op, name, width);
     if (x.in == x.out && x.in_stride == x.out_stride) return CPMCU_OK;
-    const char *a = (const char*)x.in, *b = (const char*)x.out;
-    CPMCU_CHECK_ARG(a + 2 * ((n - 1) * x.in_stride + width) <= b || b + 2 * ((n - 1) * x.out_stride + width) <= a,
-                    "%s: the results of %s are neither in place nor in memory apart", op, name);
+    CPMCU_CHECK_ARG(!share({x.in, x.in_stride, width}, {x.out, x.out_stride, width}, n), "%s: the results of %s are neither in place nor in memory apart", op, name);
     return CPMCU_OK;
 }
 
@@ -323,6 +334,10 @@ extern "C" int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, 
     RopeParams p{{positions, inv_freq, rotary_dim / 2, magnitude, transposed ? -magnitude : magnitude}, {q, q_out, q_stride, q_out_stride, Hq}, {k, k_out, k_stride, k_out_stride, Hkv}, n, head_dim, 1};
     if (int rc = check_rows("rope_rows", "q", p.q, n, head_dim)) return rc;
     if (int rc = check_rows("rope_rows", "k", p.k, n, head_dim)) return rc;
+    const long q_width = (long)Hq * head_dim, k_width = (long)Hkv * head_dim;
+    CPMCU_CHECK_ARG(!share({q_out, q_out_stride, q_width}, {k, k_stride, k_width}, n) && !share({k_out, k_out_stride, k_width}, {q, q_stride, q_width}, n) &&
+                        !share({q_out, q_out_stride, q_width}, {k_out, k_out_stride, k_width}, n),
+                    "rope_rows: results lie in the memory of the other rows");
     if (Hq + Hkv == 0) return CPMCU_OK;
     const bool wide = rotary_dim % 16 == 0 && head_dim % 16 == 0 && on_16_bytes(p.q) && on_16_bytes(p.k);
     p.parts = row_parts(n, Hq + Hkv, head_dim / (wide ? 16 : 2));

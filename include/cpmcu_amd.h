@@ -676,7 +676,7 @@ int cpmcu_batch_tables(const int32_t* kv_lens, const int32_t* new_lens, int num_
  *   inv_freq float[half]: with whatever scaling the model's long contexts have (see ops.rope_frequencies);
  *   transposed: the transposed matrix, that takes gradients of the results back to the inputs (with m = 1 the inverse);
  *   q [n][q_stride], heads of head_dim values one after the other from the row's start; q_out likewise, the same memory and stride (in
- *       place) or memory apart, from k too; k alike; Hq or Hkv may be 0.  n < 2^24.  head_dim even, up to 256; rotary_dim even.  Rows on 16 bytes with
+ *       place) or memory apart, from k and k_out too (columns apart of rows of one stride are); k alike; Hq or Hkv may be 0.  n < 2^24.  head_dim even, up to 256; rotary_dim even.  Rows on 16 bytes with
  *       rotary_dim and head_dim multiples of 16 are read and written in 16-byte pieces, others value by value. */
 int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, int rotary_dim, int interleaved, float magnitude, int transposed,
                     const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, const void* k, int64_t k_stride, void* k_out,

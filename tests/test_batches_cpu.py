@@ -49,6 +49,20 @@ def test_rope_rows_refuses(kw, match):
         _rope(**kw)
 
 
+Q, K = 1 << 32, 3 << 32  # where _rope has q and k, 60 rows of 4096 and of 256 values
+
+
+@pytest.mark.parametrize("kw", [
+    dict(qo=P(K), qos=4096), dict(qo=P(K - 2 * 59 * 4096)), dict(qo=P(K + 2 * (59 * 256 + 255)), qos=4096), dict(ko=P(Q)), dict(ko=P(Q + 2 * (59 * 4096 + 4095))), dict(qo=P(5 << 32), ko=P(5 << 32)),
+    dict(k=P(Q + 2 * 4095), ks=4352, qs=4352, qo=P(Q), qos=4352, ko=P(7 << 32)),      # the last value of each row of q is the first of k's
+    dict(k=P(Q + 2 * 4097), ks=4352, qs=4352, qo=P(Q), qos=4352, ko=P(7 << 32)),      # the last of k's the first of the next row of q
+    dict(qo=P(5 << 32), qos=4352, ko=P((5 << 32) + 2 * 4000), kos=4352), dict(qo=P(5 << 32), qos=5000, ko=P((5 << 32) + 2 * 4096), kos=5001)])
+def test_rope_rows_refuses_results_in_the_other_rows(kw):
+    """Workgroups would read rows that others have turned already, or write the same memory."""
+    with pytest.raises(ValueError, match="rope_rows: results lie in the memory of the other rows"):
+        _rope(**kw)
+
+
 def test_empty_calls_are_no_calls():
     """No rows or heads: nothing to do, and no device is asked for."""
     _rope(n=0)

@@ -261,6 +261,31 @@ def test_rope_rows_of_wider_rows_and_rows_left_out(gpu, offset, rotary):
     assert (out[:, ~used] == 7.0).all() and torch.equal(in_place[:, ~used], x[:, ~used])
 
 
+def test_rope_rows_of_one_wide_row_in_any_columns(gpu):
+    """q, k and their results as columns of one tensor, in place and beside each other; columns that overlap are refused."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    n, Hq, Hkv = 21, 3, 2
+    x = _rows(torch, 3, 0, n, 14 * D)
+    part = lambda t, at, heads: t[:, at:at + heads * D].view(n, heads, D)  # noqa: E731
+    positions, freq = torch.arange(n, dtype=torch.int32, device="cuda") * 1000, _freq(torch, 64)
+    want = [t.clone() for t in ops.rope_rows(part(x, 0, Hq), part(x, Hq * D, Hkv), positions, freq)]
+    for q_at, k_at in ((0, Hq * D), (5 * D, Hq * D), (0, 8 * D), (5 * D, 8 * D), (11 * D, 5 * D), (9 * D, 12 * D)):
+        y = x.clone()
+        ops.rope_rows(part(y, 0, Hq), part(y, Hq * D, Hkv), positions, freq, q_out=part(y, q_at, Hq), k_out=part(y, k_at, Hkv))
+        torch.cuda.synchronize()
+        assert torch.equal(part(y, q_at, Hq), want[0]) and torch.equal(part(y, k_at, Hkv), want[1])
+        written = torch.zeros(14 * D, dtype=torch.bool, device="cuda")
+        written[q_at:q_at + Hq * D] = written[k_at:k_at + Hkv * D] = True
+        assert torch.equal(y[:, ~written], x[:, ~written])
+    for q_at, k_at in ((2 * D, Hq * D), (4 * D, Hq * D), (0, 2 * D), (5 * D, 7 * D), (0, Hq * D + 8)):
+        y = x.clone()
+        with pytest.raises(ValueError, match="results"):
+            ops.rope_rows(part(y, 0, Hq), part(y, Hq * D, Hkv), positions, freq, q_out=part(y, q_at, Hq), k_out=part(y, k_at, Hkv))
+        torch.cuda.synchronize()
+        assert torch.equal(y, x)
+
+
 def test_rope_gradient_is_the_transposed_rotation(gpu):
     """Against differences: for f = sum(w * rope(x)), (f(x + h e) - f(x - h e)) / 2h = rope^T(w) . e, f being linear in x.  The sums are of
     fp16 results (half a step each, 2^-11) over 2h = 2: 32 values of |w| <= 4 and |y| <= 12 leave 32 * 4 * 12 * 2^-11 / 2 in the worst case."""
