@@ -372,6 +372,10 @@ extern "C" int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, 
     CPMCU_CHECK_ARG(k_stride >= width && v_stride >= width, "kv_append_slots: rows closer than their %ld values", width);
     CPMCU_CHECK_ARG(on_16_bytes(p.rope.q) && ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0,
                     "kv_append_slots: rows and pools have to lie on 16 bytes");
+    const long q_width = (long)Hq * kHeadDim, pool = (long)Hkv * kHeadDim * kPage;
+    CPMCU_CHECK_ARG(!share({q_out, q_out_stride, q_width}, {k, k_stride, width}, n) && !share({q_out, q_out_stride, q_width}, {v, v_stride, width}, n),
+                    "kv_append_slots: the results of q lie in the memory of k or v");
+    CPMCU_CHECK_ARG(!share({k_pool, pool, pool}, {v_pool, pool, pool}, num_pages), "kv_append_slots: the K and the V pool share memory");
     p.k_pool = (f16*)k_pool;
     p.v_pool = (f16*)v_pool;
     p.slots = slots;

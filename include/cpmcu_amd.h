@@ -683,11 +683,11 @@ int cpmcu_rope_rows(const int32_t* positions, const float* inv_freq, int rotary_
                     int64_t k_out_stride, int Hkv, int head_dim, int n, void* stream);
 
 /* The K and V rows of several requests into the paged cache of a layer, row t of [n] to slots[t] = page * 256 + place in the page (as
- * cpmcu_batch_tables writes them; no slot twice).  Rows whose slot is negative or lies behind num_pages are left out whole.
+ * cpmcu_batch_tables writes them; no slot twice, and no row that lies in a place that is written).  Rows whose slot is negative or lies behind num_pages are left out whole.
  * n < 2^24, n * Hkv < 2^27.
  *   k, v [n][stride], Hkv heads of 128 values from the row's start; rows and pools on 16 bytes.
  *   positions, inv_freq (or both NULL): K is rotated on its way as by cpmcu_rope_rows, and so are the Hq heads of q into q_out (Hq
- *       may be 0); rotary_dim a multiple of 16; rows of a negative position are left out as well. */
+ *       may be 0; q_out is q in place or memory apart from q, k and v); rotary_dim a multiple of 16; rows of a negative position are left out as well. */
 int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, const int32_t* slots, const void* k, int64_t k_stride, const void* v,
                           int64_t v_stride, int n, int Hkv, const int32_t* positions, const float* inv_freq, int rotary_dim, int interleaved,
                           float magnitude, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int Hq, void* stream);

@@ -89,6 +89,18 @@ def test_kv_append_slots_refuses(kw, match):
         _append(**kw)
 
 
+@pytest.mark.parametrize("kw, match", [
+    (dict(qo=P(3 << 32)), "results of q lie in the memory of k or v"), (dict(qo=P((4 << 32) - 2 * 59 * 4096)), "results of q lie in the memory of k or v"),
+    (dict(qo=P((4 << 32) + 2 * (59 * 256 + 248))), "results of q lie in the memory of k or v"),
+    # a fused projection in place, its k one piece too early, its v one too late for the row
+    (dict(q=P(5 << 32), qo=P(5 << 32), qs=4608, qos=4608, k=P((5 << 32) + 2 * 4088), ks=4608), "results of q lie in the memory of k or v"),
+    (dict(q=P(5 << 32), qo=P(5 << 32), qs=4608, qos=4608, v=P((5 << 32) + 2 * 4360), vs=4608), "results of q lie in the memory of k or v"),
+    (dict(vp=P(1 << 32)), "pool share memory"), (dict(vp=P((1 << 32) + 4 * 2 * 256 * 128 * 2 - 16)), "pool share memory"), (dict(kp=P((2 << 32) + 16)), "pool share memory")])
+def test_kv_append_slots_refuses_memory_that_is_shared(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _append(**kw)
+
+
 def test_int8_operators_refuse():
     L = _lib()
     for args in ((None, 64, 1, 64, B, C), (A, 64, 1, 64, None, C), (A, 64, 1, 64, B, None), (A, 64, -1, 64, B, C), (A, 64, 0, 0, B, C), (A, 64, 1, 0, B, C), (A, 1 << 20, 1, 131072, B, C), (A, 63, 1, 64, B, C),

@@ -383,6 +383,27 @@ def test_kv_append_slots(gpu, set_option, dtype, n, Hq, Hkv, kind, rotary, inter
     assert torch.equal(cache.v[0].view(torch.int16), v_was.view(torch.int16))
 
 
+@pytest.mark.parametrize("n", [1, 5, 200])
+def test_kv_append_slots_turns_q_in_place_of_a_fused_projection(gpu, n):
+    """q's results over q, between k and v of the same rows: the same as into memory of their own, k and v as they were."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    from cpm.cu_amd.kvcache import PagedKVCache
+    Hq, Hkv = 6, 2
+    x = _rows(torch, n, 0, n, (Hq + 2 * Hkv) * D)
+    slots, positions = torch.arange(n, dtype=torch.int32, device="cuda") + 100, torch.arange(n, dtype=torch.int32, device="cuda") + 70000
+    freq = _freq(torch, 64)
+    parts = lambda t: [y.view(n, -1, D) for y in t.split([Hkv * D, Hq * D, Hkv * D], 1)]  # noqa: E731
+    one, two, y = PagedKVCache(1, Hkv, 2), PagedKVCache(1, Hkv, 2), x.clone()
+    k, q, v = parts(x)
+    want = ops.kv_append_slots(one, 0, k, v, slots, q=q, positions=positions, inv_freq=freq)
+    k, q, v = parts(y)
+    ops.kv_append_slots(two, 0, k, v, slots, q=q, q_out=q, positions=positions, inv_freq=freq)
+    torch.cuda.synchronize()
+    assert torch.equal(q, want) and torch.equal(one.k[0], two.k[0]) and torch.equal(one.v[0], two.v[0])
+    assert torch.equal(k, parts(x)[0]) and torch.equal(v, parts(x)[2])
+
+
 def test_kv_append_slots_is_kv_append_for_one_sequence(gpu):
     """Rows that follow each other in one sequence: the same cache, bit for bit."""
     torch = gpu
