@@ -235,7 +235,7 @@ __global__ __launch_bounds__(THREADS) void batch_tables_kernel(TableParams p) {
 
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     const char *x = (const char*)a, *y = (const char*)b;
-    return x < y + nb && y < x + na;
+    return na > 0 && nb > 0 && x < y + nb && y < x + na;
 }
 
 }  // namespace
@@ -254,12 +254,18 @@ extern "C" int cpmcu_batch_tables(const int32_t* kv_lens, const int32_t* new_len
     CPMCU_CHECK_ARG(num_pages >= 1 && num_pages <= INT32_MAX / kPage, "batch_tables: num_pages=%d outside [1, %d]", num_pages, INT32_MAX / kPage);
     CPMCU_CHECK_ARG(max_rows >= 0 && max_rows <= kMaxRows, "batch_tables: max_rows=%d outside [0, %d]", max_rows, kMaxRows);
     CPMCU_CHECK_ARG(max_rows == 0 || (positions && slots), "batch_tables: null pointer argument");
-    // Workgroups read these inputs while others write the outputs: none may be the same memory.
+    // Workgroups read the inputs while others write the outputs and, in place, the tables and the stack: what is written has to be memory of its own.
     const size_t n = sizeof(int32_t) * (size_t)num_requests;
-    const struct { const void* at; size_t bytes; } in[] = {{kv_lens, n}, {new_lens, n}, {held, n}, {counts, 4}, {block_tables, n * max_blocks}, {free_pages, 4 * (size_t)num_pages}},
-        out[] = {{kv_lens_out, n}, {held_out, n}, {counts_out, 8}, {row_offsets, n + 4}, {positions, 4 * (size_t)max_rows}, {slots, 4 * (size_t)max_rows}};
-    for (const auto& o : out)
-        for (const auto& i : in) CPMCU_CHECK_ARG(!overlap(o.at, o.bytes, i.at, i.bytes), "batch_tables: an output is the memory of an input");
+    const struct { const void* at; size_t bytes; } all[] = {{kv_lens, n}, {new_lens, n}, {held, n}, {counts, 4}, {block_tables, n * max_blocks}, {free_pages, 4 * (size_t)num_pages},
+        {kv_lens_out, n}, {held_out, n}, {counts_out, 8}, {row_offsets, n + 4}, {positions, 4 * (size_t)max_rows}, {slots, 4 * (size_t)max_rows}};
+    constexpr int kWritten = 4, kOut = 6, kAll = sizeof(all) / sizeof(all[0]);
+    for (int o = kWritten; o < kAll; ++o)
+        for (int i = 0; i < o; ++i) {
+            const bool shared = overlap(all[o].at, all[o].bytes, all[i].at, all[i].bytes);
+            CPMCU_CHECK_ARG(!shared || o < kOut || i >= kOut, "batch_tables: an output is the memory of an input");
+            CPMCU_CHECK_ARG(!shared || o >= kOut, "batch_tables: the tables or the stack share memory with another input");
+            CPMCU_CHECK_ARG(!shared, "batch_tables: two outputs share memory");
+        }
     TableParams p{kv_lens, new_lens, held, counts, block_tables, free_pages, kv_lens_out, held_out, counts_out, row_offsets, positions, slots,
                   num_requests, max_blocks, num_pages, max_rows};
     const int threads = num_requests <= 256 ? 256 : 1024;

@@ -655,10 +655,11 @@ int cpmcu_draft_tree_finish_root(void* state, int k, int num_iter, int tree_size
  *       The others are left as they are; keep them valid page numbers (zeros, at the start), since attention may look one up.
  *   free_pages int32[num_pages] / counts int32[2]: a stack of counts[0] free pages, each of them below num_pages, the next one to give
  *       at counts[0] - 1.  Ended requests' pages are put on it first, in request order; then every request takes what it lacks for
- *       kv_lens + new_lens tokens, in request order.  Both arrays and block_tables change in place.
+ *       kv_lens + new_lens tokens, in request order.  The stack and block_tables change in place and are memory apart from each other and
+ *       from the other arrays.
  *   A request is refused -- its length, pages and table stay, its rows have no slot -- if it needs more than max_blocks pages or than are
  *       left (then so is every later one that needs any), if its rows end behind max_rows, or if kv_lens[r] is negative.
- *   outputs, apart from the inputs (a caller who does not want the step drops them: the stack below counts[0] and the pages in
+ *   outputs, apart from the inputs and from each other (a caller who does not want the step drops them: the stack below counts[0] and the pages in
  *       the tables below held[r] are as they were): kv_lens_out, held_out int32[num_requests]; counts_out int32[2] = (free pages, refused
  *       requests); row_offsets int32[num_requests + 1]: request r's rows are [row_offsets[r], row_offsets[r + 1]); positions, slots
  *       int32[max_rows]: a row's position in its request and its place page * 256 + position % 256 in the cache; both -1 for

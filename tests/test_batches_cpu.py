@@ -33,6 +33,17 @@ def test_batch_tables_refuses(kw, match):
         _tables(**kw)
 
 
+@pytest.mark.parametrize("kw, match", [
+    (dict(kv=P(3 << 32)), "tables or the stack share"), (dict(held=P((3 << 32) + 4 * 4 * 8 - 4)), "tables or the stack share"), (dict(new=P((3 << 32) - 12)), "tables or the stack share"),
+    (dict(counts=P((5 << 32) + 4 * 63)), "tables or the stack share"), (dict(kv=P((5 << 32) - 4)), "tables or the stack share"), (dict(free=P(3 << 32)), "tables or the stack share"),
+    (dict(free=P((3 << 32) - 4 * 63)), "tables or the stack share"), (dict(held_out=P(7 << 32)), "two outputs share"), (dict(counts_out=P((7 << 32) + 12)), "two outputs share"),
+    (dict(offsets=P((8 << 32) - 16)), "two outputs share"), (dict(slots=P(11 << 32)), "two outputs share"), (dict(slots=P((11 << 32) - 4)), "two outputs share")])
+def test_batch_tables_refuses_memory_that_is_shared(kw, match):
+    """What one workgroup writes another one would read, or write too."""
+    with pytest.raises(ValueError, match=match):
+        _tables(**kw)
+
+
 def _rope(**kw):
     a = dict(pos=A, freq=B, rotary=128, il=0, m=1.0, tr=0, q=P(1 << 32), qs=4096, qo=P(2 << 32), qos=4096, hq=32, k=P(3 << 32), ks=256, ko=P(4 << 32), kos=256, hkv=2, dim=128, n=60)
     a.update(kw)
