@@ -233,11 +233,6 @@ __global__ __launch_bounds__(THREADS) void batch_tables_kernel(TableParams p) {
     }
 }
 
-bool overlap(const void* a, size_t na, const void* b, size_t nb) {
-    const char *x = (const char*)a, *y = (const char*)b;
-    return na > 0 && nb > 0 && x < y + nb && y < x + na;
-}
-
 }  // namespace
 }  // namespace cpmcu
 

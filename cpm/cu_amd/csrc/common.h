@@ -93,5 +93,9 @@ hipStream_t resolve_stream(void* stream);  // NULL -> the library's blocking str
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const char *x = (const char*)a, *y = (const char*)b;
+    return na > 0 && nb > 0 && x < y + nb && y < x + na;
+}
 
 }  // namespace cpmcu

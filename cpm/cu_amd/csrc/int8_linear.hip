@@ -582,8 +582,10 @@ extern "C" int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K
     CPMCU_CHECK_ARG(x && xq && scales, "quantize_rows: null pointer argument");
     CPMCU_CHECK_ARG(n < 1 << 24, "quantize_rows: n=%d, more rows than a launch has workgroups", n);
     CPMCU_CHECK_ARG(x_stride >= K, "quantize_rows: rows closer than their %d values", K);
-    CPMCU_CHECK_ARG((uintptr_t)xq % 16 == 0, "quantize_rows: xq has to lie on 16 bytes");
     const int padded = ceil_div(K, kStep) * kStep;
+    const size_t x_bytes = 2 * ((size_t)(n - 1) * (size_t)x_stride + K), q_bytes = (size_t)n * padded, s_bytes = 4 * (size_t)n;
+    CPMCU_CHECK_ARG(!overlap(xq, q_bytes, x, x_bytes) && !overlap(scales, s_bytes, x, x_bytes) && !overlap(xq, q_bytes, scales, s_bytes), "quantize_rows: the results lie in the rows' memory or in each other's");
+    CPMCU_CHECK_ARG((uintptr_t)xq % 16 == 0, "quantize_rows: xq has to lie on 16 bytes");
     hipStream_t st = resolve_stream(stream);
     const bool whole = K % 8 == 0, waves = n >= kQuantRows && padded <= 64 * 8 * kQuantPieces;
 #define CPMCU_QUANT(E)                                                                                                                              \
@@ -633,6 +635,10 @@ extern "C" int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const 
     p.row_tiles = ceil_div(n, v.rows);
     p.channel_tiles = ceil_div(V, v.channels);
     CPMCU_CHECK_ARG((int64_t)p.row_tiles * p.channel_tiles * v.threads <= UINT32_MAX, "int8_linear: n=%d rows of V=%d channels are more than a launch has threads", n, V);
+    const size_t bytes = 2 * (size_t)n * V;
+    CPMCU_CHECK_ARG(!overlap(out, bytes, xq, (size_t)n * p.steps * kStep) && !overlap(out, bytes, x_scales, 4 * (size_t)n) && !overlap(out, bytes, w_tiled, cpmcu_int8_weight_bytes(V, K)) &&
+                        !overlap(out, bytes, w_scales, 4 * (size_t)V),
+                    "int8_linear: out is the memory of an input");
     const dim3 grid(p.row_tiles * p.channel_tiles);
     hipLaunchKernelGGL(options().dtype == 1 ? v.bf16_kernel : v.f16_kernel, grid, dim3(v.threads), 0, resolve_stream(stream), p);
     CPMCU_LAUNCH_CHECK();

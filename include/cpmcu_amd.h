@@ -695,7 +695,8 @@ int cpmcu_kv_append_slots(void* k_pool, void* v_pool, int num_pages, const int32
 
 /* Rows of 16-bit floats to 8 bits with a scale for each row: scales[t] = max |x| / 127, xq[t][k] = rint(127 x / max |x|) (ties to even,
  * the quotient as if exact).  An empty (all zero) row has scale 0 and zeros, a row with an infinity or NaN scale NaN and zeros.
- *   x [n][x_stride], n < 2^24, K <= 131071 values from the row's start; xq [n][K rounded up to 64], zeros behind column K, on 16 bytes. */
+ *   x [n][x_stride], n < 2^24, K <= 131071 values from the row's start; xq [n][K rounded up to 64], zeros behind column K, on 16 bytes; x, xq
+ *   and scales are memory apart. */
 int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K, int8_t* xq, float* scales, void* stream);
 /* 8-bit weights [V][K], row-major, in matrix-operand order [ceil(V/16)][ceil(K/64)][64 lanes][16 bytes]: once, at load time. */
 size_t cpmcu_int8_weight_bytes(int V, int K);

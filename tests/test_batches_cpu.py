@@ -128,6 +128,24 @@ def test_int8_operators_refuse():
     assert L.raw.cpmcu_int8_weight_bytes(17, 65) == 2 * 2 * 1024 and L.raw.cpmcu_int8_weight_bytes(0, 65) == 0
 
 
+@pytest.mark.parametrize("xq, scales", [(1 << 32, 9 << 32), ((1 << 32) + 2 * (9 * 200 + 100) - 16, 9 << 32), ((1 << 32) - 10 * 128 + 16, 9 << 32), (8 << 32, 1 << 32), (8 << 32, (1 << 32) - 36),
+                                        (8 << 32, 8 << 32), (8 << 32, (8 << 32) + 1276), ((9 << 32) + 32, 9 << 32)])
+def test_quantize_rows_refuses_memory_that_is_shared(xq, scales):
+    """10 rows of 100 values, 200 apart, at 1 << 32."""
+    with pytest.raises(ValueError, match="quantize_rows: the results lie"):
+        _lib().quantize_rows(P(1 << 32), 200, 10, 100, P(xq), P(scales), None)
+
+
+@pytest.mark.parametrize("n", [1, 10, 600])
+def test_int8_linear_refuses_results_over_its_inputs(n):
+    V, K = 100, 100
+    at, sizes = [P(i << 32) for i in (1, 2, 3, 4)], (n * 128, 4 * n, 112 * 128, 4 * V)
+    for i, size in enumerate(sizes):
+        for out in (i + 1 << 32, (i + 1 << 32) + size - 2, (i + 1 << 32) - 2 * n * V + 2):
+            with pytest.raises(ValueError, match="int8_linear: out is the memory of an input"):
+                _lib().int8_linear(*at, n, V, K, P(out), None)
+
+
 def test_sizes_beyond_a_launch_are_refused():
     """Before any grid is made of them: rows, channels and their products up to the largest 32-bit numbers."""
     L, I = _lib(), 2 ** 31 - 1
