@@ -210,13 +210,20 @@ __global__ __launch_bounds__(64 * kSplit) void int8_linear_split_kernel(LinearPa
             for (int b = 0; b < NX; ++b) g.x[u][b] = *reinterpret_cast<const i32x4*>(x[b] + at * kStep);
         }
     };
+    // Lanes read what other lanes of their wave wrote: LDS serves a wave in the order of its requests, which the fences keep (they cost no instruction).
+    const auto fence = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
     i32x4 acc[NX][NV] = {};
     const auto multiply = [&](int s, const Group& g) {
         i32x4(&rows)[U][NX][64] = lds.rows[wave];  // (one wave's own: no barrier)
+        fence();
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int b = 0; b < NX; ++b) rows[u][b][lane] = g.x[u][b];
+        fence();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (s + u * kSplit > last) break;  // (the same for the whole wave)

@@ -593,6 +593,25 @@ def test_int8_linear_shapes_agree(gpu, set_option, int8_shape, shape):
     assert len(names) == 1
 
 
+@pytest.mark.parametrize("shape", range(8))
+def test_int8_linear_of_every_number_of_steps(gpu, int8_shape, shape):
+    """1 to 20 steps of 64 columns and those about the waves' turns and the rings' lengths: whole numbers, compared with their exact products."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    n, V = 35, 70
+    one = torch.ones(n, device="cuda")
+    for steps in list(range(1, 21)) + [23, 24, 25, 31, 32, 33, 34, 47, 48, 49, 63, 64, 65, 66]:
+        for K in (64 * steps, 64 * steps - 37):
+            xq, w = _int8(torch, K, n, 64 * steps), _int8(torch, K + 1, V, K)
+            ref = torch.matmul(xq[:, :K].double(), w.double().t().contiguous())
+            scale = 2.0 ** -10  # sums of up to 4224 * 2^14 < 2^26.1 stay below fp16's 65504 (2^16)
+            int8_shape(shape)
+            got = ops.int8_linear(xq, one, ops.Int8Weight(w, torch.full((V,), scale, device="cuda")))
+            torch.cuda.synchronize()
+            assert torch.isfinite(ref * scale).all() and (ref.abs() * scale < 65504).all()
+            _close(got, ref * scale, 0, ref.abs() * scale * 2.0 ** -24)  # the sum's one rounding to 32 bits
+
+
 @pytest.mark.parametrize("n", [1, 20, 70, 200, 600])
 def test_int8_linear_sums_to_the_ends_of_32_bits(gpu, n):
     """The longest rows of the largest values, and a row of scale NaN."""
