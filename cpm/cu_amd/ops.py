@@ -212,7 +212,8 @@ def batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, max_
     [B, max_blocks], of which the first held[r] entries of row r are request r's pages; free_pages, a stack of which counts[0] are free.
     Returns dict(kv_lens [B], held [B], counts [2] = (free pages, refused requests), row_offsets [B + 1], positions [max_rows], slots
     [max_rows]), which the next step takes in place of the inputs; block_tables and free_pages change in place.  Rows without a slot
-    (refused requests', and behind the last one) have slot and position -1.  See PageBatch for an object that keeps all this.
+    (refused requests', and behind the last one) have slot and position -1.  Once a request lacks pages every later one that needs any
+    is refused as well, and a refused request's rows keep their range of the batch.  See PageBatch for an object that keeps all this.
     """
     lens, held, counts, offsets, positions, slots, _ = (_native or _calls()).batch_tables(kv_lens, new_lens, block_tables, held, free_pages, counts, int(max_rows))
     return dict(kv_lens=lens, held=held, counts=counts, row_offsets=offsets, positions=positions, slots=slots)
@@ -233,7 +234,11 @@ class PageBatch:
     """The pages of up to max_requests requests on one paged cache, kept on the device: tables, lengths and the stack of free pages.
 
     ``plan(new_lens, max_rows)`` gives every request room for its new rows and returns where they go (batch_tables); ``kv_lens[r:r + 1]`` and
-    ``block_tables[r]`` are then what tree_attention takes for request r (through ``cache_of``)."""
+    ``block_tables[r]`` are then what tree_attention takes for request r (through ``cache_of``), with a max_kv_len of at most max_blocks * 256.
+
+    Rows that turn out not to be wanted (nodes of a draft tree that are not accepted) are given up by writing the shorter length to
+    ``kv_lens[r]``, in place: the next plan goes on from there, in pages that the request keeps.  A request that is refused has the length
+    that it had; its rows have slot -1, and there is nothing to attend with."""
 
     def __init__(self, cache, max_requests, max_blocks, num_pages=None):
         self.cache = cache

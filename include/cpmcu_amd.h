@@ -659,6 +659,7 @@ int cpmcu_draft_tree_finish_root(void* state, int k, int num_iter, int tree_size
  *       from the other arrays.
  *   A request is refused -- its length, pages and table stay, its rows have no slot -- if it needs more than max_blocks pages or than are
  *       left (then so is every later one that needs any), if its rows end behind max_rows, or if kv_lens[r] is negative.
+ *       Its rows keep their range of the batch, so the rows of later requests lie behind it.
  *   outputs, apart from the inputs and from each other (a caller who does not want the step drops them: the stack below counts[0] and the pages in
  *       the tables below held[r] are as they were): kv_lens_out, held_out int32[num_requests]; counts_out int32[2] = (free pages, refused
  *       requests); row_offsets int32[num_requests + 1]: request r's rows are [row_offsets[r], row_offsets[r + 1]); positions, slots

@@ -757,6 +757,115 @@ def test_a_batch_from_hidden_rows_to_attention(gpu):
     assert sorted(pages) == list(range(6))
 
 
+def _attention_and_limit(torch, q, k, v, seen):
+    """Attention of q [T, Hq, D] on keys and values as they lie in the cache [S, Hkv, D] in 64 bits, and how far the kernel's may be off:
+    the probabilities and the splits' sums are rounded to fp16 (2^-11 each, of a sum of magnitudes; their sum in the denominator as well), the
+    result once more; what underflows there is below 2^-25; a score is a sum of 128 products in 32 bits with two factors, and shows
+    in its probability, in the largest one's and in their sum; the products' sum has S terms."""
+    S, group = k.shape[0], q.shape[1] // k.shape[1]
+    q, k, v = q.double().transpose(0, 1), k.double().repeat_interleave(group, 1).transpose(0, 1), v.double().repeat_interleave(group, 1).transpose(0, 1).contiguous()
+    kt = k.transpose(1, 2).contiguous()
+    p = torch.softmax((torch.matmul(q, kt) / D ** 0.5).masked_fill(~seen, float("-inf")), -1)
+    delta = (torch.matmul(q.abs(), kt.abs()) / D ** 0.5).amax(-1, keepdim=True) * (128 + 4) * 2.0 ** -24
+    ref, weight = torch.matmul(p, v), torch.matmul(p, v.abs())
+    limit = weight * (3 * 2.0 ** -11 + 4 * delta + S * 2.0 ** -24) + ref.abs() * 2.0 ** -11 + 2.0 ** -25 * (torch.matmul(seen.double(), v.abs()) + 2)
+    return ref.transpose(0, 1), limit.transpose(0, 1)
+
+
+def test_prompts_longer_than_an_attention_call(gpu):
+    """Two prompts and their next chunks, planned and appended whole, attended in pieces of up to 128 rows whose length is their last row's
+    position + 1."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    from cpm.cu_amd.kvcache import PagedKVCache
+    Hq, Hkv, max_rows = 8, 2, 512
+    cache = PagedKVCache(1, Hkv, 7)
+    batch = ops.PageBatch(cache, 2, 4)
+    inv_freq, past = _freq(torch, 64), [0, 0]
+    for step, new in enumerate(([300, 129], [200, 1], [1, 257])):
+        x = _rows(torch, step, 0, max_rows, (Hq + 2 * Hkv) * D)
+        q, k, v = (t.view(max_rows, -1, D) for t in x.split([Hq * D, Hkv * D, Hkv * D], 1))
+        where = batch.plan(torch.tensor(new, dtype=torch.int32, device="cuda"), max_rows)
+        q_rot = ops.kv_append_slots(cache, 0, k, v, where["slots"], q=q, positions=where["positions"], inv_freq=inv_freq)
+        k_rot = ops.rope_rows(k, None, where["positions"], inv_freq)[0]
+        first = 0
+        for r, n in enumerate(new):
+            end, view, out = first + n, batch.cache_of(r), torch.full((n, Hq, D), float("nan"), dtype=torch.float16, device="cuda")
+            for a in range(first, end, 128):
+                b = min(a + 128, end)
+                ops.tree_attention(q_rot[a:b], view, 0, where["positions"][b - 1:b] + 1, past[r] + b - first, out=out[a - first:b - first])
+            torch.cuda.synchronize()
+            keys, values = view.read_logical(0, 0, past[r] + n)
+            assert torch.equal(keys[past[r]:], k_rot[first:end]) and torch.equal(values[past[r]:], v[first:end])
+            seen = torch.arange(past[r] + n, device="cuda")[None, :] <= torch.arange(past[r], past[r] + n, device="cuda")[:, None]
+            ref, limit = _attention_and_limit(torch, q_rot[first:end], keys, values, seen)
+            assert ((out.double() - ref).abs() <= limit).all()
+            past[r] += n
+            first = end
+    assert batch.kv_lens.tolist() == past == [501, 387]
+
+
+def test_trees_on_a_batch_and_rows_that_are_not_accepted(gpu, orc):
+    """Two requests, each with a draft tree a step: rows in places that follow each other, rotary positions by depth, masked attention, acceptance,
+    compaction in the request's table, and the length set back to what was accepted before the next plan."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    from cpm.cu_amd.kvcache import PagedKVCache
+    Hq, Hkv, max_rows, vocab = 8, 2, 300, 1000
+    cache = PagedKVCache(1, Hkv, 6)
+    batch = ops.PageBatch(cache, 2, 3)
+    inv_freq = _freq(torch, 64)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    history = [(torch.empty((0, Hkv, D), dtype=torch.float16, device="cuda"),) * 2 for _ in range(2)]
+
+    def append(seed, new, positions=None):
+        x = _rows(torch, seed, 0, max_rows, (Hq + 2 * Hkv) * D)
+        q, k, v = (t.view(max_rows, -1, D) for t in x.split([Hq * D, Hkv * D, Hkv * D], 1))
+        where = batch.plan(torch.tensor(new, dtype=torch.int32, device="cuda"), max_rows)
+        positions = where["positions"] if positions is None else positions
+        q_rot = ops.kv_append_slots(cache, 0, k, v, where["slots"], q=q, positions=positions, inv_freq=inv_freq)
+        return where, q_rot, ops.rope_rows(k, None, positions, inv_freq)[0], v
+
+    _, _, k_rot, v = append(1, [40, 250])
+    history = [(k_rot[:40], v[:40]), (k_rot[40:290], v[40:290])]
+    accepted = []
+    for step in range(4):
+        past = [h[0].shape[0] for h in history]
+        trees = [synth.random_tree(T, 10 * step + r, max_children=3, max_depth=6) for r, T in enumerate((7, 20))]
+        cached = batch.kv_lens.clone()  # (the plan counts the trees' rows)
+        positions = np.full(max_rows, -1, np.int32)
+        positions[:27] = np.concatenate([t.positions(P) for t, P in zip(trees, past)])
+        where, q_rot, k_rot, v = append(10 + step, [7, 20], dev(positions))
+        assert where["positions"][:27].tolist() == [P + i for t, P in zip(trees, past) for i in range(t.T)]
+        for r, (tree, first) in enumerate(zip(trees, (0, 7))):
+            T, rows, view, mask = tree.T, slice(first, first + tree.T), batch.cache_of(r), dev(tree.mask.view(np.int64))
+            out = ops.tree_attention(q_rot[rows], view, 0, batch.kv_lens[r:r + 1], past[r] + T, mask)
+            torch.cuda.synchronize()
+            keys, values = view.read_logical(0, 0, past[r] + T)
+            assert torch.equal(keys, torch.cat([history[r][0], k_rot[rows]])) and torch.equal(values, torch.cat([history[r][1], v[rows]]))
+            bits = (tree.mask.reshape(T, -1)[:, :1] >> np.arange(T, dtype=np.uint64)[None, :]) & np.uint64(1)
+            seen = torch.cat([torch.ones((T, past[r]), dtype=torch.bool), torch.from_numpy(bits.astype(bool))], 1).cuda()
+            ref, limit = _attention_and_limit(torch, q_rot[rows], keys, values, seen)
+            assert ((out.double() - ref).abs() <= limit).all()
+            gt = synth.rng(step, 60 + r).integers(0, vocab, T).astype(np.int32)
+            ids, _ = synth.draft_ids_for_accept(tree, gt, min(step, int(tree.depth.max())), vocab, 100 * step + r)
+            a, _, path = orc.tree_accept(ids, gt, tree.positions(past[r]), past[r], tree.mask, tree.parent)
+            pred = dev(ids.astype(np.int32))
+            best = ops.tree_accept(pred, dev(gt), dev(tree.positions(past[r])), cached[r:r + 1], mask, dev(tree.parent))
+            ops.kv_compact(view, pred, dev(gt), cached[r:r + 1], best, T)
+            batch.kv_lens[r:r + 1] = cached[r:r + 1] + best[:1]
+            torch.cuda.synchronize()
+            assert int(best[0]) == a
+            accepted.append(a)
+            history[r] = tuple(torch.cat([h, new[rows][torch.from_numpy(np.asarray(path[:a], np.int64)).cuda()]]) for h, new in zip(history[r], (k_rot, v)))
+            assert batch.kv_lens[r].item() == past[r] + a
+            keys, values = view.read_logical(0, 0, past[r] + a)
+            assert torch.equal(keys, history[r][0]) and torch.equal(values, history[r][1])
+    assert min(accepted) == 1 and max(accepted) >= 3 and batch.held.tolist() == [1, 2]
+    pages = [p for r in range(2) for p in batch.block_tables[r, :batch.held[r]].tolist()] + batch.free_pages[:batch.counts[0]].tolist()
+    assert sorted(pages) == list(range(6))
+
+
 def test_batch_operators_in_a_graph(gpu):
     """A captured step on static buffers, replayed with other lengths and rows, between eager calls: each replay as the eager call."""
     torch = gpu
