@@ -703,7 +703,8 @@ int cpmcu_quantize_rows(const void* x, int64_t x_stride, int n, int K, int8_t* x
 size_t cpmcu_int8_weight_bytes(int V, int K);
 int cpmcu_int8_weight_tile(const int8_t* w, int V, int K, int8_t* w_tiled, void* stream);
 /* out[t][c] = (sum over k of xq[t][k] w[c][k]) * (x_scales[t] * w_scales[c]), [n][V] in the element type: the sum exact in 32-bit
- * integers, one rounding to float, one product, one rounding to the element type.  xq as cpmcu_quantize_rows leaves it (what lies
+ * integers, one rounding to float, one product, one rounding to the element type.  The scales' product is formed first, as a float: where
+ * that is infinite so is the result (NaN where the sum is 0), and where it is below 2^-126 it has lost bits.  xq as cpmcu_quantize_rows leaves it (what lies
  * behind column K does not matter), w_tiled as cpmcu_int8_weight_tile does; out apart from the inputs.  K <= 131071. */
 int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_tiled, const float* w_scales, int n, int V, int K, void* out,
                       void* stream);

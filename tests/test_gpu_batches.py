@@ -682,6 +682,23 @@ def test_int8_linear_with_results_beyond_2_gib(gpu, int8_shape, shape):
     _close(got[some], ref, 0, ref.abs() * 2.0 ** -22)
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n", [1, 20, 70, 400])
+def test_int8_linear_with_scales_at_the_ends_of_32_bits(gpu, set_option, dtype, n):
+    """The scales' product comes first: infinite or below the smallest float it is the result's too, whatever the sum; up to there all is finite."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    set_option("dtype", dtype)
+    V, K = 40, 64
+    xq, w = torch.ones((n, K), dtype=torch.int8, device="cuda"), torch.ones((V, K), dtype=torch.int8, device="cuda")
+    w[1] = -1
+    w[2, ::2] = -1  # the sum is 0
+    sums = torch.tensor([64.0, -64.0, 0.0] + [64.0] * (V - 3), device="cuda").expand(n, V)
+    for s, sw, want in ((2.0 ** 100, 2.0 ** 100, sums * float("inf")), (2.0 ** -100, 2.0 ** -100, sums * 0.0), (2.0 ** 100, 2.0 ** -100, sums), (2.0 ** -126, 2.0 ** 120, sums * 2.0 ** -6), (0.0, 5.0, sums * 0.0)):
+        got = ops.int8_linear(xq, torch.full((n,), s, device="cuda"), ops.Int8Weight(w, torch.full((V,), sw, device="cuda"))).view(_types(torch, dtype)).float()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+
+
 def test_int8_weight_from_16_bits(gpu):
     """Weights and rows quantised here: the product is near the 16-bit one, by at most half a step of either side's 8 bits a column."""
     torch = gpu
