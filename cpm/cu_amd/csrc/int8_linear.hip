@@ -531,10 +531,12 @@ __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_ke
 
 // The shapes, and what they cost, fitted to 448 sizes of 1 to 8192 rows, 512 to 73448 channels and 512 to 16384 columns: `start` us of a launch; for a
 // round (a tile on every CU) `round` us and `step` more for every 64 columns, `busy` more of them where all CUs work; and `whole` says how much of a
-// last round that is not full counts as a full one.  The choice is the shape with the least cost, 0.4 % above the best of them in the mean and 11 % at
-// most (in us, rows x columns x channels: 1 x 4096 x 4608 16 x 32 split 5.6, 16 x 16 5.8, 32 x 64 7.8; 64 x 4096 x 4608 32 x 64 8.5, 16 x 64 split 9.6, 64 x 128
-// 12.0; 64 x 4096 x 4096 16 x 64 split 6.7, 32 x 64 8.4; 256 x 4096 x 4608 64 x 128 12.6, 32 x 64 15.7, 64 x 256 19.4; 333 x 4099 x 12289 128 x 256 27.2,
-// 64 x 128 33.1, 64 x 256 33.8, 256 x 256 46.7; 2048 x 4096 x 16384: 256 x 256 117, 128 x 256 125, 64 x 256 136).
+// last round that is not full counts as a full one.  The choice is the shape with the least cost: against the best of the eight, timed again, 0.8 % more in
+// the mean of those sizes and 12 % at most (0.3 us), and 1.8 % and 52 % (600 rows of 64 columns to 4096 channels: 7.4 us, 4.9) over 182 sizes that
+// were no part of the fit, 64 to 500 channels or columns among them (profiles/int8_linear_shapes.txt; `python -m cpm.cu_amd.sweep int8` times them).
+// In us, rows x columns x channels: 1 x 4096 x 4608 16 x 32 split 5.7, 16 x 16 6.0, 32 x 64 7.7; 64 x 4096 x 4608 32 x 64 8.4, 16 x 64 split 9.6, 64 x 128
+// 12.1; 64 x 4096 x 4096 16 x 64 split 6.8, 32 x 64 8.3; 256 x 4096 x 4608 64 x 128 12.3, 32 x 64 15.5, 64 x 256 19.1; 333 x 4099 x 12289 128 x 256 26.8,
+// 64 x 128 33.0, 64 x 256 33.9, 256 x 256 46.1; 2048 x 4096 x 16384: 256 x 256 115, 128 x 256 127, 64 x 256 135.
 struct Variant {
     const char* name;
     void (*f16_kernel)(LinearParams);

@@ -16,6 +16,8 @@
     python -m cpm.cu_amd.sweep softmax                log-softmax of fp16 rows: one workgroup per row beside the operator's own choice (slices)
     python -m cpm.cu_amd.sweep window                 the drafter layer's attention (k queries, block window of 1024 tokens): the
                                                       library's plan beside both split shapes and forced split counts
+    python -m cpm.cu_amd.sweep int8                   8-bit product: every shape of its kernels beside the library's choice, at the sizes that the
+                                                      choice's costs were fitted to and at others (rows x channels x columns)
 
 Eager launches on cuda:0, random fp16 data, event-timed; attention rotates over several layers' K/V pools and the heads over
 copies of the weight matrix, so that no pass is served from the last-level cache.  Fractions are of 8 TB/s (heads) and TFLOP/s
@@ -251,8 +253,50 @@ def window(torch):
             del cache
 
 
+# The sizes that choose_variant's constants were fitted to, and sizes kept out of the fit (few channels or columns among them): rows, (channels, columns).
+INT8_FITTED = ([1, 5, 12, 16, 17, 24, 32, 40, 48, 64, 80, 96, 100, 128, 160, 200, 256, 300, 333, 400, 512, 700, 1000, 1500, 2048, 3000, 4096, 8192],
+               [(512, 512), (1000, 1000), (2560, 4096), (4608, 4096), (4096, 4096), (4096, 12288), (4096, 16384), (12289, 4099), (16384, 4096), (32768, 4096), (73448, 4096), (6000, 2048), (8192, 1024),
+                (24576, 2560), (1536, 6144), (10240, 8192)])
+INT8_OTHER = ([1, 8, 20, 36, 56, 90, 150, 222, 350, 600, 900, 2000, 5000],
+              [(1, 4096), (64, 4096), (128, 2048), (200, 8192), (400, 400), (3000, 300), (8192, 200), (30000, 128), (4096, 64), (2560, 1024), (6144, 1536), (5120, 5120), (14336, 4096), (100000, 2048)])
+
+
+def int8(torch):
+    from . import lib, ops
+    L, shapes = lib.get(), 8
+    names = []
+    for i in range(shapes):
+        L.set_option(b"int8_linear_shape", i)
+        names.append(ops.int8_linear_plan(1, 16, 64)[0].replace("int8_linear_", "").replace("_kernel", ""))
+    print("us a call by shape: " + " ".join(names))
+    print("%7s %9s %8s" % ("rows", "channels", "columns") + "".join("%9d" % i for i in range(shapes)))
+    for part, (rows, weights) in (("fitted", INT8_FITTED), ("others", INT8_OTHER)):
+        print(part, flush=True)
+        for V, K in weights:
+            padded = (K + 63) // 64 * 64
+            data = lambda *size: (torch.randn(size, device="cuda") * 32).round().clamp(-127, 127).to(torch.int8)  # noqa: E731
+            w = [ops.Int8Weight(data(V, K), torch.rand(V, device="cuda")) for _ in range(3)]
+            for n in rows:
+                x, scales, out = [data(n, padded) for _ in range(3)], torch.rand(n, device="cuda") * 0.001, torch.empty((n, V), dtype=torch.float16, device="cuda")
+                line, reps = "%7d %9d %8d" % (n, V, K), max(3, min(60, int(2e13 / (2.0 * n * V * K))))
+                for i in range(shapes):
+                    if i < 3 and n * V * K > 3e11:  # (split shapes of as many rows: far behind)
+                        line += "%9s" % "-"
+                        continue
+                    L.set_option(b"int8_linear_shape", i)
+                    turn = [0]
+
+                    def call():
+                        turn[0] = (turn[0] + 1) % 3
+                        ops.int8_linear(x[turn[0]], scales, w[turn[0]], out=out)
+                    call()
+                    line += "%9.2f" % min(_time(torch, call, reps) for _ in range(4))
+                print(line, flush=True)
+    L.set_option(b"int8_linear_shape", -1)
+
+
 def main(argv):
-    if not argv or argv[0] not in ("attention", "head", "frspec", "topk", "softmax", "window"):
+    if not argv or argv[0] not in ("attention", "head", "frspec", "topk", "softmax", "window", "int8"):
         print(__doc__)
         return 2
     import torch
@@ -270,6 +314,8 @@ def main(argv):
         softmax(torch)
     elif argv[0] == "window":
         window(torch)
+    elif argv[0] == "int8":
+        int8(torch)
     else:
         frspec(torch)
     return 0

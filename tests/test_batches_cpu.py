@@ -211,6 +211,27 @@ def test_int8_linear_plans():
             lib.get().set_option(b"int8_linear_shape", value)
 
 
+def test_int8_linear_choices_against_the_times_of_every_shape():
+    """What the choice costs over the best shape in the committed table of `python -m cpm.cu_amd.sweep int8`: the figures that stand beside the costs, at the
+    sizes they were fitted to and at those that were not."""
+    import os
+    from cpm.cu_amd import ops, sweep
+    lines = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "profiles", "int8_linear_shapes.txt")).read().splitlines()
+    names = lines[0].split(": ")[1].split()
+    over, part = dict(fitted=[], others=[]), None
+    for fields in map(str.split, lines[2:]):
+        if len(fields) == 1:
+            part = fields[0]
+            continue
+        n, V, K = map(int, fields[:3])
+        times = [math.inf if t == "-" else float(t) for t in fields[3:]]
+        chosen = ops.int8_linear_plan(n, V, K)[0].replace("int8_linear_", "").replace("_kernel", "")
+        over[part].append(((n, V, K), times[names.index(chosen)] / min(times)))
+    for part, (rows, weights), mean, worst in (("fitted", sweep.INT8_FITTED, 1.009, 1.13), ("others", sweep.INT8_OTHER, 1.019, 1.52)):
+        assert [size for size, _ in over[part]] == [(n, V, K) for V, K in weights for n in rows]
+        assert np.mean([x for _, x in over[part]]) < mean and max(x for _, x in over[part]) < worst
+
+
 def test_binding_refuses_host_tensors_and_counts_arguments():
     import torch
     from cpm.cu_amd import ops
