@@ -55,8 +55,8 @@ __device__ inline int wave_totals(int v, int cap) {
 // A wave looks up RUNS runs of 64 rows at once: the requests of their first rows with the whole wave in two reads of LDS, and each row's by
 // halving what lies between, which is nothing where requests have many rows.  One run where a workgroup per CU covers all rows, four beyond
 // (the runs' round trips overlap).  4096 requests' single rows 9.0 us with one run and 11.3 with four, a million rows of 4096 requests
-// 21.2 and 16.8.  1.1 million rows of 1000 requests: 11.8 us, of which 8.8 MB written are 1.8; the totals take 5, the round trips behind
-// them (row to request, to page, to slot) the rest.
+// 21.2 and 16.8.  1.1 million rows of 1000 requests: 11.7 us, of which a launch that loads the lengths and ends there takes 2.2, the totals
+// 1.4 more, the rows' requests and the stores 4.9 (8.8 MB, 1.8 at a copy's rate), and the loads of their pages the last 3.2.
 template <int THREADS, int EACH, int RUNS>
 __global__ __launch_bounds__(THREADS) void batch_tables_kernel(TableParams p) {
     constexpr int kMost = THREADS * EACH, kWaves = THREADS / 64;

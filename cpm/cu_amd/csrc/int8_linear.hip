@@ -452,6 +452,7 @@ __global__ __launch_bounds__(64 * WX * WV * KS, WX * WV * KS / 4) void int8_line
 // LDS and a CU takes each once.  A step is requested three in advance and has to be there one early, as above.  A CU with 256 x 256 to do takes
 // 0.6 us a step where few CUs run and 0.8 to 0.9 where all do, of which the matrix cores need 0.43 at their peak: 2260 TOP/s at 8192 x 4096 x 16384 (rows,
 // columns, channels), 2510 at 8192 x 16384 x 4096, 10 % more on zeros, which draw less power; deeper rings and other orders of the tiles change nothing.
+// LDS needs as long as the matrix cores: eight waves read 12 KiB a step and 32 KiB are written, 1024 cycles at 128 bytes each, so the two have to run side by side whole.
 template <typename E, int NX, int NV, int WX, int WV>
 __global__ __launch_bounds__(64 * WX * WV, WX * WV / 4) void int8_linear_wide_kernel(LinearParams p) {
     constexpr int kWaves = WX * WV, kRows = WX * NX, kChannels = WV * NV, kStages = 4, kStageBytes = (kRows + kChannels) * kTile, kHalf = NX / 2;

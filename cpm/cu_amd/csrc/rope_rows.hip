@@ -96,6 +96,8 @@ struct WideItem {
         }
     }
 };
+// Rows off 16 bytes and rotary parts that are no whole pieces: two 2-byte values an item, with the same two divisions, and so bound by instructions: 8191 rows
+// of 40 heads with 42 of 128 values turned 77 us (2.2 TB/s), with 64 turned in pieces 32.
 template <typename E, bool IL>
 struct NarrowItem {
     static constexpr int kWidth = 1;
@@ -218,6 +220,8 @@ __device__ inline int slot_of(const SlotParams& p, int r) {
 // the first row of a run of consecutive slots inside such a group writes all of the run, up to fifteen rows beyond its own: pieces are
 // whole wherever the rows of a request follow each other, however a workgroup's rows lie to the groups.  64 rows fill whole lines of four groups; where
 // that leaves CUs idle, 16 rows do.  Everything is requested before anything is known of the slots: a decode step's rows are one round trip.
+// 4001 rows of 4 heads: 6.1 us, K's workgroups alone 3.3, V's 5.6; with V's columns read without bank conflicts (65 % of LDS's cycles are) 5.6 and 5.0, with none
+// read at all no less: what is left is the way from memory to memory.  8192 rows of 32 + 2 heads do not show it (26.4 us either way).
 template <int ROWS>
 struct VStage {
     int slot[ROWS + 16];  // [i + 1]: row i of the workgroup's, -1: none
