@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(HERE, "libcpmcu_amd.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["runtime.hip", "tree_attention.hip", "lm_head.hip", "topk.hip", "tree_accept.hip", "draft_tree.hip", "batch_tables.hip", "rope_rows.hip", "int8_linear.hip"]
+HIP_SOURCES = ["runtime.hip", "tree_attention.hip", "lm_head.hip", "topk.hip", "tree_accept.hip", "draft_tree.hip", "batch_tables.hip", "rope_rows.hip", "int8_linear.hip",
+               "prompt_attention.hip", "decode_attention.hip", "adjust_logits.hip"]
 TIMELINE_SOURCES = ["tree_attention.hip", "lm_head.hip", "topk.hip"]  # kernels with optional wall-clock stamps (csrc/timeline.h)
 TIMELINE_LIB_PATH = os.path.join(HERE, "libcpmcu_amd_timeline.so")  # loaded only by `python -m cpm.cu_amd.timeline`
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".h"))

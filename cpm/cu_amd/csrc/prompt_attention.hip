@@ -1,0 +1,559 @@
+// Causal attention of the new rows of several requests over their pages: whole prompts, chunks far into a context, single rows between them.
+//
+//   out[t][h] = sum_x p_x v[x] / sum_x p_x,  p_x = exp(scale (q[t][h] . k[x] - max)),  x from 0 to the row's own position,
+//
+// k and v the tokens of the row's request and of the KV head of h.  The rows of a request and the heads on one KV head are one matrix of
+// rows (token-major), cut into tiles of 256; a workgroup takes a tile, or a part of its keys, through them 64 at a time, with the running
+// maximum and sum of its softmax.  What bounds it: 4 * 128 operations a row, head and key on the matrix cores, twice as many vector
+// operations a score as the matrix cores need cycles for it hidden behind them, and K and V out of L2 once for every 256 rows.
+//
+// Which tiles there are follows from lengths that only the device knows, so a launch of one workgroup lists them first: longest first, those
+// that would outlast the others by much cut into pieces, which a third launch joins.
+#include "batch_attention.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace cpmcu {
+namespace {
+
+constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kWaveRows = 32, kTileRows = kWaves * kWaveRows;
+constexpr int kStages = 4;
+constexpr int kKBytes = kTileKeys * kHeadDim * 2, kStageBytes = 2 * kKBytes;
+constexpr float kLazyLog2 = 8.f;  // how far scores may pass the softmax reference before it follows, in powers of two
+
+// ---- the list of work ----
+
+// The keys [begin, end) * 64 for rows [256 tile, 256 tile + 256) of the packed rows of a request whose `rows` rows start at row0 of the batch and
+// at position p0.  slot: where its part of the results waits for the others, -1 if it has all of its keys.
+struct Work {
+    int row0, rows, p0, request, tile, begin, end, slot;
+};
+// A tile in `pieces` parts, from slot on.
+struct Join {
+    int row0, rows, tile, slot, pieces, pad[3];
+};
+struct Listed {
+    int works, joins, pad[6];
+};
+constexpr int kPlanThreads = 1024, kPlanEach = kMostRequests / kPlanThreads;
+// Pieces are made where fewer than kParts of them, on all KV heads, would each have kLeastKeys tiles of keys or more.
+constexpr int kParts = 512, kLeastKeys = 24;
+
+struct PlanParams {
+    const int32_t *row_offsets, *positions;
+    int num_requests, max_blocks, n, group, Hkv, most_tiles;
+    Listed* listed;
+    Work* works;
+    Join* joins;
+};
+
+// Totals in front of each thread over the workgroup, `most` at most (they stop there, so their grouping does not matter).
+__device__ inline int totals_before(int v, int most, int* wave_total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int from = __shfl_up(v, d);
+        if (lane >= d) v = min(v + from, most);
+    }
+    if (lane == 63) wave_total[wave] = v;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < wave; ++w) before = min(before + wave_total[w], most);
+    const int lanes = __shfl_up(v, 1);
+    return min(before + (lane > 0 ? lanes : 0), most);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(PlanParams p) {
+    constexpr int kClasses = 64;
+    __shared__ int tile_end[kMostRequests], row0[kMostRequests], rows[kMostRequests], first[kMostRequests];
+    __shared__ int wave_total[kPlanThreads / 64], in_class[kClasses], class_at[kClasses], longest, slots, joins;
+    __shared__ unsigned long long cost;
+    const int tid = threadIdx.x, B = p.num_requests;
+    if (tid < kClasses) in_class[tid] = 0;
+    if (tid == 0) {
+        cost = 0;
+        longest = slots = joins = 0;
+    }
+    int tiles[kPlanEach], mine = 0;
+#pragma unroll
+    for (int e = 0; e < kPlanEach; ++e) {
+        const int r = tid * kPlanEach + e;
+        int lo = 0, count = 0, p0 = -1;
+        if (r < B) {
+            lo = min(max(p.row_offsets[r], 0), p.n);
+            count = min(max(p.row_offsets[r + 1], lo), p.n) - lo;
+            if (count > 0) p0 = p.positions[lo];
+            const int64_t room = (int64_t)p.max_blocks * kPage - p0;
+            count = p0 < 0 ? 0 : (int)min((int64_t)count, max(room, (int64_t)0));
+        }
+        tiles[e] = (int)(((int64_t)count * p.group + kTileRows - 1) / kTileRows);
+        mine = min(mine + tiles[e], p.most_tiles);
+        row0[r] = lo;
+        rows[r] = count;
+        first[r] = p0;
+    }
+    int before = totals_before(mine, p.most_tiles, wave_total);
+#pragma unroll
+    for (int e = 0; e < kPlanEach; ++e) {
+        before = min(before + tiles[e], p.most_tiles);
+        tile_end[tid * kPlanEach + e] = before;
+    }
+    __syncthreads();
+    const int all = tile_end[kMostRequests - 1];
+    const auto request_of = [&](int t) {
+        int lo = 0, hi = B - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (tile_end[mid] > t) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    };
+    const auto keys_of = [&](int t, int r, int& tile) {  // tiles of 64 keys that the last row of this tile sees
+        tile = t - (r > 0 ? tile_end[r - 1] : 0);
+        const int last = min(rows[r] - 1, (int)(((int64_t)(tile + 1) * kTileRows - 1) / p.group));
+        return (first[r] + last) / kTileKeys + 1;
+    };
+    unsigned long long sum = 0;
+    for (int t = tid; t < all; t += kPlanThreads) {
+        int tile;
+        sum += keys_of(t, request_of(t), tile);
+    }
+    atomicAdd(&cost, sum);
+    __syncthreads();
+    const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts);
+    const int chunk = (int)min(max(share, (int64_t)kLeastKeys), (int64_t)INT32_MAX);
+    const auto pieces_of = [&](int keys) { return (keys + chunk - 1) / chunk; };
+    int most = 0;
+    for (int t = tid; t < all; t += kPlanThreads) {
+        int tile;
+        const int keys = keys_of(t, request_of(t), tile), pieces = pieces_of(keys);
+        most = max(most, (keys + pieces - 1) / pieces);
+    }
+    atomicMax(&longest, most);
+    __syncthreads();
+    // longest first: counted by length in 64 classes, then put in their places
+    const auto class_of = [&](int length) { return kClasses - 1 - (int)((int64_t)length * (kClasses - 1) / max(longest, 1)); };
+    for (int t = tid; t < all; t += kPlanThreads) {
+        int tile;
+        const int keys = keys_of(t, request_of(t), tile), pieces = pieces_of(keys);
+        atomicAdd(&in_class[class_of((keys + pieces - 1) / pieces)], pieces);
+    }
+    __syncthreads();
+    if (tid < 64) {
+        int upto = in_class[tid];
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int from = __shfl_up(upto, d);
+            if (tid >= d) upto += from;
+        }
+        class_at[tid] = upto - in_class[tid];
+        if (tid == 63) p.listed->works = upto;
+    }
+    __syncthreads();
+    for (int t = tid; t < all; t += kPlanThreads) {
+        int tile;
+        const int r = request_of(t), keys = keys_of(t, r, tile), pieces = pieces_of(keys);
+        int at = atomicAdd(&class_at[class_of((keys + pieces - 1) / pieces)], pieces), slot = -1;
+        if (pieces > 1) {
+            slot = atomicAdd(&slots, pieces);
+            p.joins[atomicAdd(&joins, 1)] = Join{row0[r], rows[r], tile, slot, pieces, {0, 0, 0}};
+        }
+        for (int i = 0; i < pieces; ++i)
+            p.works[at + i] = Work{row0[r], rows[r], first[r], r, tile, (int)((int64_t)keys * i / pieces), (int)((int64_t)keys * (i + 1) / pieces), slot < 0 ? -1 : slot + i};
+    }
+    __syncthreads();
+    if (tid == 0) p.listed->joins = joins;
+}
+
+// ---- attention ----
+
+struct PromptParams {
+    BatchRows b;
+    const Listed* listed;
+    const Work* works;
+    const Join* joins;
+    float4* parts;  // [slot][KV head][wave][16 quads][64 lanes]: sums that have not been divided yet
+    float2* stats;  // [slot][KV head][256]: (reference in powers of two, sum)
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// K: a row of 256 bytes a key, its 16-byte pieces exchanged by the key's number; V: a row of 128 bytes a dim, by half of the dim's (even and
+// odd rows are in different halves of the banks).  Both ways the matrix operands are read without conflicts.
+__device__ inline int k_at(int key, int piece) { return key * 256 + ((piece ^ (key & 15)) << 4); }
+__device__ inline int v_at(int d, int piece) { return kKBytes + d * 128 + ((piece ^ ((d >> 1) & 7)) << 4); }
+
+// Two KB of a wave from memory to LDS, each lane's 16 bytes from where it says, in lane order from lds_at on.  Their arrival is counted by hand: written
+// as loads that the compiler knows, every read of LDS would wait for all of them.  One statement: nothing comes between m0 and its use.
+__device__ inline void request_pair(const void* base, uint32_t off_0, uint32_t off_1, uint32_t lds_at) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                 : : "v"(off_0), "v"(off_1), "s"(base), "s"(lds_at) : "memory", "m0");
+}
+
+template <typename E>
+__device__ inline bool any_not_finite(typename Elem<E>::x8 v) {  // an exponent of ones among eight values
+    constexpr uint32_t kOnes = Elem<E>::kDtype == 0 ? 0x7c00u : 0x7f80u;
+    const uint4 w = __builtin_bit_cast(uint4, v);
+    const auto has = [](uint32_t x) { return (x & kOnes) == kOnes || ((x >> 16) & kOnes) == kOnes; };
+    return has(w.x) || has(w.y) || has(w.z) || has(w.w);
+}
+template <typename E>
+__device__ inline bool not_finite(E v) {
+    constexpr uint32_t kOnes = Elem<E>::kDtype == 0 ? 0x7c00u : 0x7f80u;
+    return (__builtin_bit_cast(uint16_t, v) & kOnes) == kOnes;
+}
+
+template <typename E>
+__global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptParams p) {
+    typedef typename Elem<E>::x8 X8;
+    typedef typename Elem<E>::x4 X4;
+    typedef typename Elem<E>::x2 X2;
+    __shared__ __attribute__((aligned(1024))) char ring[kStages * kStageBytes];
+    __shared__ unsigned long long s_odd[2];  // keys of the tile with an infinity or NaN among their values
+    const BatchRows& b = p.b;
+    const int g = blockIdx.x % b.Hkv, index = blockIdx.x / b.Hkv;
+    // (the entry behind the list is memory too: one round trip for both)
+    const Work w = p.works[index];
+    if (index >= p.listed->works) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int qcol = lane & 31, hf = lane >> 5;
+    const int packed = w.rows * b.group, base_row = w.tile * kTileRows + wave * kWaveRows;
+    const int R = base_row + qcol, Rc = min(R, packed - 1);
+    const bool row_ok = R < packed, wave_ok = base_row < packed;
+    const int token = Rc / b.group, head = g * b.group + Rc % b.group;
+    const int pos = w.p0 + token;
+    const int wave_first = w.p0 + min(base_row, packed - 1) / b.group, wave_last = w.p0 + min(base_row + kWaveRows, packed) / b.group - (min(base_row + kWaveRows, packed) % b.group == 0 ? 1 : 0);
+    const int tile_first = w.p0 + w.tile * kTileRows / b.group;  // the position of the workgroup's first row
+    const int n = w.end - w.begin;
+
+    // Page numbers: 64 of them at a time, one a lane.
+    const int32_t* const table = b.block_tables + (size_t)w.request * b.max_blocks;
+    int pages_from = 0, pages = 0;
+    const auto load_pages = [&](int block) {
+        pages_from = block;
+        pages = page_within(table[min(block + lane, b.max_blocks - 1)], b.num_pages);
+    };
+    load_pages(w.begin * kTileKeys / kPage);
+
+    // What each lane requests of a tile: 2 KB of K's (8 keys) and of V's (16 dims) a wave, as two KB in lane order.
+    uint32_t k_off, v_off;
+    {
+        const int key = wave * 8 + (lane >> 4), d = wave * 16 + (lane >> 3);
+        k_off = (uint32_t)(key * kHeadDim + ((lane & 15) ^ (key & 15)) * 8) * 2u;
+        v_off = (uint32_t)(d * kPage + ((lane & 7) ^ ((d >> 1) & 7)) * 8) * 2u;
+    }
+    const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_ptr_t)ring + wave * (kKBytes / kWaves);
+    const auto request_tile = [&](int i) {
+        const int first = (w.begin + i) * kTileKeys, block = first / kPage, inside = first % kPage;
+        if (block - pages_from >= 64) load_pages(block);
+        const size_t page = (size_t)__builtin_amdgcn_readlane(pages, block - pages_from) * b.Hkv + g;
+        const uint32_t at = ring_at + (i % kStages) * kStageBytes;
+        // (four keys or eight dims on, the pieces' exchange differs in bit 2; the instruction adds 1 KB to both addresses)
+        request_pair(b.k_pool + (page * kPage + inside) * kHeadDim, k_off, k_off ^ 64u, at);
+        request_pair(b.v_pool + page * kHeadDim * kPage + inside, v_off, (v_off ^ 64u) + 8u * kPage * 2u - 1024u, at + kKBytes);
+    };
+
+    X8 qreg[8];  // Q as the second operand of S^T = K Q^T: lane (qcol, hf) has dims 16 ks + 8 hf + [0, 8)
+    {
+        const E* const row = reinterpret_cast<const E*>(b.q) + (int64_t)(w.row0 + token) * b.q_stride + head * kHeadDim;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const X8*>(row + 16 * ks + 8 * hf);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (tid < 2) s_odd[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i)
+        if (i < n) request_tile(i);
+
+    f32x16 oacc[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[db][r] = 0.f;
+    float m_ref = -INFINITY, l_run = 0.f;
+
+    for (int i = 0; i < n; ++i) {
+        // Tile i has arrived when at most the two behind it (four requests each) have not.
+        switch (min(n - 1 - i, kStages - 2)) {
+            case 0: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
+            case 1: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
+            default: asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); break;
+        }
+        __syncthreads();  // everybody's pieces are there, and everybody has left the tile before
+        if (i + kStages - 1 < n) request_tile(i + kStages - 1);
+        const int c0 = (w.begin + i) * kTileKeys;
+        char* const stage = ring + (i % kStages) * kStageBytes;
+        // A tile that not all rows see whole: a value that some row may not see must not reach its sum, not even as 0 times infinity.  (Behind
+        // the last row's position lies what the page held before.)
+        const bool edge = c0 + kTileKeys - 1 > tile_first;
+        unsigned long long odd = 0;
+        if (edge) {
+            unsigned long long found = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = tid * 2 + h, d = at >> 3, piece = at & 7;
+                const X8 v = *reinterpret_cast<const X8*>(stage + v_at(d, piece));
+                if (any_not_finite<E>(v)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (not_finite(v[e])) found |= 1ull << v_slot16(piece * 8 + e);
+                }
+            }
+            if (found) atomicOr(&s_odd[i & 1], found);
+            if (tid == 0) s_odd[(i + 1) & 1] = 0;
+            __syncthreads();
+            odd = s_odd[i & 1];
+        }
+        if (!wave_ok || c0 > wave_last) continue;
+
+        f32x16 sacc[2];
+        {
+            X8 kf[16];
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) kf[ks * 2 + kb] = *reinterpret_cast<const X8*>(stage + k_at(kb * 32 + qcol, 2 * ks + hf));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sacc[kb][r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) sacc[kb] = Elem<E>::mfma_32x32x16(kf[ks * 2 + kb], qreg[ks], sacc[kb]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // sacc[kb][r] is the score of key c0 + 32 kb + 8 (r / 4) + 4 hf + r % 4 for the row of qcol.
+        if (c0 + kTileKeys - 1 > wave_first) {
+            const int seen = pos - c0 - 4 * hf;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sacc[kb][r] = kb * 32 + 8 * (r >> 2) + (r & 3) <= seen ? sacc[kb][r] : -INFINITY;
+        }
+        float tmax = sacc[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, sacc[kb][r]);
+        {
+            // the row's other keys are 32 lanes away (assembly: the builtin hands back its first result twice; the wait states cover the write of tmax)
+            float mine = tmax, other = tmax;
+            asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(mine), "+v"(other));
+            tmax = fmaxf(mine, other) * b.scale_log2;
+        }
+        if (__any(tmax > m_ref + kLazyLog2)) {
+            const float m_new = fmaxf(m_ref, tmax), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
+            m_ref = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
+        }
+        const float m_scaled = m_ref == -INFINITY ? 0.f : m_ref;
+        X8 pb[4];  // P^T as the second operand of O^T = V^T P^T, rounded to the element type: step j has keys 16 j + {4 hf + [0, 4), 8 + 4 hf + [0, 4)}
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) pb[kb * 2 + (r >> 3)][r & 7] = (E)__builtin_amdgcn_exp2f(sacc[kb][r] * b.scale_log2 - m_scaled);
+        {
+            // the sum of what the product will see, in 32 bits
+            const X2 ones = {(E)1.f, (E)1.f};
+            float psum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const X2 pp = {pb[j][2 * e], pb[j][2 * e + 1]};
+                    psum = Elem<E>::dot2_acc(pp, ones, psum);
+                }
+            l_run += psum;
+        }
+        if (odd) {
+            // zeros for the product; then what rows do see is added by itself, value by value
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int db = 0; db < 4; ++db) {
+                    X8 v = *reinterpret_cast<const X8*>(stage + v_at(db * 32 + qcol, 2 * j + hf));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = not_finite(v[e]) ? (E)0.f : v[e];
+                    oacc[db] = Elem<E>::mfma_32x32x16(v, pb[j], oacc[db]);
+                }
+            for (unsigned long long rest = odd; rest; rest &= rest - 1) {
+                const int key = __builtin_ctzll(rest), half = (key >> 2) & 1;
+                float pk = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (16 * j + 4 * half + (e & 3) + 8 * (e >> 2) == key) pk = (float)pb[j][e];
+                pk = __shfl(pk, qcol + 32 * half);
+                const bool sees = c0 + key <= pos;
+                const int slot = v_slot16(key);
+                int at = (int)(stage - ring) + kKBytes + (slot & 7) * 2;
+                const char* const base = ring + 4 * hf * 128;
+#pragma unroll
+                for (int db = 0; db < 4; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        asm volatile("" : "+v"(at));  // (64 addresses worked out ahead would take the loop's registers)
+                        const int d = db * 32 + 8 * (r >> 2) + (r & 3);
+                        const E v = *reinterpret_cast<const E*>(base + at + d * 128 + (((slot >> 3) ^ (((d + 4 * hf) >> 1) & 7)) << 4));
+                        if (sees && not_finite(v)) oacc[db][r] += pk * (float)v;
+                    }
+            }
+            continue;
+        }
+        X8 vf[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int db = 0; db < 4; ++db) vf[j * 4 + db] = *reinterpret_cast<const X8*>(stage + v_at(db * 32 + qcol, 2 * j + hf));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int db = 0; db < 4; ++db) oacc[db] = Elem<E>::mfma_32x32x16(vf[j * 4 + db], pb[j], oacc[db]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!wave_ok) return;
+
+    // oacc[db][r] is dim 32 db + 8 (r / 4) + 4 hf + r % 4 of the row of qcol
+    const float l_all = l_run + __shfl_xor(l_run, 32);
+    if (w.slot >= 0) {
+        const size_t part = (size_t)w.slot * b.Hkv + g;
+        float4* const to = p.parts + (part * kWaves + wave) * 16 * 64;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int rq = 0; rq < 4; ++rq)
+                to[(db * 4 + rq) * 64 + lane] = make_float4(oacc[db][rq * 4], oacc[db][rq * 4 + 1], oacc[db][rq * 4 + 2], oacc[db][rq * 4 + 3]);
+        if (hf == 0) p.stats[part * kTileRows + wave * kWaveRows + qcol] = make_float2(m_ref, l_all);
+        return;
+    }
+    if (!row_ok) return;
+    const float inv = 1.f / l_all;
+    E* const row = reinterpret_cast<E*>(b.out) + (int64_t)(w.row0 + token) * b.out_stride + head * kHeadDim;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+            X4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (E)(oacc[db][rq * 4 + e] * inv);
+            *reinterpret_cast<X4*>(row + db * 32 + rq * 8 + hf * 4) = o;
+        }
+}
+
+// The pieces of a tile: with M the largest of their references m, sum = sum_i l_i 2^(m_i - M), out = sum_i O_i 2^(m_i - M) / sum, in the order of the
+// keys.  A workgroup a row block of 32.
+template <typename E>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
+    typedef typename Elem<E>::x4 X4;
+    const BatchRows& b = p.b;
+    const int block = blockIdx.x % kWaves, g = blockIdx.x / kWaves % b.Hkv, index = blockIdx.x / kWaves / b.Hkv;
+    const Join j = p.joins[index];
+    if (index >= p.listed->joins) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qcol = lane & 31, hf = lane >> 5;
+    const int R = j.tile * kTileRows + block * kWaveRows + qcol;
+    if (R >= j.rows * b.group) return;
+    float M = -INFINITY;
+    for (int i = 0; i < j.pieces; ++i) M = fmaxf(M, p.stats[((size_t)(j.slot + i) * b.Hkv + g) * kTileRows + block * kWaveRows + qcol].x);
+    const float m_scaled = M == -INFINITY ? 0.f : M;
+    float sum = 0.f;
+    f32x4 acc[4];
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) acc[rq] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < j.pieces; ++i) {
+        const size_t part = (size_t)(j.slot + i) * b.Hkv + g;
+        const float2 s = p.stats[part * kTileRows + block * kWaveRows + qcol];
+        const float f = __builtin_amdgcn_exp2f(s.x - m_scaled);
+        sum = __builtin_fmaf(s.y, f, sum);
+        const float4* const from = p.parts + (part * kWaves + block) * 16 * 64 + wave * 4 * 64 + lane;
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+            const f32x4 o = __builtin_bit_cast(f32x4, from[rq * 64]);
+            // (a piece that the row sees nothing of has zeros)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rq][e] = __builtin_fmaf(o[e], f, acc[rq][e]);
+        }
+    }
+    const float inv = 1.f / sum;
+    E* const row = reinterpret_cast<E*>(b.out) + (int64_t)(j.row0 + R / b.group) * b.out_stride + (g * b.group + R % b.group) * kHeadDim;
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+        X4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (E)(acc[rq][e] * inv);
+        *reinterpret_cast<X4*>(row + wave * 32 + rq * 8 + hf * 4) = o;
+    }
+}
+
+// ---- sizes ----
+
+struct Sizes {
+    int64_t tiles, slots, works, joins;
+    size_t works_at, joins_at, stats_at, parts_at, bytes;
+};
+Sizes sizes_of(int num_requests, int max_blocks, int n, int Hq, int Hkv) {
+    Sizes s;
+    // every request's last tile may be a part of one
+    s.tiles = ((int64_t)n * (Hq / Hkv)) / kTileRows + std::min(num_requests, n);
+    // A tile of t > chunk tiles of keys makes at most 2 t / chunk pieces, and chunk is at least the total over kParts / Hkv.  None is made of fewer than kLeastKeys.
+    const int64_t keys = (int64_t)max_blocks * (kPage / kTileKeys);
+    s.slots = keys <= kLeastKeys ? 0 : std::min<int64_t>(2 * ((kParts + Hkv - 1) / Hkv), s.tiles * ((keys + kLeastKeys - 1) / kLeastKeys));
+    s.joins = std::min(s.tiles, s.slots / 2);
+    s.works = s.tiles + s.slots;
+    s.works_at = sizeof(Listed);
+    s.joins_at = s.works_at + sizeof(Work) * (s.works + 1);
+    s.stats_at = align_up(s.joins_at + sizeof(Join) * (s.joins + 1), 256);
+    s.parts_at = s.stats_at + sizeof(float2) * kTileRows * s.slots * Hkv;
+    s.bytes = s.parts_at + sizeof(float) * kTileRows * kHeadDim * s.slots * Hkv;
+    return s;
+}
+
+}  // namespace
+}  // namespace cpmcu
+
+using namespace cpmcu;
+
+extern "C" size_t cpmcu_batch_prompt_attention_workspace_bytes(int num_requests, int max_blocks, int n, int Hq, int Hkv) {
+    if (num_requests < 1 || num_requests > kMostRequests || max_blocks < 1 || max_blocks > kMostBlocks || n < 0 || n >= 1 << 24 || Hkv < 1 || Hq < 1 || Hq > 1024 || Hq % Hkv) return 0;
+    return sizes_of(num_requests, max_blocks, n, Hq, Hkv).bytes;
+}
+
+extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, int num_pages, const int32_t* block_tables,
+                                      int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv,
+                                      float scale, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    BatchRows b{(const uint16_t*)q, (uint16_t*)out, q_stride, out_stride, (const uint16_t*)k_pool, (const uint16_t*)v_pool, block_tables, row_offsets, positions,
+                num_requests, max_blocks, num_pages, n, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, scale * 1.44269504088896341f};
+    const int rc = check_batch_rows("prompt_attention", b, scale);
+    if (rc != CPMCU_OK) return rc;
+    if (n == 0) return CPMCU_OK;
+    CPMCU_CHECK_ARG(row_offsets, "prompt_attention: null pointer argument");
+    const Sizes s = sizes_of(num_requests, max_blocks, n, Hq, Hkv);
+    CPMCU_CHECK_ARG(workspace && workspace_bytes >= s.bytes, "prompt_attention: workspace of %zu bytes, %zu needed", workspace_bytes, s.bytes);
+    CPMCU_CHECK_ARG((uintptr_t)workspace % 16 == 0, "prompt_attention: the workspace has to lie on 16 bytes");
+    const int64_t grid = s.works * Hkv;
+    CPMCU_CHECK_ARG(grid <= INT32_MAX && s.joins * Hkv * kWaves <= INT32_MAX, "prompt_attention: %lld workgroups are beyond a launch", (long long)grid);
+    char* const ws = static_cast<char*>(workspace);
+    PlanParams plan{row_offsets, positions, num_requests, max_blocks, n, b.group, Hkv, (int)s.tiles, (Listed*)ws, (Work*)(ws + s.works_at), (Join*)(ws + s.joins_at)};
+    PromptParams p{b, plan.listed, plan.works, plan.joins, (float4*)(ws + s.parts_at), (float2*)(ws + s.stats_at)};
+    const hipStream_t st = resolve_stream(stream);
+    const bool bf = options().dtype == 1;
+    hipLaunchKernelGGL(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, plan);
+    CPMCU_LAUNCH_CHECK();
+    hipLaunchKernelGGL(bf ? prompt_attention_kernel<bf16> : prompt_attention_kernel<f16>, dim3((int)grid), dim3(kThreads), 0, st, p);
+    CPMCU_LAUNCH_CHECK();
+    if (s.joins > 0) {
+        hipLaunchKernelGGL(bf ? prompt_join_kernel<bf16> : prompt_join_kernel<f16>, dim3((int)(s.joins * Hkv * kWaves)), dim3(256), 0, st, p);
+        CPMCU_LAUNCH_CHECK();
+    }
+    return CPMCU_OK;
+}

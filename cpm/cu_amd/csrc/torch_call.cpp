@@ -482,6 +482,111 @@ PyObject* call_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return THPVariable_Wrap(std::move(made));
 }
 
+// Attention of a batch's rows over its pages: (q, k_pool, v_pool, block_tables, row_offsets or None, positions, scale, out).  The workspace is the call's own,
+// as the results are: calls on several streams, and captured ones, share nothing.
+decltype(&cpmcu_batch_prompt_attention) fn_prompt_attention = nullptr;
+decltype(&cpmcu_batch_prompt_attention_workspace_bytes) fn_prompt_attention_workspace_bytes = nullptr;
+decltype(&cpmcu_batch_decode_attention) fn_decode_attention = nullptr;
+decltype(&cpmcu_batch_decode_attention_workspace_bytes) fn_decode_attention_workspace_bytes = nullptr;
+template <bool PROMPT>
+PyObject* batch_attention(PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 8)) return nullptr;
+    Call call;
+    HeadRows q, out;
+    const char* const pools = "batch attention: pools of 16-bit floats";
+    if (!head_rows(call, args[0], "batch attention: q of 16-bit floats", &q) || !head_rows(call, args[7], "batch attention: out of 16-bit floats", &out)) return nullptr;
+    const at::Tensor *k_pool = call.dense(args[1], at::kHalf, pools), *v_pool = k_pool ? call.dense(args[2], at::kHalf, pools) : nullptr, *offsets = nullptr;
+    const at::Tensor *tables = v_pool ? call.dense(args[3], at::kInt, "batch attention: int32 block_tables") : nullptr,
+                     *pos = tables ? call.dense(args[5], at::kInt, "batch attention: int32 positions") : nullptr;
+    float scale;
+    if (!pos || ((PROMPT || args[4] != Py_None) && !(offsets = call.dense(args[4], at::kInt, "batch attention: int32 row_offsets"))) || !convert(args[6], &scale)) return nullptr;
+    if (!expect(k_pool->dim() == 4 && k_pool->size(2) == CPMCU_PAGE_SIZE && k_pool->size(3) == CPMCU_HEAD_DIM && v_pool->dim() == 4 && v_pool->size(0) == k_pool->size(0) &&
+                    v_pool->size(1) == k_pool->size(1) && v_pool->size(2) == CPMCU_HEAD_DIM && v_pool->size(3) == CPMCU_PAGE_SIZE && k_pool->size(0) <= INT32_MAX && k_pool->size(1) <= INT32_MAX,
+                "batch attention: pools are [pages, Hkv, 256, 128] and [pages, Hkv, 128, 256]") ||
+        !expect(alike(q, out) && q.dim == CPMCU_HEAD_DIM && pos->numel() == q.n, "batch attention: q and out are [n, Hq, 128], positions [n]") ||
+        !expect(tables->dim() == 2 && tables->size(0) <= INT32_MAX && tables->size(1) <= INT32_MAX && (!offsets || offsets->numel() == tables->size(0) + 1),
+                "batch attention: block_tables are [B, max_blocks], row_offsets [B + 1]"))
+        return nullptr;
+    const int B = static_cast<int>(tables->size(0)), M = static_cast<int>(tables->size(1)), n = static_cast<int>(q.n), Hq = static_cast<int>(q.heads), Hkv = static_cast<int>(k_pool->size(1));
+    int64_t bytes = 0;
+    if constexpr (PROMPT) bytes = static_cast<int64_t>(fn_prompt_attention_workspace_bytes(B, M, n, Hq, Hkv));
+    else bytes = static_cast<int64_t>(fn_decode_attention_workspace_bytes(B, M, Hq, Hkv));
+    at::Tensor ws;
+    if (n > 0 && bytes > 0) ws = new_tensor(*tables, at::kByte, at::IntArrayRef(&bytes, 1));
+    void* const st = call.stream();
+    return status(without_gil([&] {
+        const auto fn = PROMPT ? fn_prompt_attention : fn_decode_attention;
+        return fn(q.at, q.stride, k_pool->data_ptr(), v_pool->data_ptr(), static_cast<int>(k_pool->size(0)), ints(tables), M, offsets ? ints(offsets) : nullptr, ints(pos), B, n, Hq, Hkv,
+                  scale, out.at, out.stride, ws.defined() ? ws.data_ptr() : nullptr, static_cast<size_t>(bytes), st);
+    }));
+}
+PyObject* call_prompt_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return batch_attention<true>(args, nargs); }
+PyObject* call_decode_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return batch_attention<false>(args, nargs); }
+
+// adjust_logits(logits, penalties, tokens, lens, requests, bias_ids, bias_values, allowed, draft_ids, tree_mask, out, want_ids): ids [n] or None.  All but
+// logits and out may be None.
+decltype(&cpmcu_adjust_logits) fn_adjust_logits = nullptr;
+decltype(&cpmcu_adjust_logits_workspace_bytes) fn_adjust_logits_workspace_bytes = nullptr;
+PyObject* call_adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (!arguments(nargs, 12)) return nullptr;
+    Call call;
+    const at::Tensor* rows[2];
+    for (int i = 0; i < 2; ++i) {
+        rows[i] = call.strided(args[i ? 10 : 0], at::kHalf, "adjust_logits: rows of 16-bit floats");
+        if (!rows[i]) return nullptr;
+        if (!expect(rows[i]->dim() == 2 && (rows[i]->numel() == 0 || rows[i]->size(1) == 1 || rows[i]->stride(1) == 1) && rows[i]->size(0) <= INT32_MAX && rows[i]->size(1) <= INT32_MAX,
+                    "adjust_logits: [n, V] with whole rows required"))
+            return nullptr;
+    }
+    const at::Tensor &in = *rows[0], &out = *rows[1];
+    const int64_t n = in.size(0), V = in.size(1), words = (V + 31) / 32;
+    if (!expect(out.size(0) == n && out.size(1) == V, "adjust_logits: out is [n, V]")) return nullptr;
+    const at::Tensor* t[9] = {};  // args 1 to 9
+    const at::ScalarType types[9] = {at::kFloat, at::kInt, at::kInt, at::kInt, at::kInt, at::kFloat, at::kInt, at::kInt, at::kLong};
+    const char* const what[9] = {"adjust_logits: float32 penalties", "adjust_logits: int32 tokens", "adjust_logits: int32 lens", "adjust_logits: int32 requests", "adjust_logits: int32 bias_ids",
+                                 "adjust_logits: float32 bias_values", "adjust_logits: int32 allowed", "adjust_logits: int32 draft_ids", "adjust_logits: int64 tree_mask"};
+    for (int i = 0; i < 9; ++i)
+        if (args[1 + i] != Py_None && !(t[i] = i == 6 ? call.strided(args[1 + i], types[i], what[i]) : call.dense(args[1 + i], types[i], what[i]))) return nullptr;
+    const at::Tensor *penalties = t[0], *tokens = t[1], *lens = t[2], *requests = t[3], *bias_ids = t[4], *bias_values = t[5], *allowed = t[6], *draft_ids = t[7], *tree_mask = t[8];
+    const int64_t R = penalties ? penalties->numel() / 3 : bias_ids && bias_ids->dim() == 2 ? bias_ids->size(0) : 0;
+    if (!expect(!penalties || (penalties->dim() == 2 && penalties->size(1) == 3), "adjust_logits: penalties are [R, 3]") ||
+        !expect((tokens != nullptr) == (lens != nullptr) && (!tokens || (penalties && tokens->dim() == 2 && tokens->size(0) == R && lens->numel() == R)),
+                "adjust_logits: tokens [R, L] and lens [R] go together, with penalties") ||
+        !expect(!requests || requests->numel() == n, "adjust_logits: requests are [n]") ||
+        !expect((bias_ids != nullptr) == (bias_values != nullptr) && (!bias_ids || (bias_ids->dim() == 2 && bias_ids->size(0) == R && bias_values->sizes() == bias_ids->sizes())),
+                "adjust_logits: bias_ids and bias_values are [R, biases]") ||
+        !expect(!allowed || (allowed->dim() == 2 && allowed->size(0) == n && allowed->size(1) == words && (words == 1 || n == 0 || allowed->stride(1) == 1)),
+                "adjust_logits: allowed is [n, ceil(V / 32)] with whole rows") ||
+        !expect((draft_ids != nullptr) == (tree_mask != nullptr) && (!draft_ids || (draft_ids->numel() == n && tree_mask->dim() == 2 && tree_mask->size(0) == n)),
+                "adjust_logits: draft_ids [n] and tree_mask [n, words] go together") ||
+        !expect(R <= INT32_MAX && (!tokens || tokens->size(1) <= INT32_MAX) && (!bias_ids || bias_ids->size(1) <= INT32_MAX) && (!tree_mask || tree_mask->size(1) <= INT32_MAX),
+                "adjust_logits: sizes beyond 32 bits"))
+        return nullptr;
+    const bool no_text = tokens && tokens->size(1) == 0, no_bias = bias_ids && bias_ids->size(1) == 0;
+    const int want = PyObject_IsTrue(args[11]);
+    if (want < 0) return nullptr;
+    at::Tensor ids, ws;
+    int64_t bytes = 0;
+    if (want) {
+        ids = new_tensor(in, at::kInt, at::IntArrayRef(&n, 1));
+        bytes = V > 0 ? static_cast<int64_t>(fn_adjust_logits_workspace_bytes(static_cast<int>(n), static_cast<int>(V))) : 0;
+        if (bytes > 0) ws = new_tensor(in, at::kByte, at::IntArrayRef(&bytes, 1));
+    }
+    const auto i32 = [](const at::Tensor* x) { return x ? ints(x) : nullptr; };
+    const auto f32 = [](const at::Tensor* x) { return x ? static_cast<const float*>(x->data_ptr()) : nullptr; };
+    void* const st = call.stream();
+    const int rc = without_gil([&] {
+        return fn_adjust_logits(in.data_ptr(), n > 1 ? in.stride(0) : V, static_cast<int>(n), static_cast<int>(V), f32(penalties), no_text ? nullptr : i32(tokens), no_text ? nullptr : i32(lens),
+                                static_cast<int>(R), tokens ? static_cast<int>(tokens->size(1)) : 0, i32(requests), no_bias ? nullptr : i32(bias_ids), no_bias ? nullptr : f32(bias_values),
+                                bias_ids ? static_cast<int>(bias_ids->size(1)) : 0, allowed ? static_cast<const uint32_t*>(allowed->data_ptr()) : nullptr, allowed && n > 1 ? allowed->stride(0) : words,
+                                i32(draft_ids), tree_mask ? static_cast<const uint64_t*>(tree_mask->data_ptr()) : nullptr, tree_mask ? static_cast<int>(tree_mask->size(1)) : 0, out.data_ptr(),
+                                n > 1 ? out.stride(0) : V, want ? ints(&ids) : nullptr, ws.defined() ? ws.data_ptr() : nullptr, static_cast<size_t>(bytes), st);
+    });
+    if (rc != CPMCU_OK) return status(rc);
+    if (!want) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(ids));
+}
+
 // empty(like, dtype, rows, cols, dtype, rows, cols, ...): uninitialised [rows, cols] tensors ([rows] where cols is 0) on like's
 // device, as a tuple.  dtype: 'h' 16-bit float, 'f' fp32, 'i' int32, 'l' int64.
 PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -542,7 +647,10 @@ PyObject* bind(PyObject*, PyObject* handle) {
               find("cpmcu_tree_attention_workspace_bytes", &fn_tree_attention_workspace_bytes) && find("cpmcu_batch_tables", &fn_batch_tables) &&
               find("cpmcu_rope_rows", &fn_rope_rows) && find("cpmcu_kv_append_slots", &fn_kv_append_slots) &&
               find("cpmcu_quantize_rows", &fn_quantize_rows) && find("cpmcu_int8_linear", &fn_int8_linear) &&
-              find("cpmcu_int8_weight_bytes", &fn_int8_weight_bytes);
+              find("cpmcu_int8_weight_bytes", &fn_int8_weight_bytes) && find("cpmcu_batch_prompt_attention", &fn_prompt_attention) &&
+              find("cpmcu_batch_prompt_attention_workspace_bytes", &fn_prompt_attention_workspace_bytes) && find("cpmcu_batch_decode_attention", &fn_decode_attention) &&
+              find("cpmcu_batch_decode_attention_workspace_bytes", &fn_decode_attention_workspace_bytes) && find("cpmcu_adjust_logits", &fn_adjust_logits) &&
+              find("cpmcu_adjust_logits_workspace_bytes", &fn_adjust_logits_workspace_bytes);
 #define X(name) ok = ok && find("cpmcu_" #name, &fn_##name);
     CPMCU_TORCH_CALLS(X)
 #undef X
@@ -563,6 +671,9 @@ PyMethodDef g_methods[] = {
     X(quantize_rows)
     X(int8_linear)
     X(int8_weight_fits)
+    X(prompt_attention)
+    X(decode_attention)
+    X(adjust_logits)
     ENTRY("empty", empty)
     {"pinned", entry<pinned>, METH_O, nullptr},
     {"synchronize", entry<synchronize>, METH_NOARGS, nullptr},

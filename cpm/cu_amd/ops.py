@@ -260,6 +260,13 @@ class PageBatch:
         self._state.copy_(state)
         return dict(kv_lens=lens, held=held, counts=counts, row_offsets=offsets, positions=positions, slots=slots)
 
+    def attention(self, q, layer, where, single=False, scale=None, out=None):
+        """Every row of a plan (``where``) over its request's pages, behind the appends: prompt_attention, or, where no request has more than one row,
+        decode_attention (single)."""
+        if single:
+            return decode_attention(q, self.cache, layer, self.block_tables, where["positions"], where["row_offsets"], scale, out)
+        return prompt_attention(q, self.cache, layer, self.block_tables, where["row_offsets"], where["positions"], scale, out)
+
     def cache_of(self, r):
         """Request r's view of the cache, for tree_attention."""
         view = copy.copy(self.cache)
@@ -297,6 +304,48 @@ class Int8Weight:
 def int8_linear(xq, x_scales, weight, out=None):
     """[n, V] = (xq . weight^T in 32-bit integers) * x_scales * weight.scales, in 16 bits; xq and x_scales from quantize_rows."""
     return (_native or _calls()).int8_linear(xq, x_scales, weight.data, weight.scales, weight.V, weight.K, out)
+
+
+def prompt_attention(q, cache, layer, block_tables, row_offsets, positions, scale=None, out=None):
+    """Causal attention of the new rows q [n, Hq, 128] of several requests over their pages, in any mixture: prompts, chunks, single rows.
+
+    block_tables int32 [B, max_blocks], row_offsets int32 [B + 1] and positions int32 [n] as batch_tables gives them: request r's rows are
+    [row_offsets[r], row_offsets[r + 1]), the first at positions[row_offsets[r]], each sees the tokens of its request up to its own, which have been appended
+    (kv_append_slots).  Rows of refused requests, and behind the last one, keep what out held (a new tensor has no values there).  q and out may be
+    parts of wider rows; out may be q.  See PageBatch.attention.
+    """
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    (_native or _calls()).prompt_attention(q, cache.k[layer], cache.v[layer], block_tables, row_offsets, positions, _SCALE if scale is None else scale, out)
+    return out
+
+
+def decode_attention(q, cache, layer, block_tables, positions, row_offsets=None, scale=None, out=None):
+    """prompt_attention for requests of one new row each (a step of decoding): row r of q is request r's, or row row_offsets[r] where it has one; requests of
+    no row or of several are left out."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    (_native or _calls()).decode_attention(q, cache.k[layer], cache.v[layer], block_tables, row_offsets, positions, _SCALE if scale is None else scale, out)
+    return out
+
+
+def adjust_logits(logits, penalties=None, tokens=None, lens=None, requests=None, bias_ids=None, bias_values=None, allowed=None, draft_ids=None, tree_mask=None,
+                  out=None, want_ids=True):
+    """Penalties for repeated tokens, biases and masks on rows of logits [n, V], and their arg-max: (out, ids int32 [n] or None).
+
+    Of a token that stands c > 0 times in the text of its row's request the logit z becomes (z / repetition if z > 0 else z * repetition) - frequency * c -
+    presence; then its bias is added, and what is not allowed becomes minus infinity.  ids is the lowest index of a row's largest result, -1 where nothing is left.
+
+    penalties fp32 [R, 3]: (repetition, presence, frequency) of each request.  tokens int32 [R, L], of which lens int32 [R] count.  requests int32 [n]: each
+    row's request (-1: none); left out, row t is request t's, or all are of the only one.  bias_ids int32 / bias_values fp32 [R, up to 1024] (-1: not used).
+    allowed int32 [n, ceil(V / 32)]: bit v % 32 of word v / 32 (``mask.expand(n, -1)``: one for all rows).  draft_ids int32 [n] / tree_mask int64
+    [n, words]: the rows are the nodes of one request's draft tree, and the drafts on a node's way, its own among them, stand behind the request's tokens.
+    out may be logits (in place).
+    """
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    ids = (_native or _calls()).adjust_logits(logits, penalties, tokens, lens, requests, bias_ids, bias_values, allowed, draft_ids, tree_mask, out, want_ids)
+    return out, ids
 
 
 def gather_rows(src, remap):

@@ -711,6 +711,55 @@ int cpmcu_int8_linear(const int8_t* xq, const float* x_scales, const int8_t* w_t
 /* The kernel a cpmcu_int8_linear call of this shape launches and its workgroup count, without launching (the outputs may be NULL). */
 int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, size_t kernel_name_bytes, int* num_workgroups);
 
+/* Attention of the new rows of several requests over their pages, causal: row i of request r, the row t = row_offsets[r] + i of the batch at position
+ * x = positions[row_offsets[r]] + i, takes the keys and values of positions 0 to x of its request, its own among them (appended before:
+ * cpmcu_kv_append_slots).  Rows of a request follow each other in position, as cpmcu_batch_tables writes them; only its first row's is read.
+ *   q [n][q_stride], Hq heads of 128 values from the row's start; out alike, q's own rows (in place) or memory apart (columns apart of rows of one stride
+ *       are); rows and pools on 16 bytes.  Hq a multiple of Hkv, heads h * Hkv / Hq on KV head h.  n < 2^24.
+ *   block_tables int32[num_requests][max_blocks]: the page of position x is block_tables[r][x / 256] (read for positions that are attended
+ *       only; a number outside [0, num_pages) is taken as the nearest one inside).  At most 2^28 entries, 4096 requests, 2^18 blocks.
+ *   row_offsets int32[num_requests + 1], never falling; a request may have no rows.
+ *   Left out, with their results as they were: rows of a request whose first position is negative (refused ones), rows of positions from
+ *   max_blocks * 256 on, rows in front of row_offsets[0] and behind row_offsets[num_requests].
+ * Values that a row does not see -- later rows' keys and values, what a page holds behind the last token -- do not reach its result, infinities
+ * and NaN among them.  Scores, sums and statistics in 32 bits; probabilities are rounded to the element type before their product with V, whose sum is that of
+ * the rounded ones.  scale > 0.  Any mixture of rows and lengths: which work there is is listed on the device, long ones are cut and joined; nothing is
+ * read back, and a captured call may be replayed with other offsets, positions and tables.
+ *   workspace: at least cpmcu_batch_prompt_attention_workspace_bytes, on 16 bytes; its contents do not matter.  Calls that may overlap need one each. */
+size_t cpmcu_batch_prompt_attention_workspace_bytes(int num_requests, int max_blocks, int n, int Hq, int Hkv);
+int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, int num_pages, const int32_t* block_tables,
+                                 int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv, float scale,
+                                 void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for requests of one new row each: a step of decoding.  Row row_offsets[r] of the batch, or row r where row_offsets is NULL (n = num_requests then),
+ * is request r's; requests with no row, with several, or with a row of a negative position or one from max_blocks * 256 on are left out. */
+size_t cpmcu_batch_decode_attention_workspace_bytes(int num_requests, int max_blocks, int Hq, int Hkv);
+int cpmcu_batch_decode_attention(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, int num_pages, const int32_t* block_tables,
+                                 int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv, float scale,
+                                 void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Penalties for repeated tokens, biases and masks on n rows of logits, and their arg-max.  With c the times that token v stands in the text of the row's request:
+ *   z' = z where c = 0, else (z > 0 ? z / repetition : z * repetition) - frequency * c - presence;
+ *   z'' = z' + bias[v]; -infinity, whatever z is, where v is not allowed,
+ * in 32 bits, each operation rounded by itself, then once to the element type.
+ *   logits [n][logits_stride], V values from the row's start, V <= 2^24; out alike, the same memory and stride (in place) or memory apart.  Rows on 2 bytes;
+ *       logits and out at equal distances from 16 bytes are read and written in pieces of those.
+ *   penalties float[num_requests][3]: repetition (> 0; 1: none), presence, frequency; or NULL.  tokens int32[num_requests][max_tokens] / lens int32[num_requests]:
+ *       the texts, of which the first lens[r] tokens count (lens is taken within [0, max_tokens]; tokens outside [0, V) do not count); or both NULL.
+ *   requests int32[n]: each row's request, one outside [0, num_requests): no text, no biases.  NULL: row t is request t's (num_requests = n) or all are of one request.
+ *   bias_ids int32[num_requests][num_biases] / bias_values float[num_requests][num_biases]: up to 1024; one outside [0, V) is not used, and of one
+ *       that stands several times the values are added up in their order first; or both NULL.
+ *   allowed uint32[n][allowed_stride]: bit v % 32 of word v / 32: whether v is allowed (a stride of 0: one mask for all rows); or NULL.
+ *   draft_ids int32[n] / tree_mask uint64[n][mask_words]: the rows are the nodes of one request's draft tree (n <= 128, as cpmcu_tree_attention has it): the drafts of
+ *       the nodes in a row's mask, itself among them, stand in its text behind the tokens; or both NULL.
+ *   ids int32[n]: the index of the largest result, the lowest of equal ones; -1 where all are minus infinity or NaN; or NULL.
+ *   workspace: at least cpmcu_adjust_logits_workspace_bytes, on 8 bytes (not used without ids). */
+size_t cpmcu_adjust_logits_workspace_bytes(int n, int V);
+int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, int n, int V, const float* penalties, const int32_t* tokens, const int32_t* lens, int num_requests,
+                        int max_tokens, const int32_t* requests, const int32_t* bias_ids, const float* bias_values, int num_biases, const uint32_t* allowed,
+                        int64_t allowed_stride, const int32_t* draft_ids, const uint64_t* tree_mask, int mask_words, void* out, int64_t out_stride, int32_t* ids,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
