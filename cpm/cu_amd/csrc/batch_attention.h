@@ -8,7 +8,7 @@
 namespace cpmcu {
 
 // Row t of q and out: Hq heads of 128 values from t * stride on.  Request r's rows are [row_offsets[r], row_offsets[r + 1]); its page of
-// position x is block_tables[r * max_blocks + x / 256].
+// position x is block_tables[r * table_stride + x / 256].
 struct BatchRows {
     const uint16_t* q;
     uint16_t* out;
@@ -18,6 +18,7 @@ struct BatchRows {
     const int32_t* block_tables;
     const int32_t* row_offsets;  // null: row r is request r's only one
     const int32_t* positions;
+    int64_t table_stride;
     int num_requests, max_blocks, num_pages;
     int n, Hq, Hkv, group;
     float scale_log2;  // the scores' factor times log2 e: probabilities are powers of two
@@ -35,6 +36,7 @@ inline int check_batch_rows(const char* what, const BatchRows& b, float scale) {
     CPMCU_CHECK_ARG(b.n >= 0 && b.n < 1 << 24, "%s: n=%d outside [0, 2^24)", what, b.n);
     CPMCU_CHECK_ARG(b.num_requests >= 1 && b.num_requests <= kMostRequests, "%s: %d requests outside [1, %d]", what, b.num_requests, kMostRequests);
     CPMCU_CHECK_ARG(b.max_blocks >= 1 && b.max_blocks <= kMostBlocks, "%s: max_blocks=%d outside [1, %d]", what, b.max_blocks, kMostBlocks);
+    CPMCU_CHECK_ARG(b.table_stride >= b.max_blocks && b.table_stride <= INT32_MAX, "%s: rows of the tables closer than max_blocks=%d, or further apart than 2^31", what, b.max_blocks);
     CPMCU_CHECK_ARG((int64_t)b.num_requests * b.max_blocks <= kMostTableEntries, "%s: block tables of more than %d entries", what, kMostTableEntries);
     CPMCU_CHECK_ARG(b.num_pages >= 1 && b.num_pages <= INT32_MAX / kPage, "%s: num_pages=%d outside [1, %d]", what, b.num_pages, INT32_MAX / kPage);
     CPMCU_CHECK_ARG(b.Hkv >= 1 && b.Hkv <= 1024 && b.Hq >= 1 && b.Hq <= 1024 && b.Hq % b.Hkv == 0, "%s: %d query heads on %d KV heads", what, b.Hq, b.Hkv);
@@ -57,7 +59,7 @@ inline int check_batch_rows(const char* what, const BatchRows& b, float scale) {
     const bool columns = b.n > 1 && b.q_stride == b.out_stride && column >= 2 * row && column + 2 * row <= step;
     CPMCU_CHECK_ARG(in_place || columns || !overlap(b.q, q_bytes, b.out, out_bytes), "%s: the results lie in other rows of q", what);
     CPMCU_CHECK_ARG(!overlap(b.k_pool, pool, b.out, out_bytes) && !overlap(b.v_pool, pool, b.out, out_bytes), "%s: the results lie in the pools", what);
-    CPMCU_CHECK_ARG(!overlap(b.block_tables, ints * b.num_requests * b.max_blocks, b.out, out_bytes) && !overlap(b.positions, ints * b.n, b.out, out_bytes) &&
+    CPMCU_CHECK_ARG(!overlap(b.block_tables, ints * ((size_t)(b.num_requests - 1) * b.table_stride + b.max_blocks), b.out, out_bytes) && !overlap(b.positions, ints * b.n, b.out, out_bytes) &&
                         !(b.row_offsets && overlap(b.row_offsets, ints * (b.num_requests + 1), b.out, out_bytes)),
                     "%s: the results lie in the tables, offsets or positions", what);
     return CPMCU_OK;

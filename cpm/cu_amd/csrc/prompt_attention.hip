@@ -37,7 +37,6 @@ struct Join {
 struct Listed {
     int works, joins, pad[6];
 };
-constexpr int kPlanThreads = 1024, kPlanEach = kMostRequests / kPlanThreads;
 // Pieces are made where fewer than kParts of them, on all KV heads, would each have kLeastKeys tiles of keys or more.
 constexpr int kParts = 512, kLeastKeys = 24;
 
@@ -49,37 +48,21 @@ struct PlanParams {
     Join* joins;
 };
 
-// Totals in front of each thread over the workgroup, `most` at most (they stop there, so their grouping does not matter).
-__device__ inline int totals_before(int v, int most, int* wave_total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int from = __shfl_up(v, d);
-        if (lane >= d) v = min(v + from, most);
-    }
-    if (lane == 63) wave_total[wave] = v;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < wave; ++w) before = min(before + wave_total[w], most);
-    const int lanes = __shfl_up(v, 1);
-    return min(before + (lane > 0 ? lanes : 0), most);
-}
-
-__global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(PlanParams p) {
-    constexpr int kClasses = 64;
-    __shared__ int tile_end[kMostRequests], row0[kMostRequests], rows[kMostRequests], first[kMostRequests];
-    __shared__ int wave_total[kPlanThreads / 64], in_class[kClasses], class_at[kClasses], longest, slots, joins;
-    __shared__ unsigned long long cost;
-    const int tid = threadIdx.x, B = p.num_requests;
+// The workgroup's threads have EACH requests each, then every THREADS-th tile of rows.  The launch is round trips -- offsets, positions, the list --
+// and meetings of its waves: with a request and a tile a thread 4.4 us, with four waves in place of sixteen 2 less.
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
+    constexpr int kMost = THREADS * EACH, kClasses = 64, kPlanWaves = THREADS / 64;
+    __shared__ int tile_end[kMost], row0[kMost], rows[kMost], first[kMost];
+    __shared__ int wave_total[kPlanWaves], in_class[kClasses], slots, joins;
+    __shared__ unsigned long long wave_cost[kPlanWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = p.num_requests;
     if (tid < kClasses) in_class[tid] = 0;
-    if (tid == 0) {
-        cost = 0;
-        longest = slots = joins = 0;
-    }
-    int tiles[kPlanEach], mine = 0;
+    if (tid == 0) slots = joins = 0;
+    int tiles[EACH], mine = 0;
 #pragma unroll
-    for (int e = 0; e < kPlanEach; ++e) {
-        const int r = tid * kPlanEach + e;
+    for (int e = 0; e < EACH; ++e) {
+        const int r = tid * EACH + e;
         int lo = 0, count = 0, p0 = -1;
         if (r < B) {
             lo = min(max(p.row_offsets[r], 0), p.n);
@@ -94,75 +77,90 @@ __global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(PlanParams p)
         rows[r] = count;
         first[r] = p0;
     }
-    int before = totals_before(mine, p.most_tiles, wave_total);
+    // Running totals of tiles, most_tiles at most (they stop there, so their grouping does not matter).
+    int upto = mine;
 #pragma unroll
-    for (int e = 0; e < kPlanEach; ++e) {
+    for (int d = 1; d < 64; d <<= 1) {
+        const int from = __shfl_up(upto, d);
+        if (lane >= d) upto = min(upto + from, p.most_tiles);
+    }
+    if (lane == 63) wave_total[wave] = upto;
+    const int lanes_before = __shfl_up(upto, 1);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        if (w == wave) before = all;
+        all = min(all + wave_total[w], p.most_tiles);
+    }
+    before = min(before + (lane > 0 ? lanes_before : 0), p.most_tiles);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
         before = min(before + tiles[e], p.most_tiles);
-        tile_end[tid * kPlanEach + e] = before;
+        tile_end[tid * EACH + e] = before;
     }
     __syncthreads();
-    const int all = tile_end[kMostRequests - 1];
-    const auto request_of = [&](int t) {
+    struct Tile {
+        int request, tile, keys;  // keys: tiles of 64 of them that the last row sees
+    };
+    const auto find = [&](int t) {
         int lo = 0, hi = B - 1;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (tile_end[mid] > t) hi = mid;
             else lo = mid + 1;
         }
-        return lo;
+        Tile f{lo, t - (lo > 0 ? tile_end[lo - 1] : 0), 0};
+        const int last = min(rows[lo] - 1, (int)(((int64_t)(f.tile + 1) * kTileRows - 1) / p.group));
+        f.keys = (first[lo] + last) / kTileKeys + 1;
+        return f;
     };
-    const auto keys_of = [&](int t, int r, int& tile) {  // tiles of 64 keys that the last row of this tile sees
-        tile = t - (r > 0 ? tile_end[r - 1] : 0);
-        const int last = min(rows[r] - 1, (int)(((int64_t)(tile + 1) * kTileRows - 1) / p.group));
-        return (first[r] + last) / kTileKeys + 1;
-    };
-    unsigned long long sum = 0;
-    for (int t = tid; t < all; t += kPlanThreads) {
-        int tile;
-        sum += keys_of(t, request_of(t), tile);
-    }
-    atomicAdd(&cost, sum);
+    const Tile own = tid < all ? find(tid) : Tile{0, 0, 0};  // (most launches have no more)
+    unsigned long long cost = own.keys;
+    for (int t = tid + THREADS; t < all; t += THREADS) cost += find(t).keys;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) cost += __shfl_xor(cost, d);
+    if (lane == 0) wave_cost[wave] = cost;
     __syncthreads();
+    cost = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) cost += wave_cost[w];
     const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts);
     const int chunk = (int)min(max(share, (int64_t)kLeastKeys), (int64_t)INT32_MAX);
     const auto pieces_of = [&](int keys) { return (keys + chunk - 1) / chunk; };
-    int most = 0;
-    for (int t = tid; t < all; t += kPlanThreads) {
-        int tile;
-        const int keys = keys_of(t, request_of(t), tile), pieces = pieces_of(keys);
-        most = max(most, (keys + pieces - 1) / pieces);
-    }
-    atomicMax(&longest, most);
-    __syncthreads();
-    // longest first: counted by length in 64 classes, then put in their places
-    const auto class_of = [&](int length) { return kClasses - 1 - (int)((int64_t)length * (kClasses - 1) / max(longest, 1)); };
-    for (int t = tid; t < all; t += kPlanThreads) {
-        int tile;
-        const int keys = keys_of(t, request_of(t), tile), pieces = pieces_of(keys);
-        atomicAdd(&in_class[class_of((keys + pieces - 1) / pieces)], pieces);
+    // Longest first: counted in classes of a quarter of an octave, then put in their places.
+    const auto class_of = [&](int keys, int pieces) {
+        const int length = (keys + pieces - 1) / pieces, msb = 31 - __clz(max(length, 1));
+        return kClasses - 1 - min(length < 4 ? length : 4 * (msb - 1) + (length >> (msb - 2) & 3), kClasses - 1);
+    };
+    for (int t = tid; t < all; t += THREADS) {
+        const Tile f = t == tid ? own : find(t);
+        const int pieces = pieces_of(f.keys);
+        atomicAdd(&in_class[class_of(f.keys, pieces)], pieces);
     }
     __syncthreads();
     if (tid < 64) {
-        int upto = in_class[tid];
+        const int here = in_class[tid];
+        int sum = here;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int from = __shfl_up(upto, d);
-            if (tid >= d) upto += from;
+            const int from = __shfl_up(sum, d);
+            if (tid >= d) sum += from;
         }
-        class_at[tid] = upto - in_class[tid];
-        if (tid == 63) p.listed->works = upto;
+        in_class[tid] = sum - here;  // from here on: the next free place
+        if (tid == 63) p.listed->works = sum;
     }
     __syncthreads();
-    for (int t = tid; t < all; t += kPlanThreads) {
-        int tile;
-        const int r = request_of(t), keys = keys_of(t, r, tile), pieces = pieces_of(keys);
-        int at = atomicAdd(&class_at[class_of((keys + pieces - 1) / pieces)], pieces), slot = -1;
+    for (int t = tid; t < all; t += THREADS) {
+        const Tile f = t == tid ? own : find(t);
+        const int r = f.request, pieces = pieces_of(f.keys), at = atomicAdd(&in_class[class_of(f.keys, pieces)], pieces);
+        int slot = -1;
         if (pieces > 1) {
             slot = atomicAdd(&slots, pieces);
-            p.joins[atomicAdd(&joins, 1)] = Join{row0[r], rows[r], tile, slot, pieces, {0, 0, 0}};
+            p.joins[atomicAdd(&joins, 1)] = Join{row0[r], rows[r], f.tile, slot, pieces, {0, 0, 0}};
         }
         for (int i = 0; i < pieces; ++i)
-            p.works[at + i] = Work{row0[r], rows[r], first[r], r, tile, (int)((int64_t)keys * i / pieces), (int)((int64_t)keys * (i + 1) / pieces), slot < 0 ? -1 : slot + i};
+            p.works[at + i] = Work{row0[r], rows[r], first[r], r, f.tile, (int)((int64_t)f.keys * i / pieces), (int)((int64_t)f.keys * (i + 1) / pieces), slot < 0 ? -1 : slot + i};
     }
     __syncthreads();
     if (tid == 0) p.listed->joins = joins;
@@ -230,7 +228,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
     const int n = w.end - w.begin;
 
     // Page numbers: 64 of them at a time, one a lane.
-    const int32_t* const table = b.block_tables + (size_t)w.request * b.max_blocks;
+    const int32_t* const table = b.block_tables + (size_t)w.request * b.table_stride;
     int pages_from = 0, pages = 0;
     const auto load_pages = [&](int block) {
         pages_from = block;
@@ -256,6 +254,8 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         request_pair(b.v_pool + page * kHeadDim * kPage + inside, v_off, (v_off ^ 64u) + 8u * kPage * 2u - 1024u, at + kKBytes);
     };
 
+    if (tid < 2) s_odd[tid] = 0;
+    request_tile(0);
     X8 qreg[8];  // Q as the second operand of S^T = K Q^T: lane (qcol, hf) has dims 16 ks + 8 hf + [0, 8)
     {
         const E* const row = reinterpret_cast<const E*>(b.q) + (int64_t)(w.row0 + token) * b.q_stride + head * kHeadDim;
@@ -263,9 +263,8 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const X8*>(row + 16 * ks + 8 * hf);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (tid < 2) s_odd[tid] = 0;
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i)
+    for (int i = 1; i < kStages - 1; ++i)
         if (i < n) request_tile(i);
 
     f32x16 oacc[4];
@@ -451,47 +450,68 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         }
 }
 
-// The pieces of a tile: with M the largest of their references m, sum = sum_i l_i 2^(m_i - M), out = sum_i O_i 2^(m_i - M) / sum, in the order of the
-// keys.  A workgroup a row block of 32.
+// The pieces of a tile: with M the largest of their references m, sum = sum_i l_i 2^(m_i - M), out = sum_i O_i 2^(m_i - M) / sum.  A workgroup takes 32 of the
+// rows and 32 of their dims at a time, its waves every fourth piece each.
+constexpr int kJoinWaves = 4, kJoinGrid = 1024;
 template <typename E>
-__global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
+__global__ __launch_bounds__(64 * kJoinWaves) void prompt_join_kernel(PromptParams p) {
     typedef typename Elem<E>::x4 X4;
+    __shared__ f32x4 s_sum[kJoinWaves][4][64];
+    __shared__ float2 s_stat[kJoinWaves][kWaveRows];
     const BatchRows& b = p.b;
-    const int block = blockIdx.x % kWaves, g = blockIdx.x / kWaves % b.Hkv, index = blockIdx.x / kWaves / b.Hkv;
-    const Join j = p.joins[index];
-    if (index >= p.listed->joins) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qcol = lane & 31, hf = lane >> 5;
-    const int R = j.tile * kTileRows + block * kWaveRows + qcol;
-    if (R >= j.rows * b.group) return;
-    float M = -INFINITY;
-    for (int i = 0; i < j.pieces; ++i) M = fmaxf(M, p.stats[((size_t)(j.slot + i) * b.Hkv + g) * kTileRows + block * kWaveRows + qcol].x);
-    const float m_scaled = M == -INFINITY ? 0.f : M;
-    float sum = 0.f;
-    f32x4 acc[4];
+    const int64_t all = (int64_t)p.listed->joins * b.Hkv * kWaves * 4;
+    for (int64_t x = blockIdx.x; x < all; x += gridDim.x) {
+        const int db = (int)(x & 3), block = (int)(x >> 2) % kWaves, g = (int)((x >> 2) / kWaves % b.Hkv);
+        const Join j = p.joins[(x >> 2) / kWaves / b.Hkv];
+        const int base_row = j.tile * kTileRows + block * kWaveRows, R = base_row + qcol;
+        if (base_row >= j.rows * b.group) continue;
+        float M = -INFINITY, L = 0.f;
+        f32x4 sum[4];
 #pragma unroll
-    for (int rq = 0; rq < 4; ++rq) acc[rq] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < j.pieces; ++i) {
-        const size_t part = (size_t)(j.slot + i) * b.Hkv + g;
-        const float2 s = p.stats[part * kTileRows + block * kWaveRows + qcol];
-        const float f = __builtin_amdgcn_exp2f(s.x - m_scaled);
-        sum = __builtin_fmaf(s.y, f, sum);
-        const float4* const from = p.parts + (part * kWaves + block) * 16 * 64 + wave * 4 * 64 + lane;
+        for (int rq = 0; rq < 4; ++rq) sum[rq] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = wave; i < j.pieces; i += kJoinWaves) {
+            const size_t part = (size_t)(j.slot + i) * b.Hkv + g;
+            const float2 st = p.stats[part * kTileRows + block * kWaveRows + qcol];
+            const float4* const from = p.parts + ((part * kWaves + block) * 16 + db * 4) * 64 + lane;
+            f32x4 o[4];
 #pragma unroll
-        for (int rq = 0; rq < 4; ++rq) {
-            const f32x4 o = __builtin_bit_cast(f32x4, from[rq * 64]);
+            for (int rq = 0; rq < 4; ++rq) o[rq] = __builtin_bit_cast(f32x4, from[rq * 64]);
+            const float m = fmaxf(M, st.x), m_scaled = m == -INFINITY ? 0.f : m;
+            const float f = __builtin_amdgcn_exp2f(M - m_scaled), w = __builtin_amdgcn_exp2f(st.x - m_scaled);
+            M = m;
+            L = __builtin_fmaf(st.y, w, L * f);
             // (a piece that the row sees nothing of has zeros)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[rq][e] = __builtin_fmaf(o[e], f, acc[rq][e]);
+            for (int rq = 0; rq < 4; ++rq)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[rq][e] = __builtin_fmaf(o[rq][e], w, sum[rq][e] * f);
         }
-    }
-    const float inv = 1.f / sum;
-    E* const row = reinterpret_cast<E*>(b.out) + (int64_t)(j.row0 + R / b.group) * b.out_stride + (g * b.group + R % b.group) * kHeadDim;
+        __syncthreads();  // (the last ones have been read)
 #pragma unroll
-    for (int rq = 0; rq < 4; ++rq) {
-        X4 o;
+        for (int rq = 0; rq < 4; ++rq) s_sum[wave][rq][lane] = sum[rq];
+        if (hf == 0) s_stat[wave][qcol] = make_float2(M, L);
+        __syncthreads();
+        if (R < j.rows * b.group) {  // each wave finishes a quarter of the dims
+            M = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (E)(acc[rq][e] * inv);
-        *reinterpret_cast<X4*>(row + wave * 32 + rq * 8 + hf * 4) = o;
+            for (int w = 0; w < kJoinWaves; ++w) M = fmaxf(M, s_stat[w][qcol].x);
+            L = 0.f;
+            f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kJoinWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(s_stat[w][qcol].x - M);
+                L = __builtin_fmaf(s_stat[w][qcol].y, f, L);
+                const f32x4 o = s_sum[w][wave][lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[e], f, y[e]);
+            }
+            const float inv = 1.f / L;
+            X4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (E)(y[e] * inv);
+            *reinterpret_cast<X4*>(reinterpret_cast<E*>(b.out) + (int64_t)(j.row0 + R / b.group) * b.out_stride + (g * b.group + R % b.group) * kHeadDim + db * 32 + wave * 8 + hf * 4) = o;
+        }
     }
 }
 
@@ -529,10 +549,10 @@ extern "C" size_t cpmcu_batch_prompt_attention_workspace_bytes(int num_requests,
 }
 
 extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, int num_pages, const int32_t* block_tables,
-                                      int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv,
+                                      int64_t table_stride, int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv,
                                       float scale, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
     BatchRows b{(const uint16_t*)q, (uint16_t*)out, q_stride, out_stride, (const uint16_t*)k_pool, (const uint16_t*)v_pool, block_tables, row_offsets, positions,
-                num_requests, max_blocks, num_pages, n, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, scale * 1.44269504088896341f};
+                table_stride, num_requests, max_blocks, num_pages, n, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, scale * 1.44269504088896341f};
     const int rc = check_batch_rows("prompt_attention", b, scale);
     if (rc != CPMCU_OK) return rc;
     if (n == 0) return CPMCU_OK;
@@ -541,18 +561,19 @@ extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, con
     CPMCU_CHECK_ARG(workspace && workspace_bytes >= s.bytes, "prompt_attention: workspace of %zu bytes, %zu needed", workspace_bytes, s.bytes);
     CPMCU_CHECK_ARG((uintptr_t)workspace % 16 == 0, "prompt_attention: the workspace has to lie on 16 bytes");
     const int64_t grid = s.works * Hkv;
-    CPMCU_CHECK_ARG(grid <= INT32_MAX && s.joins * Hkv * kWaves <= INT32_MAX, "prompt_attention: %lld workgroups are beyond a launch", (long long)grid);
+    CPMCU_CHECK_ARG(grid <= INT32_MAX, "prompt_attention: %lld workgroups are beyond a launch", (long long)grid);
     char* const ws = static_cast<char*>(workspace);
     PlanParams plan{row_offsets, positions, num_requests, max_blocks, n, b.group, Hkv, (int)s.tiles, (Listed*)ws, (Work*)(ws + s.works_at), (Join*)(ws + s.joins_at)};
     PromptParams p{b, plan.listed, plan.works, plan.joins, (float4*)(ws + s.parts_at), (float2*)(ws + s.stats_at)};
     const hipStream_t st = resolve_stream(stream);
     const bool bf = options().dtype == 1;
-    hipLaunchKernelGGL(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, plan);
+    if (num_requests <= 256 && s.tiles <= 512) hipLaunchKernelGGL((prompt_plan_kernel<256, 1>), dim3(1), dim3(256), 0, st, plan);
+    else hipLaunchKernelGGL((prompt_plan_kernel<1024, kMostRequests / 1024>), dim3(1), dim3(1024), 0, st, plan);
     CPMCU_LAUNCH_CHECK();
     hipLaunchKernelGGL(bf ? prompt_attention_kernel<bf16> : prompt_attention_kernel<f16>, dim3((int)grid), dim3(kThreads), 0, st, p);
     CPMCU_LAUNCH_CHECK();
     if (s.joins > 0) {
-        hipLaunchKernelGGL(bf ? prompt_join_kernel<bf16> : prompt_join_kernel<f16>, dim3((int)(s.joins * Hkv * kWaves)), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(bf ? prompt_join_kernel<bf16> : prompt_join_kernel<f16>, dim3((int)std::min<int64_t>(s.joins * Hkv * kWaves * 4, kJoinGrid)), dim3(64 * kJoinWaves), 0, st, p);
         CPMCU_LAUNCH_CHECK();
     }
     return CPMCU_OK;

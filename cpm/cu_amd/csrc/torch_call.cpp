@@ -496,7 +496,7 @@ PyObject* batch_attention(PyObject* const* args, Py_ssize_t nargs) {
     const char* const pools = "batch attention: pools of 16-bit floats";
     if (!head_rows(call, args[0], "batch attention: q of 16-bit floats", &q) || !head_rows(call, args[7], "batch attention: out of 16-bit floats", &out)) return nullptr;
     const at::Tensor *k_pool = call.dense(args[1], at::kHalf, pools), *v_pool = k_pool ? call.dense(args[2], at::kHalf, pools) : nullptr, *offsets = nullptr;
-    const at::Tensor *tables = v_pool ? call.dense(args[3], at::kInt, "batch attention: int32 block_tables") : nullptr,
+    const at::Tensor *tables = v_pool ? call.strided(args[3], at::kInt, "batch attention: int32 block_tables") : nullptr,
                      *pos = tables ? call.dense(args[5], at::kInt, "batch attention: int32 positions") : nullptr;
     float scale;
     if (!pos || ((PROMPT || args[4] != Py_None) && !(offsets = call.dense(args[4], at::kInt, "batch attention: int32 row_offsets"))) || !convert(args[6], &scale)) return nullptr;
@@ -504,8 +504,8 @@ PyObject* batch_attention(PyObject* const* args, Py_ssize_t nargs) {
                     v_pool->size(1) == k_pool->size(1) && v_pool->size(2) == CPMCU_HEAD_DIM && v_pool->size(3) == CPMCU_PAGE_SIZE && k_pool->size(0) <= INT32_MAX && k_pool->size(1) <= INT32_MAX,
                 "batch attention: pools are [pages, Hkv, 256, 128] and [pages, Hkv, 128, 256]") ||
         !expect(alike(q, out) && q.dim == CPMCU_HEAD_DIM && pos->numel() == q.n, "batch attention: q and out are [n, Hq, 128], positions [n]") ||
-        !expect(tables->dim() == 2 && tables->size(0) <= INT32_MAX && tables->size(1) <= INT32_MAX && (!offsets || offsets->numel() == tables->size(0) + 1),
-                "batch attention: block_tables are [B, max_blocks], row_offsets [B + 1]"))
+        !expect(tables->dim() == 2 && (tables->numel() == 0 || tables->size(1) == 1 || tables->stride(1) == 1) && tables->size(0) <= INT32_MAX && tables->size(1) <= INT32_MAX && (!offsets || offsets->numel() == tables->size(0) + 1),
+                "batch attention: block_tables are [B, max_blocks] with whole rows, row_offsets [B + 1]"))
         return nullptr;
     const int B = static_cast<int>(tables->size(0)), M = static_cast<int>(tables->size(1)), n = static_cast<int>(q.n), Hq = static_cast<int>(q.heads), Hkv = static_cast<int>(k_pool->size(1));
     int64_t bytes = 0;
@@ -516,7 +516,7 @@ PyObject* batch_attention(PyObject* const* args, Py_ssize_t nargs) {
     void* const st = call.stream();
     return status(without_gil([&] {
         const auto fn = PROMPT ? fn_prompt_attention : fn_decode_attention;
-        return fn(q.at, q.stride, k_pool->data_ptr(), v_pool->data_ptr(), static_cast<int>(k_pool->size(0)), ints(tables), M, offsets ? ints(offsets) : nullptr, ints(pos), B, n, Hq, Hkv,
+        return fn(q.at, q.stride, k_pool->data_ptr(), v_pool->data_ptr(), static_cast<int>(k_pool->size(0)), ints(tables), B > 1 ? tables->stride(0) : M, M, offsets ? ints(offsets) : nullptr, ints(pos), B, n, Hq, Hkv,
                   scale, out.at, out.stride, ws.defined() ? ws.data_ptr() : nullptr, static_cast<size_t>(bytes), st);
     }));
 }

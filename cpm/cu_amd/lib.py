@@ -99,9 +99,9 @@ SIGNATURES = {
     "cpmcu_int8_linear": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, _P, _P]),
     "cpmcu_int8_linear_plan": (c_int, [c_int, c_int, c_int, c_char_p, c_size_t, ctypes.POINTER(c_int)]),
     "cpmcu_batch_prompt_attention_workspace_bytes": (c_size_t, [c_int] * 5),
-    "cpmcu_batch_prompt_attention": (c_int, [_P, c_i64, _P, _P, c_int, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_float, _P, c_i64, _P, c_size_t, _P]),
+    "cpmcu_batch_prompt_attention": (c_int, [_P, c_i64, _P, _P, c_int, _P, c_i64, c_int, _P, _P, c_int, c_int, c_int, c_int, c_float, _P, c_i64, _P, c_size_t, _P]),
     "cpmcu_batch_decode_attention_workspace_bytes": (c_size_t, [c_int] * 4),
-    "cpmcu_batch_decode_attention": (c_int, [_P, c_i64, _P, _P, c_int, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_float, _P, c_i64, _P, c_size_t, _P]),
+    "cpmcu_batch_decode_attention": (c_int, [_P, c_i64, _P, _P, c_int, _P, c_i64, c_int, _P, _P, c_int, c_int, c_int, c_int, c_float, _P, c_i64, _P, c_size_t, _P]),
     "cpmcu_adjust_logits_workspace_bytes": (c_size_t, [c_int, c_int]),
     "cpmcu_adjust_logits": (c_int, [_P, c_i64, c_int, c_int, _P, _P, _P, c_int, c_int, _P, _P, _P, c_int, _P, c_i64, _P, _P, c_int, _P, c_i64, _P, _P, c_size_t, _P]),
     "cpmcu_draft_tree_finish_root": (c_int, [_P, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P]),

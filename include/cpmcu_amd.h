@@ -716,7 +716,7 @@ int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, size_t kernel
  * cpmcu_kv_append_slots).  Rows of a request follow each other in position, as cpmcu_batch_tables writes them; only its first row's is read.
  *   q [n][q_stride], Hq heads of 128 values from the row's start; out alike, q's own rows (in place) or memory apart (columns apart of rows of one stride
  *       are); rows and pools on 16 bytes.  Hq a multiple of Hkv, heads h * Hkv / Hq on KV head h.  n < 2^24.
- *   block_tables int32[num_requests][max_blocks]: the page of position x is block_tables[r][x / 256] (read for positions that are attended
+ *   block_tables int32[num_requests][table_stride], max_blocks of them used: the page of position x is block_tables[r][x / 256] (used for positions that are attended
  *       only; a number outside [0, num_pages) is taken as the nearest one inside).  At most 2^28 entries, 4096 requests, 2^18 blocks.
  *   row_offsets int32[num_requests + 1], never falling; a request may have no rows.
  *   Left out, with their results as they were: rows of a request whose first position is negative (refused ones), rows of positions from
@@ -728,14 +728,14 @@ int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, size_t kernel
  *   workspace: at least cpmcu_batch_prompt_attention_workspace_bytes, on 16 bytes; its contents do not matter.  Calls that may overlap need one each. */
 size_t cpmcu_batch_prompt_attention_workspace_bytes(int num_requests, int max_blocks, int n, int Hq, int Hkv);
 int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, int num_pages, const int32_t* block_tables,
-                                 int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv, float scale,
+                                 int64_t table_stride, int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv, float scale,
                                  void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same for requests of one new row each: a step of decoding.  Row row_offsets[r] of the batch, or row r where row_offsets is NULL (n = num_requests then),
  * is request r's; requests with no row, with several, or with a row of a negative position or one from max_blocks * 256 on are left out. */
 size_t cpmcu_batch_decode_attention_workspace_bytes(int num_requests, int max_blocks, int Hq, int Hkv);
 int cpmcu_batch_decode_attention(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, int num_pages, const int32_t* block_tables,
-                                 int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv, float scale,
+                                 int64_t table_stride, int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv, float scale,
                                  void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Penalties for repeated tokens, biases and masks on n rows of logits, and their arg-max.  With c the times that token v stands in the text of the row's request:

@@ -14,18 +14,18 @@ def _lib():
 
 
 def _attention(kind, **kw):
-    a = dict(q=P(1 * GIB), qs=4096, k=P(100 * GIB), v=P(200 * GIB), pages=64, tables=P(4 * GIB), blocks=8, offsets=P(5 * GIB), pos=P(6 * GIB), B=4, n=60, hq=32, hkv=2, scale=0.1, out=P(7 * GIB),
+    a = dict(q=P(1 * GIB), qs=4096, k=P(100 * GIB), v=P(200 * GIB), pages=64, tables=P(4 * GIB), ts=None, blocks=8, offsets=P(5 * GIB), pos=P(6 * GIB), B=4, n=60, hq=32, hkv=2, scale=0.1, out=P(7 * GIB),
              os=4096, ws=P(8 * GIB), wb=1 << 40)
     a.update(kw)
     fn = _lib().batch_prompt_attention if kind == "prompt" else _lib().batch_decode_attention
-    fn(a["q"], a["qs"], a["k"], a["v"], a["pages"], a["tables"], a["blocks"], a["offsets"], a["pos"], a["B"], a["n"], a["hq"], a["hkv"], ctypes.c_float(a["scale"]), a["out"], a["os"], a["ws"], a["wb"], None)
+    fn(a["q"], a["qs"], a["k"], a["v"], a["pages"], a["tables"], a["blocks"] if a["ts"] is None else a["ts"], a["blocks"], a["offsets"], a["pos"], a["B"], a["n"], a["hq"], a["hkv"], ctypes.c_float(a["scale"]), a["out"], a["os"], a["ws"], a["wb"], None)
 
 
 @pytest.mark.parametrize("kind", ["prompt", "decode"])
 @pytest.mark.parametrize("kw, match", [
     (dict(q=None), "null"), (dict(k=None), "null"), (dict(v=None), "null"), (dict(tables=None), "null"), (dict(pos=None), "null"), (dict(out=None), "null"),
     (dict(n=-1), "n=-1"), (dict(n=1 << 24), "n=16777216"), (dict(B=0), "0 requests"), (dict(B=4097), "4097 requests"), (dict(blocks=0), "max_blocks=0"), (dict(blocks=(1 << 18) + 1), "max_blocks"),
-    (dict(B=4096, blocks=1 << 17), "more than 268435456 entries"), (dict(pages=0), "num_pages=0"), (dict(pages=1 << 23), "num_pages"), (dict(hkv=0), "0 KV heads"), (dict(hkv=3), "3 KV heads"), (dict(hq=0), "0 query heads"),
+    (dict(B=4096, blocks=1 << 17), "more than 268435456 entries"), (dict(ts=7), "tables closer"), (dict(ts=1 << 31), "tables closer"), (dict(out=P(4 * GIB + (3 << 22)), ts=1 << 20), "tables, offsets"), (dict(pages=0), "num_pages=0"), (dict(pages=1 << 23), "num_pages"), (dict(hkv=0), "0 KV heads"), (dict(hkv=3), "3 KV heads"), (dict(hq=0), "0 query heads"),
     (dict(hq=1025, hkv=1), "1025 query heads"), (dict(n=(1 << 24) - 1, hq=1024, qs=1 << 18, os=1 << 18), "beyond 32 bits"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
     (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(qs=4095), "closer"), (dict(os=4000), "closer"), (dict(qs=1 << 31), "further apart"), (dict(q=P(GIB + 8)), "16 bytes"), (dict(out=P(7 * GIB + 2)), "16 bytes"),
     (dict(qs=4100), "16 bytes"), (dict(k=P(100 * GIB + 4)), "16 bytes"), (dict(ws=P(8 * GIB + 8)), "16 bytes"), (dict(ws=None), "workspace of"), (dict(wb=100), "workspace of 100 bytes"),
@@ -57,7 +57,7 @@ def test_workspaces():
     # short tables: nothing is cut, a list is all there is; long ones: 512 pieces of 256 rows at most twice over, however many rows there are
     assert raw.cpmcu_batch_prompt_attention_workspace_bytes(1, 4, 1000, 32, 2) < 1 << 14
     assert raw.cpmcu_batch_prompt_attention_workspace_bytes(4096, 1 << 16, (1 << 24) - 1, 32, 2) < (1 << 27) + (1 << 22) + 64 * (1 << 21)
-    assert raw.cpmcu_batch_decode_attention_workspace_bytes(4096, 1 << 16, 32, 2) < 1 << 24
+    assert raw.cpmcu_batch_decode_attention_workspace_bytes(4096, 1 << 16, 32, 2) < 1 << 25
     assert raw.cpmcu_adjust_logits_workspace_bytes(-1, 100) == raw.cpmcu_adjust_logits_workspace_bytes(5, 0) == raw.cpmcu_adjust_logits_workspace_bytes(5, (1 << 24) + 1) == 0
 
 

@@ -163,8 +163,12 @@ DECODES = [[0], [1], [62], [63], [64], [65], [255], [256], [0, 1, 2, 3], [700, 5
 @pytest.mark.parametrize("cached", DECODES, ids=lambda c: "_".join(map(str, c[:4])) + "x%d" % len(c))
 def test_decode_attention(gpu, set_option, dtype, heads, cached):
     set_option("dtype", dtype)
-    b = Batch(gpu, 3, [(c, 1) for c in cached], *heads, dtype=dtype, spread=1.5, filler=float("nan"))
-    b.check(b.run("decode"))
+    b = Batch(gpu, 3, [(c, 1) for c in cached], *heads, dtype=dtype, spread=1.5, filler=float("nan"), table_blocks=max(8, max(cached) // PAGE + 1))
+    expect = b.expect()
+    b.check(b.run("decode"), expect)
+    if max(cached) < 4 * PAGE:
+        b.tables = b.tables[:, :max(cached) // PAGE + 1].contiguous()
+        b.check(b.run("decode"), expect)
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
@@ -285,6 +289,15 @@ def test_scores_that_grow_along_the_keys(gpu, set_option, dtype):
                 ramp = (at / (int(L) - 1) * 2 - 1) * 42.0
                 b.k[b.tables[r].long()[at // PAGE], :, at % PAGE, 0] = ramp[:, None].to(b.k.dtype)
             b.check(b.run(kind))
+
+
+@pytest.mark.parametrize("kind", ["prompt", "decode"])
+@pytest.mark.parametrize("blocks", [2, 4, 5])
+def test_columns_of_wider_tables(gpu, kind, blocks):
+    """The first columns of tables that have more, as a server's have (up to 4 of them a decoding step has another kernel)."""
+    b = Batch(gpu, 19, [(200, 1), (PAGE * (blocks - 1) + 70, 1), (5, 1)], 32, 2, table_blocks=40, filler=float("nan"))
+    b.tables = b.tables[:, :blocks]
+    b.check(b.run(kind))
 
 
 @pytest.mark.parametrize("kind", ["prompt", "decode"])
@@ -446,7 +459,7 @@ def test_wrong_tensors_are_refused(gpu):
     bad = [
         dict(q=b.q.float()), dict(q=b.q[:, :, :64]), dict(q=b.q.transpose(1, 2)), dict(q=b.q[:1]), dict(tables=b.tables.long()), dict(tables=b.tables[:1]), dict(tables=b.tables[0]),
         dict(off=b.dev([0, 1])), dict(off=off.cpu()), dict(pos=pos.float()), dict(pos=pos[:1]), dict(out=torch.empty((2, 32, 64), dtype=torch.float16, device="cuda")),
-        dict(out=torch.empty((2, 32, D), dtype=torch.float32, device="cuda")), dict(tables=b.tables.t().contiguous().t() if b.tables.shape[1] > 1 else b.tables.cpu())]
+        dict(out=torch.empty((2, 32, D), dtype=torch.float32, device="cuda")), dict(tables=b.tables.cpu()), dict(tables=b.tables.repeat(1, 4)[:, ::2])]
     for kw in bad:
         a = dict(q=b.q, tables=b.tables, off=off, pos=pos, out=None)
         a.update(kw)
