@@ -204,13 +204,19 @@ __device__ inline bool not_finite(E v) {
     return (__builtin_bit_cast(uint16_t, v) & kOnes) == kOnes;
 }
 
+// One tile of keys is two phases of a wave: its scores become probabilities (vector instructions, while the tile's V comes into registers), and the product with V and the
+// next tile's scores are formed (matrix instructions, while that one's K comes).  A CU's vector and matrix units work side by side for different waves, so the
+// upper four waves -- one on each SIMD, beside one of the lower four -- are a phase behind: barriers between the phases keep one wave of a SIMD on either unit.
+//
+// In terms of the phases between barriers: the lower waves have tile i's probabilities in phase 2 i and its products in 2 i + 1, the upper ones a phase later.  K(j) is read in
+// phases 2 j - 1 and 2 j, V(j) in 2 j to 2 j + 2.  With tile i's probabilities (phases 2 i and 2 i + 1) V(i + 2) and then K(i + 3) are requested, in place of V(i - 2),
+// which has been read by phase 2 i - 2, and K(i - 1), by 2 i - 2.  What a wave has requested of K(j) has to be there when phase 2 j - 2 ends, of V(j) when 2 j - 1 does.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptParams p) {
     typedef typename Elem<E>::x8 X8;
     typedef typename Elem<E>::x4 X4;
     typedef typename Elem<E>::x2 X2;
     __shared__ __attribute__((aligned(1024))) char ring[kStages * kStageBytes];
-    __shared__ unsigned long long s_odd[2];  // keys of the tile with an infinity or NaN among their values
     const BatchRows& b = p.b;
     const int g = blockIdx.x % b.Hkv, index = blockIdx.x / b.Hkv;
     // (the entry behind the list is memory too: one round trip for both)
@@ -218,13 +224,14 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
     if (index >= p.listed->works) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qcol = lane & 31, hf = lane >> 5;
+    const bool behind = wave >= kWaves / 2;
     const int packed = w.rows * b.group, base_row = w.tile * kTileRows + wave * kWaveRows;
     const int R = base_row + qcol, Rc = min(R, packed - 1);
     const bool row_ok = R < packed, wave_ok = base_row < packed;
     const int token = Rc / b.group, head = g * b.group + Rc % b.group;
     const int pos = w.p0 + token;
-    const int wave_first = w.p0 + min(base_row, packed - 1) / b.group, wave_last = w.p0 + min(base_row + kWaveRows, packed) / b.group - (min(base_row + kWaveRows, packed) % b.group == 0 ? 1 : 0);
-    const int tile_first = w.p0 + w.tile * kTileRows / b.group;  // the position of the workgroup's first row
+    // positions of the wave's first and last rows
+    const int wave_first = __builtin_amdgcn_readfirstlane(pos), wave_last = __builtin_amdgcn_readlane(pos, 31);
     const int n = w.end - w.begin;
 
     // Page numbers: 64 of them at a time, one a lane.
@@ -244,18 +251,48 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         v_off = (uint32_t)(d * kPage + ((lane & 7) ^ ((d >> 1) & 7)) * 8) * 2u;
     }
     const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_ptr_t)ring + wave * (kKBytes / kWaves);
-    const auto request_tile = [&](int i) {
-        const int first = (w.begin + i) * kTileKeys, block = first / kPage, inside = first % kPage;
-        if (block - pages_from >= 64) load_pages(block);
-        const size_t page = (size_t)__builtin_amdgcn_readlane(pages, block - pages_from) * b.Hkv + g;
-        const uint32_t at = ring_at + (i % kStages) * kStageBytes;
-        // (four keys or eight dims on, the pieces' exchange differs in bit 2; the instruction adds 1 KB to both addresses)
-        request_pair(b.k_pool + (page * kPage + inside) * kHeadDim, k_off, k_off ^ 64u, at);
-        request_pair(b.v_pool + page * kHeadDim * kPage + inside, v_off, (v_off ^ 64u) + 8u * kPage * 2u - 1024u, at + kKBytes);
+    // (four keys or eight dims on, the pieces' exchange differs in bit 2; the instruction adds 1 KB to both addresses.  A page has 64 KB a head in either pool.)
+    const uint32_t k_off2 = k_off ^ 64u, v_off2 = (v_off ^ 64u) + 8u * kPage * 2u - 1024u;
+    static_assert(kPage * kHeadDim * 2 == 1 << 16, "64 KB a page and head");
+    const auto page_of = [&](int i) {
+        const int block = (w.begin + i) * kTileKeys / kPage;
+        if (block - pages_from >= 64) load_pages(block);  // (by K's requests: V(j) is requested ahead of K(j + 1))
+        return (uint64_t)(uint32_t)(__builtin_amdgcn_readlane(pages, block - pages_from) * b.Hkv + g) << 16;
+    };
+    const auto request_k = [&](int i) {
+        request_pair((const char*)b.k_pool + page_of(i) + (w.begin + i) * kTileKeys % kPage * (kHeadDim * 2), k_off, k_off2, ring_at + (i % kStages) * kStageBytes);
+    };
+    const auto request_v = [&](int i) {
+        request_pair((const char*)b.v_pool + page_of(i) + (w.begin + i) * kTileKeys % kPage * 2, v_off, v_off2, ring_at + (i % kStages) * kStageBytes + kKBytes);
+    };
+    const auto request_next = [&](int i) {
+        if (i + 2 < n) request_v(i + 2);
+        if (i + 3 < n) request_k(i + 3);
+    };
+    const auto meet = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // What may still be on its way when this wave meets the others (two instructions a request, in the order V(i + 1), K(i + 2), V(i + 2), K(i + 3)): behind tile i's
+    // probabilities, when V(i + 2) and K(i + 3) have been requested, what comes behind V(i + 1); behind its products what comes behind K(i + 2).
+    const auto wait_behind_scores = [&](int i) {
+        switch (min(n - 1 - i, 3)) {
+            case 3: asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); break;
+            case 2: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
+            default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
+        }
+    };
+    const auto wait_behind_products = [&](int i) {
+        switch (min(n - 1 - i, 3)) {
+            case 3: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
+            case 2: asm volatile("s_waitcnt vmcnt(2)" ::: "memory"); break;
+            default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
+        }
     };
 
-    if (tid < 2) s_odd[tid] = 0;
-    request_tile(0);
+    request_k(0);
+    request_v(0);
     X8 qreg[8];  // Q as the second operand of S^T = K Q^T: lane (qcol, hf) has dims 16 ks + 8 hf + [0, 8)
     {
         const E* const row = reinterpret_cast<const E*>(b.q) + (int64_t)(w.row0 + token) * b.q_stride + head * kHeadDim;
@@ -263,77 +300,45 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const X8*>(row + 16 * ks + 8 * hf);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int i = 1; i < kStages - 1; ++i)
-        if (i < n) request_tile(i);
+    if (n > 1) {
+        request_k(1);
+        request_v(1);
+    }
+    if (n > 2) request_k(2);
+    meet();
 
-    f32x16 oacc[4];
+    f32x16 oacc[4], sacc[2];
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) oacc[db][r] = 0.f;
     float m_ref = -INFINITY, l_run = 0.f;
-
-    for (int i = 0; i < n; ++i) {
-        // Tile i has arrived when at most the two behind it (four requests each) have not.
-        switch (min(n - 1 - i, kStages - 2)) {
-            case 0: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
-            case 1: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
-            default: asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); break;
-        }
-        __syncthreads();  // everybody's pieces are there, and everybody has left the tile before
-        if (i + kStages - 1 < n) request_tile(i + kStages - 1);
-        const int c0 = (w.begin + i) * kTileKeys;
-        char* const stage = ring + (i % kStages) * kStageBytes;
-        // A tile that not all rows see whole: a value that some row may not see must not reach its sum, not even as 0 times infinity.  (Behind
-        // the last row's position lies what the page held before.)
-        const bool edge = c0 + kTileKeys - 1 > tile_first;
-        unsigned long long odd = 0;
-        if (edge) {
-            unsigned long long found = 0;
+    // Operand x of a tile's K (keys 32 (x % 2) + [0, 32), dims 16 (x / 2) + [0, 16)) and V (dims 32 (x % 4) + [0, 32), keys 16 (x / 4) + [0, 16)): the pieces' exchange
+    // makes the step along a row an exclusive or.
+    typedef __attribute__((address_space(3))) const X8* lds_x8_t;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_ptr_t)ring, k_base = lds_at + k_at(qcol, hf), v_base = lds_at + v_at(qcol, hf);
+    const auto k_of = [&](int i) { return k_base + (i % kStages) * kStageBytes; };
+    const auto v_of = [&](int i) { return v_base + (i % kStages) * kStageBytes; };
+    const auto read_k = [&](uint32_t at, int x) { return *reinterpret_cast<lds_x8_t>((at ^ ((x >> 1) * 32)) + (x & 1) * 32 * 256); };
+    const auto read_v = [&](uint32_t at, int x) { return *reinterpret_cast<lds_x8_t>((at ^ ((x >> 2) * 32)) + (x & 3) * 32 * 128); };
+    const auto clear_scores = [&]() {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = tid * 2 + h, d = at >> 3, piece = at & 7;
-                const X8 v = *reinterpret_cast<const X8*>(stage + v_at(d, piece));
-                if (any_not_finite<E>(v)) {
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (not_finite(v[e])) found |= 1ull << v_slot16(piece * 8 + e);
-                }
-            }
-            if (found) atomicOr(&s_odd[i & 1], found);
-            if (tid == 0) s_odd[(i + 1) & 1] = 0;
-            __syncthreads();
-            odd = s_odd[i & 1];
-        }
-        if (!wave_ok || c0 > wave_last) continue;
-
-        f32x16 sacc[2];
-        {
-            X8 kf[16];
+            for (int r = 0; r < 16; ++r) sacc[kb][r] = 0.f;
+    };
+    const auto scores_of = [&](int i) {
+        const uint32_t at = k_of(i);
+        X8 kf[16];
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
+        for (int x = 0; x < 16; ++x) kf[x] = read_k(at, x);
+        clear_scores();
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) kf[ks * 2 + kb] = *reinterpret_cast<const X8*>(stage + k_at(kb * 32 + qcol, 2 * ks + hf));
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sacc[kb][r] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) sacc[kb] = Elem<E>::mfma_32x32x16(kf[ks * 2 + kb], qreg[ks], sacc[kb]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // sacc[kb][r] is the score of key c0 + 32 kb + 8 (r / 4) + 4 hf + r % 4 for the row of qcol.
-        if (c0 + kTileKeys - 1 > wave_first) {
-            const int seen = pos - c0 - 4 * hf;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sacc[kb][r] = kb * 32 + 8 * (r >> 2) + (r & 3) <= seen ? sacc[kb][r] : -INFINITY;
-        }
+        for (int x = 0; x < 16; ++x) sacc[x & 1] = Elem<E>::mfma_32x32x16(kf[x], qreg[x >> 1], sacc[x & 1]);
+    };
+    // P^T as the second operand of O^T = V^T P^T, rounded to the element type: step j has keys 16 j + {4 hf + [0, 4), 8 + 4 hf + [0, 4)}
+    X8 pb[4];
+    const auto probabilities = [&]() {
         float tmax = sacc[0][0];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -355,73 +360,159 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
                 for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
         }
         const float m_scaled = m_ref == -INFINITY ? 0.f : m_ref;
-        X8 pb[4];  // P^T as the second operand of O^T = V^T P^T, rounded to the element type: step j has keys 16 j + {4 hf + [0, 4), 8 + 4 hf + [0, 4)}
+        const X2 ones = {(E)1.f, (E)1.f};
+        float psum[2] = {0.f, 0.f};  // the sum of what the product will see, in 32 bits
+        X2 pp[16];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) pb[kb * 2 + (r >> 3)][r & 7] = (E)__builtin_amdgcn_exp2f(sacc[kb][r] * b.scale_log2 - m_scaled);
-        {
-            // the sum of what the product will see, in 32 bits
-            const X2 ones = {(E)1.f, (E)1.f};
-            float psum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const X2 pp = {pb[j][2 * e], pb[j][2 * e + 1]};
-                    psum = Elem<E>::dot2_acc(pp, ones, psum);
-                }
-            l_run += psum;
+        for (int x = 0; x < 16; ++x) {
+            const float lo = __builtin_amdgcn_exp2f(sacc[x >> 3][2 * x & 15] * b.scale_log2 - m_scaled);
+            const float hi = __builtin_amdgcn_exp2f(sacc[x >> 3][(2 * x & 15) + 1] * b.scale_log2 - m_scaled);
+            pp[x] = X2{(E)lo, (E)hi};
+            psum[x & 1] = Elem<E>::dot2_acc(pp[x], ones, psum[x & 1]);
         }
-        if (odd) {
-            // zeros for the product; then what rows do see is added by itself, value by value
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    X8 v = *reinterpret_cast<const X8*>(stage + v_at(db * 32 + qcol, 2 * j + hf));
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = not_finite(v[e]) ? (E)0.f : v[e];
-                    oacc[db] = Elem<E>::mfma_32x32x16(v, pb[j], oacc[db]);
-                }
-            for (unsigned long long rest = odd; rest; rest &= rest - 1) {
-                const int key = __builtin_ctzll(rest), half = (key >> 2) & 1;
-                float pk = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (16 * j + 4 * half + (e & 3) + 8 * (e >> 2) == key) pk = (float)pb[j][e];
-                pk = __shfl(pk, qcol + 32 * half);
-                const bool sees = c0 + key <= pos;
-                const int slot = v_slot16(key);
-                int at = (int)(stage - ring) + kKBytes + (slot & 7) * 2;
-                const char* const base = ring + 4 * hf * 128;
-#pragma unroll
-                for (int db = 0; db < 4; ++db)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        asm volatile("" : "+v"(at));  // (64 addresses worked out ahead would take the loop's registers)
-                        const int d = db * 32 + 8 * (r >> 2) + (r & 3);
-                        const E v = *reinterpret_cast<const E*>(base + at + d * 128 + (((slot >> 3) ^ (((d + 4 * hf) >> 1) & 7)) << 4));
-                        if (sees && not_finite(v)) oacc[db][r] += pk * (float)v;
-                    }
-            }
-            continue;
+        for (int j = 0; j < 4; ++j) {
+            struct Four {
+                X2 v[4];
+            };
+            pb[j] = __builtin_bit_cast(X8, Four{{pp[4 * j], pp[4 * j + 1], pp[4 * j + 2], pp[4 * j + 3]}});
         }
-        X8 vf[16];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int db = 0; db < 4; ++db) vf[j * 4 + db] = *reinterpret_cast<const X8*>(stage + v_at(db * 32 + qcol, 2 * j + hf));
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int db = 0; db < 4; ++db) oacc[db] = Elem<E>::mfma_32x32x16(vf[j * 4 + db], pb[j], oacc[db]);
-        __builtin_amdgcn_sched_barrier(0);
+        l_run += psum[0] + psum[1];
+    };
+
+    int i = 0;
+    if (!wave_ok) {  // no rows: its part of the requests, and the meetings
+        wait_behind_products(-1);
+        if (behind) meet();
+        for (; i < n; ++i) {
+            request_next(i);
+            wait_behind_scores(i);
+            meet();
+            wait_behind_products(i);
+            if (!behind || i + 1 < n) meet();
+        }
+        return;
     }
-    if (!wave_ok) return;
+    scores_of(0);
+    wait_behind_products(-1);
+    if (behind) meet();
+    // Tiles that every row of the workgroup sees whole, and that have one behind them.
+    const int plain = min(n - 1, (w.p0 + w.tile * kTileRows / b.group + 1) / kTileKeys - w.begin);
+    for (; i < plain; ++i) {
+        const uint32_t v_now = v_of(i), k_next = k_of(i + 1);
+        X8 vf[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) vf[x] = read_v(v_now, x);
+        request_next(i);
+        probabilities();
+        wait_behind_scores(i);
+        meet();
+        // every operand is read eight products ahead of its own
+        X8 vg[8], kf[8], kg[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            oacc[x & 3] = Elem<E>::mfma_32x32x16(vf[x], pb[x >> 2], oacc[x & 3]);
+            vg[x] = read_v(v_now, x + 8);
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            oacc[x & 3] = Elem<E>::mfma_32x32x16(vg[x], pb[2 + (x >> 2)], oacc[x & 3]);
+            kf[x] = read_k(k_next, x);
+        }
+        clear_scores();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            sacc[x & 1] = Elem<E>::mfma_32x32x16(kf[x], qreg[x >> 1], sacc[x & 1]);
+            kg[x] = read_k(k_next, x + 8);
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sacc[x & 1] = Elem<E>::mfma_32x32x16(kg[x], qreg[4 + (x >> 1)], sacc[x & 1]);
+#pragma unroll
+        for (int x = 0; x < 24; ++x) {  // a product, a read
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
+        wait_behind_products(i);
+        meet();
+    }
+    for (; i < n; ++i) {
+        const int c0 = (w.begin + i) * kTileKeys;
+        const bool active = c0 <= wave_last;
+        request_next(i);
+        if (active) {
+            // sacc[kb][r] is the score of key c0 + 32 kb + 8 (r / 4) + 4 hf + r % 4 for the row of qcol.
+            const int seen = pos - c0 - 4 * hf;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sacc[kb][r] = kb * 32 + 8 * (r >> 2) + (r & 3) <= seen ? sacc[kb][r] : -INFINITY;
+            probabilities();
+        }
+        wait_behind_scores(i);
+        meet();
+        if (active) {
+            // A tile that not all rows see whole: a value that some row may not see must not reach its sum, not even as 0 times infinity.  (Behind the last row's
+            // position lies what the page held before.)  Few tiles come here: four operands at a time, and nothing worked out ahead of the loop for them.
+            int from = (i % kStages) * kStageBytes;
+            uint32_t odd = 0;  // of this lane's keys, those that have such values: bit 8 j + e is key 16 j + 4 hf + e % 4 + 8 (e / 4)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                asm volatile("" : "+v"(from));
+                X8 some_v[4];
+                bool some = false;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    some_v[x] = read_v(v_base + from, 4 * j + x);
+                    some = some || any_not_finite<E>(some_v[x]);
+                }
+                if (__any(some)) {  // zeros for the product
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (not_finite(some_v[x][e])) {
+                                odd |= 1u << (8 * j + e);
+                                some_v[x][e] = (E)0.f;
+                            }
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) oacc[x] = Elem<E>::mfma_32x32x16(some_v[x], pb[j], oacc[x]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (__any(odd != 0)) {
+                // What rows do see of such values is added by itself, one by one.
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) odd |= __shfl_xor((int)odd, d);
+                for (int half = 0; half < 2; ++half) {
+                    for (uint32_t rest = __builtin_amdgcn_readlane(odd, 32 * half); rest; rest &= rest - 1) {
+                        const int bit = __builtin_ctz(rest), key = 16 * (bit >> 3) + 4 * half + (bit & 3) + 8 * (bit >> 2 & 1);
+                        float pk = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) pk = 8 * j + e == bit ? (float)pb[j][e] : pk;
+                        pk = __shfl(pk, (lane & 31) + 32 * half);
+                        const bool sees = c0 + key <= pos;
+                        const int slot = v_slot16(key);
+                        int at = from + kKBytes + (slot & 7) * 2, rows = 4 * (lane >> 5);
+#pragma unroll
+                        for (int db = 0; db < 4; ++db)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                asm volatile("" : "+v"(at), "+v"(rows));  // (64 addresses worked out ahead would take the loop's registers)
+                                const int d = db * 32 + 8 * (r >> 2) + (r & 3) + rows;
+                                const E v = *reinterpret_cast<const E*>(ring + at + d * 128 + (((slot >> 3) ^ ((d >> 1) & 7)) << 4));
+                                if (sees && not_finite(v)) oacc[db][r] += pk * (float)v;
+                            }
+                    }
+                }
+            }
+        }
+        if (i + 1 < n) scores_of(i + 1);
+        wait_behind_products(i);
+        if (!behind || i + 1 < n) meet();
+    }
 
     // oacc[db][r] is dim 32 db + 8 (r / 4) + 4 hf + r % 4 of the row of qcol
     const float l_all = l_run + __shfl_xor(l_run, 32);
