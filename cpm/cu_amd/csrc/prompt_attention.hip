@@ -21,7 +21,7 @@ constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32, kTileRows = kWaves * kWaveRows;
 constexpr int kStages = 4;
 constexpr int kKBytes = kTileKeys * kHeadDim * 2, kStageBytes = 2 * kKBytes;
-constexpr float kLazyLog2 = 8.f;  // how far scores may pass the softmax reference before it follows, in powers of two
+constexpr float kMostSum = 4096.f;  // of a lane's 32 probabilities of a tile, before the softmax's reference follows (fp16 ends at 65504)
 
 // ---- the list of work ----
 
@@ -209,8 +209,11 @@ __device__ inline bool not_finite(E v) {
 // upper four waves -- one on each SIMD, beside one of the lower four -- are a phase behind: barriers between the phases keep one wave of a SIMD on either unit.
 //
 // In terms of the phases between barriers: the lower waves have tile i's probabilities in phase 2 i and its products in 2 i + 1, the upper ones a phase later.  K(j) is read in
-// phases 2 j - 1 and 2 j, V(j) in 2 j to 2 j + 2.  With tile i's probabilities (phases 2 i and 2 i + 1) V(i + 2) and then K(i + 3) are requested, in place of V(i - 2),
-// which has been read by phase 2 i - 2, and K(i - 1), by 2 i - 2.  What a wave has requested of K(j) has to be there when phase 2 j - 2 ends, of V(j) when 2 j - 1 does.
+// phases 2 j - 1 and 2 j, V(j) in 2 j to 2 j + 2.  With tile i's products (phases 2 i + 1 and 2 i + 2) V(i + 3) and then K(i + 4) are requested, in place of V(i - 1) and
+// K(i), which have been read by phase 2 i.  What a wave has requested of K(j) has to be there when phase 2 j - 2 ends, of V(j) when 2 j - 1 does.
+//
+// The softmax's reference is the largest score of a row's first tile, and follows only when a tile's probabilities add up to more than kMostSum: their sum is needed anyway, their
+// largest score is not.  (Half of the vector instructions of the largest score's way: 30 a tile and lane of 130.)
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptParams p) {
     typedef typename Elem<E>::x8 X8;
@@ -254,28 +257,27 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
     // (four keys or eight dims on, the pieces' exchange differs in bit 2; the instruction adds 1 KB to both addresses.  A page has 64 KB a head in either pool.)
     const uint32_t k_off2 = k_off ^ 64u, v_off2 = (v_off ^ 64u) + 8u * kPage * 2u - 1024u;
     static_assert(kPage * kHeadDim * 2 == 1 << 16, "64 KB a page and head");
-    const auto page_of = [&](int i) {
+    uint64_t page_at = 0;  // of the tile whose K has been requested last: V(j) is requested behind K(j), ahead of K(j + 1)
+    const auto request_k = [&](int i, int stage) {
         const int block = (w.begin + i) * kTileKeys / kPage;
-        if (block - pages_from >= 64) load_pages(block);  // (by K's requests: V(j) is requested ahead of K(j + 1))
-        return (uint64_t)(uint32_t)(__builtin_amdgcn_readlane(pages, block - pages_from) * b.Hkv + g) << 16;
+        if (block - pages_from >= 64) load_pages(block);
+        page_at = (uint64_t)(uint32_t)(__builtin_amdgcn_readlane(pages, block - pages_from) * b.Hkv + g) << 16;
+        request_pair((const char*)b.k_pool + page_at + (w.begin + i) * kTileKeys % kPage * (kHeadDim * 2), k_off, k_off2, ring_at + stage * kStageBytes);
     };
-    const auto request_k = [&](int i) {
-        request_pair((const char*)b.k_pool + page_of(i) + (w.begin + i) * kTileKeys % kPage * (kHeadDim * 2), k_off, k_off2, ring_at + (i % kStages) * kStageBytes);
-    };
-    const auto request_v = [&](int i) {
-        request_pair((const char*)b.v_pool + page_of(i) + (w.begin + i) * kTileKeys % kPage * 2, v_off, v_off2, ring_at + (i % kStages) * kStageBytes + kKBytes);
+    const auto request_v = [&](int i, int stage) {
+        request_pair((const char*)b.v_pool + page_at + (w.begin + i) * kTileKeys % kPage * 2, v_off, v_off2, ring_at + stage * kStageBytes + kKBytes);
     };
     const auto request_next = [&](int i) {
-        if (i + 2 < n) request_v(i + 2);
-        if (i + 3 < n) request_k(i + 3);
+        if (i + 3 < n) request_v(i + 3, (i + 3) % kStages);
+        if (i + 4 < n) request_k(i + 4, i % kStages);
     };
     const auto meet = [&]() {
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // What may still be on its way when this wave meets the others (two instructions a request, in the order V(i + 1), K(i + 2), V(i + 2), K(i + 3)): behind tile i's
-    // probabilities, when V(i + 2) and K(i + 3) have been requested, what comes behind V(i + 1); behind its products what comes behind K(i + 2).
+    // What may still be on its way when this wave meets the others (two instructions a request, in the order V(i + 1), K(i + 2), V(i + 2), K(i + 3), V(i + 3), K(i + 4)): behind
+    // tile i's probabilities what comes behind V(i + 1), behind its products, with which the last two are requested, what comes behind K(i + 2).
     const auto wait_behind_scores = [&](int i) {
         switch (min(n - 1 - i, 3)) {
             case 3: asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); break;
@@ -284,15 +286,16 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         }
     };
     const auto wait_behind_products = [&](int i) {
-        switch (min(n - 1 - i, 3)) {
-            case 3: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
+        switch (min(n - 1 - i, 4)) {
+            case 4: asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); break;
+            case 3: asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); break;
             case 2: asm volatile("s_waitcnt vmcnt(2)" ::: "memory"); break;
             default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
         }
     };
 
-    request_k(0);
-    request_v(0);
+    request_k(0, 0);
+    request_v(0, 0);
     X8 qreg[8];  // Q as the second operand of S^T = K Q^T: lane (qcol, hf) has dims 16 ks + 8 hf + [0, 8)
     {
         const E* const row = reinterpret_cast<const E*>(b.q) + (int64_t)(w.row0 + token) * b.q_stride + head * kHeadDim;
@@ -300,11 +303,11 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const X8*>(row + 16 * ks + 8 * hf);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (n > 1) {
-        request_k(1);
-        request_v(1);
+    for (int i = 1; i < min(n, 3); ++i) {
+        request_k(i, i);
+        request_v(i, i);
     }
-    if (n > 2) request_k(2);
+    if (n > 3) request_k(3, 3);
     meet();
 
     f32x16 oacc[4], sacc[2];
@@ -338,46 +341,55 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
     };
     // P^T as the second operand of O^T = V^T P^T, rounded to the element type: step j has keys 16 j + {4 hf + [0, 4), 8 + 4 hf + [0, 4)}
     X8 pb[4];
-    const auto probabilities = [&]() {
+    const auto refer = [&]() {  // to the tile's largest score, where that is larger
         float tmax = sacc[0][0];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, sacc[kb][r]);
-        {
-            // the row's other keys are 32 lanes away (assembly: the builtin hands back its first result twice; the wait states cover the write of tmax)
-            float mine = tmax, other = tmax;
-            asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(mine), "+v"(other));
-            tmax = fmaxf(mine, other) * b.scale_log2;
-        }
-        if (__any(tmax > m_ref + kLazyLog2)) {
-            const float m_new = fmaxf(m_ref, tmax), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
-            m_ref = m_new;
-            l_run *= alpha;
+        // (the row's other keys are 32 lanes away)
+        const float m_new = fmaxf(m_ref, fmaxf(tmax, __shfl_xor(tmax, 32)) * b.scale_log2), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
+        m_ref = m_new;
+        l_run *= alpha;
 #pragma unroll
-            for (int db = 0; db < 4; ++db)
+        for (int db = 0; db < 4; ++db)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
-        }
-        const float m_scaled = m_ref == -INFINITY ? 0.f : m_ref;
-        const X2 ones = {(E)1.f, (E)1.f};
-        float psum[2] = {0.f, 0.f};  // the sum of what the product will see, in 32 bits
-        X2 pp[16];
+            for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
+    };
+    const auto probabilities = [&]() {
+        float sum;
+        for (int turn = 0;; ++turn) {
+            const float m_scaled = m_ref == -INFINITY ? 0.f : m_ref;
+            const X2 ones = {(E)1.f, (E)1.f};
+            float psum[2] = {0.f, 0.f};  // the sum of what the product will see, in 32 bits
+            X2 pp[16];
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            const float lo = __builtin_amdgcn_exp2f(sacc[x >> 3][2 * x & 15] * b.scale_log2 - m_scaled);
-            const float hi = __builtin_amdgcn_exp2f(sacc[x >> 3][(2 * x & 15) + 1] * b.scale_log2 - m_scaled);
-            pp[x] = X2{(E)lo, (E)hi};
-            psum[x & 1] = Elem<E>::dot2_acc(pp[x], ones, psum[x & 1]);
-        }
+            for (int x = 0; x < 16; ++x) {
+                const float lo = __builtin_amdgcn_exp2f(sacc[x >> 3][2 * x & 15] * b.scale_log2 - m_scaled);
+                const float hi = __builtin_amdgcn_exp2f(sacc[x >> 3][(2 * x & 15) + 1] * b.scale_log2 - m_scaled);
+                pp[x] = X2{(E)lo, (E)hi};
+                psum[x & 1] = Elem<E>::dot2_acc(pp[x], ones, psum[x & 1]);
+            }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            struct Four {
-                X2 v[4];
-            };
-            pb[j] = __builtin_bit_cast(X8, Four{{pp[4 * j], pp[4 * j + 1], pp[4 * j + 2], pp[4 * j + 3]}});
+            for (int j = 0; j < 4; ++j) {
+                struct Four {
+                    X2 v[4];
+                };
+                pb[j] = __builtin_bit_cast(X8, Four{{pp[4 * j], pp[4 * j + 1], pp[4 * j + 2], pp[4 * j + 3]}});
+            }
+            sum = psum[0] + psum[1];
+            if (turn > 0 || !__any(sum > kMostSum)) break;
+            refer();
         }
-        l_run += psum[0] + psum[1];
+        l_run += sum;
+    };
+    // sacc[kb][r] is the score of key c0 + 32 kb + 8 (r / 4) + 4 hf + r % 4 for the row of qcol.
+    const auto hide = [&](int i) {
+        const int seen = pos - (w.begin + i) * kTileKeys - 4 * hf;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sacc[kb][r] = kb * 32 + 8 * (r >> 2) + (r & 3) <= seen ? sacc[kb][r] : -INFINITY;
     };
 
     int i = 0;
@@ -385,27 +397,28 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         wait_behind_products(-1);
         if (behind) meet();
         for (; i < n; ++i) {
-            request_next(i);
             wait_behind_scores(i);
             meet();
+            request_next(i);
             wait_behind_products(i);
             if (!behind || i + 1 < n) meet();
         }
         return;
     }
-    scores_of(0);
-    wait_behind_products(-1);
-    if (behind) meet();
     // Tiles that every row of the workgroup sees whole, and that have one behind them.
     const int plain = min(n - 1, (w.p0 + w.tile * kTileRows / b.group + 1) / kTileKeys - w.begin);
+    scores_of(0);
+    if (plain <= 0) hide(0);
+    refer();
+    wait_behind_products(-1);
+    if (behind) meet();
     for (; i < plain; ++i) {
         const uint32_t v_now = v_of(i), k_next = k_of(i + 1);
         X8 vf[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) vf[x] = read_v(v_now, x);
-        request_next(i);
         probabilities();
-        wait_behind_scores(i);
+        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
         meet();
         // every operand is read eight products ahead of its own
         X8 vg[8], kf[8], kg[8];
@@ -414,11 +427,14 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
             oacc[x & 3] = Elem<E>::mfma_32x32x16(vf[x], pb[x >> 2], oacc[x & 3]);
             vg[x] = read_v(v_now, x + 8);
         }
+        // (behind the last tile that one again: where its stage is has been read, and what is waited for stays the same)
+        request_v(min(i + 3, n - 1), (i + 3) % kStages);
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             oacc[x & 3] = Elem<E>::mfma_32x32x16(vg[x], pb[2 + (x >> 2)], oacc[x & 3]);
             kf[x] = read_k(k_next, x);
         }
+        request_k(min(i + 4, n - 1), i % kStages);
         clear_scores();
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -433,24 +449,19 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
-        wait_behind_products(i);
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         meet();
     }
     for (; i < n; ++i) {
         const int c0 = (w.begin + i) * kTileKeys;
         const bool active = c0 <= wave_last;
-        request_next(i);
         if (active) {
-            // sacc[kb][r] is the score of key c0 + 32 kb + 8 (r / 4) + 4 hf + r % 4 for the row of qcol.
-            const int seen = pos - c0 - 4 * hf;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sacc[kb][r] = kb * 32 + 8 * (r >> 2) + (r & 3) <= seen ? sacc[kb][r] : -INFINITY;
+            hide(i);
             probabilities();
         }
         wait_behind_scores(i);
         meet();
+        request_next(i);
         if (active) {
             // A tile that not all rows see whole: a value that some row may not see must not reach its sum, not even as 0 times infinity.  (Behind the last row's
             // position lies what the page held before.)  Few tiles come here: four operands at a time, and nothing worked out ahead of the loop for them.
@@ -513,6 +524,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         wait_behind_products(i);
         if (!behind || i + 1 < n) meet();
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a last tile that has been requested again)
 
     // oacc[db][r] is dim 32 db + 8 (r / 4) + 4 hf + r % 4 of the row of qcol
     const float l_all = l_run + __shfl_xor(l_run, 32);
