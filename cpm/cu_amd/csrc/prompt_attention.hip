@@ -3,9 +3,9 @@
 //   out[t][h] = sum_x p_x v[x] / sum_x p_x,  p_x = exp(scale (q[t][h] . k[x] - max)),  x from 0 to the row's own position,
 //
 // k and v the tokens of the row's request and of the KV head of h.  The rows of a request and the heads on one KV head are one matrix of
-// rows (token-major), cut into tiles of 256; a workgroup takes a tile, or a part of its keys, through them 64 at a time, with the running
-// maximum and sum of its softmax.  What bounds it: 4 * 128 operations a row, head and key on the matrix cores, twice as many vector
-// operations a score as the matrix cores need cycles for it hidden behind them, and K and V out of L2 once for every 256 rows.
+// rows (token-major), cut into tiles of 128; a workgroup takes a tile, or a part of its keys, through them 64 at a time, with the running
+// reference and sum of its softmax.  What bounds it: 4 * 128 operations a row, head and key on the matrix cores, of which two workgroups a CU keep
+// as many busy as the card's power allows (one of them forms products while the other one has its scores in the vector units).
 //
 // Which tiles there are follows from lengths that only the device knows, so a launch of one workgroup lists them first: longest first, those
 // that would outlast the others by much cut into pieces, which a third launch joins.
@@ -17,9 +17,9 @@
 namespace cpmcu {
 namespace {
 
-constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32, kTileRows = kWaves * kWaveRows;
-constexpr int kStages = 4;
+constexpr int kStages = 2;
 constexpr int kKBytes = kTileKeys * kHeadDim * 2, kStageBytes = 2 * kKBytes;
 constexpr float kMostSum = 4096.f;  // of a lane's 32 probabilities of a tile, before the softmax's reference follows (fp16 ends at 65504)
 
@@ -38,7 +38,7 @@ struct Listed {
     int works, joins, pad[6];
 };
 // Pieces are made where fewer than kParts of them, on all KV heads, would each have kLeastKeys tiles of keys or more.
-constexpr int kParts = 512, kLeastKeys = 24;
+constexpr int kParts = 1024, kLeastKeys = 24;
 
 struct PlanParams {
     const int32_t *row_offsets, *positions;
@@ -184,11 +184,12 @@ typedef __attribute__((address_space(3))) void* lds_ptr_t;
 __device__ inline int k_at(int key, int piece) { return key * 256 + ((piece ^ (key & 15)) << 4); }
 __device__ inline int v_at(int d, int piece) { return kKBytes + d * 128 + ((piece ^ ((d >> 1) & 7)) << 4); }
 
-// Two KB of a wave from memory to LDS, each lane's 16 bytes from where it says, in lane order from lds_at on.  Their arrival is counted by hand: written
-// as loads that the compiler knows, every read of LDS would wait for all of them.  One statement: nothing comes between m0 and its use.
-__device__ inline void request_pair(const void* base, uint32_t off_0, uint32_t off_1, uint32_t lds_at) {
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
-                 : : "v"(off_0), "v"(off_1), "s"(base), "s"(lds_at) : "memory", "m0");
+// Four KB of a wave from memory to LDS: each lane's 16 bytes of each from where it says, in lane order; the instructions add 1 KB each to both addresses.  Their arrival is counted
+// by hand: written as loads that the compiler knows, every read of LDS would wait for all of them.  One statement: nothing comes between m0 and its use.
+__device__ inline void request_4k(const void* base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds_at) {
+    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072"
+                 : : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds_at) : "memory", "m0");
 }
 
 template <typename E>
@@ -204,18 +205,16 @@ __device__ inline bool not_finite(E v) {
     return (__builtin_bit_cast(uint16_t, v) & kOnes) == kOnes;
 }
 
-// One tile of keys is two phases of a wave: its scores become probabilities (vector instructions, while the tile's V comes into registers), and the product with V and the
-// next tile's scores are formed (matrix instructions, while that one's K comes).  A CU's vector and matrix units work side by side for different waves, so the
-// upper four waves -- one on each SIMD, beside one of the lower four -- are a phase behind: barriers between the phases keep one wave of a SIMD on either unit.
-//
-// In terms of the phases between barriers: the lower waves have tile i's probabilities in phase 2 i and its products in 2 i + 1, the upper ones a phase later.  K(j) is read in
-// phases 2 j - 1 and 2 j, V(j) in 2 j to 2 j + 2.  With tile i's products (phases 2 i + 1 and 2 i + 2) V(i + 3) and then K(i + 4) are requested, in place of V(i - 1) and
-// K(i), which have been read by phase 2 i.  What a wave has requested of K(j) has to be there when phase 2 j - 2 ends, of V(j) when 2 j - 1 does.
+// A tile of keys is two phases of a wave: its scores become probabilities (vector instructions, 650 cycles), and the product with V and the next tile's scores are formed
+// (matrix instructions, 1024).  The CU's two workgroups know nothing of each other, so the one's phases fall beside the other's.  (Eight waves in one workgroup, with
+// barriers between the phases that keep one wave of a SIMD on either unit: 2.5 % faster on the largest prompt, and 10 to 35 % slower on small ones, whose tiles are too few;
+// all eight in step: 8 % slower than that.)  K and V have two stages each: V(i + 1) and K(i + 2) are requested when everybody is through with tile i - 1's products, and have the
+// time of a tile to come.
 //
 // The softmax's reference is the largest score of a row's first tile, and follows only when a tile's probabilities add up to more than kMostSum: their sum is needed anyway, their
-// largest score is not.  (Half of the vector instructions of the largest score's way: 30 a tile and lane of 130.)
+// largest score is not (30 vector instructions of 130).
 template <typename E>
-__global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptParams p) {
+__global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptParams p) {
     typedef typename Elem<E>::x8 X8;
     typedef typename Elem<E>::x4 X4;
     typedef typename Elem<E>::x2 X2;
@@ -227,7 +226,6 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
     if (index >= p.listed->works) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qcol = lane & 31, hf = lane >> 5;
-    const bool behind = wave >= kWaves / 2;
     const int packed = w.rows * b.group, base_row = w.tile * kTileRows + wave * kWaveRows;
     const int R = base_row + qcol, Rc = min(R, packed - 1);
     const bool row_ok = R < packed, wave_ok = base_row < packed;
@@ -246,54 +244,32 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
     };
     load_pages(w.begin * kTileKeys / kPage);
 
-    // What each lane requests of a tile: 2 KB of K's (8 keys) and of V's (16 dims) a wave, as two KB in lane order.
+    // What each lane requests of a tile: 4 KB of K's (16 keys) and of V's (32 dims) a wave.  Four keys or eight dims on, the pieces' exchange differs in bits 2 and 3, or 2; a
+    // page has 64 KB a head in either pool.
     uint32_t k_off, v_off;
     {
-        const int key = wave * 8 + (lane >> 4), d = wave * 16 + (lane >> 3);
+        const int key = wave * 16 + (lane >> 4), d = wave * 32 + (lane >> 3);
         k_off = (uint32_t)(key * kHeadDim + ((lane & 15) ^ (key & 15)) * 8) * 2u;
         v_off = (uint32_t)(d * kPage + ((lane & 7) ^ ((d >> 1) & 7)) * 8) * 2u;
     }
-    const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_ptr_t)ring + wave * (kKBytes / kWaves);
-    // (four keys or eight dims on, the pieces' exchange differs in bit 2; the instruction adds 1 KB to both addresses.  A page has 64 KB a head in either pool.)
-    const uint32_t k_off2 = k_off ^ 64u, v_off2 = (v_off ^ 64u) + 8u * kPage * 2u - 1024u;
+    const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_ptr_t)ring + wave * 4096;
+    const uint32_t v_off1 = (v_off ^ 64u) + 3072u, v_off2 = v_off + 6144u, v_off3 = (v_off ^ 64u) + 9216u;
     static_assert(kPage * kHeadDim * 2 == 1 << 16, "64 KB a page and head");
     uint64_t page_at = 0;  // of the tile whose K has been requested last: V(j) is requested behind K(j), ahead of K(j + 1)
     const auto request_k = [&](int i, int stage) {
         const int block = (w.begin + i) * kTileKeys / kPage;
         if (block - pages_from >= 64) load_pages(block);
         page_at = (uint64_t)(uint32_t)(__builtin_amdgcn_readlane(pages, block - pages_from) * b.Hkv + g) << 16;
-        request_pair((const char*)b.k_pool + page_at + (w.begin + i) * kTileKeys % kPage * (kHeadDim * 2), k_off, k_off2, ring_at + stage * kStageBytes);
+        request_4k((const char*)b.k_pool + page_at + (w.begin + i) * kTileKeys % kPage * (kHeadDim * 2), k_off, k_off ^ 64u, k_off ^ 128u, k_off ^ 192u, ring_at + stage * kStageBytes);
     };
     const auto request_v = [&](int i, int stage) {
-        request_pair((const char*)b.v_pool + page_at + (w.begin + i) * kTileKeys % kPage * 2, v_off, v_off2, ring_at + stage * kStageBytes + kKBytes);
-    };
-    const auto request_next = [&](int i) {
-        if (i + 3 < n) request_v(i + 3, (i + 3) % kStages);
-        if (i + 4 < n) request_k(i + 4, i % kStages);
+        request_4k((const char*)b.v_pool + page_at + (w.begin + i) * kTileKeys % kPage * 2, v_off, v_off1, v_off2, v_off3, ring_at + stage * kStageBytes + kKBytes);
     };
     const auto meet = [&]() {
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // What may still be on its way when this wave meets the others (two instructions a request, in the order V(i + 1), K(i + 2), V(i + 2), K(i + 3), V(i + 3), K(i + 4)): behind
-    // tile i's probabilities what comes behind V(i + 1), behind its products, with which the last two are requested, what comes behind K(i + 2).
-    const auto wait_behind_scores = [&](int i) {
-        switch (min(n - 1 - i, 3)) {
-            case 3: asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); break;
-            case 2: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
-            default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
-        }
-    };
-    const auto wait_behind_products = [&](int i) {
-        switch (min(n - 1 - i, 4)) {
-            case 4: asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); break;
-            case 3: asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); break;
-            case 2: asm volatile("s_waitcnt vmcnt(2)" ::: "memory"); break;
-            default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
-        }
-    };
-
     request_k(0, 0);
     request_v(0, 0);
     X8 qreg[8];  // Q as the second operand of S^T = K Q^T: lane (qcol, hf) has dims 16 ks + 8 hf + [0, 8)
@@ -303,11 +279,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const X8*>(row + 16 * ks + 8 * hf);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    for (int i = 1; i < min(n, 3); ++i) {
-        request_k(i, i);
-        request_v(i, i);
-    }
-    if (n > 3) request_k(3, 3);
+    if (n > 1) request_k(1, 1);
     meet();
 
     f32x16 oacc[4], sacc[2];
@@ -392,49 +364,37 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
             for (int r = 0; r < 16; ++r) sacc[kb][r] = kb * 32 + 8 * (r >> 2) + (r & 3) <= seen ? sacc[kb][r] : -INFINITY;
     };
 
-    int i = 0;
-    if (!wave_ok) {  // no rows: its part of the requests, and the meetings
-        wait_behind_products(-1);
-        if (behind) meet();
-        for (; i < n; ++i) {
-            wait_behind_scores(i);
-            meet();
-            request_next(i);
-            wait_behind_products(i);
-            if (!behind || i + 1 < n) meet();
-        }
-        return;
+    const int plain = wave_ok ? min(n - 1, (w.p0 + w.tile * kTileRows / b.group + 1) / kTileKeys - w.begin) : 0;
+    if (wave_ok) {
+        scores_of(0);
+        if (plain <= 0) hide(0);
+        refer();
     }
-    // Tiles that every row of the workgroup sees whole, and that have one behind them.
-    const int plain = min(n - 1, (w.p0 + w.tile * kTileRows / b.group + 1) / kTileKeys - w.begin);
-    scores_of(0);
-    if (plain <= 0) hide(0);
-    refer();
-    wait_behind_products(-1);
-    if (behind) meet();
+    // V(i + 1) and K(i + 2) are requested behind the meeting ahead of tile i's products, in place of V(i - 1) and K(i)
+    const auto next = [&](int i) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        meet();
+        if (i + 1 < n) request_v(i + 1, (i + 1) % kStages);
+        if (i + 2 < n) request_k(i + 2, i % kStages);
+    };
+    int i = 0;
     for (; i < plain; ++i) {
         const uint32_t v_now = v_of(i), k_next = k_of(i + 1);
-        X8 vf[8];
+        probabilities();
+        next(i);
+        X8 vf[8], vg[8], kf[8], kg[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) vf[x] = read_v(v_now, x);
-        probabilities();
-        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-        meet();
-        // every operand is read eight products ahead of its own
-        X8 vg[8], kf[8], kg[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             oacc[x & 3] = Elem<E>::mfma_32x32x16(vf[x], pb[x >> 2], oacc[x & 3]);
             vg[x] = read_v(v_now, x + 8);
         }
-        // (behind the last tile that one again: where its stage is has been read, and what is waited for stays the same)
-        request_v(min(i + 3, n - 1), (i + 3) % kStages);
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             oacc[x & 3] = Elem<E>::mfma_32x32x16(vg[x], pb[2 + (x >> 2)], oacc[x & 3]);
             kf[x] = read_k(k_next, x);
         }
-        request_k(min(i + 4, n - 1), i % kStages);
         clear_scores();
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -443,25 +403,23 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
         }
 #pragma unroll
         for (int x = 0; x < 8; ++x) sacc[x & 1] = Elem<E>::mfma_32x32x16(kg[x], qreg[4 + (x >> 1)], sacc[x & 1]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
         for (int x = 0; x < 24; ++x) {  // a product, a read
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
-        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        meet();
+        __builtin_amdgcn_sched_barrier(0);
     }
     for (; i < n; ++i) {
         const int c0 = (w.begin + i) * kTileKeys;
-        const bool active = c0 <= wave_last;
+        const bool active = wave_ok && c0 <= wave_last;
         if (active) {
             hide(i);
             probabilities();
         }
-        wait_behind_scores(i);
-        meet();
-        request_next(i);
+        next(i);
         if (active) {
             // A tile that not all rows see whole: a value that some row may not see must not reach its sum, not even as 0 times infinity.  (Behind the last row's
             // position lies what the page held before.)  Few tiles come here: four operands at a time, and nothing worked out ahead of the loop for them.
@@ -520,11 +478,9 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_attention_kernel(PromptPar
                 }
             }
         }
-        if (i + 1 < n) scores_of(i + 1);
-        wait_behind_products(i);
-        if (!behind || i + 1 < n) meet();
+        if (wave_ok && i + 1 < n) scores_of(i + 1);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a last tile that has been requested again)
+    if (!wave_ok) return;
 
     // oacc[db][r] is dim 32 db + 8 (r / 4) + 4 hf + r % 4 of the row of qcol
     const float l_all = l_run + __shfl_xor(l_run, 32);
