@@ -21,6 +21,7 @@ struct BatchRows {
     int64_t table_stride;
     int num_requests, max_blocks, num_pages;
     int n, Hq, Hkv, group;
+    uint32_t group_inverse;  // 0xffffffff / group
     float scale_log2;  // the scores' factor times log2 e: probabilities are powers of two
 };
 
@@ -31,6 +32,20 @@ constexpr int kTileKeys = 64;              // keys that a workgroup or a wave ta
 
 // A row's position and a page's number as the device finds them, within what the host promised.
 __device__ inline int page_within(int page, int num_pages) { return min(max(page, 0), num_pages - 1); }
+
+// x / d and x % d for 0 <= x < 2^31 - 1 without a division: (x + 1) / d by way of d's inverse is less than one too small, so its floor is the quotient or one less.
+struct Quotient {
+    int q, r;
+};
+__device__ inline Quotient divide(int x, int d, uint32_t inverse) {
+    Quotient a;
+    a.q = (int)__umulhi((uint32_t)x + 1u, inverse);
+    a.r = x - a.q * d;
+    const bool more = a.r >= d;
+    a.q += more ? 1 : 0;
+    a.r -= more ? d : 0;
+    return a;
+}
 
 inline int check_batch_rows(const char* what, const BatchRows& b, float scale) {
     CPMCU_CHECK_ARG(b.n >= 0 && b.n < 1 << 24, "%s: n=%d outside [0, 2^24)", what, b.n);

@@ -500,10 +500,11 @@ extern "C" int cpmcu_batch_decode_attention(const void* q, int64_t q_stride, con
                                       int64_t table_stride, int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv,
                                       float scale, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
     BatchRows b{(const uint16_t*)q, (uint16_t*)out, q_stride, out_stride, (const uint16_t*)k_pool, (const uint16_t*)v_pool, block_tables, row_offsets, positions,
-                table_stride, num_requests, max_blocks, num_pages, n, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, scale * 1.44269504088896341f};
+                table_stride, num_requests, max_blocks, num_pages, n, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, 0, scale * 1.44269504088896341f};
     const int rc = check_batch_rows("decode_attention", b, scale);
     if (rc != CPMCU_OK) return rc;
     if (n == 0) return CPMCU_OK;
+    b.group_inverse = 0xffffffffu / (uint32_t)b.group;
     CPMCU_CHECK_ARG(row_offsets || n == num_requests, "decode_attention: %d rows of %d requests need row_offsets", n, num_requests);
     const Sizes s = sizes_of(num_requests, max_blocks, Hq, Hkv);
     CPMCU_CHECK_ARG(workspace && workspace_bytes >= s.bytes, "decode_attention: workspace of %zu bytes, %zu needed", workspace_bytes, s.bytes);

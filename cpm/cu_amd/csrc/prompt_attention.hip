@@ -174,7 +174,7 @@ struct PromptParams {
     const Work* works;
     const Join* joins;
     float4* parts;  // [slot][KV head][wave][16 quads][64 lanes]: sums that have not been divided yet
-    float2* stats;  // [slot][KV head][256]: (reference in powers of two, sum)
+    float2* stats;  // [slot][KV head][128]: (reference in powers of two, sum)
 };
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
@@ -192,13 +192,6 @@ __device__ inline void request_4k(const void* base, uint32_t o0, uint32_t o1, ui
                  : : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds_at) : "memory", "m0");
 }
 
-template <typename E>
-__device__ inline bool any_not_finite(typename Elem<E>::x8 v) {  // an exponent of ones among eight values
-    constexpr uint32_t kOnes = Elem<E>::kDtype == 0 ? 0x7c00u : 0x7f80u;
-    const uint4 w = __builtin_bit_cast(uint4, v);
-    const auto has = [](uint32_t x) { return (x & kOnes) == kOnes || ((x >> 16) & kOnes) == kOnes; };
-    return has(w.x) || has(w.y) || has(w.z) || has(w.w);
-}
 template <typename E>
 __device__ inline bool not_finite(E v) {
     constexpr uint32_t kOnes = Elem<E>::kDtype == 0 ? 0x7c00u : 0x7f80u;
@@ -228,9 +221,12 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     const int qcol = lane & 31, hf = lane >> 5;
     const int packed = w.rows * b.group, base_row = w.tile * kTileRows + wave * kWaveRows;
     const int R = base_row + qcol, Rc = min(R, packed - 1);
-    const bool row_ok = R < packed, wave_ok = base_row < packed;
-    const int token = Rc / b.group, head = g * b.group + Rc % b.group;
-    const int pos = w.p0 + token;
+    const bool wave_ok = base_row < packed;
+    const int pos = w.p0 + divide(Rc, b.group, b.group_inverse).q;
+    const auto row_at = [&](int R, int64_t stride) {  // where packed row R's 128 values begin
+        const Quotient row = divide(R, b.group, b.group_inverse);
+        return (int64_t)(w.row0 + row.q) * stride + (g * b.group + row.r) * kHeadDim;
+    };
     // positions of the wave's first and last rows
     const int wave_first = __builtin_amdgcn_readfirstlane(pos), wave_last = __builtin_amdgcn_readlane(pos, 31);
     const int n = w.end - w.begin;
@@ -272,15 +268,21 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     };
     request_k(0, 0);
     request_v(0, 0);
-    X8 qreg[8];  // Q as the second operand of S^T = K Q^T: lane (qcol, hf) has dims 16 ks + 8 hf + [0, 8)
-    {
-        const E* const row = reinterpret_cast<const E*>(b.q) + (int64_t)(w.row0 + token) * b.q_stride + head * kHeadDim;
+    // Q's rows come through LDS, whole, in the stage that the second tile will have.
+    char* const q_stage = ring + kStageBytes + wave * (kWaveRows * 256);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const X8*>(row + 16 * ks + 8 * hf);
+    for (int x = 0; x < kWaveRows / 4; ++x) {
+        const int r = x * 4 + (lane >> 4);
+        const uint16_t* const from = b.q + row_at(min(base_row + r, packed - 1), b.q_stride) + ((lane & 15) ^ (r & 15)) * 8;
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)(q_stage + x * 1024)) : "memory", "m0");
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (n > 1) request_k(1, 1);
+    X8 qreg[8];  // as the second operand of S^T = K Q^T: lane (qcol, hf) has dims 16 ks + 8 hf + [0, 8)
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const X8*>(q_stage + k_at(qcol, 2 * ks + hf));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     meet();
+    if (n > 1) request_k(1, 1);
 
     f32x16 oacc[4], sacc[2];
 #pragma unroll
@@ -422,31 +424,32 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
         next(i);
         if (active) {
             // A tile that not all rows see whole: a value that some row may not see must not reach its sum, not even as 0 times infinity.  (Behind the last row's
-            // position lies what the page held before.)  Few tiles come here: four operands at a time, and nothing worked out ahead of the loop for them.
+            // position lies what the page held before.)  0 times all of the values is 0 if they are finite; few tiles have others.
             int from = (i % kStages) * kStageBytes;
             uint32_t odd = 0;  // of this lane's keys, those that have such values: bit 8 j + e is key 16 j + 4 hf + e % 4 + 8 (e / 4)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                asm volatile("" : "+v"(from));
-                X8 some_v[4];
-                bool some = false;
+            for (int j = 0; j < 4; j += 2) {
+                asm volatile("" : "+v"(from));  // (nothing is worked out ahead of the loop for this)
+                X8 vf[8];
+                float none[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    some_v[x] = read_v(v_base + from, 4 * j + x);
-                    some = some || any_not_finite<E>(some_v[x]);
-                }
-                if (__any(some)) {  // zeros for the product
+                for (int x = 0; x < 8; ++x) vf[x] = read_v(v_base + from, 4 * j + x);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
+                for (int x = 0; x < 8; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) none[e] = Elem<E>::dot2_acc(X2{vf[x][2 * e], vf[x][2 * e + 1]}, X2{(E)0.f, (E)0.f}, none[e]);
+                if (__any(none[0] + none[1] + none[2] + none[3] != 0.f)) {  // zeros for the product
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (not_finite(some_v[x][e])) {
-                                odd |= 1u << (8 * j + e);
-                                some_v[x][e] = (E)0.f;
+                            if (not_finite(vf[x][e])) {
+                                odd |= 1u << (8 * (j + (x >> 2)) + e);
+                                vf[x][e] = (E)0.f;
                             }
                 }
 #pragma unroll
-                for (int x = 0; x < 4; ++x) oacc[x] = Elem<E>::mfma_32x32x16(some_v[x], pb[j], oacc[x]);
+                for (int x = 0; x < 8; ++x) oacc[x & 3] = Elem<E>::mfma_32x32x16(vf[x], pb[j + (x >> 2)], oacc[x & 3]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (__any(odd != 0)) {
@@ -495,9 +498,10 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
         if (hf == 0) p.stats[part * kTileRows + wave * kWaveRows + qcol] = make_float2(m_ref, l_all);
         return;
     }
-    if (!row_ok) return;
+    // Through LDS, so that memory gets whole rows: the wave's 32 rows take the place of a quarter of the stages' K, which everybody has read.
     const float inv = 1.f / l_all;
-    E* const row = reinterpret_cast<E*>(b.out) + (int64_t)(w.row0 + token) * b.out_stride + head * kHeadDim;
+    char* const o_stage = ring + (wave >> 1) * kStageBytes + (wave & 1) * (kWaveRows * 256);
+    static_assert(kWaves == 4 && kStages == 2 && kWaveRows * 256 * 2 == kKBytes, "two waves' rows in a stage's K");
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -505,8 +509,16 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
             X4 o;
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = (E)(oacc[db][rq * 4 + e] * inv);
-            *reinterpret_cast<X4*>(row + db * 32 + rq * 8 + hf * 4) = o;
+            *reinterpret_cast<X4*>(o_stage + k_at(qcol, db * 4 + rq) + hf * 8) = o;
         }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    int at = lane;
+    asm volatile("" : "+v"(at));  // (the rows' places of the beginning, kept, would take the loop's registers)
+#pragma unroll
+    for (int x = 0; x < kWaveRows / 4; ++x) {
+        const int r = x * 4 + (at >> 4);
+        if (base_row + r < packed) *reinterpret_cast<X8*>(b.out + row_at(base_row + r, b.out_stride) + (at & 15) * 8) = *reinterpret_cast<const X8*>(o_stage + k_at(r, at & 15));
+    }
 }
 
 // The pieces of a tile: with M the largest of their references m, sum = sum_i l_i 2^(m_i - M), out = sum_i O_i 2^(m_i - M) / sum.  A workgroup takes 32 of the
@@ -611,10 +623,11 @@ extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, con
                                       int64_t table_stride, int max_blocks, const int32_t* row_offsets, const int32_t* positions, int num_requests, int n, int Hq, int Hkv,
                                       float scale, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
     BatchRows b{(const uint16_t*)q, (uint16_t*)out, q_stride, out_stride, (const uint16_t*)k_pool, (const uint16_t*)v_pool, block_tables, row_offsets, positions,
-                table_stride, num_requests, max_blocks, num_pages, n, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, scale * 1.44269504088896341f};
+                table_stride, num_requests, max_blocks, num_pages, n, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, 0, scale * 1.44269504088896341f};
     const int rc = check_batch_rows("prompt_attention", b, scale);
     if (rc != CPMCU_OK) return rc;
     if (n == 0) return CPMCU_OK;
+    b.group_inverse = 0xffffffffu / (uint32_t)b.group;
     CPMCU_CHECK_ARG(row_offsets, "prompt_attention: null pointer argument");
     const Sizes s = sizes_of(num_requests, max_blocks, n, Hq, Hkv);
     CPMCU_CHECK_ARG(workspace && workspace_bytes >= s.bytes, "prompt_attention: workspace of %zu bytes, %zu needed", workspace_bytes, s.bytes);
