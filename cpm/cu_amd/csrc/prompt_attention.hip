@@ -111,7 +111,7 @@ __global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
             else lo = mid + 1;
         }
         Tile f{lo, t - (lo > 0 ? tile_end[lo - 1] : 0), 0};
-        const int last = min(rows[lo] - 1, (int)(((int64_t)(f.tile + 1) * kTileRows - 1) / p.group));
+        const int last = min(rows[lo] - 1, (int)(((uint32_t)(f.tile + 1) * kTileRows - 1) / (uint32_t)p.group));  // (rows times heads: 31 bits)
         f.keys = (first[lo] + last) / kTileKeys + 1;
         return f;
     };
@@ -159,8 +159,8 @@ __global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
             slot = atomicAdd(&slots, pieces);
             p.joins[atomicAdd(&joins, 1)] = Join{row0[r], rows[r], f.tile, slot, pieces, {0, 0, 0}};
         }
-        for (int i = 0; i < pieces; ++i)
-            p.works[at + i] = Work{row0[r], rows[r], first[r], r, f.tile, (int)((int64_t)f.keys * i / pieces), (int)((int64_t)f.keys * (i + 1) / pieces), slot < 0 ? -1 : slot + i};
+        for (uint32_t i = 0; i < (uint32_t)pieces; ++i)  // (2^20 tiles of keys, 2^11 pieces)
+            p.works[at + i] = Work{row0[r], rows[r], first[r], r, f.tile, (int)((uint32_t)f.keys * i / pieces), (int)((uint32_t)f.keys * (i + 1) / pieces), slot < 0 ? -1 : slot + (int)i};
     }
     __syncthreads();
     if (tid == 0) p.listed->joins = joins;
@@ -521,67 +521,70 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     }
 }
 
-// The pieces of a tile: with M the largest of their references m, sum = sum_i l_i 2^(m_i - M), out = sum_i O_i 2^(m_i - M) / sum.  A workgroup takes 32 of the
-// rows and 32 of their dims at a time, its waves every fourth piece each.
-constexpr int kJoinWaves = 4, kJoinGrid = 1024;
+// The pieces of a tile: with M the largest of their references m, sum = sum_i l_i 2^(m_i - M), out = sum_i O_i 2^(m_i - M) / sum, in their order.  A workgroup takes 32 of
+// the rows at a time, a wave 32 of their dims.
+constexpr int kJoinWaves = kHeadDim / 32, kJoinGrid = 2048, kJoinAtOnce = 4;
 template <typename E>
 __global__ __launch_bounds__(64 * kJoinWaves) void prompt_join_kernel(PromptParams p) {
     typedef typename Elem<E>::x4 X4;
-    __shared__ f32x4 s_sum[kJoinWaves][4][64];
-    __shared__ float2 s_stat[kJoinWaves][kWaveRows];
     const BatchRows& b = p.b;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qcol = lane & 31, hf = lane >> 5;
-    const int64_t all = (int64_t)p.listed->joins * b.Hkv * kWaves * 4;
-    for (int64_t x = blockIdx.x; x < all; x += gridDim.x) {
-        const int db = (int)(x & 3), block = (int)(x >> 2) % kWaves, g = (int)((x >> 2) / kWaves % b.Hkv);
-        const Join j = p.joins[(x >> 2) / kWaves / b.Hkv];
+    const int lane = threadIdx.x & 63, db = threadIdx.x >> 6, qcol = lane & 31, hf = lane >> 5;
+    const int all = p.listed->joins * b.Hkv * kWaves;
+    for (int x = blockIdx.x; x < all; x += gridDim.x) {
+        const int block = x % kWaves, g = x / kWaves % b.Hkv;
+        const Join j = p.joins[x / kWaves / b.Hkv];
         const int base_row = j.tile * kTileRows + block * kWaveRows, R = base_row + qcol;
         if (base_row >= j.rows * b.group) continue;
         float M = -INFINITY, L = 0.f;
         f32x4 sum[4];
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) sum[rq] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int i = wave; i < j.pieces; i += kJoinWaves) {
-            const size_t part = (size_t)(j.slot + i) * b.Hkv + g;
-            const float2 st = p.stats[part * kTileRows + block * kWaveRows + qcol];
-            const float4* const from = p.parts + ((part * kWaves + block) * 16 + db * 4) * 64 + lane;
-            f32x4 o[4];
+        for (int i0 = 0; i0 < j.pieces; i0 += kJoinAtOnce) {
+            float2 st[kJoinAtOnce];
+            f32x4 o[kJoinAtOnce][4];
 #pragma unroll
-            for (int rq = 0; rq < 4; ++rq) o[rq] = __builtin_bit_cast(f32x4, from[rq * 64]);
-            const float m = fmaxf(M, st.x), m_scaled = m == -INFINITY ? 0.f : m;
-            const float f = __builtin_amdgcn_exp2f(M - m_scaled), w = __builtin_amdgcn_exp2f(st.x - m_scaled);
+            for (int u = 0; u < kJoinAtOnce; ++u) {
+                st[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int rq = 0; rq < 4; ++rq) o[u][rq] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (i0 + u >= j.pieces) continue;
+                const size_t part = (size_t)(j.slot + i0 + u) * b.Hkv + g;
+                st[u] = p.stats[part * kTileRows + block * kWaveRows + qcol];
+                const float4* const from = p.parts + ((part * kWaves + block) * 16 + db * 4) * 64 + lane;
+#pragma unroll
+                for (int rq = 0; rq < 4; ++rq) o[u][rq] = __builtin_bit_cast(f32x4, from[rq * 64]);
+            }
+            float m = M;
+#pragma unroll
+            for (int u = 0; u < kJoinAtOnce; ++u) m = fmaxf(m, st[u].x);
+            const float m_scaled = m == -INFINITY ? 0.f : m, f = __builtin_amdgcn_exp2f(M - m_scaled);
             M = m;
-            L = __builtin_fmaf(st.y, w, L * f);
-            // (a piece that the row sees nothing of has zeros)
+            L *= f;
 #pragma unroll
             for (int rq = 0; rq < 4; ++rq)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[rq][e] = __builtin_fmaf(o[rq][e], w, sum[rq][e] * f);
-        }
-        __syncthreads();  // (the last ones have been read)
+                for (int e = 0; e < 4; ++e) sum[rq][e] *= f;
 #pragma unroll
-        for (int rq = 0; rq < 4; ++rq) s_sum[wave][rq][lane] = sum[rq];
-        if (hf == 0) s_stat[wave][qcol] = make_float2(M, L);
-        __syncthreads();
-        if (R < j.rows * b.group) {  // each wave finishes a quarter of the dims
-            M = -INFINITY;
+            for (int u = 0; u < kJoinAtOnce; ++u) {
+                // (a piece that the row sees nothing of has zeros)
+                const float w = __builtin_amdgcn_exp2f(st[u].x - m_scaled);
+                L = __builtin_fmaf(st[u].y, w, L);
 #pragma unroll
-            for (int w = 0; w < kJoinWaves; ++w) M = fmaxf(M, s_stat[w][qcol].x);
-            L = 0.f;
-            f32x4 y = {0.f, 0.f, 0.f, 0.f};
+                for (int rq = 0; rq < 4; ++rq)
 #pragma unroll
-            for (int w = 0; w < kJoinWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f(s_stat[w][qcol].x - M);
-                L = __builtin_fmaf(s_stat[w][qcol].y, f, L);
-                const f32x4 o = s_sum[w][wave][lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[e], f, y[e]);
+                    for (int e = 0; e < 4; ++e) sum[rq][e] = __builtin_fmaf(o[u][rq][e], w, sum[rq][e]);
             }
-            const float inv = 1.f / L;
+        }
+        if (R >= j.rows * b.group) continue;
+        const Quotient row = divide(R, b.group, b.group_inverse);
+        const float inv = 1.f / L;
+        E* const to = reinterpret_cast<E*>(b.out) + (int64_t)(j.row0 + row.q) * b.out_stride + (g * b.group + row.r) * kHeadDim + db * 32 + hf * 4;
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
             X4 o;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (E)(y[e] * inv);
-            *reinterpret_cast<X4*>(reinterpret_cast<E*>(b.out) + (int64_t)(j.row0 + R / b.group) * b.out_stride + (g * b.group + R % b.group) * kHeadDim + db * 32 + wave * 8 + hf * 4) = o;
+            for (int e = 0; e < 4; ++e) o[e] = (E)(sum[rq][e] * inv);
+            *reinterpret_cast<X4*>(to + rq * 8) = o;
         }
     }
 }
@@ -639,13 +642,13 @@ extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, con
     PromptParams p{b, plan.listed, plan.works, plan.joins, (float4*)(ws + s.parts_at), (float2*)(ws + s.stats_at)};
     const hipStream_t st = resolve_stream(stream);
     const bool bf = options().dtype == 1;
-    if (num_requests <= 256 && s.tiles <= 512) hipLaunchKernelGGL((prompt_plan_kernel<256, 1>), dim3(1), dim3(256), 0, st, plan);
+    if (num_requests <= 256 && s.tiles <= 2048) hipLaunchKernelGGL((prompt_plan_kernel<256, 1>), dim3(1), dim3(256), 0, st, plan);
     else hipLaunchKernelGGL((prompt_plan_kernel<1024, kMostRequests / 1024>), dim3(1), dim3(1024), 0, st, plan);
     CPMCU_LAUNCH_CHECK();
     hipLaunchKernelGGL(bf ? prompt_attention_kernel<bf16> : prompt_attention_kernel<f16>, dim3((int)grid), dim3(kThreads), 0, st, p);
     CPMCU_LAUNCH_CHECK();
     if (s.joins > 0) {
-        hipLaunchKernelGGL(bf ? prompt_join_kernel<bf16> : prompt_join_kernel<f16>, dim3((int)std::min<int64_t>(s.joins * Hkv * kWaves * 4, kJoinGrid)), dim3(64 * kJoinWaves), 0, st, p);
+        hipLaunchKernelGGL(bf ? prompt_join_kernel<bf16> : prompt_join_kernel<f16>, dim3((int)std::min<int64_t>(s.joins * Hkv * kWaves, kJoinGrid)), dim3(64 * kJoinWaves), 0, st, p);
         CPMCU_LAUNCH_CHECK();
     }
     return CPMCU_OK;
