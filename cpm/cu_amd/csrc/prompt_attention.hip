@@ -384,6 +384,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
         const uint32_t v_now = v_of(i), k_next = k_of(i + 1);
         probabilities();
         next(i);
+        __builtin_amdgcn_s_setprio(1);  // (the other workgroup's vector instructions would delay the products, 1 % in all)
         X8 vf[8], vg[8], kf[8], kg[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) vf[x] = read_v(v_now, x);
@@ -413,6 +414,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
     }
     for (; i < n; ++i) {
         const int c0 = (w.begin + i) * kTileKeys;
