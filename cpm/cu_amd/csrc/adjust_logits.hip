@@ -7,20 +7,25 @@
 //
 // What bounds it: a row is read and written once; the counts are not read from a table of all tokens, which somebody would have to keep and which is
 // larger than the row itself: a workgroup has a slice of the vocabulary for some rows and counts the text's tokens that lie in it, in LDS
-// (whole numbers: their order does not matter).  So a text is read once for each slice, out of L2.
+// (whole numbers: their order does not matter).  So a text is read once for each slice, out of L2.  512 rows of 73447 with texts of 1500, 40 biases
+// and masks: 44 us, 3.4 TB/s of 150 MB (a plain copy of them takes 32); the instructions that count are what is left, so waves are many (32 a CU: with
+// 20 they take 50) and registers and LDS few: the lists of biases have the room that the call's list needs.
 #include "batch_attention.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #pragma clang fp contract(off)
 
 namespace cpmcu {
 namespace {
 
-constexpr int kThreads = 256, kPieces = 2;   // pieces of 8 logits that a thread has of a row
-constexpr int kSlice = kThreads * kPieces * 8;
+constexpr int kPieces = 2;      // pieces of 8 logits that a thread has of a row
 constexpr int kAhead = 8;       // places that a row's slices may lie ahead of another one's, because rows begin anywhere on 2 bytes
-constexpr int kCounted = kSlice + kAhead;
+// Slices of 8192 where rows share a text of some length, because each slice reads it (60 tree nodes, a text of 20000: 17 us, with 4096 21, with 16384 19);
+// else of 4096 (512 rows of their own texts: 44 us, with 8192 52, with 2048 54).
+constexpr int threads_of(bool shared) { return shared ? 512 : 256; }
+constexpr int slice_of(bool shared) { return threads_of(shared) * kPieces * 8; }
 constexpr int kTextAtOnce = 8;  // tokens that a thread requests together
 constexpr int kMostBiases = 1024;
 
@@ -52,236 +57,270 @@ struct Ends {
     static constexpr uint32_t kHighest = kInfinity | 0x8000, kNone = (uint16_t)~kMinusInfinity;
 };
 
-template <typename E>
-__global__ __launch_bounds__(kThreads, 6) void adjust_logits_kernel(LogitsParams p) {
-    constexpr int kWords = kCounted / 32 + 2;
+// The largest of a wave's values, within rows of 16 lanes and then from row to row, without LDS.
+__device__ inline uint32_t wave_most(uint32_t v) {
+    const auto with = [&](auto from) { v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(from)::value, 0xf, 0xf, false)); };
+    with(std::integral_constant<int, 0x111>{});  // a lane takes its neighbour's, then that of two, four and eight lanes before it
+    with(std::integral_constant<int, 0x112>{});
+    with(std::integral_constant<int, 0x114>{});
+    with(std::integral_constant<int, 0x118>{});
+    with(std::integral_constant<int, 0x142>{});  // a row takes the last lane's of the row before it, the upper half that of lane 31
+    with(std::integral_constant<int, 0x143>{});
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// SHARED: rows of one text, one after the other, a text's draft tree among them; else a row a workgroup.
+template <typename E, bool SHARED>
+__global__ __launch_bounds__(threads_of(SHARED), SHARED ? 6 : 8) void adjust_logits_kernel(LogitsParams p) {
+    constexpr int kThreads = threads_of(SHARED), kSlice = slice_of(SHARED), kCounted = kSlice + kAhead, kWords = kCounted / 32 + 2, kBiases = kMostBiases / kThreads;
+    extern __shared__ int hit_at[];  // biases of the slice: place and number in the list, one for each of the list; behind them their values
+    float* const hit_value = reinterpret_cast<float*>(hit_at + p.biases);
     __shared__ __attribute__((aligned(16))) int count[kCounted];
     __shared__ uint32_t counted[kWords], biased[kWords];  // places that have a count, or a bias: few pieces of a row have one
-    __shared__ int hits, again, hit_at[kMostBiases];      // biases of the slice: place and number in the list
-    __shared__ float hit_value[kMostBiases];
+    __shared__ int hits, again;
     __shared__ uint64_t s_best[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int slice = blockIdx.x % p.slices, row_begin = blockIdx.x / p.slices * p.rows_each, row_end = min(row_begin + p.rows_each, p.n);
-    int request = -2;  // whose counts and biases are in LDS
-    float repetition = 1.f, presence = 0.f, frequency = 0.f;
+    const int slice = blockIdx.x % p.slices, row_begin = blockIdx.x / p.slices * (SHARED ? p.rows_each : 1), row_end = SHARED ? min(row_begin + p.rows_each, p.n) : row_begin + 1;
     // A row's pieces of 16 bytes lie where memory has them: the first one may begin in front of the row, by another number of places than the next row's.
     const int base = slice * kSlice - kAhead;  // what is counted is [base, base + kCounted)
-    const auto place_of = [&](int v) { return (unsigned)v < (unsigned)p.V && (unsigned)(v - base) < (unsigned)kCounted ? v - base : -1; };
+    const int first_place = max(base, 0), places = min(base + kCounted, p.V) - first_place;
+    const auto place_of = [&](int v) { return (unsigned)(v - first_place) < (unsigned)places ? v - base : -1; };
     const auto count_one = [&](int at) {
         atomicAdd(&count[at], 1);
         atomicOr(&counted[at >> 5], 1u << (at & 31));
     };
-    for (int t = row_begin; t < row_end; ++t) {
-        const uint16_t* const in = p.in + (int64_t)t * p.in_stride;
-        uint16_t* const out = p.out + (int64_t)t * p.out_stride;
-        const bool together = ((uintptr_t)in & 15) == ((uintptr_t)out & 15);
-        const int row_e0 = slice * kSlice - (int)((uintptr_t)in / 2 & 7);
-        // What depends on nothing is requested first: the launch is round trips, one after the other unless they overlap.
+    struct Row {
         uint4 words[kPieces];
         uint32_t mask_lo[kPieces], mask_hi[kPieces];
+        int e0, on_way;  // where the slice begins; a token on a tree node's way
+    };
+    const auto request_row = [&](int t, Row& x) {
+        const uint16_t* const in = p.in + (int64_t)t * p.in_stride;
+        x.e0 = slice * kSlice - (int)((uintptr_t)in / 2 & 7);
+        const uint32_t* const mask = p.allowed + (p.allowed ? (int64_t)t * p.allowed_stride : 0);
+        const int last = (p.V - 1) >> 5;
 #pragma unroll
-        for (int x = 0; x < kPieces; ++x) {
-            const int e0 = row_e0 + (x * kThreads + tid) * 8;
-            words[x] = uint4{0, 0, 0, 0};
-            mask_lo[x] = mask_hi[x] = ~0u;
-            if (together && e0 >= 0 && e0 + 8 <= p.V) words[x] = *reinterpret_cast<const uint4*>(in + e0);
+        for (int i = 0; i < kPieces; ++i) {
+            const int e0 = x.e0 + (i * kThreads + tid) * 8;
+            x.mask_lo[i] = x.mask_hi[i] = ~0u;
             if (p.allowed) {
-                const uint32_t* const mask = p.allowed + (int64_t)t * p.allowed_stride;
-                const int last = (p.V - 1) >> 5;
-                mask_lo[x] = mask[min(max(e0, 0) >> 5, last)];
-                mask_hi[x] = mask[min(max(e0 + 7, 0) >> 5, last)];
+                x.mask_lo[i] = mask[min(max(e0, 0) >> 5, last)];
+                x.mask_hi[i] = mask[min(max(e0 + 7, 0) >> 5, last)];
+            }
+            if (e0 >= 0 && e0 + 8 <= p.V) {
+                x.words[i] = *reinterpret_cast<const uint4*>(in + e0);
+            } else {  // a row's first and last piece; -infinity where it has none
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (uint32_t)Ends<E>::kMinusInfinity * 0x10001u;
+#pragma unroll 1
+                for (int j = max(-e0, 0); j < min(p.V - e0, 8); ++j) {
+                    const uint32_t keep = j & 1 ? 0xffffu : 0xffff0000u, put = (uint32_t)in[e0 + j] << (16 * (j & 1));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = j >> 1 == k ? (w[k] & keep) | put : w[k];
+                }
+                x.words[i] = uint4{w[0], w[1], w[2], w[3]};
             }
         }
-        int on_way = -1;  // a token on a tree node's way
-        if (p.draft_ids && tid < p.n && (p.tree_mask[(size_t)t * p.mask_words + (tid >> 6)] >> (tid & 63) & 1)) on_way = place_of(p.draft_ids[tid]);
-        int r = p.requests ? p.requests[t] : p.R == 1 ? 0 : t;
-        if ((unsigned)r >= (unsigned)p.R) r = -1;  // (a row of nobody: only its mask counts)
-        if (r != request) {
-            request = r;
-            const bool texts = r >= 0 && p.tokens, biases = r >= 0 && p.bias_ids;
-            const int32_t* const text = texts ? p.tokens + (size_t)r * p.L : nullptr;
-            int token[kTextAtOnce], len = 0, bias_id[kMostBiases / kThreads];
-            if (texts) {
-                len = min(max(p.lens[r], 0), p.L);
+        x.on_way = -1;
+        if (SHARED && p.draft_ids && tid < p.n && (p.tree_mask[(size_t)t * p.mask_words + (tid >> 6)] >> (tid & 63) & 1)) x.on_way = place_of(p.draft_ids[tid]);
+    };
+    // What depends on nothing is requested first: the launch is round trips, one after the other unless they overlap.
+    Row x;
+    request_row(row_begin, x);
+    int r = SHARED ? 0 : p.requests ? p.requests[row_begin] : p.R == 1 ? 0 : row_begin;
+    if ((unsigned)r >= (unsigned)p.R) r = -1;  // (a row of nobody: only its mask counts)
+    const bool texts = r >= 0 && p.tokens, biases = r >= 0 && p.bias_ids, draft = SHARED && p.draft_ids;
+    float repetition = 1.f, presence = 0.f, frequency = 0.f;
+    if (texts || draft || biases) {
+        const int32_t* const text = texts ? p.tokens + (size_t)r * p.L : nullptr;
+        int token[kTextAtOnce], len = 0, bias_id[kBiases];
+        if (texts) {
+            len = min(max(p.lens[r], 0), p.L);
 #pragma unroll
-                for (int u = 0; u < kTextAtOnce; ++u) token[u] = text[min(u * kThreads + tid, p.L - 1)];
+            for (int u = 0; u < kTextAtOnce; ++u) token[u] = text[min(u * kThreads + tid, p.L - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < kBiases; ++i) {
+            if (!biases || i * kThreads >= p.biases) break;
+            bias_id[i] = i * kThreads + tid < p.biases ? p.bias_ids[(size_t)r * p.biases + i * kThreads + tid] : -1;
+        }
+        if (p.penalties) {
+            repetition = p.penalties[r * 3];
+            presence = p.penalties[r * 3 + 1];
+            frequency = p.penalties[r * 3 + 2];
+        }
+        if (texts || draft) {
+#pragma unroll
+            for (int i = 0; i < kCounted / 4; i += kThreads)
+                if (i + kThreads <= kCounted / 4 || i + tid < kCounted / 4) reinterpret_cast<int4*>(count)[i + tid] = int4{0, 0, 0, 0};
+        }
+        if (tid < kWords) counted[tid] = biased[tid] = 0;
+        if (tid == 0) hits = again = 0;
+        __syncthreads();
+        for (int done = 0; done < len; done += kThreads * kTextAtOnce) {
+            if (done > 0) {
+#pragma unroll
+                for (int u = 0; u < kTextAtOnce; ++u) token[u] = text[min(done + u * kThreads + tid, p.L - 1)];
             }
 #pragma unroll
-            for (int x = 0; x < kMostBiases / kThreads; ++x) bias_id[x] = biases && x * kThreads + tid < p.biases ? p.bias_ids[(size_t)r * p.biases + x * kThreads + tid] : -1;
-            repetition = 1.f;
-            presence = frequency = 0.f;
-            if (r >= 0 && p.penalties) {
-                repetition = p.penalties[r * 3];
-                presence = p.penalties[r * 3 + 1];
-                frequency = p.penalties[r * 3 + 2];
-            }
-            if (t > row_begin) __syncthreads();  // (the last row's have been read)
-            if (texts || p.draft_ids)
-                for (int i = tid; i < kCounted / 4; i += kThreads) reinterpret_cast<int4*>(count)[i] = int4{0, 0, 0, 0};
-            if (tid < kWords) counted[tid] = biased[tid] = 0;
-            if (tid == 0) hits = again = 0;
-            __syncthreads();
-            for (int done = 0; done < len; done += kThreads * kTextAtOnce) {
-                if (done > 0) {
-#pragma unroll
-                    for (int u = 0; u < kTextAtOnce; ++u) token[u] = text[min(done + u * kThreads + tid, p.L - 1)];
-                }
-#pragma unroll
-                for (int u = 0; u < kTextAtOnce; ++u) {
-                    if (done + u * kThreads >= len) break;
-                    const int v = done + u * kThreads + tid < len ? place_of(token[u]) : -1;
-                    if (v >= 0) count_one(v);
-                }
-            }
-            if (biases) {
-#pragma unroll
-                for (int x = 0; x < kMostBiases / kThreads; ++x) {
-                    const int v = place_of(bias_id[x]), i = x * kThreads + tid;
-                    if (v < 0) continue;
-                    const int h = atomicAdd(&hits, 1);
-                    hit_at[h] = v << 10 | i;
-                    hit_value[h] = p.bias_values[(size_t)r * p.biases + i];
-                    const uint32_t bit = 1u << (v & 31);
-                    if (atomicOr(&biased[v >> 5], bit) & bit) again = 1;
-                }
-            }
-            __syncthreads();
-            if (again) {  // an index that stands several times: its first place gets all of them, added up in their order
-                for (int h = tid; h < hits; h += kThreads) {
-                    const int v = hit_at[h] >> 10;
-                    bool first = true;
-                    for (int x = 0; x < hits && first; ++x) first = !(hit_at[x] >> 10 == v && hit_at[x] < hit_at[h]);
-                    if (!first) continue;
-                    float sum = 0.f;
-                    for (int last = hit_at[h] - 1;;) {
-                        int next = INT32_MAX;
-                        for (int x = 0; x < hits; ++x)
-                            if (hit_at[x] >> 10 == v && hit_at[x] > last) next = min(next, hit_at[x]);
-                        if (next == INT32_MAX) break;
-                        sum += p.bias_values[(size_t)r * p.biases + (next & 1023)];
-                        last = next;
-                    }
-                    hit_value[h] = sum;
-                }
-                __syncthreads();
+            for (int u = 0; u < kTextAtOnce; ++u) {
+                if (done + u * kThreads >= len) break;
+                const int v = done + u * kThreads + tid < len ? place_of(token[u]) : -1;
+                if (v >= 0) count_one(v);
             }
         }
-        if (p.draft_ids) {  // (counted for this row only)
-            if (on_way >= 0) count_one(on_way);
+        if (biases) {
+#pragma unroll
+            for (int i = 0; i < kBiases; ++i) {
+                if (i * kThreads >= p.biases) break;
+                const int v = place_of(bias_id[i]), number = i * kThreads + tid;
+                if (v < 0) continue;
+                const int h = atomicAdd(&hits, 1);
+                hit_at[h] = v << 10 | number;
+                hit_value[h] = p.bias_values[(size_t)r * p.biases + number];
+                const uint32_t bit = 1u << (v & 31);
+                if (atomicOr(&biased[v >> 5], bit) & bit) again = 1;
+            }
+        }
+        __syncthreads();
+        if (biases && again) {  // an index that stands several times: its first place gets all of them, added up in their order
+            for (int h = tid; h < hits; h += kThreads) {
+                const int v = hit_at[h] >> 10;
+                bool first = true;
+                for (int i = 0; i < hits && first; ++i) first = !(hit_at[i] >> 10 == v && hit_at[i] < hit_at[h]);
+                if (!first) continue;
+                float sum = 0.f;
+                for (int last = hit_at[h] - 1;;) {
+                    int next = INT32_MAX;
+                    for (int i = 0; i < hits; ++i)
+                        if (hit_at[i] >> 10 == v && hit_at[i] > last) next = min(next, hit_at[i]);
+                    if (next == INT32_MAX) break;
+                    sum += p.bias_values[(size_t)r * p.biases + (next & 1023)];
+                    last = next;
+                }
+                hit_value[h] = sum;
+            }
             __syncthreads();
         }
-        uint64_t best = 0;
+    }
+    for (int t = row_begin;;) {
+        Row next;
+        const bool more = SHARED && t + 1 < row_end;
+        if (more) request_row(t + 1, next);
+        if (draft) {  // (counted for this row only)
+            if (x.on_way >= 0) count_one(x.on_way);
+            __syncthreads();
+        }
+        uint16_t* const out = p.out + (int64_t)t * p.out_stride;
+        const bool whole_words = ((uintptr_t)(out + x.e0) & 15) == 0;
+        uint32_t largest[kPieces];
 #pragma unroll
-        for (int x = 0; x < kPieces; ++x) {
-            const int e0 = row_e0 + (x * kThreads + tid) * 8, at = e0 - base;
-            const bool whole = together && e0 >= 0 && e0 + 8 <= p.V;
+        for (int i = 0; i < kPieces; ++i) {
+            const int e0 = x.e0 + (i * kThreads + tid) * 8, at = e0 - base;
+            uint32_t w[4] = {x.words[i].x, x.words[i].y, x.words[i].z, x.words[i].w};
             // bit j: place e0 + j (a word holds 32 places from a multiple of 32 on)
-            const uint32_t allowed = e0 < 0 ? mask_lo[x] << -e0 : (uint32_t)(((uint64_t)mask_hi[x] << 32 | mask_lo[x]) >> (e0 & 31));
-            const auto bits_at = [&](const uint32_t* set) { return (uint32_t)(((uint64_t)set[(at >> 5) + 1] << 32 | set[at >> 5]) >> (at & 31)) & 0xffu; };
-            const uint32_t has_count = bits_at(counted), has_bias = bits_at(biased);
-            const auto adjusted = [&](uint16_t bits, int j) {
-                float z = Elem<E>::from_bits(bits);
-                if (has_count >> j & 1) {
-                    const int c = count[at + j];
-                    if (c > 0) {  // (the tokens of another row's way have left their bits)
-                        const float less = z > 0.f ? z / repetition : z * repetition;
-                        z = less - frequency * (float)c - presence;
-                    }
-                }
-                if (has_bias >> j & 1) {
-                    int found = INT32_MAX;
-                    float value = 0.f;
-                    for (int h = 0; h < hits; ++h)
-                        if (hit_at[h] >> 10 == at + j && hit_at[h] < found) {
-                            found = hit_at[h];
-                            value = hit_value[h];
-                        }
-                    z += value;
-                }
-                return (allowed >> j & 1) ? Elem<E>::to_bits(z) : Ends<E>::kMinusInfinity;
-            };
-            uint32_t w[4] = {words[x].x, words[x].y, words[x].z, words[x].w};
-            if (whole) {
-                // What is masked first, two logits a word; what a text or a bias changes one by one.
-                if ((allowed & 0xffu) != 0xffu) {
+            uint32_t allowed = 0xff;
+            if (p.allowed) {
+                allowed = __builtin_amdgcn_alignbit(x.mask_hi[i], x.mask_lo[i], e0);
+                if (e0 < 0) allowed = x.mask_lo[i] << -e0;
+                if ((allowed & 0xffu) != 0xffu) {  // two logits a word
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t lo = allowed >> (2 * j) & 1 ? 0xffffu : 0u, hi = allowed >> (2 * j + 1) & 1 ? 0xffff0000u : 0u;
-                        w[j] = (w[j] & (lo | hi)) | ((uint32_t)Ends<E>::kMinusInfinity * 0x10001u & ~(lo | hi));
+                        const uint32_t lo = (uint32_t)((int)(allowed << (31 - 2 * j)) >> 31), hi = (uint32_t)((int)(allowed << (30 - 2 * j)) >> 31);
+                        const uint32_t keep = (lo & 0xffffu) | (hi & 0xffff0000u);
+                        w[j] = (w[j] & keep) | ((uint32_t)Ends<E>::kMinusInfinity * 0x10001u & ~keep);
                     }
                 }
+            }
+            if (texts || draft || biases) {
+                const auto bits_at = [&](const uint32_t* set) { return __builtin_amdgcn_alignbit(set[(at >> 5) + 1], set[at >> 5], at) & 0xffu; };
+                const uint32_t has_count = bits_at(counted), has_bias = bits_at(biased);
                 for (uint32_t rest = (has_count | has_bias) & allowed; rest; rest &= rest - 1) {
                     const int j = __builtin_ctz(rest), shift = 16 * (j & 1);
                     uint32_t old = w[0];
 #pragma unroll
-                    for (int i = 1; i < 4; ++i) old = j >> 1 == i ? w[i] : old;
-                    const uint32_t y = (old & ~(0xffffu << shift)) | (uint32_t)adjusted((uint16_t)(old >> shift), j) << shift;
+                    for (int k = 1; k < 4; ++k) old = j >> 1 == k ? w[k] : old;
+                    float z = Elem<E>::from_bits((uint16_t)(old >> shift));
+                    if (has_count >> j & 1) {
+                        const int c = count[at + j];
+                        if (c > 0) {  // (the tokens of another row's way have left their bits)
+                            const float less = z > 0.f ? z / repetition : z * repetition;
+                            z = less - frequency * (float)c - presence;
+                        }
+                    }
+                    if (has_bias >> j & 1) {
+                        int found = INT32_MAX;
+                        float value = 0.f;
+                        for (int h = 0; h < hits; ++h)
+                            if (hit_at[h] >> 10 == at + j && hit_at[h] < found) {
+                                found = hit_at[h];
+                                value = hit_value[h];
+                            }
+                        z += value;
+                    }
+                    const uint32_t y = (old & ~(0xffffu << shift)) | (uint32_t)Elem<E>::to_bits(z) << shift;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = j >> 1 == i ? y : w[i];
+                    for (int k = 0; k < 4; ++k) w[k] = j >> 1 == k ? y : w[k];
                 }
+            }
+            if (whole_words && e0 >= 0 && e0 + 8 <= p.V) {
                 *reinterpret_cast<uint4*>(out + e0) = uint4{w[0], w[1], w[2], w[3]};
             } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (uint32_t)Ends<E>::kMinusInfinity * 0x10001u;
-                for (int j = max(-e0, 0); j < min(p.V - e0, 8); ++j) {
-                    const uint16_t y = adjusted(in[e0 + j], j);
-                    out[e0 + j] = y;
-                    const uint32_t keep = j & 1 ? 0xffffu : 0xffff0000u, put = (uint32_t)y << (16 * (j & 1));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = j >> 1 == i ? (w[i] & keep) | put : w[i];
-                }
+#pragma unroll 1
+                for (int j = max(-e0, 0); j < min(p.V - e0, 8); ++j) out[e0 + j] = (uint16_t)((j & 4 ? j & 2 ? w[3] : w[2] : j & 2 ? w[1] : w[0]) >> (16 * (j & 1)));
             }
+            largest[i] = 0;
             if (!p.best) continue;
-            // the largest of a piece, of the wave's pieces, and the first place that has it
-            u16x2 key[4];
+            // The piece's largest and, behind it, how far in front of the piece's end it lies: of equals the first is the largest.
+            uint32_t most = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) key[j] = keys_of(w[j]);
-            const u16x2 two = __builtin_elementwise_max(__builtin_elementwise_max(key[0], key[1]), __builtin_elementwise_max(key[2], key[3]));
-            uint32_t most = max((uint32_t)two.x, (uint32_t)two.y);
-            if (most > Ends<E>::kHighest) {  // a NaN among them
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t key = __builtin_bit_cast(uint32_t, keys_of(w[j]));
+                most = max(most, max(key << 16 | (7 - 2 * j), (key & 0xffff0000u) | (6 - 2 * j)));
+            }
+            if (most >> 16 > Ends<E>::kHighest || (most >> 16) - 0x7fff <= 1) {  // a NaN among them; or a zero: the two zeros are one value
                 most = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (key[j].x > Ends<E>::kHighest) key[j].x = 0;
-                    if (key[j].y > Ends<E>::kHighest) key[j].y = 0;
-                    most = max(most, max((uint32_t)key[j].x, (uint32_t)key[j].y));
+                for (int j = 0; j < 8; ++j) {
+                    const u16x2 two = keys_of(w[j >> 1]);
+                    const uint32_t key = j & 1 ? two.y : two.x;
+                    if (key <= Ends<E>::kHighest) most = max(most, (key == 0x7fff ? 0x8000 : key) << 16 | (7 - j));
                 }
             }
-            if (most == 0x7fff) most = 0x8000;  // the zeros are one value
-            uint32_t top = most;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-            if (top > Ends<E>::kNone && lane == __builtin_ctzll(__ballot(most == top))) {
-                int j = 0;
-#pragma unroll
-                for (int i = 7; i >= 0; --i) {
-                    const uint32_t k = i & 1 ? key[i >> 1].y : key[i >> 1].x;
-                    if (k == top || (top == 0x8000 && k == 0x7fff)) j = i;
-                }
-                const uint64_t mine = (uint64_t)top << 32 | (0xffffffffu - (uint32_t)(e0 + j));
-                best = mine > best ? mine : best;
-            }
+            largest[i] = most;
         }
         if (p.best) {
-            // (one lane of the wave has it for each piece)
-            const uint64_t some = __ballot(best != 0);
+            // the wave's largest and the first place that has it
+            uint32_t all = largest[0];
+#pragma unroll
+            for (int i = 1; i < kPieces; ++i) all = max(all, largest[i]);
+            const uint32_t top = wave_most(all >> 16);
             uint64_t most = 0;
-            for (uint64_t rest = some; rest; rest &= rest - 1) {
-                const int from = __builtin_ctzll(rest);
-                const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(best >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)best, from);
-                most = other > most ? other : most;
+            if (top > Ends<E>::kNone) {
+#pragma unroll
+                for (int i = kPieces - 1; i >= 0; --i) {
+                    const uint64_t have = __ballot(largest[i] >> 16 == top);
+                    if (!have) continue;
+                    const int first = __builtin_ctzll(have);
+                    const int place = x.e0 + (i * kThreads + wave * 64 + first) * 8 + 7 - (__builtin_amdgcn_readlane((int)largest[i], first) & 7);
+                    most = (uint64_t)top << 32 | (0xffffffffu - (uint32_t)place);
+                }
             }
             if (lane == 0) s_best[wave] = most;
         }
-        if (p.best || p.draft_ids) __syncthreads();
-        if (on_way >= 0) atomicSub(&count[on_way], 1);
+        if (p.best || (draft && more)) __syncthreads();
+        if (draft && more && x.on_way >= 0) atomicSub(&count[x.on_way], 1);
         if (p.best && tid == 0) {
             uint64_t most = s_best[0];
 #pragma unroll
             for (int w = 1; w < kThreads / 64; ++w) most = s_best[w] > most ? s_best[w] : most;
             p.best[(size_t)t * p.slices + slice] = most;
         }
-        if ((p.best || p.draft_ids) && t + 1 < row_end) __syncthreads();
+        if (!more) break;
+        if (p.best || draft) __syncthreads();
+        ++t;
+        x = next;
     }
 }
 
@@ -303,7 +342,7 @@ __global__ __launch_bounds__(256) void adjust_logits_ids_kernel(const uint64_t* 
 }
 
 // (a row that does not begin on 16 bytes reaches up to seven places further)
-int slices_of(int V) { return ceil_div(V + 7, kSlice); }
+int slices_of(int V, bool shared) { return ceil_div(V + 7, slice_of(shared)); }
 
 }  // namespace
 }  // namespace cpmcu
@@ -312,7 +351,7 @@ using namespace cpmcu;
 
 extern "C" size_t cpmcu_adjust_logits_workspace_bytes(int n, int V) {
     if (n < 0 || n >= 1 << 24 || V < 1 || V > 1 << 24) return 0;
-    return sizeof(uint64_t) * (size_t)n * slices_of(V);
+    return sizeof(uint64_t) * (size_t)n * slices_of(V, false);
 }
 
 extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, int n, int V, const float* penalties, const int32_t* tokens, const int32_t* lens, int num_requests,
@@ -334,8 +373,12 @@ extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, in
     CPMCU_CHECK_ARG(!allowed || allowed_stride == 0 || allowed_stride >= (V + 31) / 32, "adjust_logits: rows of allowed closer than their words");
     CPMCU_CHECK_ARG(!draft_ids || (tree_mask && penalties && num_requests == 1 && !requests), "adjust_logits: draft_ids go with tree_mask and the penalties of one request");
     CPMCU_CHECK_ARG(!draft_ids || (n <= kMaxTree && mask_words >= ceil_div(n, 64)), "adjust_logits: a tree of %d nodes, masks of %d words", n, mask_words);
-    const int slices = slices_of(V);
-    const size_t need = ids ? sizeof(uint64_t) * (size_t)n * slices : 0;
+    // Rows of one text share its counts: as many of them a workgroup as leave four workgroups a CU.
+    const bool one_text = any && num_requests == 1 && !requests;
+    const int rows_each = one_text ? std::max(1, std::min(n, (int)((int64_t)n * slices_of(V, true) / 1024))) : 1;
+    const bool shared = rows_each > 1 || draft_ids;
+    const int slices = slices_of(V, shared);
+    const size_t need = ids ? sizeof(uint64_t) * (size_t)n * slices_of(V, false) : 0;
     CPMCU_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0), "adjust_logits: workspace of %zu bytes, %zu needed, on 8 bytes", workspace_bytes, need);
     const size_t in_bytes = 2 * ((size_t)(n - 1) * logits_stride + V), out_bytes = 2 * ((size_t)(n - 1) * out_stride + V), ints = 4;
     const bool in_place = logits == out && (n == 1 || logits_stride == out_stride);
@@ -348,15 +391,15 @@ extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, in
         CPMCU_CHECK_ARG(!overlap(m.at, m.bytes, out, out_bytes) && !overlap(m.at, m.bytes, ids, ids ? ints * n : 0), "adjust_logits: results in the memory of an argument");
     }
     CPMCU_CHECK_ARG(!overlap(ids, ids ? ints * n : 0, out, out_bytes) && !overlap(ids, ids ? ints * n : 0, logits, in_bytes), "adjust_logits: ids in the memory of logits");
-    // Rows of one text share its counts: as many of them a workgroup as leave four workgroups a CU.
-    const bool shared = any && num_requests == 1 && !requests;
-    const int rows_each = shared ? std::max(1, std::min(n, (int)((int64_t)n * slices / 1024))) : 1;
     const int64_t grid = (int64_t)ceil_div(n, rows_each) * slices;
     CPMCU_CHECK_ARG(grid <= INT32_MAX, "adjust_logits: %lld workgroups are beyond a launch", (long long)grid);
-    LogitsParams p{(const uint16_t*)logits, (uint16_t*)out, logits_stride, out_stride, allowed_stride, n, V, any ? num_requests : 0, max_tokens, num_biases, mask_words, rows_each, slices,
+    LogitsParams p{(const uint16_t*)logits, (uint16_t*)out, logits_stride, out_stride, allowed_stride, n, V, any ? num_requests : 0, max_tokens, bias_ids ? num_biases : 0, mask_words, rows_each, slices,
                    penalties, tokens, lens, requests, bias_ids, draft_ids, bias_values, allowed, tree_mask, ids ? (uint64_t*)workspace : nullptr, ids};
     const hipStream_t st = resolve_stream(stream);
-    hipLaunchKernelGGL(options().dtype == 1 ? adjust_logits_kernel<bf16> : adjust_logits_kernel<f16>, dim3((int)grid), dim3(kThreads), 0, st, p);
+    const bool bf = options().dtype == 1;
+    void (*kernel)(LogitsParams) = bf ? adjust_logits_kernel<bf16, false> : adjust_logits_kernel<f16, false>;
+    if (shared) kernel = bf ? adjust_logits_kernel<bf16, true> : adjust_logits_kernel<f16, true>;
+    hipLaunchKernelGGL(kernel, dim3((int)grid), dim3(threads_of(shared)), 8 * p.biases, st, p);
     CPMCU_LAUNCH_CHECK();
     if (ids) {
         hipLaunchKernelGGL(adjust_logits_ids_kernel, dim3(ceil_div(n, 4)), dim3(256), 0, st, p.best, n, slices, ids);
