@@ -25,7 +25,7 @@ constexpr float kMostSum = 4096.f;  // of a lane's 32 probabilities of a tile, b
 
 // ---- the list of work ----
 
-// The keys [begin, end) * 64 for rows [256 tile, 256 tile + 256) of the packed rows of a request whose `rows` rows start at row0 of the batch and
+// The keys [begin, end) * 64 for rows [128 tile, 128 tile + 128) of the packed rows of a request whose `rows` rows start at row0 of the batch and
 // at position p0.  slot: where its part of the results waits for the others, -1 if it has all of its keys.
 struct Work {
     int row0, rows, p0, request, tile, begin, end, slot;
