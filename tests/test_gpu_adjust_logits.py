@@ -145,6 +145,19 @@ def test_trees_of_every_size(gpu, n):
     case.check(*_run(case))
 
 
+@pytest.mark.parametrize("kw", [dict(n=640, V=40003, R=1, L=3000, nb=40, mask=True), dict(n=127, V=131073, tree=True, L=9000, nb=5), dict(n=640, V=40003, R=1, nb=3)], ids=["text", "tree", "biases"])
+@pytest.mark.parametrize("want_ids", [True, False])
+def test_many_rows_of_one_text(gpu, set_option, kw, want_ids):
+    """A workgroup has several rows, one behind the other, each beginning elsewhere on 16 bytes."""
+    set_option("dtype", int(want_ids))
+    case = Case(gpu, 8, dtype=int(want_ids), **kw)
+    skip = {} if "L" in kw else dict(penalties=None, tokens=None, lens=None)
+    if skip:
+        case.penalties[:] = [1.0, 0.0, 0.0]
+    out, ids = _run(case, want_ids=want_ids, **skip)
+    case.check(out, ids)
+
+
 def test_long_texts(gpu):
     case = Case(gpu, 1, n=3, V=5000, L=200000, lens=199999)
     case.check(*_run(case))
