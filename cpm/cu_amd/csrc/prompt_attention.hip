@@ -8,7 +8,7 @@
 // as many busy as the card's power allows (one of them forms products while the other one has its scores in the vector units).
 //
 // Which tiles there are follows from lengths that only the device knows, so a launch of one workgroup lists them first: longest first, those
-// that would outlast the others by much cut into pieces, which a third launch joins.
+// that would outlast the others by much cut into pieces, which a last launch joins.  Where they are few, each workgroup finds its own.
 #include "batch_attention.h"
 
 #include <algorithm>
@@ -48,85 +48,115 @@ struct PlanParams {
     Join* joins;
 };
 
-// The workgroup's threads have EACH requests each, then every THREADS-th tile of rows.  The launch is round trips -- offsets, positions, the list --
-// and meetings of its waves: with a request and a tile a thread 4.4 us, with four waves in place of sixteen 2 less.
+// A workgroup's threads have EACH requests each, then every THREADS-th tile of rows.
+struct Tile {
+    int request, tile, keys;  // keys: tiles of 64 of them that the last row sees
+};
 template <int THREADS, int EACH>
-__global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
-    constexpr int kMost = THREADS * EACH, kClasses = 64, kPlanWaves = THREADS / 64;
-    __shared__ int tile_end[kMost], row0[kMost], rows[kMost], first[kMost];
-    __shared__ int wave_total[kPlanWaves], in_class[kClasses], slots, joins;
-    __shared__ unsigned long long wave_cost[kPlanWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = p.num_requests;
-    if (tid < kClasses) in_class[tid] = 0;
-    if (tid == 0) slots = joins = 0;
-    int tiles[EACH], mine = 0;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        const int r = tid * EACH + e;
-        int lo = 0, count = 0, p0 = -1;
-        if (r < B) {
-            lo = min(max(p.row_offsets[r], 0), p.n);
-            count = min(max(p.row_offsets[r + 1], lo), p.n) - lo;
-            if (count > 0) p0 = p.positions[lo];
-            const int64_t room = (int64_t)p.max_blocks * kPage - p0;
-            count = p0 < 0 ? 0 : (int)min((int64_t)count, max(room, (int64_t)0));
-        }
-        tiles[e] = (int)(((int64_t)count * p.group + kTileRows - 1) / kTileRows);
-        mine = min(mine + tiles[e], p.most_tiles);
-        row0[r] = lo;
-        rows[r] = count;
-        first[r] = p0;
-    }
-    // Running totals of tiles, most_tiles at most (they stop there, so their grouping does not matter).
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int from = __shfl_up(upto, d);
-        if (lane >= d) upto = min(upto + from, p.most_tiles);
-    }
-    if (lane == 63) wave_total[wave] = upto;
-    const int lanes_before = __shfl_up(upto, 1);
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) {
-        if (w == wave) before = all;
-        all = min(all + wave_total[w], p.most_tiles);
-    }
-    before = min(before + (lane > 0 ? lanes_before : 0), p.most_tiles);
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        before = min(before + tiles[e], p.most_tiles);
-        tile_end[tid * EACH + e] = before;
-    }
-    __syncthreads();
-    struct Tile {
-        int request, tile, keys;  // keys: tiles of 64 of them that the last row sees
+struct Plan {
+    static constexpr int kMost = THREADS * EACH, kPlanWaves = THREADS / 64;
+    struct Lds {
+        int tile_end[kMost], row0[kMost], rows[kMost], first[kMost];
+        unsigned long long wave_sum[2][kPlanWaves];
     };
-    const auto find = [&](int t) {
-        int lo = 0, hi = B - 1;
+    const PlanParams& p;
+    Lds& lds;
+    int tid;
+
+    // What the threads before this one have, and what all of them have.
+    template <typename T, typename F>
+    __device__ T before(T mine, int part, F add, T& all) const {
+        const int lane = tid & 63, wave = tid >> 6;
+        T upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const T from = __shfl_up(upto, d);
+            if (lane >= d) upto = add(upto, from);
+        }
+        if (lane == 63) lds.wave_sum[part][wave] = (unsigned long long)upto;
+        T lanes = __shfl_up(upto, 1);
+        if (lane == 0) lanes = 0;
+        __syncthreads();
+        T waves = 0;
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < kPlanWaves; ++w) {
+            if (w == wave) waves = all;
+            all = add(all, (T)lds.wave_sum[part][w]);
+        }
+        return add(waves, lanes);
+    }
+    // The requests' rows and tiles: how many tiles there are.  (Totals are most_tiles at most: they stop there, so their grouping does not matter.)
+    __device__ int requests() const {
+        const auto add = [&](int x, int y) { return min(x + y, p.most_tiles); };
+        int tiles[EACH], mine = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int r = tid * EACH + e;
+            int lo = 0, count = 0, p0 = -1;
+            if (r < p.num_requests) {
+                lo = min(max(p.row_offsets[r], 0), p.n);
+                count = min(max(p.row_offsets[r + 1], lo), p.n) - lo;
+                if (count > 0) p0 = p.positions[lo];
+                const int64_t room = (int64_t)p.max_blocks * kPage - p0;
+                count = p0 < 0 ? 0 : (int)min((int64_t)count, max(room, (int64_t)0));
+            }
+            tiles[e] = (int)(((int64_t)count * p.group + kTileRows - 1) / kTileRows);
+            mine = add(mine, tiles[e]);
+            lds.row0[r] = lo;
+            lds.rows[r] = count;
+            lds.first[r] = p0;
+        }
+        int all, upto = before(mine, 0, add, all);
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            upto = add(upto, tiles[e]);
+            lds.tile_end[tid * EACH + e] = upto;
+        }
+        __syncthreads();
+        return all;
+    }
+    __device__ Tile find(int t) const {
+        int lo = 0, hi = p.num_requests - 1;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (tile_end[mid] > t) hi = mid;
+            if (lds.tile_end[mid] > t) hi = mid;
             else lo = mid + 1;
         }
-        Tile f{lo, t - (lo > 0 ? tile_end[lo - 1] : 0), 0};
-        const int last = min(rows[lo] - 1, (int)(((uint32_t)(f.tile + 1) * kTileRows - 1) / (uint32_t)p.group));  // (rows times heads: 31 bits)
-        f.keys = (first[lo] + last) / kTileKeys + 1;
+        Tile f{lo, t - (lo > 0 ? lds.tile_end[lo - 1] : 0), 0};
+        const int last = min(lds.rows[lo] - 1, (int)(((uint32_t)(f.tile + 1) * kTileRows - 1) / (uint32_t)p.group));  // (rows times heads: 31 bits)
+        f.keys = (lds.first[lo] + last) / kTileKeys + 1;
         return f;
-    };
-    const Tile own = tid < all ? find(tid) : Tile{0, 0, 0};  // (most launches have no more)
-    unsigned long long cost = own.keys;
-    for (int t = tid + THREADS; t < all; t += THREADS) cost += find(t).keys;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) cost += __shfl_xor(cost, d);
-    if (lane == 0) wave_cost[wave] = cost;
-    __syncthreads();
-    cost = 0;
-#pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) cost += wave_cost[w];
-    const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts);
-    const int chunk = (int)min(max(share, (int64_t)kLeastKeys), (int64_t)INT32_MAX);
+    }
+    // How many tiles of keys a piece has at most, from what all tiles have together.
+    __device__ int chunk_of(unsigned long long cost) const {
+        const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts);
+        return (int)min(max(share, (int64_t)kLeastKeys), (int64_t)INT32_MAX);
+    }
+    __device__ Work piece(const Tile& f, int i, int pieces, int slot) const {  // (2^20 tiles of keys, 2^11 pieces)
+        const int r = f.request;
+        return Work{lds.row0[r], lds.rows[r], lds.first[r], r, f.tile, (int)((uint32_t)f.keys * i / pieces), (int)((uint32_t)f.keys * (i + 1) / pieces), slot < 0 ? -1 : slot + i};
+    }
+    __device__ Join join(const Tile& f, int slot, int pieces) const { return Join{lds.row0[f.request], lds.rows[f.request], f.tile, slot, pieces, {0, 0, 0}}; }
+};
+
+// The launch is round trips -- offsets, positions, the list -- and meetings of its waves: with a request and a tile a thread 4.4 us, with four waves in place of sixteen
+// 3.1.
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
+    constexpr int kClasses = 64;
+    __shared__ typename Plan<THREADS, EACH>::Lds lds;
+    __shared__ int in_class[kClasses], slots, joins;
+    const int tid = threadIdx.x;
+    const Plan<THREADS, EACH> plan{p, lds, tid};
+    if (tid < kClasses) in_class[tid] = 0;
+    if (tid == 0) slots = joins = 0;
+    const int all = plan.requests();
+    const Tile own = tid < all ? plan.find(tid) : Tile{0, 0, 0};  // (most launches have no more)
+    unsigned long long mine = own.keys, cost;
+    for (int t = tid + THREADS; t < all; t += THREADS) mine += plan.find(t).keys;
+    plan.before(mine, 1, [](unsigned long long x, unsigned long long y) { return x + y; }, cost);
+    const int chunk = plan.chunk_of(cost);
     const auto pieces_of = [&](int keys) { return (keys + chunk - 1) / chunk; };
     // Longest first: counted in classes of a quarter of an octave, then put in their places.
     const auto class_of = [&](int keys, int pieces) {
@@ -134,7 +164,7 @@ __global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
         return kClasses - 1 - min(length < 4 ? length : 4 * (msb - 1) + (length >> (msb - 2) & 3), kClasses - 1);
     };
     for (int t = tid; t < all; t += THREADS) {
-        const Tile f = t == tid ? own : find(t);
+        const Tile f = t == tid ? own : plan.find(t);
         const int pieces = pieces_of(f.keys);
         atomicAdd(&in_class[class_of(f.keys, pieces)], pieces);
     }
@@ -152,27 +182,62 @@ __global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
     }
     __syncthreads();
     for (int t = tid; t < all; t += THREADS) {
-        const Tile f = t == tid ? own : find(t);
-        const int r = f.request, pieces = pieces_of(f.keys), at = atomicAdd(&in_class[class_of(f.keys, pieces)], pieces);
+        const Tile f = t == tid ? own : plan.find(t);
+        const int pieces = pieces_of(f.keys), at = atomicAdd(&in_class[class_of(f.keys, pieces)], pieces);
         int slot = -1;
         if (pieces > 1) {
             slot = atomicAdd(&slots, pieces);
-            p.joins[atomicAdd(&joins, 1)] = Join{row0[r], rows[r], f.tile, slot, pieces, {0, 0, 0}};
+            p.joins[atomicAdd(&joins, 1)] = plan.join(f, slot, pieces);
         }
-        for (uint32_t i = 0; i < (uint32_t)pieces; ++i)  // (2^20 tiles of keys, 2^11 pieces)
-            p.works[at + i] = Work{row0[r], rows[r], first[r], r, f.tile, (int)((uint32_t)f.keys * i / pieces), (int)((uint32_t)f.keys * (i + 1) / pieces), slot < 0 ? -1 : slot + (int)i};
+        for (int i = 0; i < pieces; ++i) p.works[at + i] = plan.piece(f, i, pieces, slot);
     }
     __syncthreads();
     if (tid == 0) p.listed->joins = joins;
+}
+
+// The same for a workgroup by itself, its own piece only: where the card has room for all tiles at once (two workgroups a CU) their order does not matter, and the launch of the
+// list is spared (37 rows 9.9 to 7.9 us, 1777 of 16 heads 43 to 38), for 1.5 us more in each workgroup, those behind the last piece among them: the grid is what tables of max_blocks columns may need, and up
+// to twice the card's room is worth it.  Nothing here depends on the order of atomics, so all workgroups find the same.
+constexpr int kOwnThreads = 256, kOwnGrid = 512;
+struct OwnPlan {
+    Plan<kOwnThreads, 1>::Lds lds;
+    Work work;
+};
+__device__ inline Work uniform(const Work& w) {
+    return Work{__builtin_amdgcn_readfirstlane(w.row0), __builtin_amdgcn_readfirstlane(w.rows), __builtin_amdgcn_readfirstlane(w.p0), __builtin_amdgcn_readfirstlane(w.request),
+                __builtin_amdgcn_readfirstlane(w.tile), __builtin_amdgcn_readfirstlane(w.begin), __builtin_amdgcn_readfirstlane(w.end), __builtin_amdgcn_readfirstlane(w.slot)};
+}
+__device__ bool own_work(const PlanParams& p, OwnPlan& own, int index, bool writes, Work& work) {
+    const int tid = threadIdx.x;
+    const Plan<kOwnThreads, 1> plan{p, own.lds, tid};
+    const int all = plan.requests();
+    const bool has = tid < all;
+    const Tile f = has ? plan.find(tid) : Tile{0, 0, 0};
+    unsigned long long cost;
+    plan.before((unsigned long long)f.keys, 1, [](unsigned long long x, unsigned long long y) { return x + y; }, cost);
+    const int chunk = plan.chunk_of(cost), pieces = (f.keys + chunk - 1) / chunk;
+    const bool cut = pieces > 1;
+    // pieces (2^8 tiles, 2^11 more pieces), slots and joins in 16 bits each
+    const unsigned long long mine = (unsigned long long)pieces | (cut ? (unsigned long long)pieces << 16 | 1ull << 32 : 0ull);
+    unsigned long long total;
+    const unsigned long long at = plan.before(mine, 0, [](unsigned long long x, unsigned long long y) { return x + y; }, total);
+    const int works = (int)(total & 0xffff), slot = cut ? (int)(at >> 16 & 0xffff) : -1;
+    const int x = works - 1 - index - (int)(at & 0xffff);  // the last tiles of a prompt are the longest
+    if (x >= 0 && x < pieces) own.work = plan.piece(f, x, pieces, slot);
+    if (writes) {
+        if (cut) p.joins[at >> 32] = plan.join(f, slot, pieces);
+        if (tid == 0) p.listed->joins = (int)(total >> 32);
+    }
+    __syncthreads();
+    work = own.work;
+    return index < works;
 }
 
 // ---- attention ----
 
 struct PromptParams {
     BatchRows b;
-    const Listed* listed;
-    const Work* works;
-    const Join* joins;
+    PlanParams plan;
     float4* parts;  // [slot][KV head][wave][16 quads][64 lanes]: sums that have not been divided yet
     float2* stats;  // [slot][KV head][128]: (reference in powers of two, sum)
 };
@@ -206,7 +271,8 @@ __device__ inline bool not_finite(E v) {
 //
 // The softmax's reference is the largest score of a row's first tile, and follows only when a tile's probabilities add up to more than kMostSum: their sum is needed anyway, their
 // largest score is not (30 vector instructions of 130).
-template <typename E>
+// LISTED: the list has been made by a launch before this one.
+template <typename E, bool LISTED>
 __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptParams p) {
     typedef typename Elem<E>::x8 X8;
     typedef typename Elem<E>::x4 X4;
@@ -214,9 +280,17 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     __shared__ __attribute__((aligned(1024))) char ring[kStages * kStageBytes];
     const BatchRows& b = p.b;
     const int g = blockIdx.x % b.Hkv, index = blockIdx.x / b.Hkv;
-    // (the entry behind the list is memory too: one round trip for both)
-    const Work w = p.works[index];
-    if (index >= p.listed->works) return;
+    Work w;
+    if constexpr (LISTED) {
+        // (the entry behind the list is memory too: one round trip for both)
+        w = p.plan.works[index];
+        if (index >= p.plan.listed->works) return;
+    } else {
+        static_assert(sizeof(OwnPlan) <= sizeof(ring) && kOwnThreads == kThreads, "in the place of the first tiles");
+        if (!own_work(p.plan, *reinterpret_cast<OwnPlan*>(ring), index, blockIdx.x == 0, w)) return;
+        w = uniform(w);
+        __syncthreads();  // (it has been read)
+    }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qcol = lane & 31, hf = lane >> 5;
     const int packed = w.rows * b.group, base_row = w.tile * kTileRows + wave * kWaveRows;
@@ -227,8 +301,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
         const Quotient row = divide(R, b.group, b.group_inverse);
         return (int64_t)(w.row0 + row.q) * stride + (g * b.group + row.r) * kHeadDim;
     };
-    // positions of the wave's first and last rows
-    const int wave_first = __builtin_amdgcn_readfirstlane(pos), wave_last = __builtin_amdgcn_readlane(pos, 31);
+    const int wave_last = __builtin_amdgcn_readlane(pos, 31);  // the position of the wave's last row
     const int n = w.end - w.begin;
 
     // Page numbers: 64 of them at a time, one a lane.
@@ -531,10 +604,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void prompt_join_kernel(PromptPara
     typedef typename Elem<E>::x4 X4;
     const BatchRows& b = p.b;
     const int lane = threadIdx.x & 63, db = threadIdx.x >> 6, qcol = lane & 31, hf = lane >> 5;
-    const int all = p.listed->joins * b.Hkv * kWaves;
+    const int all = p.plan.listed->joins * b.Hkv * kWaves;
     for (int x = blockIdx.x; x < all; x += gridDim.x) {
         const int block = x % kWaves, g = x / kWaves % b.Hkv;
-        const Join j = p.joins[x / kWaves / b.Hkv];
+        const Join j = p.plan.joins[x / kWaves / b.Hkv];
         const int base_row = j.tile * kTileRows + block * kWaveRows, R = base_row + qcol;
         if (base_row >= j.rows * b.group) continue;
         float M = -INFINITY, L = 0.f;
@@ -641,13 +714,18 @@ extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, con
     CPMCU_CHECK_ARG(grid <= INT32_MAX, "prompt_attention: %lld workgroups are beyond a launch", (long long)grid);
     char* const ws = static_cast<char*>(workspace);
     PlanParams plan{row_offsets, positions, num_requests, max_blocks, n, b.group, Hkv, (int)s.tiles, (Listed*)ws, (Work*)(ws + s.works_at), (Join*)(ws + s.joins_at)};
-    PromptParams p{b, plan.listed, plan.works, plan.joins, (float4*)(ws + s.parts_at), (float2*)(ws + s.stats_at)};
+    PromptParams p{b, plan, (float4*)(ws + s.parts_at), (float2*)(ws + s.stats_at)};
     const hipStream_t st = resolve_stream(stream);
     const bool bf = options().dtype == 1;
-    if (num_requests <= 256 && s.tiles <= 2048) hipLaunchKernelGGL((prompt_plan_kernel<256, 1>), dim3(1), dim3(256), 0, st, plan);
-    else hipLaunchKernelGGL((prompt_plan_kernel<1024, kMostRequests / 1024>), dim3(1), dim3(1024), 0, st, plan);
-    CPMCU_LAUNCH_CHECK();
-    hipLaunchKernelGGL(bf ? prompt_attention_kernel<bf16> : prompt_attention_kernel<f16>, dim3((int)grid), dim3(kThreads), 0, st, p);
+    const bool listed = num_requests > kOwnThreads || s.tiles > kOwnThreads || s.tiles * Hkv > kOwnGrid || grid > 2 * kOwnGrid;
+    if (listed) {
+        if (num_requests <= 256 && s.tiles <= 2048) hipLaunchKernelGGL((prompt_plan_kernel<256, 1>), dim3(1), dim3(256), 0, st, plan);
+        else hipLaunchKernelGGL((prompt_plan_kernel<1024, kMostRequests / 1024>), dim3(1), dim3(1024), 0, st, plan);
+        CPMCU_LAUNCH_CHECK();
+    }
+    void (*kernel)(PromptParams) = bf ? prompt_attention_kernel<bf16, false> : prompt_attention_kernel<f16, false>;
+    if (listed) kernel = bf ? prompt_attention_kernel<bf16, true> : prompt_attention_kernel<f16, true>;
+    hipLaunchKernelGGL(kernel, dim3((int)grid), dim3(kThreads), 0, st, p);
     CPMCU_LAUNCH_CHECK();
     if (s.joins > 0) {
         hipLaunchKernelGGL(bf ? prompt_join_kernel<bf16> : prompt_join_kernel<f16>, dim3((int)std::min<int64_t>(s.joins * Hkv * kWaves, kJoinGrid)), dim3(64 * kJoinWaves), 0, st, p);

@@ -333,6 +333,19 @@ def test_many_requests(gpu):
     b.check(b.run("prompt"))
 
 
+@pytest.mark.parametrize("requests", [[(0, 37)], [(3000, 40), (0, 0), (7, 1), (9000, 3)]], ids=["one", "cut"])
+def test_wide_tables_give_the_same_bits(gpu, requests):
+    """Tables of many columns allow for lengths at which the tiles are listed by a launch of their own."""
+    torch = gpu
+    b = Batch(torch, 17, requests, 32, 2)
+    narrow = b.run()
+    b.check(narrow)
+    tables = torch.full((len(requests), 4096), -1, dtype=torch.int32, device="cuda")
+    tables[:, :b.tables.shape[1]] = b.tables
+    b.tables = tables
+    assert torch.equal(b.run().view(torch.int16), narrow.view(torch.int16))
+
+
 def test_prompt_decode_and_tree_attention_agree(gpu):
     from cpm.cu_amd import ops
     torch = gpu
