@@ -37,12 +37,19 @@ struct Join {
 struct Listed {
     int works, joins, pad[6];
 };
-// Pieces are made where fewer than kParts of them, on all KV heads, would each have kLeastKeys tiles of keys or more.
-constexpr int kParts = 1024, kLeastKeys = 24;
+// Pieces are made of tiles that have more than 1 / kParts of all keys, on all KV heads, and more than what is worth its part of the join: kLeastKeys tiles of keys where there are
+// few tiles of rows, kMostKeys where there are enough for all CUs, by the square of their number in between.  Measured with 8, 16, 24 and 64 throughout (us): 8 rows at 12000 cached
+// (2 tiles) 24, 27, 33, 68; 64 rows at 4000 (16) 22, 26, 31, 66; 512 rows at 8000 on 8 heads (128) 90, 89, 92, 97; 1000 rows (250) 28, 24, 24, 24; 4 x 256 rows at 6000 (256)
+// 125, 125, 125, 110; 4096 rows (1024) 163, 163, 163, 146.  With this rule 24, 22, 92, 24, 116 and 151.
+constexpr int kParts = 896, kLeastKeys = 8, kMostKeys = 64;
+__host__ __device__ inline int64_t least_of(int64_t tiles, int Hkv) {
+    const int64_t full = tiles * Hkv, least = full * full / 1024;
+    return least < kLeastKeys ? kLeastKeys : least > kMostKeys ? kMostKeys : least;
+}
 
 struct PlanParams {
     const int32_t *row_offsets, *positions;
-    int num_requests, max_blocks, n, group, Hkv, most_tiles;
+    int num_requests, max_blocks, n, group, Hkv, most_tiles, slots;
     Listed* listed;
     Work* works;
     Join* joins;
@@ -128,10 +135,12 @@ struct Plan {
         f.keys = (lds.first[lo] + last) / kTileKeys + 1;
         return f;
     }
-    // How many tiles of keys a piece has at most, from what all tiles have together.
-    __device__ int chunk_of(unsigned long long cost) const {
-        const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts);
-        return (int)min(max(share, (int64_t)kLeastKeys), (int64_t)INT32_MAX);
+    // How many tiles of keys a piece has at most, from how many tiles of rows there are and what they have together.
+    __device__ int chunk_of(int all, unsigned long long cost) const {
+        // What is cut fits the slots: of more than 1 / kParts of all keys, a tile of t makes at most 2 t / chunk pieces; else t / chunk + 1, and there are twice as many slots as tiles.
+        if (p.slots == 0) return INT32_MAX;
+        const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts), room = p.slots - all, fits = room > 0 ? ((int64_t)cost + room - 1) / room : 0;
+        return (int)min(max(max(share, p.slots < 2 * ((kParts + p.Hkv - 1) / p.Hkv) ? fits : 0), least_of(all, p.Hkv)), (int64_t)INT32_MAX);
     }
     __device__ Work piece(const Tile& f, int i, int pieces, int slot) const {  // (2^20 tiles of keys, 2^11 pieces)
         const int r = f.request;
@@ -156,8 +165,8 @@ __global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
     unsigned long long mine = own.keys, cost;
     for (int t = tid + THREADS; t < all; t += THREADS) mine += plan.find(t).keys;
     plan.before(mine, 1, [](unsigned long long x, unsigned long long y) { return x + y; }, cost);
-    const int chunk = plan.chunk_of(cost);
-    const auto pieces_of = [&](int keys) { return (keys + chunk - 1) / chunk; };
+    const int chunk = plan.chunk_of(all, cost);
+    const auto pieces_of = [&](int keys) { return (int)(((int64_t)keys + chunk - 1) / chunk); };
     // Longest first: counted in classes of a quarter of an octave, then put in their places.
     const auto class_of = [&](int keys, int pieces) {
         const int length = (keys + pieces - 1) / pieces, msb = 31 - __clz(max(length, 1));
@@ -215,7 +224,7 @@ __device__ bool own_work(const PlanParams& p, OwnPlan& own, int index, bool writ
     const Tile f = has ? plan.find(tid) : Tile{0, 0, 0};
     unsigned long long cost;
     plan.before((unsigned long long)f.keys, 1, [](unsigned long long x, unsigned long long y) { return x + y; }, cost);
-    const int chunk = plan.chunk_of(cost), pieces = (f.keys + chunk - 1) / chunk;
+    const int chunk = plan.chunk_of(all, cost), pieces = (int)(((int64_t)f.keys + chunk - 1) / chunk);
     const bool cut = pieces > 1;
     // pieces (2^8 tiles, 2^11 more pieces), slots and joins in 16 bits each
     const unsigned long long mine = (unsigned long long)pieces | (cut ? (unsigned long long)pieces << 16 | 1ull << 32 : 0ull);
@@ -674,9 +683,8 @@ Sizes sizes_of(int num_requests, int max_blocks, int n, int Hq, int Hkv) {
     Sizes s;
     // every request's last tile may be a part of one
     s.tiles = ((int64_t)n * (Hq / Hkv)) / kTileRows + std::min(num_requests, n);
-    // A tile of t > chunk tiles of keys makes at most 2 t / chunk pieces, and chunk is at least the total over kParts / Hkv.  None is made of fewer than kLeastKeys.
-    const int64_t keys = (int64_t)max_blocks * (kPage / kTileKeys);
-    s.slots = keys <= kLeastKeys ? 0 : std::min<int64_t>(2 * ((kParts + Hkv - 1) / Hkv), s.tiles * ((keys + kLeastKeys - 1) / kLeastKeys));
+    const int64_t keys = (int64_t)max_blocks * (kPage / kTileKeys), least = least_of(s.tiles, Hkv);
+    s.slots = keys <= least ? 0 : std::min<int64_t>(2 * ((kParts + Hkv - 1) / Hkv), s.tiles * ((keys + least - 1) / least));
     s.joins = std::min(s.tiles, s.slots / 2);
     s.works = s.tiles + s.slots;
     s.works_at = sizeof(Listed);
@@ -713,7 +721,7 @@ extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, con
     const int64_t grid = s.works * Hkv;
     CPMCU_CHECK_ARG(grid <= INT32_MAX, "prompt_attention: %lld workgroups are beyond a launch", (long long)grid);
     char* const ws = static_cast<char*>(workspace);
-    PlanParams plan{row_offsets, positions, num_requests, max_blocks, n, b.group, Hkv, (int)s.tiles, (Listed*)ws, (Work*)(ws + s.works_at), (Join*)(ws + s.joins_at)};
+    PlanParams plan{row_offsets, positions, num_requests, max_blocks, n, b.group, Hkv, (int)s.tiles, (int)s.slots, (Listed*)ws, (Work*)(ws + s.works_at), (Join*)(ws + s.joins_at)};
     PromptParams p{b, plan, (float4*)(ws + s.parts_at), (float2*)(ws + s.stats_at)};
     const hipStream_t st = resolve_stream(stream);
     const bool bf = options().dtype == 1;
