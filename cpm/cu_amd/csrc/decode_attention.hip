@@ -22,10 +22,11 @@ namespace {
 constexpr int kHeads = 16;       // columns of the products: heads that a workgroup has at a time
 constexpr int kWaves = 2;        // of a workgroup that has a part of the line: 64 KB of tiles, two a CU
 constexpr int kGrid = 512;       // workgroups that share the line
-// Where there is little, in short requests, a part of the line is a wave's, kAloneTiles tiles at most; else it is a workgroup's, whose waves take a request's tiles in
-// turn and meet in LDS (a tile a wave spares that, and leaves more for the second launch).
-constexpr int kAloneTiles = 2, kAloneMean = 16;  // and tiles of a request in the mean
-// Where no request can have more tiles than this, a workgroup takes all of one's on a KV head: no line, nothing to join, one launch.
+// Where requests are short in the mean, a part of the line is a wave's; else it is a workgroup's, whose waves take a request's tiles in turn and meet in LDS (a tile a wave
+// spares that, and leaves more for the second launch: 100 requests of up to 2000 on 8 heads 103 us, with parts of workgroups 118; one of 131000 55 more).
+constexpr int kAloneMean = 16;  // tiles of a request
+// Where no request has more tiles than this, and there are as many tiles as workgroups, a workgroup takes all of a request's on a KV head: no line, nothing to join.  Where the tables have no room
+// for more it does so anyway, in one launch.  (200 requests of up to 900: 20 us in narrow tables, 25 in wide ones, 29 cut in parts; one of 500: 6, and in wide tables 12 whole, 10 in parts.)
 constexpr int kWholeTiles = 16, kWideGrid = 256;
 constexpr int kPartFloats = kHeads * kHeadDim;
 constexpr int kKBytes = kTileKeys * kHeadDim * 2, kStageBytes = 2 * kKBytes;  // of a wave: a tile's K, then its V
@@ -103,18 +104,19 @@ __global__ __launch_bounds__(64 * WAVES) void decode_attention_kernel(DecodePara
     char* const stage = stages + wave * kStageBytes;
     const uint32_t stage_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr_t)stage);
 
-    bool alone = false;
+    bool alone = false, all_whole = WHOLE;
     int parts = 0, part = 0;
-    int64_t all = 0, at = 0, end = 1;
+    int64_t all = 0, at = WHOLE ? 0 : blockIdx.x, end = WHOLE ? 1 : (int64_t)B * p.units;
     if constexpr (!WHOLE) {
         // The line: each thread has a run of requests; their running totals.
         const int each = (B + kThreads - 1) / kThreads;
-        int mine = 0;
+        int mine = 0, most = 0;
         for (int e = 0; e < each; ++e) {
             const int r = tid * each + e;
             int row, pos;
             const int tiles = r < B ? tiles_of(b, r, row, pos) : 0;
             mine += tiles;
+            most = max(most, tiles);
             if (r < B) tile_end[r] = mine;
         }
         int upto = mine;
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(64 * WAVES) void decode_attention_kernel(DecodePara
             if (lane >= d) upto += from;
         }
         if (lane == 63) wave_total[wave] = upto;
-        __syncthreads();
+        all_whole = !__syncthreads_or(most > kWholeTiles);
         int before = upto - mine, total = 0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
@@ -137,25 +139,33 @@ __global__ __launch_bounds__(64 * WAVES) void decode_attention_kernel(DecodePara
         }
         __syncthreads();
         all = (int64_t)total * p.units;
-        alone = all <= (int64_t)kAloneTiles * WAVES * gridDim.x && total <= kAloneMean * B;
-        parts = (int)min(alone ? (int64_t)WAVES * gridDim.x : (int64_t)gridDim.x, alone ? all : (all + WAVES - 1) / WAVES);
+        all_whole = all_whole && all >= gridDim.x;
+        alone = !all_whole && total <= kAloneMean * B;
+        parts = all_whole ? 0 : (int)min(alone ? (int64_t)WAVES * gridDim.x : (int64_t)gridDim.x, alone ? all : (all + WAVES - 1) / WAVES);
         if (blockIdx.x == 0) {
             if (tid == 0) *p.line = Line{parts, {0, 0, 0}};
-            for (int r = tid; r < B; r += kThreads) p.tiles[r] = tile_end[r] - (r > 0 ? tile_end[r - 1] : 0);
+            for (int r = tid; r < B; r += kThreads) p.tiles[r] = all_whole ? 0 : tile_end[r] - (r > 0 ? tile_end[r - 1] : 0);
         }
-        part = alone ? wave * gridDim.x + blockIdx.x : blockIdx.x;
-        if (part >= parts) return;  // (whole workgroups where they share a part)
-        at = part_begin(all, parts, part);
-        end = part_begin(all, parts, part + 1);
+        if (!all_whole) {
+            part = alone ? wave * gridDim.x + blockIdx.x : blockIdx.x;
+            if (part >= parts) return;  // (whole workgroups where they share a part)
+            at = part_begin(all, parts, part);
+            end = part_begin(all, parts, part + 1);
+        }
     }
     const int first_wave = alone ? 0 : wave, step = alone ? 1 : WAVES;
     for (bool begins = true; at < end; begins = false) {
         int r, unit, tiles, t0, t1, row, pos;
-        if constexpr (WHOLE) {
-            r = blockIdx.x / p.units;
-            unit = blockIdx.x % p.units;
+        if (all_whole) {
+            const int x = WHOLE ? blockIdx.x : (int)at;
+            r = x / p.units;
+            unit = x % p.units;
             tiles = tiles_of(b, r, row, pos);
-            if (tiles == 0) return;
+            if (tiles == 0) {
+                if (WHOLE) return;
+                at += gridDim.x;
+                continue;
+            }
             t0 = 0;
             t1 = tiles;
         } else {
@@ -331,7 +341,7 @@ __global__ __launch_bounds__(64 * WAVES) void decode_attention_kernel(DecodePara
         l_run += __shfl_xor(l_run, 16);
         l_run += __shfl_xor(l_run, 32);
         // o[db][i] is dim 16 db + 4 lg + i of head col
-        const bool whole = WHOLE || (t0 == 0 && t1 == tiles);
+        const bool whole = all_whole || (t0 == 0 && t1 == tiles);
         const int slot = 2 * part + (t0 == 0 ? 1 : 0);  // of a part that begins a unit's keys and of one that goes on with them
         const auto put = [&](int db, const f32x4& sum, float inv) {
             if (!whole) {
@@ -380,7 +390,7 @@ __global__ __launch_bounds__(64 * WAVES) void decode_attention_kernel(DecodePara
             if (!whole && wave == 0 && lg == 0) p.stats[slot * kHeads + col] = make_float2(M, L);
             if (!WHOLE) __syncthreads();  // (the next segment's tiles may come)
         }
-        at += WHOLE ? 1 : t1 - t0;
+        at += WHOLE ? 1 : all_whole ? (int)gridDim.x : t1 - t0;
     }
 }
 

@@ -346,6 +346,24 @@ def test_wide_tables_give_the_same_bits(gpu, requests):
     assert torch.equal(b.run().view(torch.int16), narrow.view(torch.int16))
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("heads, count", [((32, 2), 300), ((32, 8), 70), ((4, 1), 1500), ((34, 2), 200)], ids=str)
+def test_short_requests_in_wide_tables(gpu, set_option, dtype, heads, count):
+    """Many of them are taken whole, as in narrow tables; some have no row, one has two."""
+    torch = gpu
+    set_option("dtype", dtype)
+    g = synth.rng(18, count)
+    requests = [(int(c), 0 if i % 17 == 5 else 2 if i == 9 else 1) for i, c in enumerate(g.integers(0, 1023, count))]
+    b = Batch(torch, 18, requests, *heads, dtype=dtype, filler=float("nan"), table_blocks=50)
+    out = b.run("decode")
+    two = int(b.offsets[9])
+    assert bool((out[two:two + 2] == 7.0).all())
+    ref, lim = b.expect()
+    ref[two:two + 2], lim[two:two + 2] = 7.0, 0.0
+    b.check(out, (ref, lim))
+    assert torch.equal(b.run("decode").view(torch.int16), out.view(torch.int16))
+
+
 def test_prompt_decode_and_tree_attention_agree(gpu):
     from cpm.cu_amd import ops
     torch = gpu
