@@ -22,12 +22,13 @@ namespace {
 
 constexpr int kPieces = 2;      // pieces of 8 logits that a thread has of a row
 constexpr int kAhead = 8;       // places that a row's slices may lie ahead of another one's, because rows begin anywhere on 2 bytes
-// Slices of 8192 where rows share a text of some length, because each slice reads it (60 tree nodes, a text of 20000: 17 us, with 4096 21, with 16384 19);
-// else of 4096 (512 rows of their own texts: 44 us, with 8192 52, with 2048 54).
-constexpr int threads_of(bool shared) { return shared ? 512 : 256; }
-constexpr int slice_of(bool shared) { return threads_of(shared) * kPieces * 8; }
+// A slice reads the whole text, so longer texts take larger ones: 4096, 8192 and 16384 logits, two pieces a thread.  512 rows with texts of 300: 28, 29 and 32 us, of 4000 42, 38 and 41,
+// of 16000 86, 68 and 61; one row with 100000 42, 27 and 25.  (What the call has room for decides, the lengths are the device's.)  Rows of one text: 8192, 60 tree nodes
+// and 20000 tokens 17 us, with the others 21 and 19.
+constexpr int kSmall = 256, kMiddle = 512, kLarge = 1024, kShortText = 4096, kMiddleText = 8192;
+constexpr int slice_of(int threads) { return threads * kPieces * 8; }
 constexpr int kTextAtOnce = 8;  // tokens that a thread requests together
-constexpr int kMostBiases = 1024;
+constexpr int kMostBiases = 1024, kCountBits = 21, kMostTokens = 1 << 20;  // (a draft tree's 128 besides)
 
 struct LogitsParams {
     const uint16_t* in;
@@ -70,13 +71,13 @@ __device__ inline uint32_t wave_most(uint32_t v) {
 }
 
 // SHARED: rows of one text, one after the other, a text's draft tree among them; else a row a workgroup.
-template <typename E, bool SHARED>
-__global__ __launch_bounds__(threads_of(SHARED), SHARED ? 6 : 8) void adjust_logits_kernel(LogitsParams p) {
-    constexpr int kThreads = threads_of(SHARED), kSlice = slice_of(SHARED), kCounted = kSlice + kAhead, kWords = kCounted / 32 + 2, kBiases = kMostBiases / kThreads;
+template <typename E, bool SHARED, int THREADS>
+__global__ __launch_bounds__(THREADS, SHARED ? 6 : 8) void adjust_logits_kernel(LogitsParams p) {
+    constexpr int kThreads = THREADS, kSlice = slice_of(THREADS), kCounted = kSlice + kAhead, kWords = kCounted / 32 + 2, kBiases = kMostBiases / kThreads;
     extern __shared__ int hit_at[];  // biases of the slice: place and number in the list, one for each of the list; behind them their values
     float* const hit_value = reinterpret_cast<float*>(hit_at + p.biases);
-    __shared__ __attribute__((aligned(16))) int count[kCounted];
-    __shared__ uint32_t counted[kWords], biased[kWords];  // places that have a count, or a bias: few pieces of a row have one
+    __shared__ __attribute__((aligned(16))) uint32_t count[kCounted];  // of a place: its count, and above it the number of its bias among the hits, from 1 on
+    __shared__ uint32_t counted[kWords], biased[kWords], twice[kWords];  // places that have either: few pieces of a row have one; with a bias; with several
     __shared__ int hits, again;
     __shared__ uint64_t s_best[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(threads_of(SHARED), SHARED ? 6 : 8) void adjust_log
     const int first_place = max(base, 0), places = min(base + kCounted, p.V) - first_place;
     const auto place_of = [&](int v) { return (unsigned)(v - first_place) < (unsigned)places ? v - base : -1; };
     const auto count_one = [&](int at) {
-        atomicAdd(&count[at], 1);
+        atomicAdd(&count[at], 1u);
         atomicOr(&counted[at >> 5], 1u << (at & 31));
     };
     struct Row {
@@ -150,12 +151,10 @@ __global__ __launch_bounds__(threads_of(SHARED), SHARED ? 6 : 8) void adjust_log
             presence = p.penalties[r * 3 + 1];
             frequency = p.penalties[r * 3 + 2];
         }
-        if (texts || draft) {
 #pragma unroll
-            for (int i = 0; i < kCounted / 4; i += kThreads)
-                if (i + kThreads <= kCounted / 4 || i + tid < kCounted / 4) reinterpret_cast<int4*>(count)[i + tid] = int4{0, 0, 0, 0};
-        }
-        if (tid < kWords) counted[tid] = biased[tid] = 0;
+        for (int i = 0; i < kCounted / 4; i += kThreads)
+            if (i + kThreads <= kCounted / 4 || i + tid < kCounted / 4) reinterpret_cast<int4*>(count)[i + tid] = int4{0, 0, 0, 0};
+        if (tid < kWords) counted[tid] = biased[tid] = twice[tid] = 0;
         if (tid == 0) hits = again = 0;
         __syncthreads();
         for (int done = 0; done < len; done += kThreads * kTextAtOnce) {
@@ -180,23 +179,32 @@ __global__ __launch_bounds__(threads_of(SHARED), SHARED ? 6 : 8) void adjust_log
                 hit_at[h] = v << 10 | number;
                 hit_value[h] = p.bias_values[(size_t)r * p.biases + number];
                 const uint32_t bit = 1u << (v & 31);
-                if (atomicOr(&biased[v >> 5], bit) & bit) again = 1;
+                if (atomicOr(&biased[v >> 5], bit) & bit) {
+                    again = 1;
+                    atomicOr(&twice[v >> 5], bit);
+                } else {
+                    atomicAdd(&count[v], (uint32_t)(h + 1) << kCountBits);
+                    atomicOr(&counted[v >> 5], bit);
+                }
             }
         }
         __syncthreads();
-        if (biases && again) {  // an index that stands several times: its first place gets all of them, added up in their order
+        if (biases && again) {  // an index that stands several times: the hit that its place names gets all of them, added up in their order
             for (int h = tid; h < hits; h += kThreads) {
                 const int v = hit_at[h] >> 10;
-                bool first = true;
-                for (int i = 0; i < hits && first; ++i) first = !(hit_at[i] >> 10 == v && hit_at[i] < hit_at[h]);
-                if (!first) continue;
+                if (!(twice[v >> 5] >> (v & 31) & 1) || (int)(count[v] >> kCountBits) != h + 1) continue;
                 float sum = 0.f;
-                for (int last = hit_at[h] - 1;;) {
-                    int next = INT32_MAX;
-                    for (int i = 0; i < hits; ++i)
-                        if (hit_at[i] >> 10 == v && hit_at[i] > last) next = min(next, hit_at[i]);
+                for (int last = (v << 10) - 1;;) {
+                    int next = INT32_MAX, from = 0;
+                    for (int i = 0; i < hits; ++i) {
+                        const int other = hit_at[i];
+                        if (other >> 10 == v && other > last && other < next) {
+                            next = other;
+                            from = i;
+                        }
+                    }
                     if (next == INT32_MAX) break;
-                    sum += p.bias_values[(size_t)r * p.biases + (next & 1023)];
+                    sum += hit_value[from];  // (of this place only)
                     last = next;
                 }
                 hit_value[h] = sum;
@@ -234,31 +242,19 @@ __global__ __launch_bounds__(threads_of(SHARED), SHARED ? 6 : 8) void adjust_log
                 }
             }
             if (texts || draft || biases) {
-                const auto bits_at = [&](const uint32_t* set) { return __builtin_amdgcn_alignbit(set[(at >> 5) + 1], set[at >> 5], at) & 0xffu; };
-                const uint32_t has_count = bits_at(counted), has_bias = bits_at(biased);
-                for (uint32_t rest = (has_count | has_bias) & allowed; rest; rest &= rest - 1) {
+                const uint32_t has = __builtin_amdgcn_alignbit(counted[(at >> 5) + 1], counted[at >> 5], at) & 0xffu;
+                for (uint32_t rest = has & allowed; rest; rest &= rest - 1) {
                     const int j = __builtin_ctz(rest), shift = 16 * (j & 1);
                     uint32_t old = w[0];
 #pragma unroll
                     for (int k = 1; k < 4; ++k) old = j >> 1 == k ? w[k] : old;
                     float z = Elem<E>::from_bits((uint16_t)(old >> shift));
-                    if (has_count >> j & 1) {
-                        const int c = count[at + j];
-                        if (c > 0) {  // (the tokens of another row's way have left their bits)
-                            const float less = z > 0.f ? z / repetition : z * repetition;
-                            z = less - frequency * (float)c - presence;
-                        }
+                    const uint32_t both = count[at + j], c = both & ((1u << kCountBits) - 1), h = both >> kCountBits;
+                    if (c > 0) {  // (the tokens of another row's way have left their bits)
+                        const float less = z > 0.f ? z / repetition : z * repetition;
+                        z = less - frequency * (float)c - presence;
                     }
-                    if (has_bias >> j & 1) {
-                        int found = INT32_MAX;
-                        float value = 0.f;
-                        for (int h = 0; h < hits; ++h)
-                            if (hit_at[h] >> 10 == at + j && hit_at[h] < found) {
-                                found = hit_at[h];
-                                value = hit_value[h];
-                            }
-                        z += value;
-                    }
+                    if (h > 0) z += hit_value[h - 1];
                     const uint32_t y = (old & ~(0xffffu << shift)) | (uint32_t)Elem<E>::to_bits(z) << shift;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] = j >> 1 == k ? y : w[k];
@@ -310,7 +306,7 @@ __global__ __launch_bounds__(threads_of(SHARED), SHARED ? 6 : 8) void adjust_log
             if (lane == 0) s_best[wave] = most;
         }
         if (p.best || (draft && more)) __syncthreads();
-        if (draft && more && x.on_way >= 0) atomicSub(&count[x.on_way], 1);
+        if (draft && more && x.on_way >= 0) atomicSub(&count[x.on_way], 1u);
         if (p.best && tid == 0) {
             uint64_t most = s_best[0];
 #pragma unroll
@@ -342,7 +338,7 @@ __global__ __launch_bounds__(256) void adjust_logits_ids_kernel(const uint64_t* 
 }
 
 // (a row that does not begin on 16 bytes reaches up to seven places further)
-int slices_of(int V, bool shared) { return ceil_div(V + 7, slice_of(shared)); }
+int slices_of(int V, int threads) { return ceil_div(V + 7, slice_of(threads)); }
 
 }  // namespace
 }  // namespace cpmcu
@@ -351,7 +347,7 @@ using namespace cpmcu;
 
 extern "C" size_t cpmcu_adjust_logits_workspace_bytes(int n, int V) {
     if (n < 0 || n >= 1 << 24 || V < 1 || V > 1 << 24) return 0;
-    return sizeof(uint64_t) * (size_t)n * slices_of(V, false);
+    return sizeof(uint64_t) * (size_t)n * slices_of(V, kSmall);
 }
 
 extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, int n, int V, const float* penalties, const int32_t* tokens, const int32_t* lens, int num_requests,
@@ -367,7 +363,7 @@ extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, in
     const bool any = penalties || bias_ids;
     CPMCU_CHECK_ARG(!any || num_requests >= 1, "adjust_logits: %d requests", num_requests);
     CPMCU_CHECK_ARG(!any || requests || num_requests == 1 || num_requests == n, "adjust_logits: %d rows of %d requests need requests", n, num_requests);
-    CPMCU_CHECK_ARG(max_tokens <= 1 << 30, "adjust_logits: max_tokens=%d beyond 2^30", max_tokens);
+    CPMCU_CHECK_ARG(max_tokens <= kMostTokens, "adjust_logits: max_tokens=%d beyond 2^20", max_tokens);
     CPMCU_CHECK_ARG(!tokens || (penalties && lens && max_tokens >= 1), "adjust_logits: tokens go with penalties and lens, one place each at least");
     CPMCU_CHECK_ARG(!bias_ids || (bias_values && num_biases >= 1 && num_biases <= kMostBiases), "adjust_logits: %d biases outside [1, %d], or without values", num_biases, kMostBiases);
     CPMCU_CHECK_ARG(!allowed || allowed_stride == 0 || allowed_stride >= (V + 31) / 32, "adjust_logits: rows of allowed closer than their words");
@@ -375,10 +371,10 @@ extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, in
     CPMCU_CHECK_ARG(!draft_ids || (n <= kMaxTree && mask_words >= ceil_div(n, 64)), "adjust_logits: a tree of %d nodes, masks of %d words", n, mask_words);
     // Rows of one text share its counts: as many of them a workgroup as leave four workgroups a CU.
     const bool one_text = any && num_requests == 1 && !requests;
-    const int rows_each = one_text ? std::max(1, std::min(n, (int)((int64_t)n * slices_of(V, true) / 1024))) : 1;
+    const int rows_each = one_text ? std::max(1, std::min(n, (int)((int64_t)n * slices_of(V, kMiddle) / 1024))) : 1;
     const bool shared = rows_each > 1 || draft_ids;
-    const int slices = slices_of(V, shared);
-    const size_t need = ids ? sizeof(uint64_t) * (size_t)n * slices_of(V, false) : 0;
+    const int threads = shared ? kMiddle : !tokens || max_tokens <= kShortText ? kSmall : max_tokens <= kMiddleText ? kMiddle : kLarge, slices = slices_of(V, threads);
+    const size_t need = ids ? sizeof(uint64_t) * (size_t)n * slices_of(V, kSmall) : 0;
     CPMCU_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0), "adjust_logits: workspace of %zu bytes, %zu needed, on 8 bytes", workspace_bytes, need);
     const size_t in_bytes = 2 * ((size_t)(n - 1) * logits_stride + V), out_bytes = 2 * ((size_t)(n - 1) * out_stride + V), ints = 4;
     const bool in_place = logits == out && (n == 1 || logits_stride == out_stride);
@@ -397,9 +393,11 @@ extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, in
                    penalties, tokens, lens, requests, bias_ids, draft_ids, bias_values, allowed, tree_mask, ids ? (uint64_t*)workspace : nullptr, ids};
     const hipStream_t st = resolve_stream(stream);
     const bool bf = options().dtype == 1;
-    void (*kernel)(LogitsParams) = bf ? adjust_logits_kernel<bf16, false> : adjust_logits_kernel<f16, false>;
-    if (shared) kernel = bf ? adjust_logits_kernel<bf16, true> : adjust_logits_kernel<f16, true>;
-    hipLaunchKernelGGL(kernel, dim3((int)grid), dim3(threads_of(shared)), 8 * p.biases, st, p);
+    void (*kernel)(LogitsParams) = bf ? adjust_logits_kernel<bf16, false, kSmall> : adjust_logits_kernel<f16, false, kSmall>;
+    if (threads == kMiddle) kernel = bf ? adjust_logits_kernel<bf16, false, kMiddle> : adjust_logits_kernel<f16, false, kMiddle>;
+    if (threads == kLarge) kernel = bf ? adjust_logits_kernel<bf16, false, kLarge> : adjust_logits_kernel<f16, false, kLarge>;
+    if (shared) kernel = bf ? adjust_logits_kernel<bf16, true, kMiddle> : adjust_logits_kernel<f16, true, kMiddle>;
+    hipLaunchKernelGGL(kernel, dim3((int)grid), dim3(threads), 8 * p.biases, st, p);
     CPMCU_LAUNCH_CHECK();
     if (ids) {
         hipLaunchKernelGGL(adjust_logits_ids_kernel, dim3(ceil_div(n, 4)), dim3(256), 0, st, p.best, n, slices, ids);

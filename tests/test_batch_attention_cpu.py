@@ -54,7 +54,7 @@ def test_workspaces():
     for args in ((0, 8, 60, 32, 2), (4097, 8, 60, 32, 2), (4, 0, 60, 32, 2), (4, 8, -1, 32, 2), (4, 8, 60, 32, 3), (4, 8, 60, 32, 0)):
         assert raw.cpmcu_batch_prompt_attention_workspace_bytes(*args) == 0
         assert raw.cpmcu_batch_decode_attention_workspace_bytes(args[0], args[1], args[3], args[4]) == 0 or args[2] < 0
-    # short tables: nothing is cut, a list is all there is; long ones: 512 pieces of 256 rows at most twice over, however many rows there are
+    # short tables: nothing is cut, a list is all there is; long ones: 896 pieces of 128 rows at most twice over, however many rows there are
     assert raw.cpmcu_batch_prompt_attention_workspace_bytes(1, 4, 1000, 32, 2) < 1 << 14
     assert raw.cpmcu_batch_prompt_attention_workspace_bytes(4096, 1 << 16, (1 << 24) - 1, 32, 2) < (1 << 27) + (1 << 22) + 64 * (1 << 21)
     assert raw.cpmcu_batch_decode_attention_workspace_bytes(4096, 1 << 16, 32, 2) < 1 << 25
@@ -83,6 +83,12 @@ TREE = dict(di=P(11 * GIB), tm=P(12 * GIB), mw=1, R=1)
 def test_adjust_logits_refuses(kw, match):
     with pytest.raises(ValueError, match=match):
         _logits(**kw)
+
+
+def test_texts_beyond_a_place_s_count_are_refused():
+    """A place has 21 bits for its count."""
+    with pytest.raises(ValueError, match="max_tokens=1048577"):
+        _logits(L=(1 << 20) + 1)
 
 
 def test_no_logits_need_nothing():

@@ -145,6 +145,15 @@ def test_trees_of_every_size(gpu, n):
     case.check(*_run(case))
 
 
+@pytest.mark.parametrize("L", [4096, 4097, 8192, 8193])
+@pytest.mark.parametrize("V", [40, 8191, 16385, 50001])
+def test_slices_of_every_size(gpu, set_option, L, V):
+    """What the text has room for decides how much of the vocabulary a workgroup takes."""
+    set_option("dtype", L & 1)
+    case = Case(gpu, L, n=4, V=V, R=3, L=L, nb=200, mask=True, requests=True, dtype=L & 1)
+    case.check(*_run(case))
+
+
 @pytest.mark.parametrize("kw", [dict(n=640, V=40003, R=1, L=3000, nb=40, mask=True), dict(n=127, V=131073, tree=True, L=9000, nb=5), dict(n=640, V=40003, R=1, nb=3)], ids=["text", "tree", "biases"])
 @pytest.mark.parametrize("want_ids", [True, False])
 def test_many_rows_of_one_text(gpu, set_option, kw, want_ids):
