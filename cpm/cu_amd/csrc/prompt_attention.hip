@@ -42,6 +42,7 @@ struct Listed {
 // (2 tiles) 24, 27, 33, 68; 64 rows at 4000 (16) 22, 26, 31, 66; 512 rows at 8000 on 8 heads (128) 90, 89, 92, 97; 1000 rows (250) 28, 24, 24, 24; 4 x 256 rows at 6000 (256)
 // 125, 125, 125, 110; 4096 rows (1024) 163, 163, 163, 146.  With this rule 24, 22, 92, 24, 116 and 151.
 constexpr int kParts = 896, kLeastKeys = 8, kMostKeys = 64;
+constexpr int kMostChunk = 1 << 21;  // longer than any tile's keys
 __host__ __device__ inline int64_t least_of(int64_t tiles, int Hkv) {
     const int64_t full = tiles * Hkv, least = full * full / 1024;
     return least < kLeastKeys ? kLeastKeys : least > kMostKeys ? kMostKeys : least;
@@ -138,10 +139,14 @@ struct Plan {
     // How many tiles of keys a piece has at most, from how many tiles of rows there are and what they have together.
     __device__ int chunk_of(int all, unsigned long long cost) const {
         // What is cut fits the slots: of more than 1 / kParts of all keys, a tile of t makes at most 2 t / chunk pieces; else t / chunk + 1, and there are twice as many slots as tiles.
-        if (p.slots == 0) return INT32_MAX;
-        const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts), room = p.slots - all, fits = room > 0 ? ((int64_t)cost + room - 1) / room : 0;
-        return (int)min(max(max(share, p.slots < 2 * ((kParts + p.Hkv - 1) / p.Hkv) ? fits : 0), least_of(all, p.Hkv)), (int64_t)INT32_MAX);
+        if (p.slots == 0) return kMostChunk;
+        const int64_t share = (int64_t)((cost * p.Hkv + kParts - 1) / kParts);
+        const int room = p.slots - all, cap = 2 * ((kParts + p.Hkv - 1) / p.Hkv);
+        // (a quotient of 64-bit floats, one tile too long at most, is a fraction of a division of 64-bit whole numbers)
+        const int64_t fits = room > 0 && p.slots < cap ? (int64_t)((double)cost / (double)room) + 2 : 0;
+        return (int)min(max(max(share, fits), least_of(all, p.Hkv)), (int64_t)kMostChunk);
     }
+    __device__ int pieces_of(int keys, int chunk) const { return (int)(((uint32_t)keys + chunk - 1) / (uint32_t)chunk); }
     __device__ Work piece(const Tile& f, int i, int pieces, int slot) const {  // (2^20 tiles of keys, 2^11 pieces)
         const int r = f.request;
         return Work{lds.row0[r], lds.rows[r], lds.first[r], r, f.tile, (int)((uint32_t)f.keys * i / pieces), (int)((uint32_t)f.keys * (i + 1) / pieces), slot < 0 ? -1 : slot + i};
@@ -150,7 +155,7 @@ struct Plan {
 };
 
 // The launch is round trips -- offsets, positions, the list -- and meetings of its waves: with a request and a tile a thread 4.4 us, with four waves in place of sixteen
-// 3.1.
+// 3.1; 1025 tiles, behind a launch that has taken the clock down, 11.6 with four waves and 9 with sixteen.
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
     constexpr int kClasses = 64;
@@ -166,7 +171,7 @@ __global__ __launch_bounds__(THREADS) void prompt_plan_kernel(PlanParams p) {
     for (int t = tid + THREADS; t < all; t += THREADS) mine += plan.find(t).keys;
     plan.before(mine, 1, [](unsigned long long x, unsigned long long y) { return x + y; }, cost);
     const int chunk = plan.chunk_of(all, cost);
-    const auto pieces_of = [&](int keys) { return (int)(((int64_t)keys + chunk - 1) / chunk); };
+    const auto pieces_of = [&](int keys) { return plan.pieces_of(keys, chunk); };
     // Longest first: counted in classes of a quarter of an octave, then put in their places.
     const auto class_of = [&](int keys, int pieces) {
         const int length = (keys + pieces - 1) / pieces, msb = 31 - __clz(max(length, 1));
@@ -224,7 +229,7 @@ __device__ bool own_work(const PlanParams& p, OwnPlan& own, int index, bool writ
     const Tile f = has ? plan.find(tid) : Tile{0, 0, 0};
     unsigned long long cost;
     plan.before((unsigned long long)f.keys, 1, [](unsigned long long x, unsigned long long y) { return x + y; }, cost);
-    const int chunk = plan.chunk_of(all, cost), pieces = (int)(((int64_t)f.keys + chunk - 1) / chunk);
+    const int chunk = plan.chunk_of(all, cost), pieces = plan.pieces_of(f.keys, chunk);
     const bool cut = pieces > 1;
     // pieces (2^8 tiles, 2^11 more pieces), slots and joins in 16 bits each
     const unsigned long long mine = (unsigned long long)pieces | (cut ? (unsigned long long)pieces << 16 | 1ull << 32 : 0ull);
@@ -727,7 +732,8 @@ extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, con
     const bool bf = options().dtype == 1;
     const bool listed = num_requests > kOwnThreads || s.tiles > kOwnThreads || s.tiles * Hkv > kOwnGrid || grid > 2 * kOwnGrid;
     if (listed) {
-        if (num_requests <= 256 && s.tiles <= 2048) hipLaunchKernelGGL((prompt_plan_kernel<256, 1>), dim3(1), dim3(256), 0, st, plan);
+        if (num_requests <= 256 && s.tiles <= 512) hipLaunchKernelGGL((prompt_plan_kernel<256, 1>), dim3(1), dim3(256), 0, st, plan);
+        else if (num_requests <= 1024) hipLaunchKernelGGL((prompt_plan_kernel<1024, 1>), dim3(1), dim3(1024), 0, st, plan);
         else hipLaunchKernelGGL((prompt_plan_kernel<1024, kMostRequests / 1024>), dim3(1), dim3(1024), 0, st, plan);
         CPMCU_LAUNCH_CHECK();
     }
