@@ -336,7 +336,7 @@ def adjust_logits(logits, penalties=None, tokens=None, lens=None, requests=None,
     Of a token that stands c > 0 times in the text of its row's request the logit z becomes (z / repetition if z > 0 else z * repetition) - frequency * c -
     presence; then its bias is added, and what is not allowed becomes minus infinity.  ids is the lowest index of a row's largest result, -1 where nothing is left.
 
-    penalties fp32 [R, 3]: (repetition, presence, frequency) of each request.  tokens int32 [R, L], of which lens int32 [R] count.  requests int32 [n]: each
+    penalties fp32 [R, 3]: (repetition, presence, frequency) of each request.  tokens int32 [R, L up to 2^20], of which lens int32 [R] count.  requests int32 [n]: each
     row's request (-1: none); left out, row t is request t's, or all are of the only one.  bias_ids int32 / bias_values fp32 [R, up to 1024] (-1: not used).
     allowed int32 [n, ceil(V / 32)]: bit v % 32 of word v / 32 (``mask.expand(n, -1)``: one for all rows).  draft_ids int32 [n] / tree_mask int64
     [n, words]: the rows are the nodes of one request's draft tree, and the drafts on a node's way, its own among them, stand behind the request's tokens.
