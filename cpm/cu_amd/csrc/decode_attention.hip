@@ -83,7 +83,7 @@ __device__ inline int tiles_of(const BatchRows& b, int r, int& row, int& pos) {
 // is counted by hand.
 __device__ inline void request_4k(const void* base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds_at) {
     asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072"
+                 "global_load_lds_dwordx4 %2, %4 offset:2*1024\n\tglobal_load_lds_dwordx4 %3, %4 offset:3*1024"
                  : : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds_at) : "memory", "m0");
 }
 
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * WAVES) void decode_attention_kernel(DecodePara
         const auto request_v = [&](size_t page, int t) {
             const char* const from = reinterpret_cast<const char*>(b.v_pool + page * kHeadDim * kPage + t * kTileKeys % kPage);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) request_4k(from + i * 16384, v_off, (v_off ^ 64u) + 3072u, v_off + 6144u, (v_off ^ 64u) + 9216u, stage_at + kKBytes + i * 4096);
+            for (int i = 0; i < 4; ++i) request_4k(from + i * 16384, v_off, (v_off ^ 64u) + 3u * 1024u, v_off + 6u * 1024u, (v_off ^ 64u) + 9u * 1024u, stage_at + kKBytes + i * 4096);
         };
         f32x4 o[8];
 #pragma unroll

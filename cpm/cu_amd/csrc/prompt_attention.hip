@@ -267,7 +267,7 @@ __device__ inline int v_at(int d, int piece) { return kKBytes + d * 128 + ((piec
 // by hand: written as loads that the compiler knows, every read of LDS would wait for all of them.  One statement: nothing comes between m0 and its use.
 __device__ inline void request_4k(const void* base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds_at) {
     asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072"
+                 "global_load_lds_dwordx4 %2, %4 offset:2*1024\n\tglobal_load_lds_dwordx4 %3, %4 offset:3*1024"
                  : : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds_at) : "memory", "m0");
 }
 
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
         v_off = (uint32_t)(d * kPage + ((lane & 7) ^ ((d >> 1) & 7)) * 8) * 2u;
     }
     const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_ptr_t)ring + wave * 4096;
-    const uint32_t v_off1 = (v_off ^ 64u) + 3072u, v_off2 = v_off + 6144u, v_off3 = (v_off ^ 64u) + 9216u;
+    const uint32_t v_off1 = (v_off ^ 64u) + 3u * 1024u, v_off2 = v_off + 6u * 1024u, v_off3 = (v_off ^ 64u) + 9u * 1024u;
     static_assert(kPage * kHeadDim * 2 == 1 << 16, "64 KB a page and head");
     uint64_t page_at = 0;  // of the tile whose K has been requested last: V(j) is requested behind K(j), ahead of K(j + 1)
     const auto request_k = [&](int i, int stage) {
