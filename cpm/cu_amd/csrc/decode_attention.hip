@@ -30,8 +30,8 @@ constexpr int kAloneMean = 16;  // tiles of a request
 constexpr int kWholeTiles = 16, kWideGrid = 256;
 constexpr int kPartFloats = kHeads * kHeadDim;
 constexpr int kKBytes = kTileKeys * kHeadDim * 2, kStageBytes = 2 * kKBytes;  // of a wave: a tile's K, then its V
-// The second launch: a workgroup joins up to kFewParts parts of a unit, eight of them more; a wave requests kAtOnce of them together.
-constexpr int kJoinWaves = 16, kFewParts = 32, kAtOnce = 8;
+// The second launch: a workgroup joins up to kFewParts parts of a unit, eight of them more (with 32 one request of 3000 takes 15.1 us instead of 13.6); a wave requests kAtOnce of them together.
+constexpr int kJoinWaves = 16, kFewParts = 16, kAtOnce = 8;
 constexpr int kFewRequests = 1024;  // up to which the line's ends leave room for two workgroups a CU
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
