@@ -388,7 +388,7 @@ extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, in
     }
     CPMCU_CHECK_ARG(!overlap(ids, ids ? ints * n : 0, out, out_bytes) && !overlap(ids, ids ? ints * n : 0, logits, in_bytes), "adjust_logits: ids in the memory of logits");
     const int64_t grid = (int64_t)ceil_div(n, rows_each) * slices;
-    CPMCU_CHECK_ARG(grid <= INT32_MAX, "adjust_logits: %lld workgroups are beyond a launch", (long long)grid);
+    CPMCU_CHECK_ARG(grid * threads <= UINT32_MAX, "adjust_logits: %lld workgroups of %d threads are beyond a launch", (long long)grid, threads);
     LogitsParams p{(const uint16_t*)logits, (uint16_t*)out, logits_stride, out_stride, allowed_stride, n, V, any ? num_requests : 0, max_tokens, bias_ids ? num_biases : 0, mask_words, rows_each, slices,
                    penalties, tokens, lens, requests, bias_ids, draft_ids, bias_values, allowed, tree_mask, ids ? (uint64_t*)workspace : nullptr, ids};
     const hipStream_t st = resolve_stream(stream);

@@ -519,6 +519,8 @@ extern "C" int cpmcu_batch_decode_attention(const void* q, int64_t q_stride, con
     const Sizes s = sizes_of(num_requests, max_blocks, Hq, Hkv);
     CPMCU_CHECK_ARG(workspace && workspace_bytes >= s.bytes, "decode_attention: workspace of %zu bytes, %zu needed", workspace_bytes, s.bytes);
     CPMCU_CHECK_ARG((uintptr_t)workspace % 16 == 0, "decode_attention: the workspace has to lie on 16 bytes");
+    const int64_t few = (int64_t)num_requests * units_of(Hq, Hkv), many = s.parts > kFewParts ? 8 * ceil_div(s.parts, kFewParts) : 0;
+    CPMCU_CHECK_ARG((few + many) * 64 * kJoinWaves <= UINT32_MAX, "decode_attention: %lld workgroups of %d threads are beyond a launch", (long long)(few + many), 64 * kJoinWaves);
     char* const ws = static_cast<char*>(workspace);
     DecodeParams p{b, units_of(Hq, Hkv), ceil_div(b.group, kHeads), (Line*)ws, (int*)(ws + s.tiles_at), (Unit*)(ws + s.cut_at), (Unit*)(ws + s.owners_at), (float2*)(ws + s.stats_at), (float4*)(ws + s.sums_at)};
     const hipStream_t st = resolve_stream(stream);
@@ -538,8 +540,7 @@ extern "C" int cpmcu_batch_decode_attention(const void* q, int64_t q_stride, con
     CPMCU_LAUNCH_CHECK();
     // (one part is the whole line: nothing is cut)
     if (s.parts > 1) {
-        const int few = num_requests * p.units, many = s.parts > kFewParts ? 8 * ceil_div(s.parts, kFewParts) : 0;
-        hipLaunchKernelGGL(bf ? decode_join_kernel<bf16> : decode_join_kernel<f16>, dim3(few + many), dim3(64 * kJoinWaves), 0, st, p, few);
+        hipLaunchKernelGGL(bf ? decode_join_kernel<bf16> : decode_join_kernel<f16>, dim3((int)(few + many)), dim3(64 * kJoinWaves), 0, st, p, (int)few);
         CPMCU_LAUNCH_CHECK();
     }
     return CPMCU_OK;

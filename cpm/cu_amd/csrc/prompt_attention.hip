@@ -724,7 +724,7 @@ extern "C" int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, con
     CPMCU_CHECK_ARG(workspace && workspace_bytes >= s.bytes, "prompt_attention: workspace of %zu bytes, %zu needed", workspace_bytes, s.bytes);
     CPMCU_CHECK_ARG((uintptr_t)workspace % 16 == 0, "prompt_attention: the workspace has to lie on 16 bytes");
     const int64_t grid = s.works * Hkv;
-    CPMCU_CHECK_ARG(grid <= INT32_MAX, "prompt_attention: %lld workgroups are beyond a launch", (long long)grid);
+    CPMCU_CHECK_ARG(grid * kThreads <= UINT32_MAX, "prompt_attention: %lld workgroups of %d threads are beyond a launch", (long long)grid, kThreads);
     char* const ws = static_cast<char*>(workspace);
     PlanParams plan{row_offsets, positions, num_requests, max_blocks, n, b.group, Hkv, (int)s.tiles, (int)s.slots, (Listed*)ws, (Work*)(ws + s.works_at), (Join*)(ws + s.joins_at)};
     PromptParams p{b, plan, (float4*)(ws + s.parts_at), (float2*)(ws + s.stats_at)};

@@ -85,6 +85,17 @@ def test_adjust_logits_refuses(kw, match):
         _logits(**kw)
 
 
+def test_more_threads_than_a_launch_has_are_refused():
+    """A launch has fewer than 2^32 threads."""
+    far = dict(q=P(1 << 50), out=P(1 << 52), qs=1 << 17, os=1 << 17, hq=1024, hkv=1024, wb=1 << 60)
+    with pytest.raises(ValueError, match="prompt_attention: .* beyond a launch"):
+        _attention("prompt", **dict(far, B=4096, n=(1 << 21) - 5))
+    with pytest.raises(ValueError, match="decode_attention: .* beyond a launch"):
+        _attention("decode", **dict(far, B=4096, n=4096))
+    with pytest.raises(ValueError, match="adjust_logits: .* beyond a launch"):
+        _logits(z=P(1 << 50), zs=5000, out=P(1 << 52), os=5000, n=(1 << 24) - 1, V=5000, R=1, al=None, ids=None, pen=None, tok=None, lens=None, bi=None, bv=None)
+
+
 def test_texts_beyond_a_place_s_count_are_refused():
     """A place has 21 bits for its count."""
     with pytest.raises(ValueError, match="max_tokens=1048577"):
