@@ -60,6 +60,25 @@ struct PlanParams {
 struct Tile {
     int request, tile, keys;  // keys: tiles of 64 of them that the last row sees
 };
+// A lane's value and those of the lanes before it, added up within rows of 16 lanes and then from row to row, without LDS (0 is nothing).
+template <typename T, typename F>
+__device__ inline T wave_upto(T v, F add) {
+    const auto moved = [&](auto from, auto rows) {
+        T x = 0;
+#pragma unroll
+        for (int part = 0; part < (int)sizeof(T); part += 4)
+            x |= (T)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)((unsigned long long)v >> (8 * part)), decltype(from)::value, decltype(rows)::value, 0xf, false) << (part ? 32 : 0);
+        return x;
+    };
+    typedef std::integral_constant<int, 0xf> All;
+    v = add(v, moved(std::integral_constant<int, 0x111>{}, All{}));  // the lane one before, two, four, eight
+    v = add(v, moved(std::integral_constant<int, 0x112>{}, All{}));
+    v = add(v, moved(std::integral_constant<int, 0x114>{}, All{}));
+    v = add(v, moved(std::integral_constant<int, 0x118>{}, All{}));
+    v = add(v, moved(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));  // every second row: the last lane's of the row before
+    v = add(v, moved(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));  // the upper half: lane 31's
+    return v;
+}
 template <int THREADS, int EACH>
 struct Plan {
     static constexpr int kMost = THREADS * EACH, kPlanWaves = THREADS / 64;
@@ -75,12 +94,7 @@ struct Plan {
     template <typename T, typename F>
     __device__ T before(T mine, int part, F add, T& all) const {
         const int lane = tid & 63, wave = tid >> 6;
-        T upto = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const T from = __shfl_up(upto, d);
-            if (lane >= d) upto = add(upto, from);
-        }
+        const T upto = wave_upto(mine, add);
         if (lane == 63) lds.wave_sum[part][wave] = (unsigned long long)upto;
         T lanes = __shfl_up(upto, 1);
         if (lane == 0) lanes = 0;
@@ -227,20 +241,22 @@ __device__ bool own_work(const PlanParams& p, OwnPlan& own, int index, bool writ
     const int all = plan.requests();
     const bool has = tid < all;
     const Tile f = has ? plan.find(tid) : Tile{0, 0, 0};
-    unsigned long long cost;
-    plan.before((unsigned long long)f.keys, 1, [](unsigned long long x, unsigned long long y) { return x + y; }, cost);
+    uint32_t cost;  // (2^8 tiles of 2^20 tiles of keys)
+    const auto plus = [](uint32_t x, uint32_t y) { return x + y; };
+    plan.before((uint32_t)f.keys, 1, plus, cost);
     const int chunk = plan.chunk_of(all, cost), pieces = plan.pieces_of(f.keys, chunk);
     const bool cut = pieces > 1;
-    // pieces (2^8 tiles, 2^11 more pieces), slots and joins in 16 bits each
-    const unsigned long long mine = (unsigned long long)pieces | (cut ? (unsigned long long)pieces << 16 | 1ull << 32 : 0ull);
-    unsigned long long total;
-    const unsigned long long at = plan.before(mine, 0, [](unsigned long long x, unsigned long long y) { return x + y; }, total);
-    const int works = (int)(total & 0xffff), slot = cut ? (int)(at >> 16 & 0xffff) : -1;
+    // pieces (2^8 tiles, 2^11 more pieces) and slots in 16 bits each
+    uint32_t total;
+    const uint32_t at = plan.before((uint32_t)pieces | (cut ? (uint32_t)pieces << 16 : 0u), 0, plus, total);
+    const int works = (int)(total & 0xffff), slot = cut ? (int)(at >> 16) : -1;
     const int x = works - 1 - index - (int)(at & 0xffff);  // the last tiles of a prompt are the longest
     if (x >= 0 && x < pieces) own.work = plan.piece(f, x, pieces, slot);
-    if (writes) {
-        if (cut) p.joins[at >> 32] = plan.join(f, slot, pieces);
-        if (tid == 0) p.listed->joins = (int)(total >> 32);
+    if (writes) {  // (by the whole workgroup)
+        uint32_t joins;
+        const uint32_t join = plan.before((uint32_t)cut, 1, plus, joins);
+        if (cut) p.joins[join] = plan.join(f, slot, pieces);
+        if (tid == 0) p.listed->joins = (int)joins;
     }
     __syncthreads();
     work = own.work;
@@ -311,9 +327,20 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     const int R = base_row + qcol, Rc = min(R, packed - 1);
     const bool wave_ok = base_row < packed;
     const int pos = w.p0 + divide(Rc, b.group, b.group_inverse).q;
-    const auto row_at = [&](int R, int64_t stride) {  // where packed row R's 128 values begin
+    // Where the rows of a lane's sixteen, four apart, begin: one division for the first of them.
+    const Quotient four = divide(4, b.group, b.group_inverse);
+    struct Rows {
+        int64_t at;
+        int head;
+    };
+    const auto first_row = [&](int R, int64_t stride) {
         const Quotient row = divide(R, b.group, b.group_inverse);
-        return (int64_t)(w.row0 + row.q) * stride + (g * b.group + row.r) * kHeadDim;
+        return Rows{(int64_t)(w.row0 + row.q) * stride + (g * b.group + row.r) * kHeadDim, row.r};
+    };
+    const auto next_row = [&](Rows& x, int64_t stride) {
+        const bool over = x.head + four.r >= b.group;
+        x.head += over ? four.r - b.group : four.r;
+        x.at += four.q * stride + four.r * kHeadDim + (over ? stride - b.group * kHeadDim : 0);
     };
     const int wave_last = __builtin_amdgcn_readlane(pos, 31);  // the position of the wave's last row
     const int n = w.end - w.begin;
@@ -357,10 +384,13 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     request_v(0, 0);
     // Q's rows come through LDS, whole, in the stage that the second tile will have.
     char* const q_stage = ring + kStageBytes + wave * (kWaveRows * 256);
+    Rows q_row = first_row(base_row + (lane >> 4), b.q_stride);
+    const int64_t q_last = first_row(packed - 1, b.q_stride).at;
 #pragma unroll
     for (int x = 0; x < kWaveRows / 4; ++x) {
         const int r = x * 4 + (lane >> 4);
-        const uint16_t* const from = b.q + row_at(min(base_row + r, packed - 1), b.q_stride) + ((lane & 15) ^ (r & 15)) * 8;
+        const uint16_t* const from = b.q + (base_row + r < packed ? q_row.at : q_last) + ((lane & 15) ^ (r & 15)) * 8;
+        next_row(q_row, b.q_stride);
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)(q_stage + x * 1024)) : "memory", "m0");
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -603,10 +633,12 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     int at = lane;
     asm volatile("" : "+v"(at));  // (the rows' places of the beginning, kept, would take the loop's registers)
+    Rows o_row = first_row(base_row + (at >> 4), b.out_stride);
 #pragma unroll
     for (int x = 0; x < kWaveRows / 4; ++x) {
         const int r = x * 4 + (at >> 4);
-        if (base_row + r < packed) *reinterpret_cast<X8*>(b.out + row_at(base_row + r, b.out_stride) + (at & 15) * 8) = *reinterpret_cast<const X8*>(o_stage + k_at(r, at & 15));
+        if (base_row + r < packed) *reinterpret_cast<X8*>(b.out + o_row.at + (at & 15) * 8) = *reinterpret_cast<const X8*>(o_stage + k_at(r, at & 15));
+        next_row(o_row, b.out_stride);
     }
 }
 
