@@ -12,6 +12,7 @@
 #include "batch_attention.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace cpmcu {
@@ -299,8 +300,8 @@ __device__ inline bool not_finite(E v) {
 // all eight in step: 8 % slower than that.)  K and V have two stages each: V(i + 1) and K(i + 2) are requested when everybody is through with tile i - 1's products, and have the
 // time of a tile to come.
 //
-// The softmax's reference is the largest score of a row's first tile, and follows only when a tile's probabilities add up to more than kMostSum: their sum is needed anyway, their
-// largest score is not (30 vector instructions of 130).
+// The softmax's reference is the largest score of a row's first tile (of the first that has any but minus infinities), and follows only when a tile's probabilities add up to more than
+// kMostSum: their sum is needed anyway, their largest score is not (30 vector instructions of 130).
 // LISTED: the list has been made by a launch before this one.
 template <typename E, bool LISTED>
 __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptParams p) {
@@ -450,7 +451,8 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     const auto probabilities = [&]() {
         float sum;
         for (int turn = 0;; ++turn) {
-            const float m_scaled = m_ref == -INFINITY ? 0.f : m_ref;
+            // (no reference yet: hidden scores, minus infinity, are zeros; any other one is infinity here, so that the reference follows it)
+            const float m_scaled = m_ref == -INFINITY ? -FLT_MAX : m_ref;
             const X2 ones = {(E)1.f, (E)1.f};
             float psum[2] = {0.f, 0.f};  // the sum of what the product will see, in 32 bits
             X2 pp[16];
