@@ -32,6 +32,10 @@ constexpr int kPartFloats = kHeads * kHeadDim;
 constexpr int kKBytes = kTileKeys * kHeadDim * 2, kStageBytes = 2 * kKBytes;  // of a wave: a tile's K, then its V
 // The second launch: a workgroup joins up to kFewParts parts of a unit, eight of them more (with 32 one request of 3000 takes 15.1 us instead of 13.6); a wave requests kAtOnce of them together.
 constexpr int kJoinWaves = 16, kFewParts = 16, kAtOnce = 8;
+// Probabilities are powers of two of a score less a reference, kLift below the largest: up to 4096 in fp16, which ends at 65504 and has fewer bits below 2^-14, so that a probability keeps all of its bits
+// down to e^-18 of the largest (without, to e^-9.7: behind one key that has e^16.5 times the weight of each other, the others' sum was 2 % off).  bf16 has the range of 32 bits.
+template <typename E>
+constexpr float kLift = Elem<E>::kDtype == 0 ? 12.f : 0.f;
 constexpr int kFewRequests = 1024;  // up to which the line's ends leave room for two workgroups a CU
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
@@ -311,7 +315,7 @@ __global__ __launch_bounds__(64 * WAVES) void decode_attention_kernel(DecodePara
 #pragma unroll
                     for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, s[sp][ab][i]);
             tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
-            tmax = fmaxf(tmax, __shfl_xor(tmax, 32)) * b.scale_log2;
+            tmax = fmaxf(tmax, __shfl_xor(tmax, 32)) * b.scale_log2 - kLift<E>;
             const float m_new = fmaxf(m_ref, tmax);
             const float m_scaled = m_new == -INFINITY ? 0.f : m_new, alpha = __builtin_amdgcn_exp2f(m_ref - m_scaled);
             m_ref = m_new;

@@ -22,7 +22,13 @@ constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32, kTileRows = kWaves * kWaveRows;
 constexpr int kStages = 2;
 constexpr int kKBytes = kTileKeys * kHeadDim * 2, kStageBytes = 2 * kKBytes;
-constexpr float kMostSum = 4096.f;  // of a lane's 32 probabilities of a tile, before the softmax's reference follows (fp16 ends at 65504)
+// Probabilities are powers of two of a score less the softmax's reference, which is kLift below the largest score that it has followed and stays until a lane's 32 of a tile add up to
+// more than kMostSum.  fp16 has fewer bits below 2^-14: with a lift of 10 a probability keeps all of them down to e^-16.6 of the largest (without, to e^-9.7: behind one key of e^16.5
+// times the weight of each other, the others' sum was 2 % off), and what passes 65504 is infinity, as the sum is then.  bf16 has the range of 32 bits.
+template <typename E>
+struct Range {
+    static constexpr float kLift = Elem<E>::kDtype == 0 ? 10.f : 0.f, kMostSum = Elem<E>::kDtype == 0 ? FLT_MAX : 4096.f;
+};
 
 // ---- the list of work ----
 
@@ -433,14 +439,14 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
     };
     // P^T as the second operand of O^T = V^T P^T, rounded to the element type: step j has keys 16 j + {4 hf + [0, 4), 8 + 4 hf + [0, 4)}
     X8 pb[4];
-    const auto refer = [&]() {  // to the tile's largest score, where that is larger
+    const auto refer = [&]() {  // to the tile's largest score (kLift below), where that is larger
         float tmax = sacc[0][0];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, sacc[kb][r]);
         // (the row's other keys are 32 lanes away)
-        const float m_new = fmaxf(m_ref, fmaxf(tmax, __shfl_xor(tmax, 32)) * b.scale_log2), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
+        const float m_new = fmaxf(m_ref, fmaxf(tmax, __shfl_xor(tmax, 32)) * b.scale_log2 - Range<E>::kLift), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
         m_ref = m_new;
         l_run *= alpha;
 #pragma unroll
@@ -471,7 +477,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_attention_kernel(PromptPar
                 pb[j] = __builtin_bit_cast(X8, Four{{pp[4 * j], pp[4 * j + 1], pp[4 * j + 2], pp[4 * j + 3]}});
             }
             sum = psum[0] + psum[1];
-            if (turn > 0 || !__any(sum > kMostSum)) break;
+            if (turn > 0 || !__any(sum > Range<E>::kMostSum)) break;
             refer();
         }
         l_run += sum;

@@ -77,3 +77,23 @@ def test_tiles_whose_scores_are_minus_infinity(gpu, set_option, dtype, heads, le
         b.k[page, :, at % PAGE, 1] = (octaves * math.log(2) / (16.0 * SCALE))[:, None].to(b.k.dtype)
         b.k[page, :, at % PAGE, 0] = torch.where(hidden(at), -math.inf, 0.0)[:, None].to(b.k.dtype)
     b.check(b.run(rows.split("_")[0]), _expect(b, hidden)[:2])
+
+
+@pytest.mark.parametrize("kind, heads, requests", [
+    ("decode", (7, 1), [(1000, 1)] * 5), ("decode", (32, 2), [(2500, 1)] * 200), ("decode", (16, 16), [(60, 1), (3000, 1)]), ("prompt", (32, 2), [(0, 900), (700, 130)]), ("prompt", (7, 1), [(3000, 200)])],
+    ids=["decode_1000", "decode_2500", "decode_mha", "prompt_two", "prompt_far"])
+@pytest.mark.parametrize("gap", [12.0, 14.0, 16.5, 18.0])
+@pytest.mark.parametrize("place", ["first", "middle"])
+def test_one_key_far_above_the_others(gpu, kind, heads, requests, gap, place):
+    """e^gap times as much weight on one key, whose value is 0: the result is what the many small probabilities of the others add up to (fp16)."""
+    torch = gpu
+    b = Batch(torch, 51, requests, *heads, spread=0.3)
+    b.q[:, :, 0] = 16.0
+    for r in range(len(b.requests)):
+        at, page = _places(b, r)
+        above = at == (0 if place == "first" else int(b.requests[r][0]) // 2)
+        b.k[page, :, at % PAGE, 0] = torch.where(above, gap / (16.0 * SCALE), 0.0)[:, None].half()
+        v = torch.where(above[:, None, None], 0.0, 32.0 + 16.0 * b.v[page, :, :, b.slot[at % PAGE]].float())
+        b.v[page, :, :, b.slot[at % PAGE]] = v.half()
+    shift = {"prompt": 10, "decode": 12}[kind]
+    b.check(b.run(kind), _expect(b, shift=shift)[:2])
