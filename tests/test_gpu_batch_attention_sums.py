@@ -97,3 +97,29 @@ def test_one_key_far_above_the_others(gpu, kind, heads, requests, gap, place):
         b.v[page, :, :, b.slot[at % PAGE]] = v.half()
     shift = {"prompt": 10, "decode": 12}[kind]
     b.check(b.run(kind), _expect(b, shift=shift)[:2])
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("kind, heads, requests", [
+    ("decode", (32, 2), [(100000, 1)]), ("decode", (7, 1), [(131000, 1)]), ("decode", (32, 8), [(40000, 1), (3, 1), (17, 1), (26000, 1), (900, 1)]), ("decode", (16, 16), [(9000, 1)] * 3),
+    ("prompt", (32, 2), [(9001, 40), (50000, 1), (3, 1), (17000, 129)]), ("prompt", (4, 1), [(30011, 64)])],
+    ids=["decode_2_heads", "decode_1_head", "decode_ragged", "decode_mha", "prompt_ragged", "prompt_chunk"])
+def test_every_tile_of_long_requests_counts(gpu, set_option, dtype, kind, heads, requests):
+    """The values of a tile of 64 keys are 1 in a dim of its own and 0 elsewhere, 128 tiles at a time: each dim is its tile's share of the probabilities.  A tile that is lost or counted
+    twice moves its dim by far more than the limit, as is checked first."""
+    torch = gpu
+    set_option("dtype", dtype)
+    b = Batch(torch, 52, requests, *heads, dtype=dtype, spread=1.0)
+    _, _, share, of_one = _expect(b)
+    tiles = share.shape[2]
+    mark = torch.cat([torch.eye(D, device="cuda"), torch.zeros((1, D), device="cuda")]).to(b.v.dtype)
+    for first in range(0, tiles, D):
+        for r in range(len(requests)):
+            at, page = _places(b, r)
+            tile = at // 64 - first
+            b.v[page, :, :, b.slot[at % PAGE]] = mark[torch.where((tile >= 0) & (tile < D), tile, D)][:, None, :].expand(-1, heads[1], -1)
+        ref = torch.nn.functional.pad(share[:, :, first:first + D], (0, max(0, first + D - tiles)))
+        lim = of_one[:, :, None] * ref + 2.0 ** -25
+        several = (ref > 2.0 ** -20) & (ref < 0.9)  # (all of a row that sees one tile is that tile's; a row's last tile may be next to nothing)
+        assert bool((ref * (1 - ref) / (1 + ref) > 2 * lim)[several].all()) and bool(several.any())
+        b.check(b.run(kind), (ref, lim))
