@@ -74,11 +74,11 @@ __device__ inline uint32_t wave_most(uint32_t v) {
 template <typename E, bool SHARED, int THREADS>
 __global__ __launch_bounds__(THREADS, SHARED ? 6 : 8) void adjust_logits_kernel(LogitsParams p) {
     constexpr int kThreads = THREADS, kSlice = slice_of(THREADS), kCounted = kSlice + kAhead, kWords = kCounted / 32 + 2, kBiases = kMostBiases / kThreads;
-    extern __shared__ int hit_at[];  // biases of the slice: place and number in the list, one for each of the list; behind them their values
-    float* const hit_value = reinterpret_cast<float*>(hit_at + p.biases);
-    __shared__ __attribute__((aligned(16))) uint32_t count[kCounted];  // of a place: its count, and above it the number of its bias among the hits, from 1 on
+    extern __shared__ int bias_at[];  // the list of biases: each one's place in the slice, or -1; behind them their values
+    float* const bias_value = reinterpret_cast<float*>(bias_at + p.biases);
+    __shared__ __attribute__((aligned(16))) uint32_t count[kCounted];  // of a place: its count, and above it the number of its bias in the list, from 1 on
     __shared__ uint32_t counted[kWords], biased[kWords], twice[kWords];  // places that have either: few pieces of a row have one; with a bias; with several
-    __shared__ int hits, again;
+    __shared__ int again;
     __shared__ uint64_t s_best[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int slice = blockIdx.x % p.slices, row_begin = blockIdx.x / p.slices * (SHARED ? p.rows_each : 1), row_end = SHARED ? min(row_begin + p.rows_each, p.n) : row_begin + 1;
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 6 : 8) void adjust_logits_kernel(
         for (int i = 0; i < kCounted / 4; i += kThreads)
             if (i + kThreads <= kCounted / 4 || i + tid < kCounted / 4) reinterpret_cast<int4*>(count)[i + tid] = int4{0, 0, 0, 0};
         if (tid < kWords) counted[tid] = biased[tid] = twice[tid] = 0;
-        if (tid == 0) hits = again = 0;
+        if (tid == 0) again = 0;
         __syncthreads();
         for (int done = 0; done < len; done += kThreads * kTextAtOnce) {
             if (done > 0) {
@@ -174,40 +174,32 @@ __global__ __launch_bounds__(THREADS, SHARED ? 6 : 8) void adjust_logits_kernel(
             for (int i = 0; i < kBiases; ++i) {
                 if (i * kThreads >= p.biases) break;
                 const int v = place_of(bias_id[i]), number = i * kThreads + tid;
+                if (number < p.biases) bias_at[number] = v;
                 if (v < 0) continue;
-                const int h = atomicAdd(&hits, 1);
-                hit_at[h] = v << 10 | number;
-                hit_value[h] = p.bias_values[(size_t)r * p.biases + number];
+                bias_value[number] = p.bias_values[(size_t)r * p.biases + number];
                 const uint32_t bit = 1u << (v & 31);
                 if (atomicOr(&biased[v >> 5], bit) & bit) {
                     again = 1;
                     atomicOr(&twice[v >> 5], bit);
                 } else {
-                    atomicAdd(&count[v], (uint32_t)(h + 1) << kCountBits);
+                    atomicAdd(&count[v], (uint32_t)(number + 1) << kCountBits);
                     atomicOr(&counted[v >> 5], bit);
                 }
             }
         }
         __syncthreads();
-        if (biases && again) {  // an index that stands several times: the hit that its place names gets all of them, added up in their order
-            for (int h = tid; h < hits; h += kThreads) {
-                const int v = hit_at[h] >> 10;
-                if (!(twice[v >> 5] >> (v & 31) & 1) || (int)(count[v] >> kCountBits) != h + 1) continue;
+        if (biases && again) {  // an index that stands several times: the one that its place names gets all of them, added up in the list's order
+#pragma unroll 1
+            for (int number = tid; number < p.biases; number += kThreads) {
+                const int v = bias_at[number];
+                if (v < 0 || !(twice[v >> 5] >> (v & 31) & 1) || (int)(count[v] >> kCountBits) != number + 1) continue;
                 float sum = 0.f;
-                for (int last = (v << 10) - 1;;) {
-                    int next = INT32_MAX, from = 0;
-                    for (int i = 0; i < hits; ++i) {
-                        const int other = hit_at[i];
-                        if (other >> 10 == v && other > last && other < next) {
-                            next = other;
-                            from = i;
-                        }
-                    }
-                    if (next == INT32_MAX) break;
-                    sum += hit_value[from];  // (of this place only)
-                    last = next;
+#pragma unroll 8
+                for (int i = 0; i < p.biases; ++i) {
+                    const float next = sum + bias_value[i];  // (another place's may be anything)
+                    sum = bias_at[i] == v ? next : sum;
                 }
-                hit_value[h] = sum;
+                bias_value[number] = sum;
             }
             __syncthreads();
         }
@@ -254,7 +246,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 6 : 8) void adjust_logits_kernel(
                         const float less = z > 0.f ? z / repetition : z * repetition;
                         z = less - frequency * (float)c - presence;
                     }
-                    if (h > 0) z += hit_value[h - 1];
+                    if (h > 0) z += bias_value[h - 1];
                     const uint32_t y = (old & ~(0xffffu << shift)) | (uint32_t)Elem<E>::to_bits(z) << shift;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] = j >> 1 == k ? y : w[k];
