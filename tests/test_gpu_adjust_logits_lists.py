@@ -1,4 +1,4 @@
-"""adjust_logits: long lists of biases that name the same tokens again and again."""
+"""adjust_logits: long lists of biases that name the same tokens again and again, and what a call's indexes hold."""
 import numpy as np
 import pytest
 
@@ -50,3 +50,14 @@ def test_a_list_of_one_token_takes_no_longer(gpu):
             end.synchronize()
             times[i].append(begin.elapsed_time(end))
     assert min(times[1]) < 20 * min(times[0]), times
+
+
+@pytest.mark.parametrize("n", [0, 1, 2, 7, 512])
+def test_indexes_hold_nothing_else(gpu, n):
+    """A kept tensor of indexes keeps no workspace, and a saved one writes none."""
+    torch = gpu
+    from cpm.cu_amd import ops
+    z = torch.randn((n, 9001), device="cuda").half()
+    _, ids = ops.adjust_logits(z)
+    assert ids.storage_offset() == 0 and ids.untyped_storage().nbytes() == 4 * n
+    assert torch.equal(ids.long(), z.float().argmax(1))
