@@ -353,7 +353,7 @@ extern "C" int cpmcu_adjust_logits(const void* logits, int64_t logits_stride, in
     CPMCU_CHECK_ARG(n == 1 || (logits_stride >= V && out_stride >= V), "adjust_logits: rows closer than their %d values", V);
     CPMCU_CHECK_ARG(((uintptr_t)logits | (uintptr_t)out) % 2 == 0, "adjust_logits: rows have to lie on 2 bytes");
     const bool any = penalties || bias_ids;
-    CPMCU_CHECK_ARG(!any || num_requests >= 1, "adjust_logits: %d requests", num_requests);
+    CPMCU_CHECK_ARG(!any || (num_requests >= 1 && num_requests < 1 << 24), "adjust_logits: %d requests outside [1, 2^24)", num_requests);
     CPMCU_CHECK_ARG(!any || requests || num_requests == 1 || num_requests == n, "adjust_logits: %d rows of %d requests need requests", n, num_requests);
     CPMCU_CHECK_ARG(max_tokens <= kMostTokens, "adjust_logits: max_tokens=%d beyond 2^20", max_tokens);
     CPMCU_CHECK_ARG(!tokens || (penalties && lens && max_tokens >= 1), "adjust_logits: tokens go with penalties and lens, one place each at least");

@@ -744,7 +744,7 @@ int cpmcu_batch_decode_attention(const void* q, int64_t q_stride, const void* k_
  * in 32 bits, each operation rounded by itself, then once to the element type.
  *   logits [n][logits_stride], V values from the row's start, V <= 2^24; out alike, the same memory and stride (in place) or memory apart.  Rows on 2 bytes;
  *       logits and out at equal distances from 16 bytes are read and written in pieces of those.
- *   penalties float[num_requests][3]: repetition (> 0; 1: none), presence, frequency; or NULL.  tokens int32[num_requests][max_tokens <= 2^20] / lens int32[num_requests]:
+ *   penalties float[num_requests < 2^24][3]: repetition (> 0; 1: none), presence, frequency; or NULL.  tokens int32[num_requests][max_tokens <= 2^20] / lens int32[num_requests]:
  *       the texts, of which the first lens[r] tokens count (lens is taken within [0, max_tokens]; tokens outside [0, V) do not count); or both NULL.
  *   requests int32[n]: each row's request, one outside [0, num_requests): no text, no biases.  NULL: row t is request t's (num_requests = n) or all are of one request.
  *   bias_ids int32[num_requests][num_biases] / bias_values float[num_requests][num_biases]: up to 1024; one outside [0, V) is not used, and of one

@@ -104,3 +104,12 @@ def test_texts_beyond_a_place_s_count_are_refused():
 
 def test_no_logits_need_nothing():
     _logits(n=0, z=None, out=None, ids=None, ws=None)
+
+
+def test_more_requests_than_rows_may_be_are_refused():
+    """A request's penalties are found by a 32-bit product."""
+    for more in (dict(), dict(pen=None, tok=None, lens=None)):
+        with pytest.raises(ValueError, match="16777216 requests outside"):
+            _logits(R=1 << 24, req=P(13 * GIB), out=P(1 << 50), ids=P(1 << 52), **more)
+    with pytest.raises(ValueError, match="715827883 requests outside"):
+        _logits(R=715827883, req=P(13 * GIB), out=P(1 << 50), ids=P(1 << 52))
