@@ -21,7 +21,7 @@ struct BatchRows {
     int64_t table_stride;
     int num_requests, max_blocks, num_pages;
     int n, Hq, Hkv, group;
-    uint32_t group_inverse;  // 0xffffffff / group
+    uint32_t group_inverse;  // 0xffffffff / group (prompts)
     float scale_log2;  // the scores' factor times log2 e: probabilities are powers of two
 };
 
@@ -45,6 +45,16 @@ __device__ inline Quotient divide(int x, int d, uint32_t inverse) {
     a.q += more ? 1 : 0;
     a.r -= more ? d : 0;
     return a;
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// Four KB of a wave from memory to LDS, whole lines: each lane's 16 bytes of each from where it says, in lane order; the instructions add 1 KB each to both addresses.  Their arrival is
+// counted by hand: written as loads that the compiler knows, every read of LDS would wait for all of them.  One statement: nothing comes between m0 and its use.
+__device__ inline void request_4k(const void* base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds_at) {
+    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %2, %4 offset:2*1024\n\tglobal_load_lds_dwordx4 %3, %4 offset:3*1024"
+                 : : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds_at) : "memory", "m0");
 }
 
 inline int check_batch_rows(const char* what, const BatchRows& b, float scale) {

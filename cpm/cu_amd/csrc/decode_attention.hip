@@ -38,7 +38,6 @@ template <typename E>
 constexpr float kLift = Elem<E>::kDtype == 0 ? 12.f : 0.f;
 constexpr int kFewRequests = 1024;  // up to which the line's ends leave room for two workgroups a CU
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 struct Line {
     int parts;  // that are cut
@@ -81,14 +80,6 @@ __device__ inline int tiles_of(const BatchRows& b, int r, int& row, int& pos) {
     pos = b.positions[row];
     if (pos < 0 || pos >= (int64_t)b.max_blocks * kPage) return 0;
     return pos / kTileKeys + 1;
-}
-
-// Four KB from memory to LDS, whole lines: lane's 16 bytes of each from where it says, in lane order; the instructions add 1 KB each to both addresses.  Their arrival
-// is counted by hand.
-__device__ inline void request_4k(const void* base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds_at) {
-    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %2, %4 offset:2*1024\n\tglobal_load_lds_dwordx4 %3, %4 offset:3*1024"
-                 : : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds_at) : "memory", "m0");
 }
 
 // MOST: requests that the line may have (0: no line, a workgroup has a request's keys on a KV head).
@@ -518,7 +509,6 @@ extern "C" int cpmcu_batch_decode_attention(const void* q, int64_t q_stride, con
     const int rc = check_batch_rows("decode_attention", b, scale);
     if (rc != CPMCU_OK) return rc;
     if (n == 0) return CPMCU_OK;
-    b.group_inverse = 0xffffffffu / (uint32_t)b.group;
     CPMCU_CHECK_ARG(row_offsets || n == num_requests, "decode_attention: %d rows of %d requests need row_offsets", n, num_requests);
     const Sizes s = sizes_of(num_requests, max_blocks, Hq, Hkv);
     CPMCU_CHECK_ARG(workspace && workspace_bytes >= s.bytes, "decode_attention: workspace of %zu bytes, %zu needed", workspace_bytes, s.bytes);

@@ -279,20 +279,10 @@ struct PromptParams {
     float2* stats;  // [slot][KV head][128]: (reference in powers of two, sum)
 };
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
 // K: a row of 256 bytes a key, its 16-byte pieces exchanged by the key's number; V: a row of 128 bytes a dim, by half of the dim's (even and
 // odd rows are in different halves of the banks).  Both ways the matrix operands are read without conflicts.
 __device__ inline int k_at(int key, int piece) { return key * 256 + ((piece ^ (key & 15)) << 4); }
 __device__ inline int v_at(int d, int piece) { return kKBytes + d * 128 + ((piece ^ ((d >> 1) & 7)) << 4); }
-
-// Four KB of a wave from memory to LDS: each lane's 16 bytes of each from where it says, in lane order; the instructions add 1 KB each to both addresses.  Their arrival is counted
-// by hand: written as loads that the compiler knows, every read of LDS would wait for all of them.  One statement: nothing comes between m0 and its use.
-__device__ inline void request_4k(const void* base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3, uint32_t lds_at) {
-    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %2, %4 offset:2*1024\n\tglobal_load_lds_dwordx4 %3, %4 offset:3*1024"
-                 : : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds_at) : "memory", "m0");
-}
 
 template <typename E>
 __device__ inline bool not_finite(E v) {
