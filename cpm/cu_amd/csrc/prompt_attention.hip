@@ -48,6 +48,7 @@ struct Listed {
 // few tiles of rows, kMostKeys where there are enough for all CUs, by the square of their number in between.  Measured with 8, 16, 24 and 64 throughout (us): 8 rows at 12000 cached
 // (2 tiles) 24, 27, 33, 68; 64 rows at 4000 (16) 22, 26, 31, 66; 512 rows at 8000 on 8 heads (128) 90, 89, 92, 97; 1000 rows (250) 28, 24, 24, 24; 4 x 256 rows at 6000 (256)
 // 125, 125, 125, 110; 4096 rows (1024) 163, 163, 163, 146.  With this rule 24, 22, 92, 24, 116 and 151.
+// (The lengths do not count: 1777 rows of 16 heads, 224 tiles of up to 33 tiles of keys, are not cut, 38.9; with pieces of 8, 12 and 17 at least 46.5, 38.7 and 38.1.)
 constexpr int kParts = 896, kLeastKeys = 8, kMostKeys = 64;
 constexpr int kMostChunk = 1 << 21;  // longer than any tile's keys
 __host__ __device__ inline int64_t least_of(int64_t tiles, int Hkv) {

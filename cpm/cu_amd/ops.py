@@ -262,7 +262,7 @@ class PageBatch:
 
     def attention(self, q, layer, where, single=False, scale=None, out=None):
         """Every row of a plan (``where``) over its request's pages, behind the appends: prompt_attention, or, where no request has more than one row,
-        decode_attention (single)."""
+        decode_attention (single).  The tables go whole: where a bound on the requests' lengths is known, these with its columns are faster for short ones."""
         if single:
             return decode_attention(q, self.cache, layer, self.block_tables, where["positions"], where["row_offsets"], scale, out)
         return prompt_attention(q, self.cache, layer, self.block_tables, where["row_offsets"], where["positions"], scale, out)
@@ -312,7 +312,8 @@ def prompt_attention(q, cache, layer, block_tables, row_offsets, positions, scal
     block_tables int32 [B, max_blocks], row_offsets int32 [B + 1] and positions int32 [n] as batch_tables gives them: request r's rows are
     [row_offsets[r], row_offsets[r + 1]), the first at positions[row_offsets[r]], each sees the tokens of its request up to its own, which have been appended
     (kv_append_slots).  Rows of refused requests, and behind the last one, keep what out held (a new tensor has no values there).  q and out may be
-    parts of wider rows; out may be q.  See PageBatch.attention.
+    parts of wider rows; out may be q.  How many columns the tables have decides the launches and the workspace (about 120 MB where they have room for long
+    requests): columns that no request reaches are best left out (block_tables[:, :columns]).  See PageBatch.attention.
     """
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -340,7 +341,7 @@ def adjust_logits(logits, penalties=None, tokens=None, lens=None, requests=None,
     row's request (-1: none); left out, row t is request t's, or all are of the only one.  bias_ids int32 / bias_values fp32 [R, up to 1024] (-1: not used).
     allowed int32 [n, ceil(V / 32)]: bit v % 32 of word v / 32 (``mask.expand(n, -1)``: one for all rows).  draft_ids int32 [n] / tree_mask int64
     [n, words]: the rows are the nodes of one request's draft tree, and the drafts on a node's way, its own among them, stand behind the request's tokens.
-    out may be logits (in place).
+    All three penalties count the same text.  out may be logits (in place).
     """
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)

@@ -723,8 +723,9 @@ int cpmcu_int8_linear_plan(int n, int V, int K, char* kernel_name, size_t kernel
  *   max_blocks * 256 on, rows in front of row_offsets[0] and behind row_offsets[num_requests].
  * Values that a row does not see -- later rows' keys and values, what a page holds behind the last token -- do not reach its result, infinities
  * and NaN among them.  Scores, sums and statistics in 32 bits; probabilities are rounded to the element type before their product with V, whose sum is that of
- * the rounded ones.  scale > 0.  Any mixture of rows and lengths: which work there is is listed on the device, long ones are cut and joined; nothing is
- * read back, and a captured call may be replayed with other offsets, positions and tables.
+ * the rounded ones (fp16: those below e^-16.6 of a row's largest, in decoding e^-18, with fewer bits).  scale > 0.  Any mixture of rows and lengths: which work there is is listed on the device, long ones are cut and joined; nothing is
+ * read back, and a captured call may be replayed with other offsets, positions and tables.  max_blocks decides which launches are made (short tables need neither
+ * list nor join) and the workspace's size: about 120 MB, whatever the batch is, where tables have room for long requests.
  *   workspace: at least cpmcu_batch_prompt_attention_workspace_bytes, on 16 bytes; its contents do not matter.  Calls that may overlap need one each. */
 size_t cpmcu_batch_prompt_attention_workspace_bytes(int num_requests, int max_blocks, int n, int Hq, int Hkv);
 int cpmcu_batch_prompt_attention(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, int num_pages, const int32_t* block_tables,

@@ -25,6 +25,8 @@ def _expect(b, hidden=lambda at: at < 0, shift=0):
     h = HALF_STEP[b.dtype]
     for r, (cached, n) in enumerate(b.requests):
         lo = int(b.offsets[r])
+        if n == 0:
+            continue
         for g in range(b.Hkv):
             k, v = b.keys(r, g)
             k = torch.where(k.isfinite(), k, 0.0)
